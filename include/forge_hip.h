@@ -127,6 +127,54 @@ int forge_rope(int dtype,
                int64_t head_dim, int backward, void* stream);
 
 /* ------------------------------------------------------------------------
+ * RMS norm of q and k heads + RoPE in one pass (no reference counterpart: the
+ * reference's patched attention calls q_norm, k_norm and apply_rotary_pos_emb,
+ * forge/forge/patching/kernels/lora.py:254-264)
+ * ------------------------------------------------------------------------ */
+
+/* q_out = R(q r (q_weight + offset)) with r = 1/sqrt(mean(q^2) + eps) of each
+ * head and R the half-split rotation of the token's position; the same for k.
+ * q, k, cos, sin, positions, table_dtype, table_rows: as in forge_rope
+ * (positions outside the table: NaN for that token, nothing read).  q dtype
+ * fp32 / bf16 / fp16; weights [head_dim] fp32 / bf16 / fp16 (w_dtype).
+ * head_dim even, up to 1024; any n_q, n_kv; fewer than 2^30 heads in a call.
+ * In place (q_out == q with q's strides) is allowed. */
+int forge_qk_norm_rope_fwd(int dtype,
+                           const void* q, int64_t q_sb, int64_t q_sh, int64_t q_ss,
+                           const void* k, int64_t k_sb, int64_t k_sh, int64_t k_ss,
+                           void* q_out, int64_t qo_sb, int64_t qo_sh, int64_t qo_ss,
+                           void* k_out, int64_t ko_sb, int64_t ko_sh, int64_t ko_ss,
+                           const void* q_weight, const void* k_weight, int w_dtype,
+                           const void* cos, int64_t cos_sb, int64_t cos_ss,
+                           const void* sin, int64_t sin_sb, int64_t sin_ss,
+                           int table_dtype, int64_t table_rows, const int64_t* positions,
+                           int64_t batch, int64_t n_q, int64_t n_kv, int64_t seq_len, int64_t head_dim,
+                           double eps, double offset, void* stream);
+
+/* Bytes of `work` for a forge_qk_norm_rope_bwd call with weight gradients. */
+int64_t forge_qk_norm_rope_bwd_workspace(int64_t head_dim);
+
+/* Backward: dq, dk are the gradients of q_out, k_out; q, k the forward's
+ * inputs; dq_in, dk_in the gradients of q, k.  dq_weight / dk_weight (w_dtype,
+ * [head_dim]) may be NULL (a frozen norm); with either, `work` holds
+ * forge_qk_norm_rope_bwd_workspace bytes, and the sums over tokens and heads
+ * are taken in a fixed order. */
+int forge_qk_norm_rope_bwd(int dtype,
+                           const void* dq, int64_t dq_sb, int64_t dq_sh, int64_t dq_ss,
+                           const void* dk, int64_t dk_sb, int64_t dk_sh, int64_t dk_ss,
+                           const void* q, int64_t q_sb, int64_t q_sh, int64_t q_ss,
+                           const void* k, int64_t k_sb, int64_t k_sh, int64_t k_ss,
+                           void* dq_in, int64_t qi_sb, int64_t qi_sh, int64_t qi_ss,
+                           void* dk_in, int64_t ki_sb, int64_t ki_sh, int64_t ki_ss,
+                           const void* q_weight, const void* k_weight, int w_dtype,
+                           const void* cos, int64_t cos_sb, int64_t cos_ss,
+                           const void* sin, int64_t sin_sb, int64_t sin_ss,
+                           int table_dtype, int64_t table_rows, const int64_t* positions,
+                           void* dq_weight, void* dk_weight, void* work,
+                           int64_t batch, int64_t n_q, int64_t n_kv, int64_t seq_len, int64_t head_dim,
+                           double eps, double offset, void* stream);
+
+/* ------------------------------------------------------------------------
  * Cross-entropy (online softmax, dlogits written in place)
  * ------------------------------------------------------------------------ */
 

@@ -1,0 +1,408 @@
+// RMS norm of every query and key head and its rotary embedding, in one pass
+// over q and k, for gfx950; forward and backward.
+//
+// Per head x of D values, with r = 1 / sqrt(mean(x^2) + eps), n = x r,
+// w = weight + offset and the half-split rotation R of the token's position:
+//     out = R (n w)
+// and, with dy = R^T dout (R is orthogonal: the same rotation by -theta),
+//     dweight = sum over tokens and heads of dy n
+//     g = dy w,   dx = r (g - n mean(g n)).
+// Everything is fp32 between the loads and the one rounding of each output.
+//
+// Bound by HBM: forward 2 and backward 3 passes over q and k.  A head is
+// shared by L lanes (a power of two): lane c owns 16 bytes at c of the lower
+// half and the 16 bytes they rotate with in the upper half, so nothing leaves
+// the lane but the sum of squares (and the mean of g n).
+#include "common.h"
+
+namespace {
+
+constexpr int kBlock = 256;
+constexpr int kMaxHalf = 512;      // head_dim up to 1024
+constexpr int kMaxBlocks = 16384;  // 64 workgroups per CU
+constexpr int kDwBlocks = 2048;    // workgroups (each one row of partial sums) where weights take gradients
+
+// (batch, head, seq) element strides of a [B, heads, S, D] tensor
+struct View {
+  int64_t sb, sh, ss;
+};
+
+struct Side {  // q or k
+  const void* x; View xv;
+  const void* dy; View dv;   // backward: gradient of the output
+  void* out; View ov;        // forward: the output; backward: dx
+  const void* w;
+  float* part;               // backward: [blocks][D] partial sums of dweight, or nullptr
+  uint32_t rows, heads;      // rows = B * S * heads
+  uint32_t blocks;
+};
+
+struct Args {
+  Side q, k;
+  const void* cos; int64_t cos_sb, cos_ss;
+  const void* sin; int64_t sin_sb, sin_ss;
+  const int64_t* positions;
+  int64_t table_rows;
+  uint32_t seq_len;
+  int half, lanes;
+  float eps, offset, inv_d;
+  int w_dtype;
+};
+
+__device__ __forceinline__ float load_w(const void* w, int dtype, int i) {
+  if (dtype == FORGE_DTYPE_BF16) return (float)((const bf16_t*)w)[i];
+  if (dtype == FORGE_DTYPE_F16) return (float)((const fp16_t*)w)[i];
+  return ((const float*)w)[i];
+}
+
+// Sum over the L lanes that share a head.
+__device__ __forceinline__ float head_sum(float v, int lanes) {
+  for (int off = lanes >> 1; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+// A lane's values of one half of a head.  VEC: 16 bytes at column c * E;
+// otherwise (unaligned, or a half that is no multiple of 16 bytes) elements c,
+// c + L, ...
+template <class T, bool VEC>
+struct Lane {
+  static constexpr int E = VEC ? 16 / (int)sizeof(T) : 8;
+  int c, lanes, half;
+  __device__ __forceinline__ int col(int j) const { return VEC ? c * E + j : c + j * lanes; }
+  __device__ __forceinline__ bool on(int j) const { return col(j) < half; }
+  template <bool NT>
+  __device__ __forceinline__ void load(const T* p, float (&v)[E]) const {
+    if constexpr (VEC) {
+      Vec16<T> t = NT ? load16_nt(p + c * E) : load16(p + c * E);
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = to_f32(t.v[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = on(j) ? to_f32(p[col(j)]) : 0.f;
+    }
+  }
+  __device__ __forceinline__ void store(T* p, const float (&v)[E]) const {
+    if constexpr (VEC) {
+      Vec16<T> t;
+#pragma unroll
+      for (int j = 0; j < E; ++j) t.v[j] = from_f32<T>(v[j]);
+      store16_nt(p + c * E, t);
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (on(j)) p[col(j)] = from_f32<T>(v[j]);
+    }
+  }
+  // cos or sin values of type TC at the same columns
+  template <class TC>
+  __device__ __forceinline__ void table(const TC* p, float (&v)[E]) const {
+    if constexpr (VEC) {
+      constexpr int PER = 16 / (int)sizeof(TC);
+#pragma unroll
+      for (int k = 0; k < E / PER; ++k) {
+        Vec16<TC> t = load16(p + c * E + k * PER);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) v[k * PER + j] = to_f32(t.v[j]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = on(j) ? to_f32(p[col(j)]) : 0.f;
+    }
+  }
+};
+
+template <class T, class TC, bool VEC, bool BWD>
+__global__ __launch_bounds__(kBlock) void qk_norm_rope_kernel(Args a) {
+  using LaneT = Lane<T, VEC>;
+  constexpr int E = LaneT::E;
+  extern __shared__ float lds[];  // backward with weight gradients: [waves][D]
+  const bool is_k = blockIdx.x >= a.q.blocks;
+  const Side& s = is_k ? a.k : a.q;
+  const uint32_t block = is_k ? blockIdx.x - a.q.blocks : blockIdx.x;
+  const int lanes = a.lanes, half = a.half;
+  const LaneT lane{(int)threadIdx.x & (lanes - 1), lanes, half};
+  const bool active = VEC ? lane.c * E < half : lane.c < half;
+  const uint32_t per_block = kBlock / lanes;
+
+  float wl[E], wh[E], al[E], ah[E];  // weight of the lower and upper half, and their gradients' sums
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    wl[j] = active && lane.on(j) ? load_w(s.w, a.w_dtype, lane.col(j)) + a.offset : 0.f;
+    wh[j] = active && lane.on(j) ? load_w(s.w, a.w_dtype, half + lane.col(j)) + a.offset : 0.f;
+    al[j] = ah[j] = 0.f;
+  }
+
+  for (uint32_t row = block * per_block + threadIdx.x / lanes; row < s.rows; row += s.blocks * per_block) {
+    const uint32_t t = row / s.heads, h = row - t * s.heads;
+    const uint32_t b = t / a.seq_len, sq = t - b * a.seq_len;
+    const int64_t pos = a.positions ? a.positions[t] : (int64_t)sq;
+    const bool in_table = pos >= 0 && pos < a.table_rows;
+    float xl[E] = {}, xh[E] = {}, cs[E] = {}, sn[E] = {}, gl[E] = {}, gh[E] = {};
+    if (active) {
+      const T* x = (const T*)s.x + ((int64_t)b * s.xv.sb + (int64_t)h * s.xv.sh + (int64_t)sq * s.xv.ss);
+      lane.template load<true>(x, xl);
+      lane.template load<true>(x + half, xh);
+      if constexpr (BWD) {
+        const T* dy = (const T*)s.dy + ((int64_t)b * s.dv.sb + (int64_t)h * s.dv.sh + (int64_t)sq * s.dv.ss);
+        lane.template load<true>(dy, gl);
+        lane.template load<true>(dy + half, gh);
+      }
+      if (in_table) {
+        lane.table((const TC*)a.cos + ((int64_t)b * a.cos_sb + pos * a.cos_ss), cs);
+        lane.table((const TC*)a.sin + ((int64_t)b * a.sin_sb + pos * a.sin_ss), sn);
+      } else {
+        // a position outside the table: nothing is read, the token's outputs are NaN
+#pragma unroll
+        for (int j = 0; j < E; ++j) cs[j] = sn[j] = __builtin_nanf("");
+      }
+    }
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < E; ++j) ss += xl[j] * xl[j] + xh[j] * xh[j];
+    const float r = rsqrtf(head_sum(ss, lanes) * a.inv_d + a.eps);
+    if constexpr (!BWD) {
+      float ol[E], oh[E];
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float yl = xl[j] * r * wl[j], yh = xh[j] * r * wh[j];
+        ol[j] = yl * cs[j] - yh * sn[j];
+        oh[j] = yh * cs[j] + yl * sn[j];
+      }
+      if (active) {
+        T* o = (T*)s.out + ((int64_t)b * s.ov.sb + (int64_t)h * s.ov.sh + (int64_t)sq * s.ov.ss);
+        lane.store(o, ol);
+        lane.store(o + half, oh);
+      }
+    } else {
+      float dot = 0.f;
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float dl = gl[j] * cs[j] + gh[j] * sn[j], dh = gh[j] * cs[j] - gl[j] * sn[j];
+        xl[j] *= r;  // n
+        xh[j] *= r;
+        al[j] += dl * xl[j];
+        ah[j] += dh * xh[j];
+        gl[j] = dl * wl[j];
+        gh[j] = dh * wh[j];
+        dot += gl[j] * xl[j] + gh[j] * xh[j];
+      }
+      const float mean = head_sum(dot, lanes) * a.inv_d;
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        gl[j] = r * (gl[j] - xl[j] * mean);
+        gh[j] = r * (gh[j] - xh[j] * mean);
+      }
+      if (active) {
+        T* o = (T*)s.out + ((int64_t)b * s.ov.sb + (int64_t)h * s.ov.sh + (int64_t)sq * s.ov.ss);
+        lane.store(o, gl);
+        lane.store(o + half, gh);
+      }
+    }
+  }
+
+  if constexpr (BWD) {
+    if (!s.part) return;  // (uniform over the workgroup)
+    // this workgroup's row of partial sums, in a fixed order: the groups of a
+    // wave by shuffles, then the waves
+    const int wave = threadIdx.x >> 6, wl_ = threadIdx.x & 63;
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      for (int off = lanes; off < 64; off <<= 1) {
+        al[j] += __shfl_xor(al[j], off, 64);
+        ah[j] += __shfl_xor(ah[j], off, 64);
+      }
+    if (wl_ < lanes && active) {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (lane.on(j)) {
+          lds[wave * 2 * half + lane.col(j)] = al[j];
+          lds[wave * 2 * half + half + lane.col(j)] = ah[j];
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * half; i += kBlock) {
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < kBlock / 64; ++w) v += lds[w * 2 * half + i];
+      s.part[(int64_t)block * 2 * half + i] = v;
+    }
+  }
+}
+
+// dweight[i] = sum over the workgroups' partial sums, in a fixed order: 32
+// columns a workgroup, 32 threads to a column.  blockIdx.y: q or k.
+__global__ __launch_bounds__(1024) void qk_dweight_kernel(const float* qp, uint32_t q_blocks, void* dqw, const float* kp,
+                                                          uint32_t k_blocks, void* dkw, int d, int w_dtype) {
+  __shared__ float red[32][33];
+  const float* part = blockIdx.y ? kp : qp;
+  const int n = (int)(blockIdx.y ? k_blocks : q_blocks);
+  void* out = blockIdx.y ? dkw : dqw;
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int i = blockIdx.x * 32 + x;
+  if (!part) return;  // (uniform)
+  float v = 0.f;
+  if (i < d) {
+#pragma unroll 8
+    for (int b = y; b < n; b += 32) v += part[(int64_t)b * d + i];
+  }
+  red[y][x] = v;
+  __syncthreads();
+  if (y == 0 && i < d) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) t += red[k][x];
+    if (w_dtype == FORGE_DTYPE_BF16) ((bf16_t*)out)[i] = (bf16_t)t;
+    else if (w_dtype == FORGE_DTYPE_F16) ((fp16_t*)out)[i] = (fp16_t)t;
+    else ((float*)out)[i] = t;
+  }
+}
+
+int lanes_for(int64_t half, bool vec, size_t es) {
+  const int64_t chunks = vec ? half * (int64_t)es / 16 : half;
+  int lanes = 1;
+  while (lanes < chunks && lanes < 64) lanes <<= 1;
+  return lanes;
+}
+
+uint32_t blocks_for(uint32_t rows, int lanes, uint32_t most) {
+  const uint32_t per = kBlock / lanes;
+  const uint32_t b = (rows + per - 1) / per;
+  return b > most ? most : b;
+}
+
+// Workgroups of q and k: all they can use up to the cap, shared by their rows.
+void split_blocks(uint32_t q_rows, uint32_t k_rows, int lanes, bool dw, uint32_t& qb, uint32_t& kb) {
+  const uint64_t cap = dw ? kDwBlocks : kMaxBlocks, all = (uint64_t)q_rows + k_rows;
+  const uint32_t q_cap = (uint32_t)((cap * q_rows + all - 1) / all), k_cap = (uint32_t)((cap * k_rows + all - 1) / all);
+  qb = blocks_for(q_rows, lanes, q_cap);
+  kb = blocks_for(k_rows, lanes, k_cap);
+}
+
+template <class T, class TC, bool BWD>
+void launch(const Args& a, bool vec, uint32_t blocks, size_t lds, hipStream_t s) {
+  if (vec) qk_norm_rope_kernel<T, TC, true, BWD><<<blocks, kBlock, lds, s>>>(a);
+  else qk_norm_rope_kernel<T, TC, false, BWD><<<blocks, kBlock, lds, s>>>(a);
+}
+
+template <bool BWD>
+int run(int dtype, const char* what, Args& a, int w_dtype, int table_dtype, int64_t batch, int64_t n_q, int64_t n_kv,
+        int64_t seq_len, int64_t head_dim, double eps, double offset, void* dqw, void* dkw, float* work, void* stream) {
+  if (batch < 0 || n_q < 0 || n_kv < 0 || seq_len < 0)
+    return forge_set_error(FORGE_ERR_INVALID, "%s: negative shape", what);
+  if (head_dim <= 0 || head_dim % 2 != 0 || head_dim / 2 > kMaxHalf)
+    return forge_set_error(FORGE_ERR_INVALID, "%s: head_dim %lld (even, up to %d)", what, (long long)head_dim, 2 * kMaxHalf);
+  if (dtype != FORGE_DTYPE_F32 && dtype != FORGE_DTYPE_BF16 && dtype != FORGE_DTYPE_F16)
+    return forge_set_error(FORGE_ERR_UNSUPPORTED, "%s: dtype %d", what, dtype);
+  if (w_dtype != FORGE_DTYPE_F32 && w_dtype != FORGE_DTYPE_BF16 && w_dtype != FORGE_DTYPE_F16)
+    return forge_set_error(FORGE_ERR_UNSUPPORTED, "%s: weight dtype %d", what, w_dtype);
+  if (table_dtype != dtype && table_dtype != FORGE_DTYPE_F32)
+    return forge_set_error(FORGE_ERR_UNSUPPORTED, "%s: cos/sin dtype %d with q dtype %d (tables are q's dtype or fp32)",
+                           what, table_dtype, dtype);
+  if (a.table_rows < 0) return forge_set_error(FORGE_ERR_INVALID, "%s: negative table_rows", what);
+  if (!a.positions && a.table_rows < seq_len)
+    return forge_set_error(FORGE_ERR_INVALID, "%s: cos/sin have %lld rows for seq_len %lld", what,
+                           (long long)a.table_rows, (long long)seq_len);
+  const int64_t lim = 0x40000000;  // rows, and a grid's step past them, stay below 2^32
+  if (batch > lim || n_q > lim || n_kv > lim || seq_len > lim || batch * seq_len > lim ||
+      batch * seq_len * (n_q > n_kv ? n_q : n_kv) > lim)
+    return forge_set_error(FORGE_ERR_UNSUPPORTED, "%s: more than 2^30 heads in a call", what);
+  if ((dqw || dkw) && !work) return forge_set_error(FORGE_ERR_INVALID, "%s: weight gradients need the workspace", what);
+
+  const size_t es = dtype_size(dtype), ets = dtype_size(table_dtype);
+  const int64_t V = (int64_t)(16 / es), Vt = (int64_t)(16 / ets);
+  a.half = (int)(head_dim / 2);
+  bool vec = a.half % V == 0 && a.half / V <= 64 && aligned16(a.cos) && aligned16(a.sin);
+  for (const Side* s : {&a.q, &a.k}) {
+    vec = vec && aligned16(s->x) && aligned16(s->out) && (!BWD || aligned16(s->dy));
+    for (int64_t st : {s->xv.sb, s->xv.sh, s->xv.ss, s->ov.sb, s->ov.sh, s->ov.ss}) vec = vec && st % V == 0;
+    if (BWD)
+      for (int64_t st : {s->dv.sb, s->dv.sh, s->dv.ss}) vec = vec && st % V == 0;
+  }
+  for (int64_t st : {a.cos_sb, a.cos_ss, a.sin_sb, a.sin_ss}) vec = vec && st % Vt == 0;
+  a.lanes = lanes_for(a.half, vec, es);
+  a.seq_len = (uint32_t)seq_len;
+  a.eps = (float)eps;
+  a.offset = (float)offset;
+  a.inv_d = (float)(1.0 / (double)head_dim);
+  a.w_dtype = w_dtype;
+  a.q.heads = (uint32_t)n_q;
+  a.k.heads = (uint32_t)n_kv;
+  a.q.rows = (uint32_t)(batch * seq_len * n_q);
+  a.k.rows = (uint32_t)(batch * seq_len * n_kv);
+  hipStream_t s = (hipStream_t)stream;
+  const bool dw = dqw || dkw;
+  a.q.blocks = a.k.blocks = 0;
+  if (a.q.rows + a.k.rows) split_blocks(a.q.rows, a.k.rows, a.lanes, dw, a.q.blocks, a.k.blocks);
+  if (dw) {  // both sides' partial sums, one after the other
+    a.q.part = dqw ? work : nullptr;
+    a.k.part = dkw ? work + (int64_t)a.q.blocks * head_dim : nullptr;
+  }
+  const uint32_t blocks = a.q.blocks + a.k.blocks;
+  if (blocks) {
+    const size_t lds = dw ? (kBlock / 64) * (size_t)head_dim * sizeof(float) : 0;
+    const bool f32_table = table_dtype != dtype;
+    switch (dtype) {
+      case FORGE_DTYPE_F32: launch<float, float, BWD>(a, vec, blocks, lds, s); break;
+      case FORGE_DTYPE_BF16:
+        if (f32_table) launch<bf16_t, float, BWD>(a, vec, blocks, lds, s);
+        else launch<bf16_t, bf16_t, BWD>(a, vec, blocks, lds, s);
+        break;
+      default:
+        if (f32_table) launch<fp16_t, float, BWD>(a, vec, blocks, lds, s);
+        else launch<fp16_t, fp16_t, BWD>(a, vec, blocks, lds, s);
+    }
+    FORGE_CHECK_LAUNCH();
+  }
+  if (dw) {  // (no rows: zeros)
+    qk_dweight_kernel<<<dim3((unsigned)((head_dim + 31) / 32), 2), 1024, 0, s>>>(
+        a.q.part, a.q.blocks, dqw, a.k.part, a.k.blocks, dkw, (int)head_dim, w_dtype);
+    FORGE_CHECK_LAUNCH();
+  }
+  return FORGE_OK;
+}
+
+}  // namespace
+
+extern "C" int forge_qk_norm_rope_fwd(int dtype, const void* q, int64_t q_sb, int64_t q_sh, int64_t q_ss, const void* k,
+                                      int64_t k_sb, int64_t k_sh, int64_t k_ss, void* q_out, int64_t qo_sb,
+                                      int64_t qo_sh, int64_t qo_ss, void* k_out, int64_t ko_sb, int64_t ko_sh,
+                                      int64_t ko_ss, const void* q_weight, const void* k_weight, int w_dtype,
+                                      const void* cos, int64_t cos_sb, int64_t cos_ss, const void* sin, int64_t sin_sb,
+                                      int64_t sin_ss, int table_dtype, int64_t table_rows, const int64_t* positions,
+                                      int64_t batch, int64_t n_q, int64_t n_kv, int64_t seq_len, int64_t head_dim,
+                                      double eps, double offset, void* stream) {
+  Args a = {};
+  a.q = {q, {q_sb, q_sh, q_ss}, nullptr, {}, q_out, {qo_sb, qo_sh, qo_ss}, q_weight, nullptr, 0, 0, 0};
+  a.k = {k, {k_sb, k_sh, k_ss}, nullptr, {}, k_out, {ko_sb, ko_sh, ko_ss}, k_weight, nullptr, 0, 0, 0};
+  a.cos = cos; a.cos_sb = cos_sb; a.cos_ss = cos_ss;
+  a.sin = sin; a.sin_sb = sin_sb; a.sin_ss = sin_ss;
+  a.positions = positions;
+  a.table_rows = table_rows;
+  return run<false>(dtype, "qk_norm_rope_fwd", a, w_dtype, table_dtype, batch, n_q, n_kv, seq_len, head_dim, eps, offset,
+                    nullptr, nullptr, nullptr, stream);
+}
+
+extern "C" int64_t forge_qk_norm_rope_bwd_workspace(int64_t head_dim) {
+  return (kDwBlocks + 2) * head_dim * (int64_t)sizeof(float);
+}
+
+extern "C" int forge_qk_norm_rope_bwd(int dtype, const void* dq, int64_t dq_sb, int64_t dq_sh, int64_t dq_ss,
+                                      const void* dk, int64_t dk_sb, int64_t dk_sh, int64_t dk_ss, const void* q,
+                                      int64_t q_sb, int64_t q_sh, int64_t q_ss, const void* k, int64_t k_sb,
+                                      int64_t k_sh, int64_t k_ss, void* dq_in, int64_t qi_sb, int64_t qi_sh,
+                                      int64_t qi_ss, void* dk_in, int64_t ki_sb, int64_t ki_sh, int64_t ki_ss,
+                                      const void* q_weight, const void* k_weight, int w_dtype, const void* cos,
+                                      int64_t cos_sb, int64_t cos_ss, const void* sin, int64_t sin_sb, int64_t sin_ss,
+                                      int table_dtype, int64_t table_rows, const int64_t* positions, void* dq_weight,
+                                      void* dk_weight, void* work, int64_t batch, int64_t n_q, int64_t n_kv,
+                                      int64_t seq_len, int64_t head_dim, double eps, double offset, void* stream) {
+  Args a = {};
+  a.q = {q, {q_sb, q_sh, q_ss}, dq, {dq_sb, dq_sh, dq_ss}, dq_in, {qi_sb, qi_sh, qi_ss}, q_weight, nullptr, 0, 0, 0};
+  a.k = {k, {k_sb, k_sh, k_ss}, dk, {dk_sb, dk_sh, dk_ss}, dk_in, {ki_sb, ki_sh, ki_ss}, k_weight, nullptr, 0, 0, 0};
+  a.cos = cos; a.cos_sb = cos_sb; a.cos_ss = cos_ss;
+  a.sin = sin; a.sin_sb = sin_sb; a.sin_ss = sin_ss;
+  a.positions = positions;
+  a.table_rows = table_rows;
+  return run<true>(dtype, "qk_norm_rope_bwd", a, w_dtype, table_dtype, batch, n_q, n_kv, seq_len, head_dim, eps, offset,
+                   dq_weight, dk_weight, (float*)work, stream);
+}

@@ -1,6 +1,7 @@
 """RoPE re-export and the HF-signature adapter (reference
 forge/forge/kernels/rope.py:12-43)."""
 from kernels.rope.forge_rope_v3 import ForgeRoPEv3, ForgeRoPEv3Function, apply_rope
+from kernels.rope.qk_norm_rope import ForgeQKNormRoPE, ForgeQKNormRoPEFunction, apply_qk_norm_rope
 
 
 def forge_apply_rotary_pos_emb(q, k, cos, sin, position_ids=None, unsqueeze_dim=1):
@@ -19,4 +20,5 @@ def forge_apply_rotary_pos_emb(q, k, cos, sin, position_ids=None, unsqueeze_dim=
     return apply_rope(q, k, cos, sin)
 
 
-__all__ = ["apply_rope", "ForgeRoPEv3", "ForgeRoPEv3Function", "forge_apply_rotary_pos_emb"]
+__all__ = ["apply_rope", "ForgeRoPEv3", "ForgeRoPEv3Function", "forge_apply_rotary_pos_emb",
+           "apply_qk_norm_rope", "ForgeQKNormRoPE", "ForgeQKNormRoPEFunction"]

@@ -11,6 +11,7 @@ so no kernel path can silently run without the HIP code.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from pathlib import Path
@@ -96,6 +97,17 @@ forge_rope = _decl(
     + [c_vp, c_i64, c_i64] * 2
     + [c_int, c_i64]
     + [c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_int, c_vp],
+)
+_QK_STRIDED = [c_vp, c_i64, c_i64, c_i64]
+_QK_TABLES = [c_vp, c_i64, c_i64] * 2 + [c_int, c_i64, c_vp]
+_QK_SIZES = [c_i64] * 5 + [ctypes.c_double] * 2 + [c_vp]
+forge_qk_norm_rope_fwd = _decl(
+    "forge_qk_norm_rope_fwd", [c_int] + _QK_STRIDED * 4 + [c_vp, c_vp, c_int] + _QK_TABLES + _QK_SIZES
+)
+forge_qk_norm_rope_bwd_workspace = _decl("forge_qk_norm_rope_bwd_workspace", [c_i64], c_i64)
+forge_qk_norm_rope_bwd = _decl(
+    "forge_qk_norm_rope_bwd",
+    [c_int] + _QK_STRIDED * 6 + [c_vp, c_vp, c_int] + _QK_TABLES + [c_vp] * 3 + _QK_SIZES,
 )
 forge_ce_fwd = _decl(
     "forge_ce_fwd",
@@ -193,6 +205,7 @@ forge_cast_f32_bf16 = _decl("forge_cast_f32_bf16", [c_vp, c_i64, c_vp, c_i64, c_
 EXPORTED = [
     "forge_version", "forge_last_error", "forge_arch_ok",
     "forge_swiglu_fwd", "forge_swiglu_bwd", "forge_geglu_fwd", "forge_geglu_bwd", "forge_rope",
+    "forge_qk_norm_rope_fwd", "forge_qk_norm_rope_bwd", "forge_qk_norm_rope_bwd_workspace",
     "forge_ce_fwd", "forge_ce_target_stats", "forge_ce_fwd_reduce", "forge_ce_stats_wait", "forge_ce_scale",
     "forge_sum_f32",
     "forge_gemm", "forge_gemm_f16", "forge_lora_mlp_gate_up", "forge_lora_mlp_gate_up_v", "forge_lora_mlp_down_bwd", "forge_lora_mlp_down_bwd_v", "forge_lora_mlp_glu_bwd",
@@ -226,6 +239,15 @@ def stream_of(t: torch.Tensor) -> int:
     it).  The raw accessor skips building a Stream object (2 us -> 0.1 us per
     launch on the host)."""
     return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def on_device(t: torch.Tensor):
+    """Makes t's device the current one for a launch (its stream belongs to
+    that device); nothing to do where it is already."""
+    return _NO_SWITCH if torch._C._cuda_getDevice() == t.device.index else torch.cuda.device(t.device)
 
 
 def ptr(t):

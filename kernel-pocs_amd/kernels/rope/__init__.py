@@ -7,3 +7,8 @@ from .forge_rope_v3 import (  # noqa: F401
     get_autotune_cache_for,
     rope_cos_sin,
 )
+from .qk_norm_rope import (  # noqa: F401
+    ForgeQKNormRoPE,
+    ForgeQKNormRoPEFunction,
+    apply_qk_norm_rope,
+)
