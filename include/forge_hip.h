@@ -96,6 +96,30 @@ int forge_geglu_bwd(int dtype, const void* dout, int64_t ld_dout,
                     int64_t rows, int64_t cols, int approximate_tanh, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Gated activation that keeps gate and up in 8 bits for its backward (no
+ * reference counterpart)
+ * ------------------------------------------------------------------------ */
+
+/* Bytes of the `kept` buffer of a [rows, cols] call. */
+int64_t forge_glu_act8_bytes(int64_t rows, int64_t cols);
+
+/* out = act(gate) * up in fp32, rounded once; activation FORGE_ACT_*; rows of
+ * `cols` elements, pitches ld_* >= cols, any element alignment; fp32 / bf16 /
+ * fp16.  With kept != NULL (16-byte aligned, forge_glu_act8_bytes) gate and up
+ * are also written there in 8 bits: groups of 32 values of a row share the
+ * least power of two 2^e, e >= -126, with |x| <= 127 * 2^e, and a value is the
+ * integer round(x / 2^e); an infinity or NaN is kept as NaN.  Fewer than 2^34
+ * values in a call. */
+int forge_glu_act8_fwd(int dtype, int activation, const void* gate, int64_t ld_gate,
+                       const void* up, int64_t ld_up, void* out, int64_t ld_out,
+                       void* kept, int64_t rows, int64_t cols, void* stream);
+
+/* dgate = dout u act'(g), dup = dout act(g) with g, u the values in `kept`. */
+int forge_glu_act8_bwd(int dtype, int activation, const void* dout, int64_t ld_dout,
+                       const void* kept, void* dgate, void* dup, int64_t ld_grad,
+                       int64_t rows, int64_t cols, void* stream);
+
+/* ------------------------------------------------------------------------
  * RoPE (half-split rotation; any n_q, n_kv)
  * ------------------------------------------------------------------------ */
 

@@ -90,6 +90,13 @@ forge_geglu_fwd = _decl("forge_geglu_fwd", [c_int, c_vp, c_vp, c_i64, c_vp, c_i6
 forge_geglu_bwd = _decl(
     "forge_geglu_bwd", [c_int, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_int, c_vp]
 )
+forge_glu_act8_bytes = _decl("forge_glu_act8_bytes", [c_i64, c_i64], c_i64)
+forge_glu_act8_fwd = _decl(
+    "forge_glu_act8_fwd", [c_int, c_int, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_vp]
+)
+forge_glu_act8_bwd = _decl(
+    "forge_glu_act8_bwd", [c_int, c_int, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp]
+)
 forge_rope = _decl(
     "forge_rope",
     [c_int]
@@ -206,6 +213,7 @@ EXPORTED = [
     "forge_version", "forge_last_error", "forge_arch_ok",
     "forge_swiglu_fwd", "forge_swiglu_bwd", "forge_geglu_fwd", "forge_geglu_bwd", "forge_rope",
     "forge_qk_norm_rope_fwd", "forge_qk_norm_rope_bwd", "forge_qk_norm_rope_bwd_workspace",
+    "forge_glu_act8_bytes", "forge_glu_act8_fwd", "forge_glu_act8_bwd",
     "forge_ce_fwd", "forge_ce_target_stats", "forge_ce_fwd_reduce", "forge_ce_stats_wait", "forge_ce_scale",
     "forge_sum_f32",
     "forge_gemm", "forge_gemm_f16", "forge_lora_mlp_gate_up", "forge_lora_mlp_gate_up_v", "forge_lora_mlp_down_bwd", "forge_lora_mlp_down_bwd_v", "forge_lora_mlp_glu_bwd",
