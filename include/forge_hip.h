@@ -309,6 +309,82 @@ int forge_row_scale(int dtype, void* x, int64_t ld, int64_t n_rows, int64_t n_co
                     void* stream);
 
 /* ------------------------------------------------------------------------
+ * Log-probabilities of target tokens, preference and policy losses (no
+ * reference counterpart)
+ *
+ * Logits [N, S, V] by element strides ld_n, ld_s (unit column stride, any
+ * element alignment), fp32 / bf16 / fp16; target int64 [N, S] by strides t_n,
+ * t_s; other per-token arrays fp32 by their own strides (0 broadcasts).  Rows
+ * whose target is ignore_index are not read: their log-probability, loss and
+ * gradient are 0.  A target outside [0, V) that is not ignore_index makes its
+ * row NaN (and so the loss); nothing is read by it.  `work` holds
+ * forge_logp_workspace bytes, 16-byte aligned.  Every sum is taken in a fixed
+ * order.
+ * ------------------------------------------------------------------------ */
+enum {
+  FORGE_REDUCE_NONE = 0,
+  FORGE_REDUCE_MEAN = 1,      /* over kept tokens (policy) or pairs (preference) */
+  FORGE_REDUCE_SUM = 2,
+  FORGE_REDUCE_SEQUENCE = 3,  /* mean over the sequences of each one's mean */
+};
+
+enum {
+  FORGE_PREF_SIGMOID = 0, /* -(1 - e) log s(h) - e log s(-h), e = label smoothing */
+  FORGE_PREF_HINGE = 1,   /* max(0, 1 - h) */
+  FORGE_PREF_IPO = 2,     /* (h / beta - 1 / (2 beta))^2 */
+};
+
+int64_t forge_logp_workspace(int dtype, int64_t n, int64_t s, int64_t v);
+
+/* logps[n, s] (dense fp32) = log softmax(logits / temperature) at the target.
+ * state (2 floats a row, may be NULL): what forge_token_logps_bwd needs. */
+int forge_token_logps_fwd(int dtype, const void* logits, int64_t ld_n, int64_t ld_s,
+                          int64_t n, int64_t s, int64_t v,
+                          const int64_t* target, int64_t t_n, int64_t t_s, int64_t ignore_index,
+                          double temperature, float* logps, float* state, void* work, void* stream);
+
+/* dlogits[n, s, :] = c / temperature (onehot - softmax), c = coef[n, s], times
+ * up[(n % up_count) * up_stride] where up is given.  A row with c == 0 is
+ * written as zeros without being read.  dlogits may be the logits. */
+int forge_token_logps_bwd(int dtype, const void* logits, int64_t ld_n, int64_t ld_s,
+                          int64_t n, int64_t s, int64_t v,
+                          const int64_t* target, int64_t t_n, int64_t t_s, int64_t ignore_index,
+                          double temperature, const float* logps, const float* state,
+                          const float* coef, int64_t c_n, int64_t c_s,
+                          const float* up, int64_t up_stride, int64_t up_count,
+                          void* dlogits, int64_t d_n, int64_t d_s, void* stream);
+
+/* Preference loss over `pairs` pairs: N = 2 pairs sequences, the chosen
+ * answers, then the rejected ones in the same order.  h = beta ((pi_c - ref_c)
+ * - (pi_r - ref_r)) with pi the sum (normalized != 0: the mean) of an answer's
+ * log-probabilities and ref [2 pairs] the reference model's (NULL: 0).
+ * loss: one fp32 value, or [pairs] with FORGE_REDUCE_NONE; seq_logps, rewards =
+ * beta (pi - ref), coef (dloss/dlogp of a sequence's tokens): [2 pairs];
+ * logps, state: as in forge_token_logps_fwd.  The gradient is
+ * forge_token_logps_bwd with coef (c_n = 1, c_s = 0). */
+int forge_preference_fwd(int dtype, const void* logits, int64_t ld_n, int64_t ld_s,
+                         int64_t pairs, int64_t s, int64_t v,
+                         const int64_t* target, int64_t t_n, int64_t t_s, int64_t ignore_index,
+                         const float* ref, double beta, double label_smoothing, int kind,
+                         int normalized, int reduction, float* loss, float* seq_logps, float* rewards,
+                         float* coef, float* logps, float* state, void* work, void* stream);
+
+/* Clipped policy loss with a divergence from a reference model; per kept token
+ *   -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^f - f - 1),
+ *   r = exp(logp - old) (old_logps NULL: 1), f = ref - logp (ref_logps NULL: no
+ * such term), reduced to one fp32 value.  logps, kl (e^f - f - 1): dense fp32
+ * [N, S].  dlogits (NULL: loss only) gets dloss/dlogits and may be the logits. */
+int forge_policy_loss(int dtype, const void* logits, int64_t ld_n, int64_t ld_s,
+                      int64_t n, int64_t s, int64_t v,
+                      const int64_t* target, int64_t t_n, int64_t t_s, int64_t ignore_index,
+                      double temperature, const float* advantages, int64_t a_n, int64_t a_s,
+                      const float* old_logps, int64_t o_n, int64_t o_s,
+                      const float* ref_logps, int64_t r_n, int64_t r_s,
+                      double clip_low, double clip_high, double kl_coef, int reduction,
+                      float* loss, float* logps, float* kl,
+                      void* dlogits, int64_t d_n, int64_t d_s, void* work, void* stream);
+
+/* ------------------------------------------------------------------------
  * RMSNorm (forward + backward, deterministic weight gradient)
  * ------------------------------------------------------------------------ */
 

@@ -166,6 +166,23 @@ forge_lora_a_noalloc = _decl(
 )
 LORA_A_SCRATCH_BYTES = 16 * 1024 * 1024
 
+REDUCE_NONE, REDUCE_MEAN, REDUCE_SUM, REDUCE_SEQUENCE = 0, 1, 2, 3
+PREF_SIGMOID, PREF_HINGE, PREF_IPO = 0, 1, 2
+c_f64 = ctypes.c_double
+_LP_ROWS = [c_int, c_vp] + [c_i64] * 5 + [c_vp] + [c_i64] * 3  # logits [N, S, V] and targets
+forge_logp_workspace = _decl("forge_logp_workspace", [c_int, c_i64, c_i64, c_i64], c_i64)
+forge_token_logps_fwd = _decl("forge_token_logps_fwd", _LP_ROWS + [c_f64] + [c_vp] * 4)
+forge_token_logps_bwd = _decl(
+    "forge_token_logps_bwd",
+    _LP_ROWS + [c_f64, c_vp, c_vp, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp]
+)
+forge_preference_fwd = _decl(
+    "forge_preference_fwd", _LP_ROWS + [c_vp, c_f64, c_f64, c_int, c_int, c_int] + [c_vp] * 8
+)
+forge_policy_loss = _decl(
+    "forge_policy_loss",
+    _LP_ROWS + [c_f64] + [c_vp, c_i64, c_i64] * 3 + [c_f64] * 3 + [c_int] + [c_vp] * 4 + [c_i64] * 2 + [c_vp] * 2
+)
 forge_ce_target_prob = _decl(
     "forge_ce_target_prob", [c_int, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_f32, c_vp, c_vp]
 )
@@ -213,6 +230,8 @@ EXPORTED = [
     "forge_version", "forge_last_error", "forge_arch_ok",
     "forge_swiglu_fwd", "forge_swiglu_bwd", "forge_geglu_fwd", "forge_geglu_bwd", "forge_rope",
     "forge_qk_norm_rope_fwd", "forge_qk_norm_rope_bwd", "forge_qk_norm_rope_bwd_workspace",
+    "forge_logp_workspace", "forge_token_logps_fwd", "forge_token_logps_bwd", "forge_preference_fwd",
+    "forge_policy_loss",
     "forge_glu_act8_bytes", "forge_glu_act8_fwd", "forge_glu_act8_bwd",
     "forge_ce_fwd", "forge_ce_target_stats", "forge_ce_fwd_reduce", "forge_ce_stats_wait", "forge_ce_scale",
     "forge_sum_f32",
