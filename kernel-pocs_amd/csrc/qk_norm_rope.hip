@@ -12,7 +12,18 @@
 // Bound by HBM: forward 2 and backward 3 passes over q and k.  A head is
 // shared by L lanes (a power of two): lane c owns 16 bytes at c of the lower
 // half and the 16 bytes they rotate with in the upper half, so nothing leaves
-// the lane but the sum of squares (and the mean of g n).
+// the lane but the sum of squares (and the mean of g n).  A lane takes two
+// heads of a token together, which share the token's place, its row of the
+// table and the loads in flight.  Measured on MI355X, bf16 [4, 4096], 32 + 8
+// heads of 128, nothing cached: forward 63 us (5.3 TB/s; a copy 5.8), backward
+// 92 us without and 104 us with the weights' gradients (5.5 and 4.8 TB/s).
+//
+// Weight gradients: a workgroup adds up its heads in registers and writes one
+// row of partial sums, so there are few of them, each with the same share of
+// the heads: 768 (3 per CU, what the registers of two heads allow) 104 us; 1024
+// with one head a lane 106; 2048 114, 4096 119 (more rows to add up, and a last
+// round that is not full).  The adds within a wave go by DPP: by ds_bpermute the
+// backward took 119 us.
 #include "common.h"
 
 namespace {
@@ -20,7 +31,8 @@ namespace {
 constexpr int kBlock = 256;
 constexpr int kMaxHalf = 512;      // head_dim up to 1024
 constexpr int kMaxBlocks = 16384;  // 64 workgroups per CU
-constexpr int kDwBlocks = 2048;    // workgroups (each one row of partial sums) where weights take gradients
+constexpr int kDwBlocks = 768;     // with weight gradients: 3 workgroups per CU, each one row of partial sums
+constexpr int kHeads = 2;          // heads of a token that a lane takes together
 
 // (batch, head, seq) element strides of a [B, heads, S, D] tensor
 struct View {
@@ -33,7 +45,7 @@ struct Side {  // q or k
   void* out; View ov;        // forward: the output; backward: dx
   const void* w;
   float* part;               // backward: [blocks][D] partial sums of dweight, or nullptr
-  uint32_t rows, heads;      // rows = B * S * heads
+  uint32_t tokens, heads;    // tokens = B * S
   uint32_t blocks;
 };
 
@@ -49,15 +61,20 @@ struct Args {
   int w_dtype;
 };
 
-__device__ __forceinline__ float load_w(const void* w, int dtype, int i) {
-  if (dtype == FORGE_DTYPE_BF16) return (float)((const bf16_t*)w)[i];
-  if (dtype == FORGE_DTYPE_F16) return (float)((const fp16_t*)w)[i];
-  return ((const float*)w)[i];
+// Sum over the L lanes that share a head, by DPP within 16 lanes: neighbours,
+// pairs of a quad, then mirrored halves, whose lanes already agree.
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
 }
 
-// Sum over the L lanes that share a head.
 __device__ __forceinline__ float head_sum(float v, int lanes) {
-  for (int off = lanes >> 1; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+  if (lanes >= 2) v = add_dpp<0xb1>(v);    // quad_perm [1, 0, 3, 2]
+  if (lanes >= 4) v = add_dpp<0x4e>(v);    // quad_perm [2, 3, 0, 1]
+  if (lanes >= 8) v = add_dpp<0x141>(v);   // row_half_mirror
+  if (lanes >= 16) v = add_dpp<0x140>(v);  // row_mirror
+  if (lanes >= 32) v += __shfl_xor(v, 16, 64);
+  if (lanes >= 64) v += __shfl_xor(v, 32, 64);
   return v;
 }
 
@@ -70,16 +87,47 @@ struct Lane {
   int c, lanes, half;
   __device__ __forceinline__ int col(int j) const { return VEC ? c * E + j : c + j * lanes; }
   __device__ __forceinline__ bool on(int j) const { return col(j) < half; }
-  template <bool NT>
-  __device__ __forceinline__ void load(const T* p, float (&v)[E]) const {
+
+  // The values as they are in memory (cos and sin may be of another type TC).
+  template <class S, bool NT>
+  struct Raw {
+    static constexpr int PER = 16 / (int)sizeof(S);
+    Vec16<S> v[VEC ? E / PER : 1];
+    S e[VEC ? 1 : E];
+  };
+  template <class S, bool NT>
+  __device__ __forceinline__ void load(const S* p, Raw<S, NT>& r) const {
     if constexpr (VEC) {
-      Vec16<T> t = NT ? load16_nt(p + c * E) : load16(p + c * E);
 #pragma unroll
-      for (int j = 0; j < E; ++j) v[j] = to_f32(t.v[j]);
+      for (int k = 0; k < E / Raw<S, NT>::PER; ++k) {
+        const S* q = p + c * E + k * Raw<S, NT>::PER;
+        r.v[k] = NT ? load16_nt(q) : load16(q);
+      }
     } else {
 #pragma unroll
-      for (int j = 0; j < E; ++j) v[j] = on(j) ? to_f32(p[col(j)]) : 0.f;
+      for (int j = 0; j < E; ++j) r.e[j] = on(j) ? p[col(j)] : from_f32<S>(0.f);
     }
+  }
+  template <class S, bool NT>
+  __device__ __forceinline__ void values(const Raw<S, NT>& r, float (&v)[E]) const {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      if constexpr (VEC) v[j] = to_f32(r.v[j / Raw<S, NT>::PER].v[j % Raw<S, NT>::PER]);
+      else v[j] = to_f32(r.e[j]);
+    }
+  }
+  template <class S>
+  __device__ __forceinline__ void plus(const S* p, float offset, float (&v)[E]) const {
+    Raw<S, false> r;
+    load(p, r);
+    values(r, v);
+#pragma unroll
+    for (int j = 0; j < E; ++j) v[j] += offset;
+  }
+  __device__ __forceinline__ void weight(const void* w, int dtype, int first, float offset, float (&v)[E]) const {
+    if (dtype == FORGE_DTYPE_BF16) plus((const bf16_t*)w + first, offset, v);
+    else if (dtype == FORGE_DTYPE_F16) plus((const fp16_t*)w + first, offset, v);
+    else plus((const float*)w + first, offset, v);
   }
   __device__ __forceinline__ void store(T* p, const float (&v)[E]) const {
     if constexpr (VEC) {
@@ -93,125 +141,125 @@ struct Lane {
         if (on(j)) p[col(j)] = from_f32<T>(v[j]);
     }
   }
-  // cos or sin values of type TC at the same columns
-  template <class TC>
-  __device__ __forceinline__ void table(const TC* p, float (&v)[E]) const {
-    if constexpr (VEC) {
-      constexpr int PER = 16 / (int)sizeof(TC);
-#pragma unroll
-      for (int k = 0; k < E / PER; ++k) {
-        Vec16<TC> t = load16(p + c * E + k * PER);
-#pragma unroll
-        for (int j = 0; j < PER; ++j) v[k * PER + j] = to_f32(t.v[j]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < E; ++j) v[j] = on(j) ? to_f32(p[col(j)]) : 0.f;
-    }
-  }
 };
 
-template <class T, class TC, bool VEC, bool BWD>
+template <class T, class TC, bool VEC, bool BWD, bool DW>
 __global__ __launch_bounds__(kBlock) void qk_norm_rope_kernel(Args a) {
   using LaneT = Lane<T, VEC>;
+  using X = typename LaneT::template Raw<T, true>;
+  using C = typename LaneT::template Raw<TC, false>;
   constexpr int E = LaneT::E;
-  extern __shared__ float lds[];  // backward with weight gradients: [waves][D]
+  constexpr int HEADS = VEC ? kHeads : 1;
+  extern __shared__ float lds[];  // DW: [waves][D]
   const bool is_k = blockIdx.x >= a.q.blocks;
   const Side& s = is_k ? a.k : a.q;
   const uint32_t block = is_k ? blockIdx.x - a.q.blocks : blockIdx.x;
   const int lanes = a.lanes, half = a.half;
   const LaneT lane{(int)threadIdx.x & (lanes - 1), lanes, half};
   const bool active = VEC ? lane.c * E < half : lane.c < half;
-  const uint32_t per_block = kBlock / lanes;
+  const uint32_t per_block = kBlock / lanes, step = s.blocks * per_block;
+  const uint32_t groups = (s.heads + HEADS - 1) / HEADS, items = s.tokens * groups;
 
-  float wl[E], wh[E], al[E], ah[E];  // weight of the lower and upper half, and their gradients' sums
-#pragma unroll
-  for (int j = 0; j < E; ++j) {
-    wl[j] = active && lane.on(j) ? load_w(s.w, a.w_dtype, lane.col(j)) + a.offset : 0.f;
-    wh[j] = active && lane.on(j) ? load_w(s.w, a.w_dtype, half + lane.col(j)) + a.offset : 0.f;
-    al[j] = ah[j] = 0.f;
+  float wl[E] = {}, wh[E] = {}, al[E], ah[E];  // weight of the lower and upper half, and their gradients' sums
+  if (active) {
+    lane.weight(s.w, a.w_dtype, 0, a.offset, wl);
+    lane.weight(s.w, a.w_dtype, half, a.offset, wh);
   }
+#pragma unroll
+  for (int j = 0; j < E; ++j) al[j] = ah[j] = 0.f;
 
-  for (uint32_t row = block * per_block + threadIdx.x / lanes; row < s.rows; row += s.blocks * per_block) {
-    const uint32_t t = row / s.heads, h = row - t * s.heads;
+  for (uint32_t item = block * per_block + threadIdx.x / lanes; item < items; item += step) {
+    const uint32_t t = item / groups, h0 = (item - t * groups) * HEADS;
     const uint32_t b = t / a.seq_len, sq = t - b * a.seq_len;
+    X rl[HEADS] = {}, rh[HEADS] = {}, dl[HEADS] = {}, dh[HEADS] = {};
+    C rc = {}, rs = {};
+    const T* x = (const T*)s.x + ((int64_t)b * s.xv.sb + (int64_t)h0 * s.xv.sh + (int64_t)sq * s.xv.ss);
+#pragma unroll
+    for (int u = 0; u < HEADS; ++u)
+      if (active && h0 + u < s.heads) {
+        lane.load(x + u * s.xv.sh, rl[u]);
+        lane.load(x + u * s.xv.sh + half, rh[u]);
+      }
+    if constexpr (BWD) {
+      const T* dy = (const T*)s.dy + ((int64_t)b * s.dv.sb + (int64_t)h0 * s.dv.sh + (int64_t)sq * s.dv.ss);
+#pragma unroll
+      for (int u = 0; u < HEADS; ++u)
+        if (active && h0 + u < s.heads) {
+          lane.load(dy + u * s.dv.sh, dl[u]);
+          lane.load(dy + u * s.dv.sh + half, dh[u]);
+        }
+    }
     const int64_t pos = a.positions ? a.positions[t] : (int64_t)sq;
     const bool in_table = pos >= 0 && pos < a.table_rows;
-    float xl[E] = {}, xh[E] = {}, cs[E] = {}, sn[E] = {}, gl[E] = {}, gh[E] = {};
-    if (active) {
-      const T* x = (const T*)s.x + ((int64_t)b * s.xv.sb + (int64_t)h * s.xv.sh + (int64_t)sq * s.xv.ss);
-      lane.template load<true>(x, xl);
-      lane.template load<true>(x + half, xh);
-      if constexpr (BWD) {
-        const T* dy = (const T*)s.dy + ((int64_t)b * s.dv.sb + (int64_t)h * s.dv.sh + (int64_t)sq * s.dv.ss);
-        lane.template load<true>(dy, gl);
-        lane.template load<true>(dy + half, gh);
-      }
-      if (in_table) {
-        lane.table((const TC*)a.cos + ((int64_t)b * a.cos_sb + pos * a.cos_ss), cs);
-        lane.table((const TC*)a.sin + ((int64_t)b * a.sin_sb + pos * a.sin_ss), sn);
-      } else {
-        // a position outside the table: nothing is read, the token's outputs are NaN
-#pragma unroll
-        for (int j = 0; j < E; ++j) cs[j] = sn[j] = __builtin_nanf("");
-      }
+    if (active && in_table) {
+      lane.load((const TC*)a.cos + ((int64_t)b * a.cos_sb + pos * a.cos_ss), rc);
+      lane.load((const TC*)a.sin + ((int64_t)b * a.sin_sb + pos * a.sin_ss), rs);
     }
-    float ss = 0.f;
+    float cs[E], sn[E];
+    lane.values(rc, cs);
+    lane.values(rs, sn);
+    T* o = (T*)s.out + ((int64_t)b * s.ov.sb + (int64_t)h0 * s.ov.sh + (int64_t)sq * s.ov.ss);
 #pragma unroll
-    for (int j = 0; j < E; ++j) ss += xl[j] * xl[j] + xh[j] * xh[j];
-    const float r = rsqrtf(head_sum(ss, lanes) * a.inv_d + a.eps);
-    if constexpr (!BWD) {
-      float ol[E], oh[E];
+    for (int u = 0; u < HEADS; ++u) {
+      float xl[E], xh[E];
+      lane.values(rl[u], xl);
+      lane.values(rh[u], xh);
+      float ss = 0.f;
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const float yl = xl[j] * r * wl[j], yh = xh[j] * r * wh[j];
-        ol[j] = yl * cs[j] - yh * sn[j];
-        oh[j] = yh * cs[j] + yl * sn[j];
-      }
-      if (active) {
-        T* o = (T*)s.out + ((int64_t)b * s.ov.sb + (int64_t)h * s.ov.sh + (int64_t)sq * s.ov.ss);
-        lane.store(o, ol);
-        lane.store(o + half, oh);
-      }
-    } else {
-      float dot = 0.f;
+      for (int j = 0; j < E; ++j) ss += xl[j] * xl[j] + xh[j] * xh[j];
+      float r = rsqrtf(head_sum(ss, lanes) * a.inv_d + a.eps);
+      if (!in_table) r = __builtin_nanf("");  // nothing of the table was read: the token's outputs are NaN
+      if constexpr (!BWD) {
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const float dl = gl[j] * cs[j] + gh[j] * sn[j], dh = gh[j] * cs[j] - gl[j] * sn[j];
-        xl[j] *= r;  // n
-        xh[j] *= r;
-        al[j] += dl * xl[j];
-        ah[j] += dh * xh[j];
-        gl[j] = dl * wl[j];
-        gh[j] = dh * wh[j];
-        dot += gl[j] * xl[j] + gh[j] * xh[j];
-      }
-      const float mean = head_sum(dot, lanes) * a.inv_d;
+        for (int j = 0; j < E; ++j) {
+          const float yl = xl[j] * r * wl[j], yh = xh[j] * r * wh[j];
+          xl[j] = yl * cs[j] - yh * sn[j];
+          xh[j] = yh * cs[j] + yl * sn[j];
+        }
+      } else {
+        float gl[E], gh[E];
+        lane.values(dl[u], gl);
+        lane.values(dh[u], gh);
+        float dot = 0.f;
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        gl[j] = r * (gl[j] - xl[j] * mean);
-        gh[j] = r * (gh[j] - xh[j] * mean);
+        for (int j = 0; j < E; ++j) {
+          // r dy; then r g = r dy w, and with sum g n = sum (r g) x
+          const float yl = (gl[j] * cs[j] + gh[j] * sn[j]) * r, yh = (gh[j] * cs[j] - gl[j] * sn[j]) * r;
+          if constexpr (DW) {  // (a head past the last one has x = dy = 0)
+            al[j] += yl * xl[j];
+            ah[j] += yh * xh[j];
+          }
+          gl[j] = yl * wl[j];
+          gh[j] = yh * wh[j];
+          dot += gl[j] * xl[j] + gh[j] * xh[j];
+        }
+        // dx = r g - n r mean(g n)
+        const float m = head_sum(dot, lanes) * a.inv_d * r * r;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          xl[j] = gl[j] - xl[j] * m;
+          xh[j] = gh[j] - xh[j] * m;
+        }
       }
-      if (active) {
-        T* o = (T*)s.out + ((int64_t)b * s.ov.sb + (int64_t)h * s.ov.sh + (int64_t)sq * s.ov.ss);
-        lane.store(o, gl);
-        lane.store(o + half, gh);
+      if (active && h0 + u < s.heads) {
+        lane.store(o + u * s.ov.sh, xl);
+        lane.store(o + u * s.ov.sh + half, xh);
       }
     }
   }
 
-  if constexpr (BWD) {
+  if constexpr (DW) {
     if (!s.part) return;  // (uniform over the workgroup)
     // this workgroup's row of partial sums, in a fixed order: the groups of a
     // wave by shuffles, then the waves
-    const int wave = threadIdx.x >> 6, wl_ = threadIdx.x & 63;
+    const int wave = threadIdx.x >> 6;
 #pragma unroll
     for (int j = 0; j < E; ++j)
       for (int off = lanes; off < 64; off <<= 1) {
         al[j] += __shfl_xor(al[j], off, 64);
         ah[j] += __shfl_xor(ah[j], off, 64);
       }
-    if (wl_ < lanes && active) {
+    if ((int)(threadIdx.x & 63) < lanes && active) {
 #pragma unroll
       for (int j = 0; j < E; ++j)
         if (lane.on(j)) {
@@ -264,24 +312,28 @@ int lanes_for(int64_t half, bool vec, size_t es) {
   return lanes;
 }
 
-uint32_t blocks_for(uint32_t rows, int lanes, uint32_t most) {
-  const uint32_t per = kBlock / lanes;
-  const uint32_t b = (rows + per - 1) / per;
-  return b > most ? most : b;
-}
-
-// Workgroups of q and k: all they can use up to the cap, shared by their rows.
-void split_blocks(uint32_t q_rows, uint32_t k_rows, int lanes, bool dw, uint32_t& qb, uint32_t& kb) {
-  const uint64_t cap = dw ? kDwBlocks : kMaxBlocks, all = (uint64_t)q_rows + k_rows;
-  const uint32_t q_cap = (uint32_t)((cap * q_rows + all - 1) / all), k_cap = (uint32_t)((cap * k_rows + all - 1) / all);
-  qb = blocks_for(q_rows, lanes, q_cap);
-  kb = blocks_for(k_rows, lanes, k_cap);
+// Workgroups of q and k: all they can use up to the cap, shared by their heads
+// (at least one each: the cap is far above two).
+void split_blocks(Args& a, int heads_each, uint64_t cap) {
+  const uint64_t all = (uint64_t)a.q.heads + a.k.heads, per = kBlock / a.lanes;
+  for (Side* s : {&a.q, &a.k}) {
+    const uint64_t items = (uint64_t)s->tokens * ((s->heads + heads_each - 1) / heads_each);
+    uint64_t most = all ? cap * s->heads / all : 0;
+    if (most == 0) most = 1;
+    const uint64_t b = (items + per - 1) / per;
+    s->blocks = (uint32_t)(b > most ? most : b);
+  }
 }
 
 template <class T, class TC, bool BWD>
 void launch(const Args& a, bool vec, uint32_t blocks, size_t lds, hipStream_t s) {
-  if (vec) qk_norm_rope_kernel<T, TC, true, BWD><<<blocks, kBlock, lds, s>>>(a);
-  else qk_norm_rope_kernel<T, TC, false, BWD><<<blocks, kBlock, lds, s>>>(a);
+  if (BWD && lds) {
+    if (vec) qk_norm_rope_kernel<T, TC, true, BWD, BWD><<<blocks, kBlock, lds, s>>>(a);
+    else qk_norm_rope_kernel<T, TC, false, BWD, BWD><<<blocks, kBlock, lds, s>>>(a);
+  } else {
+    if (vec) qk_norm_rope_kernel<T, TC, true, BWD, false><<<blocks, kBlock, 0, s>>>(a);
+    else qk_norm_rope_kernel<T, TC, false, BWD, false><<<blocks, kBlock, 0, s>>>(a);
+  }
 }
 
 template <bool BWD>
@@ -311,7 +363,8 @@ int run(int dtype, const char* what, Args& a, int w_dtype, int table_dtype, int6
   const size_t es = dtype_size(dtype), ets = dtype_size(table_dtype);
   const int64_t V = (int64_t)(16 / es), Vt = (int64_t)(16 / ets);
   a.half = (int)(head_dim / 2);
-  bool vec = a.half % V == 0 && a.half / V <= 64 && aligned16(a.cos) && aligned16(a.sin);
+  bool vec = a.half % V == 0 && a.half / V <= 64 && aligned16(a.cos) && aligned16(a.sin) && aligned16(a.q.w) &&
+             aligned16(a.k.w);
   for (const Side* s : {&a.q, &a.k}) {
     vec = vec && aligned16(s->x) && aligned16(s->out) && (!BWD || aligned16(s->dy));
     for (int64_t st : {s->xv.sb, s->xv.sh, s->xv.ss, s->ov.sb, s->ov.sh, s->ov.ss}) vec = vec && st % V == 0;
@@ -327,12 +380,10 @@ int run(int dtype, const char* what, Args& a, int w_dtype, int table_dtype, int6
   a.w_dtype = w_dtype;
   a.q.heads = (uint32_t)n_q;
   a.k.heads = (uint32_t)n_kv;
-  a.q.rows = (uint32_t)(batch * seq_len * n_q);
-  a.k.rows = (uint32_t)(batch * seq_len * n_kv);
+  a.q.tokens = a.k.tokens = (uint32_t)(batch * seq_len);
   hipStream_t s = (hipStream_t)stream;
   const bool dw = dqw || dkw;
-  a.q.blocks = a.k.blocks = 0;
-  if (a.q.rows + a.k.rows) split_blocks(a.q.rows, a.k.rows, a.lanes, dw, a.q.blocks, a.k.blocks);
+  split_blocks(a, vec ? kHeads : 1, dw ? kDwBlocks : kMaxBlocks);
   if (dw) {  // both sides' partial sums, one after the other
     a.q.part = dqw ? work : nullptr;
     a.k.part = dkw ? work + (int64_t)a.q.blocks * head_dim : nullptr;
