@@ -108,8 +108,8 @@ int64_t forge_glu_act8_bytes(int64_t rows, int64_t cols);
  * fp16.  With kept != NULL (16-byte aligned, forge_glu_act8_bytes) gate and up
  * are also written there in 8 bits: groups of 32 values of a row share the
  * least power of two 2^e, e >= -126, with |x| <= 127 * 2^e, and a value is the
- * integer round(x / 2^e); an infinity or NaN is kept as NaN.  Fewer than 2^34
- * values in a call. */
+ * integer round(x / 2^e); an infinity or NaN is kept as NaN.  Up to 2^30
+ * vectors of 16 bytes (2^33 16-bit values) in a call. */
 int forge_glu_act8_fwd(int dtype, int activation, const void* gate, int64_t ld_gate,
                        const void* up, int64_t ld_up, void* out, int64_t ld_out,
                        void* kept, int64_t rows, int64_t cols, void* stream);

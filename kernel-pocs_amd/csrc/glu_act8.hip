@@ -16,10 +16,18 @@
 // with pitch = cols rounded up to 32, then [rows][pitch / 32] pairs of bytes
 // e + 127 (gate's, up's).
 //
-// Bound by HBM.  A thread owns 16 consecutive columns: 32 bytes of each 16-bit
-// operand and one 16-byte vector of each q; two neighbouring lanes share a
-// group.  Every operand is touched once (nontemporal).  Rows need no
-// alignment: global memory takes 16-byte accesses at any element's address.
+// Bound by HBM.  A thread owns one 16-byte vector of each operand (8 columns, 4
+// of fp32), so that a wave's accesses are whole lines, and 8 (4) bytes of each
+// q; 4 (8) neighbouring lanes share a group.  Every operand is touched once
+// (nontemporal).  Rows need no alignment: global memory takes 16-byte accesses
+// at any element's address.  Measured on MI355X, nothing cached, forward /
+// backward: bf16 [8192, 14336] silu 161 / 157 us (5.9 / 6.0 TB/s; a copy 5.8),
+// tanh 167 / 165; fp16 [4096, 14337] erf 85 / 89; fp32 [4096, 11008] silu 99 /
+// 99.  With 16 columns a thread the 16-bit backward took 235 us (two stores 32
+// bytes apart in place of whole lines); one vector in flight 166 / 158, four
+// 165 / 159; two in fp32 103 / 107.  The forward's arithmetic (two activations'
+// worth) is close behind the memory: testing every value for infinities took
+// it to 176 us, so a wave tests its largest and looks closer only then.
 #include "gelu.h"
 
 #include "common.h"
@@ -27,48 +35,43 @@
 namespace {
 
 constexpr int kBlock = 256;
-constexpr int kOwn = 16;    // columns of a thread
 constexpr int kGroup = 32;  // columns that share a scale
 
 // 16 bytes at an address that is a multiple of the element only
 typedef unsigned int u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
 template <class T>
-__device__ __forceinline__ void load_own(const T* p, int n, float (&v)[kOwn]) {
-  constexpr int PER = 16 / (int)sizeof(T);
-  if (n >= kOwn) {
-    Vec16<T> t[kOwn / PER];
-#pragma unroll
-    for (int k = 0; k < kOwn / PER; ++k) {
-      const u32x4_any w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p + k * PER));
-      t[k].raw = make_uint4(w.x, w.y, w.z, w.w);
-    }
-#pragma unroll
-    for (int j = 0; j < kOwn; ++j) v[j] = to_f32(t[j / PER].v[j % PER]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < kOwn; ++j) v[j] = j < n ? to_f32(p[j]) : 0.f;
-  }
-}
+struct Own {
+  static constexpr int N = 16 / (int)sizeof(T);  // columns of a thread
+  static constexpr int LANES = kGroup / N;       // threads of a group
+  static constexpr int VECTORS = sizeof(T) == 4 ? 1 : 2;  // in flight for each operand
 
-template <class T>
-__device__ __forceinline__ void store_own(T* p, int n, const float (&v)[kOwn]) {
-  constexpr int PER = 16 / (int)sizeof(T);
-  if (n >= kOwn) {
+  static __device__ __forceinline__ Vec16<T> load(const T* p, int n) {
+    Vec16<T> t;
+    if (n >= N) {
+      const u32x4_any w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p));
+      t.raw = make_uint4(w.x, w.y, w.z, w.w);
+    } else {
 #pragma unroll
-    for (int k = 0; k < kOwn / PER; ++k) {
-      Vec16<T> t;
-#pragma unroll
-      for (int j = 0; j < PER; ++j) t.v[j] = from_f32<T>(v[k * PER + j]);
-      const u32x4_any w = {t.raw.x, t.raw.y, t.raw.z, t.raw.w};
-      __builtin_nontemporal_store(w, reinterpret_cast<u32x4_any*>(p + k * PER));
+      for (int j = 0; j < N; ++j) t.v[j] = j < n ? p[j] : from_f32<T>(0.f);
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < kOwn; ++j)
-      if (j < n) p[j] = from_f32<T>(v[j]);
+    return t;
   }
-}
+
+  static __device__ __forceinline__ void store(T* p, int n, const float (&v)[N]) {
+    Vec16<T> t;
+#pragma unroll
+    for (int j = 0; j < N; ++j) t.v[j] = from_f32<T>(v[j]);
+    if (n >= N) {
+      const u32x4_any w = {t.raw.x, t.raw.y, t.raw.z, t.raw.w};
+      __builtin_nontemporal_store(w, reinterpret_cast<u32x4_any*>(p));
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (j < n) p[j] = t.v[j];
+    }
+  }
+};
 
 // act(x) and act'(x) in fp32.
 template <int ACT>
@@ -88,47 +91,105 @@ __device__ __forceinline__ void act_and_slope(float x, float& act, float& slope)
   }
 }
 
-// A thread's 16 values in 8 bits: q, and the group's e + 127.
-__device__ __forceinline__ uint4 keep(const float (&x)[kOwn], uint32_t& scale) {
-  float m = 0.f;
+template <int CTRL>
+__device__ __forceinline__ uint32_t max_dpp(uint32_t v) {
+  const uint32_t w = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+  return v > w ? v : w;
+}
+
+// The largest over the lanes of a group of N values a lane: neighbours
+// (quad_perm [1, 0, 3, 2]), pairs (quad_perm [2, 3, 0, 1]), and where 8 lanes
+// share one the other quad (row_half_mirror).
+template <int N>
+__device__ __forceinline__ uint32_t group_max(uint32_t m) {
+  m = max_dpp<0xb1>(m);
+  m = max_dpp<0x4e>(m);
+  if constexpr (N == 4) m = max_dpp<0x141>(m);
+  return m;
+}
+
+constexpr uint32_t kInf = 0x7f800000;
+
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_amdgcn_perm(b, a, 0x0c0c0400) | __builtin_amdgcn_perm(d, c, 0x04000c0c);
+}
+
+// A thread's values in 8 bits: q, and the group's e + 127.  Magnitudes are
+// compared as bits, whose order they share, so that one look at the largest
+// tells whether a wave has infinities or NaN to leave out.
+template <int N>
+__device__ __forceinline__ void keep(const float (&x)[N], uint32_t (&q)[N / 4], uint32_t& scale) {
+  uint32_t m = 0;
 #pragma unroll
-  for (int j = 0; j < kOwn; ++j) {
-    const float t = fabsf(x[j]);
-    m = fmaxf(m, t < INFINITY ? t : 0.f);  // infinities and NaN do not count
+  for (int j = 0; j < N; ++j) {
+    const uint32_t t = __float_as_uint(x[j]) & 0x7fffffff;
+    m = m > t ? m : t;
   }
-  m = fmaxf(m, __shfl_xor(m, 1, 64));  // the group's other lane
+  const bool special = __any(m >= kInf);
+  if (special) {
+    m = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const uint32_t t = __float_as_uint(x[j]) & 0x7fffffff;
+      m = t < kInf && t > m ? t : m;
+    }
+  }
+  m = group_max<N>(m);
   // m = f 2^(b - 127) with f in [1, 2): 127 * 2^e >= m from e = b - 133 on, or
   // one more where f > 127 / 64
-  const uint32_t bits = __float_as_uint(m);
-  int e = (int)(bits >> 23) - 133 + ((bits & 0x7fffff) > 0x7e0000 ? 1 : 0);
+  int e = (int)(m >> 23) - 133 + ((m & 0x7fffff) > 0x7e0000 ? 1 : 0);
   e = e < -126 ? -126 : e;
   scale = (uint32_t)(e + 127);
   const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-  uint32_t q[4];
+  uint32_t r[N];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    uint32_t w = 0;
+  for (int j = 0; j < N; ++j) r[j] = __float_as_uint(fmaf(x[j], inv, 12582912.f));  // rounded to even in the low bits of 1.5 * 2^23 + .
+  if (special) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float v = x[4 * k + j];
-      // v / 2^e + 1.5 * 2^23 rounds to an integer, to even, in the low bits
-      const uint32_t r = __float_as_uint(fmaf(v, inv, 12582912.f));
-      const uint32_t b = fabsf(v) < INFINITY ? r & 0xff : 0x80u;
-      w |= b << (8 * j);
-    }
-    q[k] = w;
+    for (int j = 0; j < N; ++j)
+      if ((__float_as_uint(x[j]) & 0x7fffffff) >= kInf) r[j] = 0x80;
   }
-  return make_uint4(q[0], q[1], q[2], q[3]);
+#pragma unroll
+  for (int k = 0; k < N / 4; ++k) q[k] = low_bytes(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
 }
 
-__device__ __forceinline__ void kept_values(const uint4& q, uint32_t scale, float (&v)[kOwn]) {
+template <int N>
+__device__ __forceinline__ void kept_values(const uint32_t (&q)[N / 4], uint32_t scale, float (&v)[N]) {
   const float s = __uint_as_float(scale << 23);
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  uint32_t hit = 0;  // a byte 0x80 leaves its top bit here (and may leave others')
 #pragma unroll
-  for (int j = 0; j < kOwn; ++j) {
-    const int b = (int8_t)(w[j / 4] >> (8 * (j % 4)));
-    v[j] = b == -128 ? __builtin_nanf("") : (float)b * s;
+  for (int k = 0; k < N / 4; ++k) {
+    const uint32_t t = q[k] ^ 0x80808080u;
+    hit |= (t - 0x01010101u) & ~t & 0x80808080u;
   }
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = (float)(int8_t)(q[j / 4] >> (8 * (j % 4))) * s;
+  if (__any(hit)) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (((q[j / 4] >> (8 * (j % 4))) & 0xff) == 0x80) v[j] = __builtin_nanf("");
+  }
+}
+
+// q of a thread's columns: N bytes.
+template <int N>
+__device__ __forceinline__ void load_q(const uint8_t* p, uint32_t (&q)[N / 4]) {
+  if constexpr (N == 8) {
+    const uint64_t w = __builtin_nontemporal_load(reinterpret_cast<const uint64_t*>(p));
+    q[0] = (uint32_t)w;
+    q[1] = (uint32_t)(w >> 32);
+  } else {
+    q[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
+  }
+}
+
+template <int N>
+__device__ __forceinline__ void store_q(uint8_t* p, const uint32_t (&q)[N / 4]) {
+  if constexpr (N == 8)
+    __builtin_nontemporal_store((uint64_t)q[0] | (uint64_t)q[1] << 32, reinterpret_cast<uint64_t*>(p));
+  else
+    __builtin_nontemporal_store(q[0], reinterpret_cast<uint32_t*>(p));
 }
 
 struct Args {
@@ -137,74 +198,108 @@ struct Args {
   void* out; int64_t ld_out;       // backward: the gradient of the output (read)
   void* dgate; void* dup; int64_t ld_grad;
   uint8_t* kept;
-  uint32_t n, per_row;             // threads' pieces: in all, and of a row (even)
-  uint32_t rows, cols;
+  uint32_t n, per_row;             // threads' vectors: in all, and of a row (whole groups)
+  uint32_t cols;
 };
 
+template <class T>
 __device__ __forceinline__ uint8_t* kept_q(const Args& a, uint32_t i, bool up) {
-  return a.kept + ((int64_t)(up ? a.n : 0) + i) * kOwn;
+  return a.kept + ((int64_t)(up ? a.n : 0) + i) * Own<T>::N;
 }
 
+template <class T>
 __device__ __forceinline__ uint16_t* kept_scales(const Args& a, uint32_t i) {
-  return reinterpret_cast<uint16_t*>(a.kept + (int64_t)2 * a.n * kOwn) + (i >> 1);
+  return reinterpret_cast<uint16_t*>(a.kept + (int64_t)2 * a.n * Own<T>::N) + i / Own<T>::LANES;
 }
 
 template <class T, int ACT, bool KEEP>
 __global__ __launch_bounds__(kBlock) void glu_act8_fwd_kernel(Args a) {
-  const uint32_t i = blockIdx.x * kBlock + threadIdx.x;
-  if (i >= a.n) return;  // (n is even: both lanes of a group)
-  const uint32_t r = i / a.per_row, c = (i - r * a.per_row) * kOwn;
-  const int left = (int)a.cols - (int)c;  // <= 0 in the second half of a last, short group
-  float g[kOwn], u[kOwn], o[kOwn];
-  load_own((const T*)a.gate + (int64_t)r * a.ld_gate + c, left, g);
-  load_own((const T*)a.up + (int64_t)r * a.ld_up + c, left, u);
+  using O = Own<T>;
+  constexpr int N = O::N, U = O::VECTORS;
+  const uint32_t i0 = blockIdx.x * (kBlock * U) + threadIdx.x;
+  Vec16<T> g[U], u[U];
+  uint32_t row[U];
+  int col[U];
 #pragma unroll
-  for (int j = 0; j < kOwn; ++j) {
-    float act, slope;
-    act_and_slope<ACT>(g[j], act, slope);
-    o[j] = act * u[j];
+  for (int k = 0; k < U; ++k) {
+    const uint32_t i = i0 + k * kBlock;
+    if (i >= a.n) continue;  // (n is whole groups)
+    row[k] = i / a.per_row;
+    col[k] = (int)(i - row[k] * a.per_row) * N;
+    const int left = (int)a.cols - col[k];  // <= 0 past the end of a last, short group
+    g[k] = O::load((const T*)a.gate + (int64_t)row[k] * a.ld_gate + col[k], left);
+    u[k] = O::load((const T*)a.up + (int64_t)row[k] * a.ld_up + col[k], left);
   }
-  store_own((T*)a.out + (int64_t)r * a.ld_out + c, left, o);
-  if constexpr (KEEP) {
-    uint32_t sg, su;
-    const uint4 qg = keep(g, sg), qu = keep(u, su);
-    Vec16<uint8_t> t;
-    t.raw = qg;
-    store16_nt(kept_q(a, i, false), t);
-    t.raw = qu;
-    store16_nt(kept_q(a, i, true), t);
-    if (!(i & 1)) *kept_scales(a, i) = (uint16_t)(sg | su << 8);
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const uint32_t i = i0 + k * kBlock;
+    if (i >= a.n) continue;
+    float x[N], y[N], o[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      x[j] = to_f32(g[k].v[j]);
+      y[j] = to_f32(u[k].v[j]);
+      float act, slope;
+      act_and_slope<ACT>(x[j], act, slope);
+      o[j] = act * y[j];
+    }
+    O::store((T*)a.out + (int64_t)row[k] * a.ld_out + col[k], (int)a.cols - col[k], o);
+    if constexpr (KEEP) {
+      uint32_t qx[N / 4], qy[N / 4], sx, sy;
+      keep(x, qx, sx);
+      keep(y, qy, sy);
+      store_q<N>(kept_q<T>(a, i, false), qx);
+      store_q<N>(kept_q<T>(a, i, true), qy);
+      if (i % O::LANES == 0) *kept_scales<T>(a, i) = (uint16_t)(sx | sy << 8);
+    }
   }
 }
 
 template <class T, int ACT>
 __global__ __launch_bounds__(kBlock) void glu_act8_bwd_kernel(Args a) {
-  const uint32_t i = blockIdx.x * kBlock + threadIdx.x;
-  if (i >= a.n) return;
-  const uint32_t r = i / a.per_row, c = (i - r * a.per_row) * kOwn;
-  const int left = (int)a.cols - (int)c;
-  const Vec16<uint8_t> qg = load16_nt(kept_q(a, i, false)), qu = load16_nt(kept_q(a, i, true));
-  const uint32_t scales = *kept_scales(a, i);
-  float d[kOwn], g[kOwn], u[kOwn];
-  load_own((const T*)a.out + (int64_t)r * a.ld_out + c, left, d);
-  kept_values(qg.raw, scales & 0xff, g);
-  kept_values(qu.raw, scales >> 8, u);
+  using O = Own<T>;
+  constexpr int N = O::N, U = O::VECTORS;
+  const uint32_t i0 = blockIdx.x * (kBlock * U) + threadIdx.x;
+  Vec16<T> d[U];
+  uint32_t qg[U][N / 4], qu[U][N / 4], scales[U], row[U];
+  int col[U];
 #pragma unroll
-  for (int j = 0; j < kOwn; ++j) {
-    float act, slope;
-    act_and_slope<ACT>(g[j], act, slope);
-    g[j] = d[j] * u[j] * slope;
-    u[j] = d[j] * act;
+  for (int k = 0; k < U; ++k) {
+    const uint32_t i = i0 + k * kBlock;
+    if (i >= a.n) continue;
+    row[k] = i / a.per_row;
+    col[k] = (int)(i - row[k] * a.per_row) * N;
+    d[k] = O::load((const T*)a.out + (int64_t)row[k] * a.ld_out + col[k], (int)a.cols - col[k]);
+    load_q<N>(kept_q<T>(a, i, false), qg[k]);
+    load_q<N>(kept_q<T>(a, i, true), qu[k]);
+    scales[k] = *kept_scales<T>(a, i);
   }
-  store_own((T*)a.dgate + (int64_t)r * a.ld_grad + c, left, g);
-  store_own((T*)a.dup + (int64_t)r * a.ld_grad + c, left, u);
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const uint32_t i = i0 + k * kBlock;
+    if (i >= a.n) continue;
+    const int left = (int)a.cols - col[k];
+    float g[N], u[N];
+    kept_values(qg[k], scales[k] & 0xff, g);
+    kept_values(qu[k], scales[k] >> 8, u);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float dout = to_f32(d[k].v[j]);
+      float act, slope;
+      act_and_slope<ACT>(g[j], act, slope);
+      g[j] = dout * u[j] * slope;
+      u[j] = dout * act;
+    }
+    O::store((T*)a.dgate + (int64_t)row[k] * a.ld_grad + col[k], left, g);
+    O::store((T*)a.dup + (int64_t)row[k] * a.ld_grad + col[k], left, u);
+  }
 }
 
-int64_t pieces(int64_t cols) { return (cols + kGroup - 1) / kGroup * (kGroup / kOwn); }
+int64_t groups_of(int64_t cols) { return (cols + kGroup - 1) / kGroup; }
 
 template <class T, int ACT>
 int launch(const Args& a, bool bwd, hipStream_t s) {
-  const unsigned grid = (a.n + kBlock - 1) / kBlock;
+  const unsigned per = kBlock * Own<T>::VECTORS, grid = (a.n + per - 1) / per;
   if (bwd) glu_act8_bwd_kernel<T, ACT><<<grid, kBlock, 0, s>>>(a);
   else if (a.kept) glu_act8_fwd_kernel<T, ACT, true><<<grid, kBlock, 0, s>>>(a);
   else glu_act8_fwd_kernel<T, ACT, false><<<grid, kBlock, 0, s>>>(a);
@@ -226,13 +321,13 @@ int prepare(const char* what, int dtype, int act, int64_t rows, int64_t cols, Ar
     return forge_set_error(FORGE_ERR_INVALID, "%s: activation %d", what, act);
   if (dtype != FORGE_DTYPE_F32 && dtype != FORGE_DTYPE_BF16 && dtype != FORGE_DTYPE_F16)
     return forge_set_error(FORGE_ERR_UNSUPPORTED, "%s: dtype %d", what, dtype);
-  const int64_t lim = 0x40000000;  // pieces of a call, and the threads of its grid, stay below 2^31
-  if (rows > lim || cols > lim || rows * pieces(cols) > lim)
-    return forge_set_error(FORGE_ERR_UNSUPPORTED, "%s: more than 2^34 values in a call", what);
-  a.rows = (uint32_t)rows;
+  const int64_t lim = 0x40000000;  // vectors of a call, and the threads of its grid, stay below 2^31
+  const int64_t per_row = groups_of(cols) * kGroup * (int64_t)dtype_size(dtype) / 16;
+  if (rows > lim || cols > lim || rows * per_row > lim)
+    return forge_set_error(FORGE_ERR_UNSUPPORTED, "%s: more than 2^30 vectors of 16 bytes in a call", what);
   a.cols = (uint32_t)cols;
-  a.per_row = (uint32_t)pieces(cols);
-  a.n = a.rows * a.per_row;
+  a.per_row = (uint32_t)per_row;
+  a.n = (uint32_t)(rows * per_row);
   return FORGE_OK;
 }
 
@@ -249,8 +344,8 @@ bool element_aligned(const void* p, int dtype) { return reinterpret_cast<uintptr
 
 extern "C" int64_t forge_glu_act8_bytes(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  const int64_t n = rows * pieces(cols);
-  return 2 * n * kOwn + n / 2 * 2;
+  const int64_t n = rows * groups_of(cols);
+  return n * (2 * kGroup + 2);
 }
 
 extern "C" int forge_glu_act8_fwd(int dtype, int activation, const void* gate, int64_t ld_gate, const void* up,
