@@ -456,6 +456,16 @@ struct Grad {
 
 constexpr int kGradVec = 4;  // vectors of a thread
 
+// *sum = the rows' losses in a fixed order, by one workgroup.
+template <int NT>
+__device__ void sum_rows(const double* rows, int64_t n, float* sum, double* red) {
+  double t = 0.0;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < n; i += NT) t += rows[i];
+  t = block_total<double, NT>(t, red);
+  if (threadIdx.x == 0) *sum = (float)t;
+}
+
 template <class T>
 __global__ __launch_bounds__(kBlock) void lp_grad_kernel(Rows a, Grad g, int64_t chunks) {
   constexpr int VEC = 16 / sizeof(T);
@@ -464,11 +474,7 @@ __global__ __launch_bounds__(kBlock) void lp_grad_kernel(Rows a, Grad g, int64_t
   if (g.sum) {
     if (blockIdx.x == 0) {
       __shared__ double red[kBlock / 64];
-      double t = 0.0;
-#pragma unroll 8
-      for (int64_t i = tid; i < a.n * a.s; i += kBlock) t += g.rows64[i];
-      t = block_total<double, kBlock>(t, red);
-      if (tid == 0) *g.sum = (float)t;
+      sum_rows<kBlock>(g.rows64, a.n * a.s, g.sum, red);
       return;
     }
     first -= 1;
@@ -525,6 +531,195 @@ __global__ __launch_bounds__(kBlock) void lp_grad_kernel(Rows a, Grad g, int64_t
       o[at] = from_f32<T>(at == y ? at_y : v);
     }
   }
+}
+
+// ---------------------------------------------------------------------------
+// policy loss with a row held on chip
+//
+// One 512-thread workgroup a row of 16-bit logits, which is read once and
+// written once: thread t owns the 16-byte vectors t + 512 i, the first NL in LDS
+// (filled by loads that go there by themselves), the others in registers (8 + 24
+// vectors: 131072 columns, two workgroups on a CU; one computes while the other
+// loads or stores).
+//   A  the largest value, as packed 16-bit integers (bits of non-negative values
+//      are in their order; a row of negative ones takes a second look)
+//   B  d = sum of 2^(x k - m k)
+//   C  one thread, in 64 bits: the token's loss and coefficient
+//   D  the gradient, each exponential again (kept in 16 bits it would be rounded
+//      twice)
+// One fma gives x k - m k: what rounding m k leaves is the same factor on every
+// exponential and on d, and the log-probability takes it into account.  Where m k
+// passes 2^29 (a row of a mask's lowest values) that factor could leave fp32;
+// values that differ are then 2^18 apart or more in the exponent, so a power of
+// two in place of k, whose products are exact, gives the same 1 or 0.
+// ---------------------------------------------------------------------------
+constexpr int kRow = 512;
+
+typedef short short2_t __attribute__((ext_vector_type(2)));
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_rsrc(const void* base, uint32_t bytes) {
+  const uint64_t b = reinterpret_cast<uint64_t>(base);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)b);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(b >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(((uint64_t)hi << 32) | lo), (short)0, (int)bytes,
+                                           0x00020000);
+}
+
+template <class T, int NL, int NR>
+__global__ __launch_bounds__(kRow) __attribute__((amdgpu_waves_per_eu(NR > 8 ? 4 : 6))) void lp_policy_kernel(
+    Rows a, Work w, Policy p, Grad g) {
+  constexpr int VEC = 16 / sizeof(T);
+  __shared__ __attribute__((aligned(16))) uint4 lds[NL > 0 ? NL * kRow : 1];
+  __shared__ float red[kRow / 64], say[2];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t row = blockIdx.x, n = row / a.s, s = row - n * a.s;
+  const int64_t y = a.target[n * a.tn + s * a.ts];
+  const T* x = (const T*)a.x + (n * a.xn + s * a.xs);
+  T* o = (T*)g.out + (n * g.on + s * g.os);
+  const int nvec = (int)(a.v / VEC), tail = (int)(a.v - (int64_t)nvec * VEC);
+  auto on = [&](int i) { return tid < nvec - i * kRow; };
+  auto fill = [&](float f) {
+    Vec16<T> z;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) z.v[j] = from_f32<T>(f);
+    for (int i = tid; i < nvec; i += kRow) store_any(o + (int64_t)i * VEC, z);
+    if (tid < tail) o[(int64_t)nvec * VEC + tid] = from_f32<T>(f);
+  };
+  if (y == a.ignore || !in_vocab(a, y)) {
+    const float f = y == a.ignore ? 0.f : __builtin_nanf("");
+    if (tid == 0) {
+      w.logps[row] = f;
+      w.row64[row] = f;
+      p.kl[row] = f;
+    }
+    fill(f);
+    return;
+  }
+
+  uint4 reg[NR];
+  if constexpr (NL > 0) {
+    const __amdgpu_buffer_rsrc_t rs = row_rsrc(x, (uint32_t)(nvec * 16));
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+      if (on(i)) {
+        __attribute__((address_space(3))) char* dst =
+            (__attribute__((address_space(3))) char*)lds + (i * (kRow / 64) + wave) * 1024;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)dst, 16, (uint32_t)tid * 16u,
+                                                 i * kRow * 16, 0, 2);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    reg[i] = make_uint4(0, 0, 0, 0);
+    if (on(NL + i)) reg[i] = load_any<T, true>(x + ((int64_t)(NL + i) * kRow + tid) * VEC).raw;
+  }
+  const float last = tid < tail ? to_f32(x[(int64_t)nvec * VEC + tid]) : -INFINITY;
+  const float xy = to_f32(x[y]);
+  if constexpr (NL > 0) {
+    __builtin_amdgcn_s_waitcnt(0);  // this wave's part of lds is there
+    __syncthreads();                // and every other's
+  }
+  uint4* mine = lds + tid;
+  auto each = [&](auto f) {  // f(vector, its index)
+#pragma unroll 1
+    for (int i = 0; i < NL; ++i)
+      if (on(i)) f(mine[i * kRow], i);
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+      if (on(NL + i)) f(reg[i], NL + i);
+  };
+  auto unpack = [](const uint4& r, float (&v)[VEC]) {
+    Vec16<T> t;
+    t.raw = r;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = to_f32(t.v[j]);
+  };
+
+  // A
+  short2_t mi = {(short)0x8000, (short)0x8000};
+  each([&](const uint4& r, int) {
+    mi = __builtin_elementwise_max(mi, __builtin_bit_cast(short2_t, r.x));
+    mi = __builtin_elementwise_max(mi, __builtin_bit_cast(short2_t, r.y));
+    mi = __builtin_elementwise_max(mi, __builtin_bit_cast(short2_t, r.z));
+    mi = __builtin_elementwise_max(mi, __builtin_bit_cast(short2_t, r.w));
+  });
+  const short top = mi.x > mi.y ? mi.x : mi.y;
+  float m = top >= 0 ? to_f32(__builtin_bit_cast(T, top)) : -INFINITY;
+  m = block_largest<kRow>(fmaxf(m, last), red);
+  if (m < 0.f) {  // nothing that is not negative but perhaps in the tail
+    each([&](const uint4& r, int) {
+      float v[VEC];
+      unpack(r, v);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) m = fmaxf(m, v[j]);
+    });
+    m = block_largest<kRow>(m, red);
+  }
+  float k = a.k, mk = m * k;
+  const bool far = fabsf(mk) >= 0x1p29f && fabsf(m) < INFINITY;
+  if (far) {
+    k = __uint_as_float(__float_as_uint(k) & 0x7f800000);
+    mk = m * k;
+  }
+
+  // B
+  float d = fast_exp2(fmaf(last, k, -mk));  // (0 without a tail)
+  each([&](const uint4& r, int) {
+    float v[VEC];
+    unpack(r, v);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = fast_exp2(fmaf(v[j], k, -mk));
+#pragma unroll
+    for (int h = VEC / 2; h >= 1; h /= 2)
+#pragma unroll
+      for (int j = 0; j < h; ++j) v[j] += v[j + h];
+    d += v[0];
+  });
+  d = block_total<float, kRow>(d, red);
+
+  // C
+  if (tid == 0) {
+    const double z = far ? ((double)xy - (double)m) * (double)a.k : (double)xy * (double)k - (double)mk;
+    const double lp = kLn2 * (z - log2((double)d));
+    double loss, dl;
+    float kl;
+    policy_token(p, n, s, lp, loss, dl, kl);
+    const double weight = token_weight(a, w.counts, p.reduction, n);
+    w.logps[row] = (float)lp;
+    w.row64[row] = loss * weight;
+    p.kl[row] = kl;
+    const float c = (float)(dl * weight) * g.inv_t;
+    say[0] = c == 0.f ? 0.f : -c / d;
+    say[1] = c == 0.f ? 0.f : -c * (float)expm1(lp);
+  }
+  __syncthreads();
+  const float scale = say[0], at_y = say[1];
+
+  // D
+  if (scale == 0.f && at_y == 0.f) {
+    fill(0.f);
+    return;
+  }
+  each([&](const uint4& r, int i) {
+    float v[VEC];
+    unpack(r, v);
+    Vec16<T> t;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) t.v[j] = from_f32<T>(scale * fast_exp2(fmaf(v[j], k, -mk)));
+    store_any(o + ((int64_t)i * kRow + tid) * VEC, t);
+  });
+  if (tid < tail) o[(int64_t)nvec * VEC + tid] = from_f32<T>(scale * fast_exp2(fmaf(last, k, -mk)));
+  // the target's column by the thread that has stored it, after that store
+  const int64_t yv = y / VEC;
+  if (yv < nvec ? (int)(yv % kRow) == tid : (int)(y - (int64_t)nvec * VEC) == tid) o[y] = from_f32<T>(at_y);
+}
+
+__global__ __launch_bounds__(1024) void lp_count_kernel(Rows a, int* counts) { count_tokens<1024>(a, counts); }
+
+__global__ __launch_bounds__(1024) void lp_sum_kernel(const double* rows, int64_t n, float* sum) {
+  __shared__ double red[16];
+  sum_rows<1024>(rows, n, sum, red);
 }
 
 // ---------------------------------------------------------------------------
@@ -631,6 +826,33 @@ int launch_grad(int dtype, const Rows& a, const Grad& g, bool rows, hipStream_t 
   });
 }
 
+// The kernel that holds a row, where it takes this call: 16-bit logits whose row
+// fits (in registers alone at any alignment), and rows enough for the card.
+#ifndef LP_RES_ROWS
+#define LP_RES_ROWS 512
+#endif
+constexpr int64_t kResidentRows = LP_RES_ROWS;
+
+template <class T>
+bool launch_policy(const Rows& a, const Work& w, const Policy& p, const Grad& g, hipStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    const int64_t rows = a.n * a.s, per = (a.v / 8 + kRow - 1) / kRow;  // vectors of a thread
+    if (rows < kResidentRows || rows > kMaxGrid || per > 32) return false;
+    const bool aligned = aligned16(a.x) && a.xn % 8 == 0 && a.xs % 8 == 0;
+    if (per > 16 && !aligned) return false;
+    const unsigned grid = (unsigned)rows;
+    lp_count_kernel<<<1, 1024, 0, s>>>(a, w.counts);
+    if (per <= 4) lp_policy_kernel<T, 0, 4><<<grid, kRow, 0, s>>>(a, w, p, g);
+    else if (per <= 8) lp_policy_kernel<T, 0, 8><<<grid, kRow, 0, s>>>(a, w, p, g);
+    else if (per <= 16) lp_policy_kernel<T, 0, 16><<<grid, kRow, 0, s>>>(a, w, p, g);
+    else if (per <= 24) lp_policy_kernel<T, 8, 16><<<grid, kRow, 0, s>>>(a, w, p, g);
+    else lp_policy_kernel<T, 8, 24><<<grid, kRow, 0, s>>>(a, w, p, g);
+    lp_sum_kernel<<<1, 1024, 0, s>>>(w.row64, rows, g.sum);
+    return true;
+  }
+  return false;
+}
+
 Rows make_rows(const void* x, int64_t xn, int64_t xs, int64_t n, int64_t s, int64_t v, const int64_t* target, int64_t tn,
                int64_t ts, int64_t ignore, double temperature) {
   const double k = temperature > 0.0 ? 1.4426950408889634074 / temperature : 0.0;
@@ -720,6 +942,11 @@ extern "C" int forge_policy_loss(int dtype, const void* logits, int64_t ld_n, in
   const Grad g = {dlogits, d_n, d_s, w.coef, s, 1, nullptr, 0, 1, w.state, logps, (float)(1.0 / temperature), w.row64, loss};
   hipStream_t st = (hipStream_t)stream;
   if (n * s > 0) {
+    bool done = false;
+    if (dlogits)
+      if (int rc = by_dtype(dtype, [&](auto* t) { done = launch_policy<std::remove_pointer_t<decltype(t)>>(a, w, p, g, st); }))
+        return rc;
+    if (done) return FORGE_OK;
     if (int rc = launch_partial(dtype, a, w, true, st)) return rc;
     if (int rc = launch_rows(dtype, a, w, &p, st)) return rc;
   }

@@ -574,6 +574,64 @@ def test_policy_many_rows(dtype, v):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16], ids=str)
+@pytest.mark.parametrize("v,inplace", [(5, False), (3003, True), (20000, False), (40001, True), (70000, True),
+                                       (120000, False)])
+def test_policy_awkward_rows(v, inplace, dtype):
+    """Rows of negative values, of a mask's lowest values, with infinities and
+    NaN, targets out of range and clipped tokens, in a batch large enough for a
+    row to a workgroup: a call of its own for each must give the same."""
+    from kernels.logprob import forge_policy_loss
+
+    s, inf, low = 600, float("inf"), torch.finfo(dtype).min
+    g = torch.Generator(device="cuda").manual_seed(v)
+    x = torch.empty(1, s, v, device="cuda", dtype=dtype).normal_(0, 2, generator=g)
+    y = torch.randint(0, v, (1, s), device="cuda", generator=g)
+    x[0, 0] = -x[0, 0].abs() - 3          # nothing but negative values
+    x[0, 1] = low                          # nothing but the lowest value
+    x[0, 2] = low
+    x[0, 2, v // 2] = 1.5                  # one value left, and it is not the target's
+    x[0, 3] = -inf
+    x[0, 4, 1] = inf
+    x[0, 5, v - 1] = float("nan")
+    x[0, 6, v // 3:] = -inf
+    y[0, 6] = 0
+    x[0, 7, y[0, 7]] = -inf                # the target is masked
+    x[0, 8], x[0, 8, y[0, 8]] = low / 2, low / 4
+    y[0, 9], y[0, 10] = v, -7
+    x[0, 11] = 0.0
+    x[0, 12] = torch.finfo(dtype).max
+    y[0, 13], y[0, 14] = v - 1, 0
+    y[0, 15:40] = IGNORE
+    adv = torch.empty(1, s, device="cuda").normal_(generator=g)
+    old = torch.full((1, s), -11.0, device="cuda")
+    old[0, 41], adv[0, 41] = -200.0, 1.0   # the ratio is past its clip: no gradient
+    ref = torch.full((1, s), -10.0, device="cuda")
+    ref[0, 41] = 0.0
+
+    def call(rows, inplace):
+        leaf = x[:, rows].clone().requires_grad_(True)
+        t = leaf * 1.0
+        o = forge_policy_loss(t, y[:, rows], adv[:, rows], old[:, rows], reduction="sum", inplace=inplace)
+        return (o, *torch.autograd.grad(o.loss, leaf))
+
+    o, d = call(slice(None), inplace)
+    assert o.loss.isnan() and (d[0, 15:40] == 0).all() and (d[0, 41] == 0).all()
+    rows = list(range(15)) + [41, 42, 599]
+    for r in rows:
+        one, d1 = call(slice(r, r + 1), False)
+        a, b = o.logps[0, r], one.logps[0, 0]
+        assert a == b or (a.isnan() and b.isnan()) or abs(a - b) <= 4 * float(_e(torch.tensor([[0.0, 20.0]])).max()) + \
+            abs(b) * 2 * U, (r, a, b)
+        assert torch.equal(d[0, r].isnan(), d1[0, 0].isnan()), r
+        eps = torch.finfo(dtype).eps
+        off = (d[0, r].float() - d1[0, 0].float()).abs() - d1[0, 0].float().abs() * eps * 1.1
+        fin = d1[0, 0].isfinite()
+        assert (off[fin] <= torch.finfo(dtype).smallest_normal).all(), (r, off[fin].max())
+        assert torch.equal(d[0, r][~fin & ~d1[0, 0].isnan()], d1[0, 0][~fin & ~d1[0, 0].isnan()]), r
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("scale", [1.0, 0.25, -3.7])
 @pytest.mark.parametrize("dtype", [BF16, FP32], ids=str)
 def test_policy_inplace_strides_and_scale(dtype, scale):
