@@ -16,11 +16,11 @@
 // heads of a token together, which share the token's place, its row of the
 // table and the loads in flight.  Measured on MI355X, bf16 [4, 4096], 32 + 8
 // heads of 128, nothing cached: forward 63 us (5.3 TB/s; a copy 5.8), backward
-// 92 us without and 104 us with the weights' gradients (5.5 and 4.8 TB/s).
+// 92 us without and 102 us with the weights' gradients (5.5 and 4.9 TB/s).
 //
 // Weight gradients: a workgroup adds up its heads in registers and writes one
 // row of partial sums, so there are few of them, each with the same share of
-// the heads: 768 (3 per CU, what the registers of two heads allow) 104 us; 1024
+// the heads: 768 (3 per CU, what the registers of two heads allow) 102 us; 1024
 // with one head a lane 106; 2048 114, 4096 119 (more rows to add up, and a last
 // round that is not full).  The adds within a wave go by DPP: by ds_bpermute the
 // backward took 119 us.
@@ -143,7 +143,7 @@ struct Lane {
   }
 };
 
-template <class T, class TC, bool VEC, bool BWD, bool DW>
+template <class T, class TC, bool VEC, bool BWD, bool DW, bool LATE>
 __global__ __launch_bounds__(kBlock) void qk_norm_rope_kernel(Args a) {
   using LaneT = Lane<T, VEC>;
   using X = typename LaneT::template Raw<T, true>;
@@ -161,7 +161,8 @@ __global__ __launch_bounds__(kBlock) void qk_norm_rope_kernel(Args a) {
   const uint32_t groups = (s.heads + HEADS - 1) / HEADS, items = s.tokens * groups;
 
   float wl[E] = {}, wh[E] = {}, al[E], ah[E];  // weight of the lower and upper half, and their gradients' sums
-  if (active) {
+  bool fresh = LATE;
+  if (!LATE && active) {
     lane.weight(s.w, a.w_dtype, 0, a.offset, wl);
     lane.weight(s.w, a.w_dtype, half, a.offset, wh);
   }
@@ -194,6 +195,13 @@ __global__ __launch_bounds__(kBlock) void qk_norm_rope_kernel(Args a) {
     if (active && in_table) {
       lane.load((const TC*)a.cos + ((int64_t)b * a.cos_sb + pos * a.cos_ss), rc);
       lane.load((const TC*)a.sin + ((int64_t)b * a.sin_sb + pos * a.sin_ss), rs);
+    }
+    if constexpr (LATE) {
+      if (fresh && active) {
+        lane.weight(s.w, a.w_dtype, 0, a.offset, wl);
+        lane.weight(s.w, a.w_dtype, half, a.offset, wh);
+      }
+      fresh = false;
     }
     float cs[E], sn[E];
     lane.values(rc, cs);
@@ -325,15 +333,28 @@ void split_blocks(Args& a, int heads_each, uint64_t cap) {
   }
 }
 
+// A call of few workgroups, a serving step's, is as long as its chain of loads:
+// there the weights are asked for behind the first heads (bf16, 16 tokens, 32 + 8
+// heads of 128: 4.5 us against 6.1), and so they are by the few workgroups that
+// add up weight gradients.  Where many workgroups follow each other the order
+// does not matter, and the test in the loop costs 3 us of 63 ([4, 4096]).
+constexpr uint32_t kFewBlocks = 1024;
+
+template <class T, class TC, bool VEC, bool BWD>
+void launch_vec(const Args& a, uint32_t blocks, size_t lds, hipStream_t s) {
+  if constexpr (BWD) {
+    if (lds) qk_norm_rope_kernel<T, TC, VEC, true, true, true><<<blocks, kBlock, lds, s>>>(a);
+    else qk_norm_rope_kernel<T, TC, VEC, true, false, false><<<blocks, kBlock, 0, s>>>(a);
+  } else {
+    if (blocks <= kFewBlocks) qk_norm_rope_kernel<T, TC, VEC, false, false, true><<<blocks, kBlock, 0, s>>>(a);
+    else qk_norm_rope_kernel<T, TC, VEC, false, false, false><<<blocks, kBlock, 0, s>>>(a);
+  }
+}
+
 template <class T, class TC, bool BWD>
 void launch(const Args& a, bool vec, uint32_t blocks, size_t lds, hipStream_t s) {
-  if (BWD && lds) {
-    if (vec) qk_norm_rope_kernel<T, TC, true, BWD, BWD><<<blocks, kBlock, lds, s>>>(a);
-    else qk_norm_rope_kernel<T, TC, false, BWD, BWD><<<blocks, kBlock, lds, s>>>(a);
-  } else {
-    if (vec) qk_norm_rope_kernel<T, TC, true, BWD, false><<<blocks, kBlock, 0, s>>>(a);
-    else qk_norm_rope_kernel<T, TC, false, BWD, false><<<blocks, kBlock, 0, s>>>(a);
-  }
+  if (vec) launch_vec<T, TC, true, BWD>(a, blocks, lds, s);
+  else launch_vec<T, TC, false, BWD>(a, blocks, lds, s);
 }
 
 template <bool BWD>

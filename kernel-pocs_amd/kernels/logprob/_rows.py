@@ -101,16 +101,37 @@ def workspace(x: torch.Tensor) -> torch.Tensor:
     return torch.empty(L.forge_logp_workspace(L.dtype_code(x.dtype), *x.shape), dtype=torch.uint8, device=x.device)
 
 
-def gradient(x, target, ignore_index, temperature, logps, state, coef, coef_strides, up, up_stride, up_count, out=None):
+def held(x: torch.Tensor):
+    """One buffer of a forward whose backward reads the logits again: each
+    row's state (2 floats) and log-probability, each sequence's coefficient,
+    and the forward's workspace behind them -> (buffer, the four addresses)."""
+    n, s, _ = x.shape
+    rows = -(-n * s // 4) * 4
+    logps = 8 * rows
+    coef = logps + 4 * rows
+    work = coef + -(-n // 4) * 16
+    buf = torch.empty(work + L.forge_logp_workspace(L.dtype_code(x.dtype), *x.shape), dtype=torch.uint8, device=x.device)
+    at = buf.data_ptr()
+    return buf, (at, at + logps, at + coef, at + work)
+
+
+def gradient(x, target, ignore_index, temperature, state, logps, coef, coef_strides, up, up_stride, up_count, out=None):
     """dlogits of coef (times up) times each row's log-probability, dense
-    unless `out` (the logits themselves) takes it."""
+    unless `out` (the logits themselves) takes it.  state, logps and coef are
+    addresses."""
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if x.numel():
         with L.on_device(x):
             L.check(
-                L.forge_token_logps_bwd(*rows_args(x, target, ignore_index), temperature, logps.data_ptr(),
-                                        state.data_ptr(), coef.data_ptr(), *coef_strides, L.ptr(up), up_stride, up_count,
-                                        out.data_ptr(), out.stride(0), out.stride(1), L.stream_of(x)),
+                L.forge_token_logps_bwd(*rows_args(x, target, ignore_index), temperature, logps, state, coef,
+                                        *coef_strides, L.ptr(up), up_stride, up_count, out.data_ptr(), out.stride(0),
+                                        out.stride(1), L.stream_of(x)),
                 "forge_token_logps_bwd")
     return out
+
+
+def held_addresses(buf: torch.Tensor, n: int, s: int):
+    """(state, log-probabilities, coefficients) of a buffer of `held`."""
+    rows, at = -(-n * s // 4) * 4, buf.data_ptr()
+    return at, at + 8 * rows, at + 12 * rows

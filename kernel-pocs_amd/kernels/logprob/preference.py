@@ -36,18 +36,17 @@ class ForgePreferenceLossFunction(torch.autograd.Function):
         n, s, _ = x.shape
         f32 = {"dtype": torch.float32, "device": x.device}
         loss = torch.empty((n // 2,) if reduction == L.REDUCE_NONE else (), **f32)
-        seq_logps, rewards, coef = (torch.empty(n, **f32) for _ in range(3))
-        logps, state, work = torch.empty((n, s), **f32), torch.empty((n, s, 2), **f32), R.workspace(x)
+        seq_logps, rewards = torch.empty(n, **f32), torch.empty(n, **f32)
+        held, (state, logps, coef, work) = R.held(x)
         with L.on_device(x):
             L.check(
                 L.forge_preference_fwd(*R.rows_args(x[: n // 2], target, ignore_index), L.ptr(ref), beta, smoothing, kind,
                                        int(normalized), reduction, loss.data_ptr(), seq_logps.data_ptr(),
-                                       rewards.data_ptr(), coef.data_ptr(), logps.data_ptr(), state.data_ptr(),
-                                       work.data_ptr(), L.stream_of(x)),
+                                       rewards.data_ptr(), coef, logps, state, work, L.stream_of(x)),
                 "forge_preference_fwd")
         # with inplace the backward writes over the logits, so they are kept
         # outside autograd's version check, and checked here
-        ctx.save_for_backward(target, logps, state, coef, *(() if inplace else (x,)))
+        ctx.save_for_backward(target, held, *(() if inplace else (x,)))
         ctx.x, ctx.version = (x.detach(), x._version) if inplace else (None, 0)
         ctx.ignore_index, ctx.inplace = ignore_index, inplace
         ctx.mark_non_differentiable(seq_logps, rewards)
@@ -56,7 +55,7 @@ class ForgePreferenceLossFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad, _logps, _rewards):
-        target, logps, state, coef, *saved = ctx.saved_tensors
+        target, held, *saved = ctx.saved_tensors
         x = ctx.x if ctx.inplace else saved[0]
         if x is None:
             raise RuntimeError("forge_preference_loss: the backward with inplace=True has written over the logits and "
@@ -64,7 +63,7 @@ class ForgePreferenceLossFunction(torch.autograd.Function):
         if ctx.inplace and x._version != ctx.version:
             raise RuntimeError("forge_preference_loss: the logits have been modified in place since the forward")
         grad = grad.to(torch.float32)
-        out = R.gradient(x, target, ctx.ignore_index, 1.0, logps, state, coef, (1, 0), grad,
+        out = R.gradient(x, target, ctx.ignore_index, 1.0, *R.held_addresses(held, *x.shape[:2]), (1, 0), grad,
                          grad.stride(0) if grad.dim() else 0, x.shape[0] // 2, out=x if ctx.inplace else None)
         if ctx.inplace:
             ctx.x = None

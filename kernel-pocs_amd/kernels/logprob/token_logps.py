@@ -40,8 +40,8 @@ class ForgeTokenLogpsFunction(torch.autograd.Function):
     def backward(ctx, grad):
         x, target, logps, state = ctx.saved_tensors
         grad = grad.to(torch.float32)
-        return (R.gradient(x, target, ctx.ignore_index, ctx.temperature, logps, state, grad, grad.stride(), None, 0, 1),
-                None, None, None)
+        return (R.gradient(x, target, ctx.ignore_index, ctx.temperature, state.data_ptr(), logps.data_ptr(),
+                           grad.data_ptr(), grad.stride(), None, 0, 1), None, None, None)
 
 
 def forge_token_logps(logits: torch.Tensor, target: torch.Tensor, ignore_index: int = -100, temperature: float = 1.0,

@@ -25,6 +25,7 @@ from kernels._positions import check_positions
 from .forge_rope_v3 import _tables, _unit_last
 
 _DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+_INTEGERS = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 MAX_HEAD_DIM = 1024
 
 
@@ -32,19 +33,20 @@ def _check(q, k, q_weight, k_weight, cos, sin, positions, eps):
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError(f"q and k must be [batch, heads, seq, head_dim], got {tuple(q.shape)} and {tuple(k.shape)}")
     B, _, S, D = q.shape
-    if (k.shape[0], k.shape[2], k.shape[3]) != (B, S, D):
+    kb, _, ks, kd = k.shape
+    if kb != B or ks != S or kd != D:
         raise ValueError(f"k {tuple(k.shape)} does not match q {tuple(q.shape)} in batch, seq or head_dim")
     if D == 0 or D % 2 or D > MAX_HEAD_DIM:
         raise ValueError(f"head_dim must be even and at most {MAX_HEAD_DIM}, got {D}")
-    for name, t in (("q", q), ("k", k), ("q_weight", q_weight), ("k_weight", k_weight)):
-        if t.dtype not in _DTYPES:
-            raise TypeError(f"{name} must be fp16, bf16 or fp32, got {t.dtype}")
-    if q.dtype != k.dtype:
-        raise TypeError(f"q and k must have the same dtype, got {q.dtype} and {k.dtype}")
+    dtype, w_dtype = q.dtype, q_weight.dtype
+    if dtype not in _DTYPES or w_dtype not in _DTYPES:
+        raise TypeError(f"q, k and the weights must be fp16, bf16 or fp32, got {dtype} and {w_dtype}")
+    if k.dtype != dtype:
+        raise TypeError(f"q and k must have the same dtype, got {dtype} and {k.dtype}")
     if q_weight.shape != (D,) or k_weight.shape != (D,):
         raise ValueError(f"q_weight and k_weight must be [{D}], got {tuple(q_weight.shape)} and {tuple(k_weight.shape)}")
-    if q_weight.dtype != k_weight.dtype:
-        raise TypeError(f"q_weight and k_weight must have the same dtype, got {q_weight.dtype} and {k_weight.dtype}")
+    if k_weight.dtype != w_dtype:
+        raise TypeError(f"q_weight and k_weight must have the same dtype, got {w_dtype} and {k_weight.dtype}")
     if cos.dim() != 3 or cos.shape != sin.shape or cos.shape[0] not in (1, B) or cos.shape[2] != D:
         raise ValueError(f"cos and sin must be [1 or {B}, rows, {D}], got {tuple(cos.shape)} and {tuple(sin.shape)}")
     if not cos.is_floating_point() or not sin.is_floating_point():
@@ -53,15 +55,16 @@ def _check(q, k, q_weight, k_weight, cos, sin, positions, eps):
         if cos.shape[1] != S:
             raise ValueError(f"cos and sin have {cos.shape[1]} rows for {S} tokens; pass positions to index a table")
     else:
-        if positions.dtype.is_floating_point or positions.dtype == torch.bool:
+        if positions.dtype not in _INTEGERS:
             raise TypeError(f"positions must be an integer tensor (got {positions.dtype})")
         if positions.numel() != B * S:
             raise ValueError(f"positions must have batch * seq = {B * S} entries, got {positions.numel()}")
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    for t in (k, q_weight, k_weight, cos, sin) + (() if positions is None else (positions,)):
-        if t.device != q.device:
-            raise ValueError(f"every tensor must be on q's device {q.device}, got {t.device}")
+    device = q.device
+    if (k.device != device or q_weight.device != device or k_weight.device != device or cos.device != device
+            or sin.device != device or (positions is not None and positions.device != device)):
+        raise ValueError(f"every tensor must be on q's device {device}")
     L.require_gpu(q)
 
 
@@ -154,13 +157,15 @@ def apply_qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
     if positions is not None:
         if validate_positions:
             check_positions(positions, cos.shape[1])
-        positions = positions.reshape(-1).to(torch.int64).contiguous()
+        if positions.dtype != torch.int64 or not positions.is_contiguous():
+            positions = positions.to(torch.int64).contiguous()
     cos, sin = _tables(cos, sin, q)
-    args = (_unit_last(q), _unit_last(k), q_weight.contiguous(), k_weight.contiguous(), cos.detach(), sin.detach(),
-            positions, float(eps), float(offset))
-    if torch.is_grad_enabled() and any(t.requires_grad for t in args[:4]):
-        return ForgeQKNormRoPEFunction.apply(*args)
-    return _forward(*args)
+    q, k, q_weight, k_weight = _unit_last(q), _unit_last(k), q_weight.contiguous(), k_weight.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad
+                                    or k_weight.requires_grad):
+        return ForgeQKNormRoPEFunction.apply(q, k, q_weight, k_weight, cos.detach(), sin.detach(), positions, float(eps),
+                                             float(offset))
+    return _forward(q, k, q_weight, k_weight, cos, sin, positions, float(eps), float(offset))
 
 
 class ForgeQKNormRoPE(torch.nn.Module):
