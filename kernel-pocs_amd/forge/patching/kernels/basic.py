@@ -28,11 +28,21 @@ _GELU_EXACT = {"gelu", "gelu_python"}
 _GELU_TANH = {"gelu_pytorch_tanh", "gelu_new"}
 
 
+def _saved_in_8_bits(config) -> bool:
+    """config["saved_activations"]: None (gate and up are saved as they are) or
+    "8bit" (glu_act8: an 8-bit copy of them is, on a GPU)."""
+    saved = config.get("saved_activations")
+    if saved not in (None, "8bit"):
+        raise ValueError(f"forge.patch: saved_activations must be None or '8bit', got {saved!r}")
+    return saved == "8bit"
+
+
 def make_geglu_forward(module, config):
     """Gemma MLP.forward -> down_proj(geglu(gate_proj(x), up_proj(x)))
     (basic.py:53-90).  The GELU form comes from config["approximate"] or the
     HF config's hidden_activation / hidden_act; NotImplementedError when
-    neither names a known form."""
+    neither names a known form.  config["saved_activations"] = "8bit" keeps gate
+    and up in 8 bits for the backward."""
     from forge.kernels.geglu import geglu
 
     approximate = config.get("approximate")
@@ -50,6 +60,19 @@ def make_geglu_forward(module, config):
                 f"forge.patch: geglu kernel cannot infer GELU variant for hidden_activation={act!r}. "
                 f"Pass approximate='tanh' or approximate='none' via the mapping config to override.")
 
+    if _saved_in_8_bits(config):
+        from forge.kernels.glu_act8 import glu_act8
+
+        kind = "gelu_tanh" if approximate == "tanh" else "gelu_exact"
+
+        def forward8(x):
+            gate, up = module.gate_proj(x), module.up_proj(x)
+            if not gate.is_cuda:
+                return module.down_proj(geglu(gate, up, approximate=approximate))
+            return module.down_proj(glu_act8(gate, up, kind))
+
+        return forward8
+
     def forward(x):
         return module.down_proj(geglu(module.gate_proj(x), module.up_proj(x), approximate=approximate))
 
@@ -58,13 +81,25 @@ def make_geglu_forward(module, config):
 
 def make_swiglu_forward(module, config):
     """Qwen/Llama MLP.forward -> down_proj(swiglu(gate_proj(x), up_proj(x)))
-    (basic.py:93-107); only activation "silu"."""
+    (basic.py:93-107); only activation "silu".  config["saved_activations"] =
+    "8bit" keeps gate and up in 8 bits for the backward."""
     activation = config.get("activation", "silu")
     if activation != "silu":
         raise NotImplementedError(
             f"forge.patch: swiglu kernel only supports activation='silu', got {activation!r}. "
             f"Route this module to the 'geglu' kernel instead.")
     from forge.kernels.swiglu import swiglu
+
+    if _saved_in_8_bits(config):
+        from forge.kernels.glu_act8 import glu_act8
+
+        def forward8(x):
+            gate, up = module.gate_proj(x), module.up_proj(x)
+            if not gate.is_cuda:
+                return module.down_proj(swiglu(gate, up))
+            return module.down_proj(glu_act8(gate, up, "silu"))
+
+        return forward8
 
     def forward(x):
         return module.down_proj(swiglu(module.gate_proj(x), module.up_proj(x)))

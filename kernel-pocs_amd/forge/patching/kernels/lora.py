@@ -40,7 +40,9 @@ Fused paths:
     to Q and K in its epilogue (replaces view -> transpose ->
     apply_rotary_pos_emb, lora.py:240-264).  With q/k norms (Qwen3) the norm
     sits between the projection and RoPE, so the fused QKV GEMM runs without
-    RoPE and the model's own norm and apply_rotary_pos_emb follow.
+    RoPE and the model's own norm and apply_rotary_pos_emb follow; with
+    config["fuse_qk_norm"] both norms and RoPE are one pass instead
+    (apply_qk_norm_rope, which rounds once where the modules round four times).
 """
 from __future__ import annotations
 
@@ -351,7 +353,36 @@ def _attention_interface(module, modeling, kwargs):
     return modeling.ALL_ATTENTION_FUNCTIONS[impl]
 
 
-def _qkv_states(module, modeling, hidden_states, cos, sin):
+def qk_norm_args(module, Q, K, cos, sin, config):
+    """(q weight, k weight, eps, offset) when the two norms and RoPE can run as
+    one pass over Q, K [B, S, heads, D], else None: both norms plain RMS norms
+    over head_dim (class names end in RMSNorm) with one eps and no hooks, GPU
+    tensors, cos/sin [B or 1, S, D] of a half-split rotation.  The stored weight
+    is the difference from one (offset 1.0) in Gemma's classes;
+    config["qk_norm_offset"] overrides."""
+    q_norm, k_norm = getattr(module, "q_norm", None), getattr(module, "k_norm", None)
+    if q_norm is None or k_norm is None or not Q.is_cuda or _is_dtensor(Q):
+        return None
+    names, eps = [], []
+    for norm in (q_norm, k_norm):
+        w = getattr(norm, "weight", None)
+        if not type(norm).__name__.endswith("RMSNorm") or w is None or _is_dtensor(w) or w.shape != Q.shape[-1:]:
+            return None
+        if w.device != Q.device or norm._forward_hooks or norm._forward_pre_hooks:
+            return None
+        names.append(type(norm).__name__)
+        eps.append(getattr(norm, "variance_epsilon", getattr(norm, "eps", None)))
+    if eps[0] is None or eps[0] != eps[1] or names[0] != names[1] or q_norm.weight.dtype != k_norm.weight.dtype:
+        return None
+    if cos.dim() != 3 or cos.shape != sin.shape or cos.shape[0] not in (1, Q.shape[0]):
+        return None
+    if tuple(cos.shape[1:]) != (Q.shape[1], Q.shape[-1]) or cos.device != Q.device:
+        return None
+    offset = float(config.get("qk_norm_offset", 1.0 if names[0].startswith("Gemma") else 0.0))
+    return q_norm.weight, k_norm.weight, float(eps[0]), offset
+
+
+def _qkv_states(module, modeling, hidden_states, cos, sin, config):
     """(query, key, value) as [B, heads, S, D] with RoPE applied to query and
     key: fused when the live tensors allow it, else the reference's chain."""
     from kernels.lora_qkv.experiments.v4.lora_qkv_kernel_v4 import LoRAQKVRoPEFunction, LoRAQKVv4Function
@@ -373,6 +404,13 @@ def _qkv_states(module, modeling, hidden_states, cos, sin):
     else:
         Q, K, V = module.q_proj(hidden_states), module.k_proj(hidden_states), module.v_proj(hidden_states)
     Q, K, V = Q.view(hidden_shape), K.view(hidden_shape), V.view(hidden_shape)
+    norm = qk_norm_args(module, Q, K, cos, sin, config) if config.get("fuse_qk_norm", False) else None
+    if norm is not None:
+        from kernels.rope.qk_norm_rope import apply_qk_norm_rope
+
+        qw, kw, eps, offset = norm
+        Q, K = apply_qk_norm_rope(Q.transpose(1, 2), K.transpose(1, 2), qw, kw, cos, sin, eps=eps, offset=offset)
+        return Q, K, V.transpose(1, 2)
     if hasattr(module, "q_norm"):
         Q = module.q_norm(Q)
     if hasattr(module, "k_norm"):
@@ -386,7 +424,9 @@ def make_lora_qkv_forward(module, config):
     """PEFT LoRA attention forward with fused Q/K/V (+RoPE), per
     lora.py:200-312: same signature (past_key_value or past_key_values,
     cache_position, **kwargs), KV-cache update, sliding window, attention
-    interface selection, Gemma2's softcap, o_proj through its submodule."""
+    interface selection, Gemma2's softcap, o_proj through its submodule.
+    config["fuse_qk_norm"] (default False): q/k norms and RoPE in one pass where
+    `qk_norm_args` allows."""
     for proj in (module.q_proj, module.k_proj, module.v_proj):
         _check_lora_active(proj)
     modeling = importlib.import_module(module.__class__.__module__)
@@ -396,7 +436,7 @@ def make_lora_qkv_forward(module, config):
         kv_cache = past_key_values if past_key_values is not None else past_key_value
         input_shape = hidden_states.shape[:-1]
         cos, sin = position_embeddings
-        query, key, value = _qkv_states(module, modeling, hidden_states, cos, sin)
+        query, key, value = _qkv_states(module, modeling, hidden_states, cos, sin, config)
         if kv_cache is not None:
             key, value = kv_cache.update(key, value, module.layer_idx,
                                          {"sin": sin, "cos": cos, "cache_position": cache_position})
@@ -415,4 +455,4 @@ def make_lora_qkv_forward(module, config):
 
 
 __all__ = ["LiveLoRA", "live_lora", "make_lora_mlp_forward", "make_lora_qkv_forward", "mlp_fused_args",
-           "qkv_fused_args", "rope_tables"]
+           "qk_norm_args", "qkv_fused_args", "rope_tables"]

@@ -1,6 +1,6 @@
 """RMS norm of every query and key head and RoPE, in one pass over q and k.
 
-Models with q/k norms (Qwen3, Gemma3) norm each head between the projections
+Models with q/k norms (Qwen3) norm each head between the projections
 and the rotation: `q_norm`, `k_norm`, then `apply_rotary_pos_emb`
 (forge/forge/patching/kernels/lora.py:254-264 of the reference runs them as
 separate modules).  `apply_qk_norm_rope` does both at once, forward and
