@@ -336,7 +336,8 @@ enum {
 
 int64_t forge_logp_workspace(int dtype, int64_t n, int64_t s, int64_t v);
 
-/* logps[n, s] (dense fp32) = log softmax(logits / temperature) at the target.
+/* logps[n, s] (dense fp32) = log softmax(logits / temperature) at the target;
+ * temperature from 1e-6 to 1e6.
  * state (2 floats a row, may be NULL): what forge_token_logps_bwd needs. */
 int forge_token_logps_fwd(int dtype, const void* logits, int64_t ld_n, int64_t ld_s,
                           int64_t n, int64_t s, int64_t v,

@@ -164,17 +164,24 @@ __device__ __forceinline__ float block_largest(float v, float* red) {
 }
 
 // counts[n]: tokens of sequence n that are not ignored; counts[N], counts[N + 1]:
-// tokens in all and sequences that have any.  By one workgroup, a wave to a sequence.
+// tokens in all and sequences that have any.  By one workgroup: a wave to a
+// sequence, or the whole workgroup where there are fewer sequences than waves (a
+// packed batch is one long sequence).
 template <int NT>
 __device__ void count_tokens(const Rows& a, int* counts) {
   __shared__ int red[NT / 64];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const bool whole = a.n < NT / 64;
+  const int lane = whole ? threadIdx.x : threadIdx.x & 63, lanes = whole ? NT : 64;
   int tokens = 0, filled = 0;
-  for (int64_t n = wave; n < a.n; n += NT / 64) {
+  for (int64_t n = whole ? 0 : threadIdx.x >> 6; n < a.n; n += whole ? 1 : NT / 64) {
     int c = 0;
 #pragma unroll 8
-    for (int64_t s = lane; s < a.s; s += 64) c += a.target[n * a.tn + s * a.ts] != a.ignore;
-    for (int off = 32; off >= 1; off >>= 1) c += __shfl_xor(c, off, 64);
+    for (int64_t s = lane; s < a.s; s += lanes) c += a.target[n * a.tn + s * a.ts] != a.ignore;
+    if (whole) {
+      c = block_total<int, NT>(c, red);
+    } else {
+      for (int off = 32; off >= 1; off >>= 1) c += __shfl_xor(c, off, 64);
+    }
     if (lane == 0) {
       counts[n] = c;
       tokens += c;
@@ -783,7 +790,8 @@ int check_rows(const char* what, int dtype, const Rows& a, double temperature) {
   if (a.n < 0 || a.s < 0 || a.v < 0) return forge_set_error(FORGE_ERR_INVALID, "%s: negative shape", what);
   if (dtype != FORGE_DTYPE_F32 && dtype != FORGE_DTYPE_BF16 && dtype != FORGE_DTYPE_F16)
     return forge_set_error(FORGE_ERR_UNSUPPORTED, "%s: dtype %d", what, dtype);
-  if (!(temperature > 0.0)) return forge_set_error(FORGE_ERR_INVALID, "%s: temperature %g", what, temperature);
+  if (!(temperature >= 1e-6 && temperature <= 1e6))
+    return forge_set_error(FORGE_ERR_INVALID, "%s: temperature %g (1e-6 to 1e6)", what, temperature);
   const int64_t lim = 0x7fffffff;
   if (a.n > lim || a.s > lim || a.v > lim || a.n * a.s > lim)
     return forge_set_error(FORGE_ERR_UNSUPPORTED, "%s: 2^31 rows or columns", what);

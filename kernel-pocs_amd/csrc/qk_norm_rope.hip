@@ -217,6 +217,7 @@ __global__ __launch_bounds__(kBlock) void qk_norm_rope_kernel(Args a) {
       for (int j = 0; j < E; ++j) ss += xl[j] * xl[j] + xh[j] * xh[j];
       float r = rsqrtf(head_sum(ss, lanes) * a.inv_d + a.eps);
       if (!in_table) r = __builtin_nanf("");  // nothing of the table was read: the token's outputs are NaN
+      if (HEADS > 1 && h0 + u >= s.heads) r = 0.f;  // no head: x = dy = 0, which an eps of 0 would turn into NaN
       if constexpr (!BWD) {
 #pragma unroll
         for (int j = 0; j < E; ++j) {
@@ -233,7 +234,7 @@ __global__ __launch_bounds__(kBlock) void qk_norm_rope_kernel(Args a) {
         for (int j = 0; j < E; ++j) {
           // r dy; then r g = r dy w, and with sum g n = sum (r g) x
           const float yl = (gl[j] * cs[j] + gh[j] * sn[j]) * r, yh = (gh[j] * cs[j] - gl[j] * sn[j]) * r;
-          if constexpr (DW) {  // (a head past the last one has x = dy = 0)
+          if constexpr (DW) {  // (a head past the last one adds zeros)
             al[j] += yl * xl[j];
             ah[j] += yh * xh[j];
           }

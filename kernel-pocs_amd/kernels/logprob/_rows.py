@@ -18,8 +18,8 @@ def check_logits(logits: torch.Tensor, target: torch.Tensor, temperature: float 
         raise TypeError(f"target must be an integer tensor, got {target.dtype}")
     if logits.shape[-1] == 0 and target.numel():
         raise ValueError("logits have no columns")
-    if not temperature > 0.0:
-        raise ValueError(f"temperature must be positive, got {temperature}")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"temperature must be between 1e-6 and 1e6, got {temperature}")
     if target.device != logits.device:
         raise ValueError(f"target must be on the logits' device {logits.device}, got {target.device}")
 
@@ -76,8 +76,10 @@ def target_2d(target: torch.Tensor, dim: int) -> torch.Tensor:
 
 
 def check_inplace(logits: torch.Tensor) -> None:
-    """The gradient can be written over [N, S, V] logits only where no two of
-    their elements share memory and columns are adjacent."""
+    """The gradient can be written over [N, S, V] logits only where they are an
+    operation's result, columns are adjacent and no two elements share memory."""
+    if logits.requires_grad and logits.is_leaf:
+        raise ValueError("inplace needs logits that are not a leaf: their gradient would be themselves")
     (n, s, v), (sn, ss, sv) = logits.shape, logits.stride()
     inner, outer = ((s, ss), (n, sn)) if ss <= sn else ((n, sn), (s, ss))
     ok = v <= 1 or sv == 1

@@ -21,7 +21,6 @@ from typing import Optional
 import torch
 
 from forge_hip import _lib as L
-from kernels._positions import check_positions
 from .forge_rope_v3 import _tables, _unit_last
 
 _DTYPES = (torch.float16, torch.bfloat16, torch.float32)
@@ -155,8 +154,10 @@ def apply_qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
     Gradients: q, k, and the weights where they require it."""
     _check(q, k, q_weight, k_weight, cos, sin, positions, eps)
     if positions is not None:
-        if validate_positions:
-            check_positions(positions, cos.shape[1])
+        if validate_positions and positions.numel():
+            lo, hi = (int(v) for v in torch.aminmax(positions))
+            if lo < 0 or hi >= cos.shape[1]:
+                raise IndexError(f"positions must lie in [0, {cos.shape[1]}) (the cos/sin rows); got min {lo}, max {hi}")
         if positions.dtype != torch.int64 or not positions.is_contiguous():
             positions = positions.to(torch.int64).contiguous()
     cos, sin = _tables(cos, sin, q)

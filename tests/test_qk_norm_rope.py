@@ -239,6 +239,15 @@ def test_zero_rows_large_values_and_no_tokens():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=str)
+def test_no_eps_with_odd_heads(dtype):
+    """eps = 0: nothing but the heads themselves may be divided by their norm."""
+    q, k = _make(2, 5, 3, 7, 96, dtype)
+    cos, sin = (t.cuda() for t in _cos_sin(7, 96, dtype))
+    _check(q, k, *_weights(96, dtype, 0.0), cos, sin, None, 0.0, eps=0.0)
+
+
+@pytest.mark.gpu
 def test_a_head_with_an_infinity_or_nan_stays_alone():
     from kernels.rope import apply_qk_norm_rope
 
