@@ -165,27 +165,41 @@ __device__ __forceinline__ float block_largest(float v, float* red) {
 
 // counts[n]: tokens of sequence n that are not ignored; counts[N], counts[N + 1]:
 // tokens in all and sequences that have any.  By one workgroup: a wave to a
-// sequence, or the whole workgroup where there are fewer sequences than waves (a
-// packed batch is one long sequence).
+// sequence, or several where there are fewer sequences than waves (a packed batch
+// is one long sequence).
 template <int NT>
 __device__ void count_tokens(const Rows& a, int* counts) {
-  __shared__ int red[NT / 64];
-  const bool whole = a.n < NT / 64;
-  const int lane = whole ? threadIdx.x : threadIdx.x & 63, lanes = whole ? NT : 64;
-  int tokens = 0, filled = 0;
-  for (int64_t n = whole ? 0 : threadIdx.x >> 6; n < a.n; n += whole ? 1 : NT / 64) {
+  constexpr int NW = NT / 64;
+  __shared__ int red[NW], part[NW];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  auto count = [&](int64_t n, int first, int step) {  // by a wave: tokens first * 64 + lane, + step * 64, ...
     int c = 0;
 #pragma unroll 8
-    for (int64_t s = lane; s < a.s; s += lanes) c += a.target[n * a.tn + s * a.ts] != a.ignore;
-    if (whole) {
-      c = block_total<int, NT>(c, red);
-    } else {
-      for (int off = 32; off >= 1; off >>= 1) c += __shfl_xor(c, off, 64);
+    for (int64_t s = first * 64 + lane; s < a.s; s += step * 64) c += a.target[n * a.tn + s * a.ts] != a.ignore;
+    for (int off = 32; off >= 1; off >>= 1) c += __shfl_xor(c, off, 64);
+    return c;
+  };
+  int tokens = 0, filled = 0;
+  auto store = [&](int64_t n, int c) {
+    counts[n] = c;
+    tokens += c;
+    filled += c > 0;
+  };
+  if (a.n >= NW) {
+    for (int64_t n = wave; n < a.n; n += NW) {
+      const int c = count(n, 0, 1);
+      if (lane == 0) store(n, c);
     }
-    if (lane == 0) {
-      counts[n] = c;
-      tokens += c;
-      filled += c > 0;
+  } else {
+    const int each = NW / (int)a.n;  // waves of a sequence
+    const int n = wave / each;
+    const int c = n < a.n ? count(n, wave % each, each) : 0;
+    if (lane == 0) part[wave] = c;
+    __syncthreads();
+    if ((int)threadIdx.x < a.n) {
+      int t = 0;
+      for (int w = 0; w < each; ++w) t += part[threadIdx.x * each + w];
+      store(threadIdx.x, t);
     }
   }
   tokens = block_total<int, NT>(tokens, red);
