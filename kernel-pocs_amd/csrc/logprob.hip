@@ -387,22 +387,23 @@ __global__ __launch_bounds__(1024) void lp_sequences_kernel(Rows a, Work w, int 
   __shared__ double redd[16];
   __shared__ int redi[16];
   const int lane = threadIdx.x & (lanes - 1), per = 1024 / lanes;
-  const int64_t n = blockIdx.x;
-  double sum = 0.0;
-  int count = 0;
-  for (int64_t s = threadIdx.x / lanes; s < a.s; s += per) {
-    const int64_t y = a.target[n * a.tn + s * a.ts];
-    const double lp = join_row<T>(a, w, n * a.s + s, lane, lanes, y);
-    if (lane == 0) {
-      sum += lp;
-      count += y != a.ignore;
+  for (int64_t n = blockIdx.x; n < a.n; n += gridDim.x) {
+    double sum = 0.0;
+    int count = 0;
+    for (int64_t s = threadIdx.x / lanes; s < a.s; s += per) {
+      const int64_t y = a.target[n * a.tn + s * a.ts];
+      const double lp = join_row<T>(a, w, n * a.s + s, lane, lanes, y);
+      if (lane == 0) {
+        sum += lp;
+        count += y != a.ignore;
+      }
     }
-  }
-  sum = block_total<double, 1024>(sum, redd);
-  count = block_total<int, 1024>(count, redi);
-  if (threadIdx.x == 0) {
-    seq[n] = mean && count ? sum / count : sum;
-    w.counts[n] = count;
+    sum = block_total<double, 1024>(sum, redd);
+    count = block_total<int, 1024>(count, redi);
+    if (threadIdx.x == 0) {
+      seq[n] = mean && count ? sum / count : sum;
+      w.counts[n] = count;
+    }
   }
 }
 
@@ -940,7 +941,7 @@ extern "C" int forge_preference_fwd(int dtype, const void* logits, int64_t ld_n,
   const int lanes = lanes_of(w.splits);
   if (int rc = by_dtype(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        lp_sequences_kernel<T><<<(unsigned)n, 1024, 0, st>>>(a, w, lanes, normalized != 0, seq);
+        lp_sequences_kernel<T><<<(unsigned)(n > kMaxGrid / 4 ? kMaxGrid / 4 : n), 1024, 0, st>>>(a, w, lanes, normalized != 0, seq);
       }))
     return rc;
   const Pairs p = {seq, w.counts, ref, pairs, beta, label_smoothing, kind, reduction, normalized != 0, loss, seq_logps,
