@@ -17,7 +17,9 @@
 //   lp_grad_kernel      c / t (1{j = y} - p_j) over every row, zeros where the
 //                       target is ignored (those rows are not read).
 // Bound by HBM: one read of the kept rows, and for the gradient another and one
-// write.
+// write.  Measured on MI355X, bf16, nothing cached, log-probabilities / gradient:
+// 4096 rows of 128256 197 / 342 us (5.3 / 6.1 TB/s; a copy 5.8), 2048 of 50257
+// (rows off 16 bytes) 56 / 76, 512 of 32000 14 / 16, 16 of 128256 9 / 5.
 //
 // Numbers: the softmax runs in base 2, with k = log2(e) / t in two fp32 parts
 // (the first alone is a temperature off by up to 2^-24, the same way for every
@@ -36,7 +38,7 @@
 namespace {
 
 constexpr int kBlock = 256;
-constexpr int kU = 4;                   // vectors in flight per thread
+constexpr int kU = 4;                   // vectors in flight per thread (2: the same; 8: 5% slower, 20% at 512 rows of 32000)
 constexpr int kMaxSplits = 64;          // pieces of a row
 constexpr int64_t kMaxGrid = 1 << 22;   // workgroups of a launch; more work loops
 constexpr double kLn2 = 0.693147180559945309417;
@@ -476,7 +478,9 @@ struct Grad {
   float* sum;                             // ... into here, where given
 };
 
-constexpr int kGradVec = 4;  // vectors of a thread
+// Vectors of a thread: 4096 rows of 128256, 342 us; with 1 576, 2 378, 8 348 (8
+// on 2048 rows of 50257: 95 against 76).
+constexpr int kGradVec = 4;
 
 // *sum = the rows' losses in a fixed order, by one workgroup.
 template <int NT>
@@ -569,9 +573,9 @@ __global__ __launch_bounds__(kBlock) void lp_grad_kernel(Rows a, Grad g, int64_t
 //   C  one thread, in 64 bits: the token's loss and coefficient
 //   D  the gradient, each exponential again (kept in 16 bits it would be rounded
 //      twice)
-// Measured on MI355X, bf16 [8, 1024, 128256], 73% of the rows kept, nothing
-// cached: 655 us, 5.5 TB/s of reads and writes (a copy 5.8), against 815 us for
-// the passes above, which read those rows twice at 6.3 TB/s.
+// Measured on MI355X, bf16 [8, 1024, 128256], 66% of the rows kept, nothing
+// cached: 655 us, 5.3 TB/s of reads and writes (a copy 5.8), against 815 us for
+// the passes above, which read those rows twice at 6.0 TB/s.
 // One fma gives x k - m k: what rounding m k leaves is the same factor on every
 // exponential and on d, and the log-probability takes it into account.  Where m k
 // passes 2^29 (a row of a mask's lowest values) that factor could leave fp32;
@@ -753,7 +757,8 @@ __global__ __launch_bounds__(1024) void lp_sum_kernel(const double* rows, int64_
 int vec_of(int dtype) { return (int)(16 / dtype_size(dtype)); }
 
 // Pieces of a row: enough workgroups for the card (4 on each CU), none with
-// less than a vector a thread.
+// less than a vector a thread.  512 rows of 32000 / 16 of 128256: 13.7 / 9.0 us;
+// with 2 on each CU 14.0 / 8.0, 8 14.9 / 9.0, 16 17.5 / 8.9.
 int splits_for(int64_t rows, int64_t v, int dtype) {
   const int64_t most = v / ((int64_t)vec_of(dtype) * kBlock);
   int64_t s = rows ? (1024 + rows - 1) / rows : 1;
