@@ -356,6 +356,7 @@ extern "C" int forge_glu_act8_fwd(int dtype, int activation, const void* gate, i
   if (a.n == 0) return FORGE_OK;
   if (ld_gate < cols || ld_up < cols || ld_out < cols)
     return forge_set_error(FORGE_ERR_INVALID, "glu_act8_fwd: leading dimension smaller than cols");
+  if (!gate || !up || !out) return forge_set_error(FORGE_ERR_INVALID, "glu_act8_fwd: a required pointer is NULL");
   if (!element_aligned(gate, dtype) || !element_aligned(up, dtype) || !element_aligned(out, dtype) || !aligned16(kept))
     return forge_set_error(FORGE_ERR_INVALID, "glu_act8_fwd: misaligned pointer");
   a.gate = gate; a.ld_gate = ld_gate;
@@ -372,7 +373,8 @@ extern "C" int forge_glu_act8_bwd(int dtype, int activation, const void* dout, i
   if (a.n == 0) return FORGE_OK;
   if (ld_dout < cols || ld_grad < cols)
     return forge_set_error(FORGE_ERR_INVALID, "glu_act8_bwd: leading dimension smaller than cols");
-  if (!kept) return forge_set_error(FORGE_ERR_INVALID, "glu_act8_bwd: kept is NULL");
+  if (!kept || !dout || !dgate || !dup)
+    return forge_set_error(FORGE_ERR_INVALID, "glu_act8_bwd: kept or another required pointer is NULL");
   if (!element_aligned(dout, dtype) || !element_aligned(dgate, dtype) || !element_aligned(dup, dtype) || !aligned16(kept))
     return forge_set_error(FORGE_ERR_INVALID, "glu_act8_bwd: misaligned pointer");
   a.out = const_cast<void*>(dout); a.ld_out = ld_dout;

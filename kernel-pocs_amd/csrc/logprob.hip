@@ -33,6 +33,9 @@
 // a mask's -1e30.)  A row with a NaN or +infinity, or with nothing but
 // -infinity, comes out as NaN; so does a row whose target is outside [0, V)
 // without being ignored, of which nothing is read.
+#include <initializer_list>
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
@@ -819,6 +822,13 @@ int check_rows(const char* what, int dtype, const Rows& a, double temperature) {
   return FORGE_OK;
 }
 
+// The arrays that a call with rows cannot do without.
+int check_given(const char* what, std::initializer_list<const void*> ptrs) {
+  for (const void* p : ptrs)
+    if (!p) return forge_set_error(FORGE_ERR_INVALID, "%s: a required pointer is NULL", what);
+  return FORGE_OK;
+}
+
 template <class F>
 int by_dtype(int dtype, F f) {
   if (dtype == FORGE_DTYPE_F32) f((float*)nullptr);
@@ -904,6 +914,7 @@ extern "C" int forge_token_logps_fwd(int dtype, const void* logits, int64_t ld_n
   const Rows a = make_rows(logits, ld_n, ld_s, n, s, v, target, t_n, t_s, ignore_index, temperature);
   if (int rc = check_rows("token_logps_fwd", dtype, a, temperature)) return rc;
   if (n * s == 0) return FORGE_OK;
+  if (int rc = check_given("token_logps_fwd", {logits, target, logps, work})) return rc;
   const Work w = Layout(dtype, n, s, v).work(work, logps, (float2*)state);
   hipStream_t st = (hipStream_t)stream;
   if (int rc = launch_partial(dtype, a, w, false, st)) return rc;
@@ -918,6 +929,7 @@ extern "C" int forge_token_logps_bwd(int dtype, const void* logits, int64_t ld_n
   const Rows a = make_rows(logits, ld_n, ld_s, n, s, v, target, t_n, t_s, ignore_index, temperature);
   if (int rc = check_rows("token_logps_bwd", dtype, a, temperature)) return rc;
   if (n * s == 0) return FORGE_OK;
+  if (int rc = check_given("token_logps_bwd", {logits, target, logps, state, coef, dlogits})) return rc;
   if (up && up_count <= 0) return forge_set_error(FORGE_ERR_INVALID, "token_logps_bwd: up_count %lld", (long long)up_count);
   const Grad g = {dlogits, d_n, d_s, coef, c_n, c_s, up, up_stride, up_count, (const float2*)state, logps,
                   (float)(1.0 / temperature), nullptr, nullptr};
@@ -937,6 +949,9 @@ extern "C" int forge_preference_fwd(int dtype, const void* logits, int64_t ld_n,
   if (reduction != FORGE_REDUCE_MEAN && reduction != FORGE_REDUCE_SUM && reduction != FORGE_REDUCE_NONE)
     return forge_set_error(FORGE_ERR_INVALID, "preference_fwd: reduction %d", reduction);
   if (pairs < 1) return forge_set_error(FORGE_ERR_INVALID, "preference_fwd: no pairs");
+  if (int rc = check_given("preference_fwd", {loss, seq_logps, rewards, coef, work})) return rc;
+  if (s > 0)
+    if (int rc = check_given("preference_fwd", {logits, target, logps, state})) return rc;
   const Layout l(dtype, n, s, v);
   const Work w = l.work(work, logps, (float2*)state);
   double* seq = (double*)((char*)work + l.seq);
@@ -967,6 +982,9 @@ extern "C" int forge_policy_loss(int dtype, const void* logits, int64_t ld_n, in
   if (int rc = check_rows("policy_loss", dtype, a, temperature)) return rc;
   if (reduction != FORGE_REDUCE_MEAN && reduction != FORGE_REDUCE_SUM && reduction != FORGE_REDUCE_SEQUENCE)
     return forge_set_error(FORGE_ERR_INVALID, "policy_loss: reduction %d", reduction);
+  if (int rc = check_given("policy_loss", {loss, work})) return rc;
+  if (n * s > 0)
+    if (int rc = check_given("policy_loss", {logits, target, advantages, logps, kl})) return rc;
   const Layout l(dtype, n, s, v);
   const Work w = l.work(work, logps, (float2*)((char*)work + l.state));
   const Policy p = {advantages, a_n, a_s, old_logps, o_n, o_s, ref_logps, r_n, r_s, 1.0 - clip_low, 1.0 + clip_high,

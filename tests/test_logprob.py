@@ -215,7 +215,12 @@ def test_c_entry_errors():
     assert L.forge_preference_fwd(*rows(n=0), *pref) == 1 and b"no pairs" in L.forge_last_error()
     assert L.forge_preference_fwd(*rows(), None, 0.1, 0.0, 3, 0, 1, *pref[6:]) == 1 and b"kind" in L.forge_last_error()
     assert L.forge_preference_fwd(*rows(), None, 0.1, 0.0, 0, 0, 3, *pref[6:]) == 1
+    assert L.forge_token_logps_fwd(*rows(), 1.0, None, None, 16, None) == 1 and b"NULL" in L.forge_last_error()
+    assert L.forge_token_logps_bwd(*rows(), 1.0, 16, None, 16, 3, 1, None, 0, 1, 16, 24, 8, None) == 1
+    assert L.forge_preference_fwd(*rows(), *pref[:-2], None, None) == 1 and b"NULL" in L.forge_last_error()
     none = (None, 0, 0)
+    rc = L.forge_policy_loss(*rows(), 1.0, None, 1, 0, *none, *none, 0.2, 0.2, 0.0, 1, 16, 16, 16, None, 0, 0, 16, None)
+    assert rc == 1 and b"NULL" in L.forge_last_error()
     rc = L.forge_policy_loss(*rows(), 1.0, 16, 1, 0, *none, *none, 0.2, 0.2, 0.0, 0, 16, 16, 16, None, 0, 0, 16, None)
     assert rc == 1 and b"reduction" in L.forge_last_error()
 
