@@ -41,6 +41,7 @@
 namespace {
 
 constexpr int kBlock = 256;
+constexpr int kWave = 64;
 constexpr int kU = 4;                   // vectors in flight per thread (2: the same; 8: 5% slower, 20% at 512 rows of 32000)
 constexpr int kMaxSplits = 64;          // pieces of a row
 constexpr int64_t kMaxGrid = 1 << 22;   // workgroups of a launch; more work loops
@@ -218,15 +219,15 @@ __device__ void count_tokens(const Rows& a, int* counts) {
 // ---------------------------------------------------------------------------
 // reference and sum of a piece of a row
 // ---------------------------------------------------------------------------
-template <class T>
-__global__ __launch_bounds__(kBlock) void lp_partial_kernel(Rows a, Work w, bool count) {
+template <class T, int NT>
+__global__ __launch_bounds__(NT) void lp_partial_kernel(Rows a, Work w, bool count) {
   constexpr int VEC = 16 / sizeof(T);
-  __shared__ float red[kBlock / 64];
+  __shared__ float red[NT / 64];
   const int tid = threadIdx.x;
   int64_t first = blockIdx.x, step = gridDim.x;
   if (count) {  // workgroup 0 counts
     if (blockIdx.x == 0) {
-      count_tokens<kBlock>(a, w.counts);
+      count_tokens<NT>(a, w.counts);
       return;
     }
     first -= 1;
@@ -257,10 +258,10 @@ __global__ __launch_bounds__(kBlock) void lp_partial_kernel(Rows a, Work w, bool
       d += sum_exp2(v, m == -INFINITY ? 0.f : m, a);
     };
     int64_t c = lo;
-    for (; c + kBlock * kU <= hi; c += kBlock * kU) {
+    for (; c + NT * kU <= hi; c += NT * kU) {
       Vec16<T> t[kU];
 #pragma unroll
-      for (int u = 0; u < kU; ++u) t[u] = load_any<T, false>(x + (c + u * kBlock + tid) * VEC);
+      for (int u = 0; u < kU; ++u) t[u] = load_any<T, false>(x + (c + u * NT + tid) * VEC);
       float v[kU * VEC];
 #pragma unroll
       for (int u = 0; u < kU; ++u)
@@ -268,7 +269,7 @@ __global__ __launch_bounds__(kBlock) void lp_partial_kernel(Rows a, Work w, bool
         for (int j = 0; j < VEC; ++j) v[u * VEC + j] = to_f32(t[u].v[j]);
       take(v);
     }
-    for (c += tid; c < hi; c += kBlock) {
+    for (c += tid; c < hi; c += NT) {
       const Vec16<T> t = load_any<T, false>(x + c * VEC);
       float v[VEC];
 #pragma unroll
@@ -279,8 +280,8 @@ __global__ __launch_bounds__(kBlock) void lp_partial_kernel(Rows a, Work w, bool
       float v[1] = {to_f32(x[nvec * VEC + tid])};
       take(v);
     }
-    const float to = block_largest<kBlock>(m, red);
-    d = block_total<float, kBlock>(d * factor_to(m, to, a), red);
+    const float to = block_largest<NT>(m, red);
+    d = block_total<float, NT>(d * factor_to(m, to, a), red);
     if (tid == 0) w.part[i] = make_float2(to, d);
   }
 }
@@ -495,15 +496,15 @@ __device__ void sum_rows(const double* rows, int64_t n, float* sum, double* red)
   if (threadIdx.x == 0) *sum = (float)t;
 }
 
-template <class T>
-__global__ __launch_bounds__(kBlock) void lp_grad_kernel(Rows a, Grad g, int64_t chunks) {
+template <class T, int NT>
+__global__ __launch_bounds__(NT) void lp_grad_kernel(Rows a, Grad g, int64_t chunks) {
   constexpr int VEC = 16 / sizeof(T);
   const int tid = threadIdx.x;
   int64_t first = blockIdx.x, step = gridDim.x;
   if (g.sum) {
     if (blockIdx.x == 0) {
-      __shared__ double red[kBlock / 64];
-      sum_rows<kBlock>(g.rows64, a.n * a.s, g.sum, red);
+      __shared__ double red[NT / 64];
+      sum_rows<NT>(g.rows64, a.n * a.s, g.sum, red);
       return;
     }
     first -= 1;
@@ -523,14 +524,14 @@ __global__ __launch_bounds__(kBlock) void lp_grad_kernel(Rows a, Grad g, int64_t
       if (!in_vocab(a, y)) c = __builtin_nanf("");
     }
     const int64_t nvec = a.v / VEC;
-    const int64_t c0 = chunk * (kBlock * kGradVec);
+    const int64_t c0 = chunk * (NT * kGradVec);
     const bool last = chunk == chunks - 1;
     if (c == 0.f) {  // nothing to read
       Vec16<T> z;
       z.raw = make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int u = 0; u < kGradVec; ++u)
-        if (const int64_t at = c0 + u * kBlock + tid; at < nvec) store_any(o + at * VEC, z);
+        if (const int64_t at = c0 + u * NT + tid; at < nvec) store_any(o + at * VEC, z);
       if (last && nvec * VEC + tid < a.v) o[nvec * VEC + tid] = from_f32<T>(0.f);
       continue;
     }
@@ -540,10 +541,10 @@ __global__ __launch_bounds__(kBlock) void lp_grad_kernel(Rows a, Grad g, int64_t
     Vec16<T> t[kGradVec];
 #pragma unroll
     for (int u = 0; u < kGradVec; ++u)
-      if (const int64_t at = c0 + u * kBlock + tid; at < nvec) t[u] = load_any<T, true>(x + at * VEC);
+      if (const int64_t at = c0 + u * NT + tid; at < nvec) t[u] = load_any<T, true>(x + at * VEC);
 #pragma unroll
     for (int u = 0; u < kGradVec; ++u) {
-      const int64_t at = c0 + u * kBlock + tid;
+      const int64_t at = c0 + u * NT + tid;
       if (at >= nvec) continue;
       const int64_t hit = y - at * VEC;
 #pragma unroll
@@ -565,8 +566,9 @@ __global__ __launch_bounds__(kBlock) void lp_grad_kernel(Rows a, Grad g, int64_t
 // ---------------------------------------------------------------------------
 // policy loss with a row held on chip
 //
-// One 512-thread workgroup a row of 16-bit logits, which is read once and
-// written once: thread t owns the 16-byte vectors t + 512 i, the first NL in LDS
+// One workgroup a row of 16-bit logits (512 threads; a wave where many rows are
+// short), which is read once and written once: thread t of NT owns the 16-byte
+// vectors t + NT i, the first NL in LDS
 // (filled by loads that go there by themselves), the others in registers (8 + 24
 // vectors: 131072 columns, two workgroups on a CU; one computes while the other
 // loads or stores).
@@ -585,7 +587,7 @@ __global__ __launch_bounds__(kBlock) void lp_grad_kernel(Rows a, Grad g, int64_t
 // values that differ are then 2^18 apart or more in the exponent, so a power of
 // two in place of k, whose products are exact, gives the same 1 or 0.
 // ---------------------------------------------------------------------------
-constexpr int kRow = 512;
+constexpr int kRow = 512;  // threads of a row
 
 typedef short short2_t __attribute__((ext_vector_type(2)));
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
@@ -598,24 +600,24 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t row_rsrc(const void* base, uin
                                            0x00020000);
 }
 
-template <class T, int NL, int NR>
-__global__ __launch_bounds__(kRow) __attribute__((amdgpu_waves_per_eu(NR > 8 ? 4 : 6))) void lp_policy_kernel(
+template <class T, int NT, int NL, int NR>
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NR > 8 ? 4 : 6))) void lp_policy_kernel(
     Rows a, Work w, Policy p, Grad g) {
   constexpr int VEC = 16 / sizeof(T);
-  __shared__ __attribute__((aligned(16))) uint4 lds[NL > 0 ? NL * kRow : 1];
-  __shared__ float red[kRow / 64], say[2];
+  __shared__ __attribute__((aligned(16))) uint4 lds[NL > 0 ? NL * NT : 1];
+  __shared__ float red[NT / 64], say[2];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t row = blockIdx.x, n = row / a.s, s = row - n * a.s;
   const int64_t y = a.target[n * a.tn + s * a.ts];
   const T* x = (const T*)a.x + (n * a.xn + s * a.xs);
   T* o = (T*)g.out + (n * g.on + s * g.os);
   const int nvec = (int)(a.v / VEC), tail = (int)(a.v - (int64_t)nvec * VEC);
-  auto on = [&](int i) { return tid < nvec - i * kRow; };
+  auto on = [&](int i) { return tid < nvec - i * NT; };
   auto fill = [&](float f) {
     Vec16<T> z;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) z.v[j] = from_f32<T>(f);
-    for (int i = tid; i < nvec; i += kRow) store_any(o + (int64_t)i * VEC, z);
+    for (int i = tid; i < nvec; i += NT) store_any(o + (int64_t)i * VEC, z);
     if (tid < tail) o[(int64_t)nvec * VEC + tid] = from_f32<T>(f);
   };
   if (y == a.ignore || !in_vocab(a, y)) {
@@ -636,15 +638,15 @@ __global__ __launch_bounds__(kRow) __attribute__((amdgpu_waves_per_eu(NR > 8 ? 4
     for (int i = 0; i < NL; ++i)
       if (on(i)) {
         __attribute__((address_space(3))) char* dst =
-            (__attribute__((address_space(3))) char*)lds + (i * (kRow / 64) + wave) * 1024;
+            (__attribute__((address_space(3))) char*)lds + (i * (NT / 64) + wave) * 1024;
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)dst, 16, (uint32_t)tid * 16u,
-                                                 i * kRow * 16, 0, 2);
+                                                 i * NT * 16, 0, 2);
       }
   }
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
     reg[i] = make_uint4(0, 0, 0, 0);
-    if (on(NL + i)) reg[i] = load_any<T, true>(x + ((int64_t)(NL + i) * kRow + tid) * VEC).raw;
+    if (on(NL + i)) reg[i] = load_any<T, true>(x + ((int64_t)(NL + i) * NT + tid) * VEC).raw;
   }
   const float last = tid < tail ? to_f32(x[(int64_t)nvec * VEC + tid]) : -INFINITY;
   const float xy = to_f32(x[y]);
@@ -656,7 +658,7 @@ __global__ __launch_bounds__(kRow) __attribute__((amdgpu_waves_per_eu(NR > 8 ? 4
   auto each = [&](auto f) {  // f(vector, its index)
 #pragma unroll 1
     for (int i = 0; i < NL; ++i)
-      if (on(i)) f(mine[i * kRow], i);
+      if (on(i)) f(mine[i * NT], i);
 #pragma unroll
     for (int i = 0; i < NR; ++i)
       if (on(NL + i)) f(reg[i], NL + i);
@@ -678,7 +680,7 @@ __global__ __launch_bounds__(kRow) __attribute__((amdgpu_waves_per_eu(NR > 8 ? 4
   });
   const short top = mi.x > mi.y ? mi.x : mi.y;
   float m = top >= 0 ? to_f32(__builtin_bit_cast(T, top)) : -INFINITY;
-  m = block_largest<kRow>(fmaxf(m, last), red);
+  m = block_largest<NT>(fmaxf(m, last), red);
   if (m < 0.f) {  // nothing that is not negative but perhaps in the tail
     each([&](const uint4& r, int) {
       float v[VEC];
@@ -686,7 +688,7 @@ __global__ __launch_bounds__(kRow) __attribute__((amdgpu_waves_per_eu(NR > 8 ? 4
 #pragma unroll
       for (int j = 0; j < VEC; ++j) m = fmaxf(m, v[j]);
     });
-    m = block_largest<kRow>(m, red);
+    m = block_largest<NT>(m, red);
   }
   float k = a.k, mk = m * k;
   const bool far = fabsf(mk) >= 0x1p29f && fabsf(m) < INFINITY;
@@ -708,7 +710,7 @@ __global__ __launch_bounds__(kRow) __attribute__((amdgpu_waves_per_eu(NR > 8 ? 4
       for (int j = 0; j < h; ++j) v[j] += v[j + h];
     d += v[0];
   });
-  d = block_total<float, kRow>(d, red);
+  d = block_total<float, NT>(d, red);
 
   // C
   if (tid == 0) {
@@ -739,12 +741,12 @@ __global__ __launch_bounds__(kRow) __attribute__((amdgpu_waves_per_eu(NR > 8 ? 4
     Vec16<T> t;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) t.v[j] = from_f32<T>(scale * fast_exp2(fmaf(v[j], k, -mk)));
-    store_any(o + ((int64_t)i * kRow + tid) * VEC, t);
+    store_any(o + ((int64_t)i * NT + tid) * VEC, t);
   });
   if (tid < tail) o[(int64_t)nvec * VEC + tid] = from_f32<T>(scale * fast_exp2(fmaf(last, k, -mk)));
   // the target's column by the thread that has stored it, after that store
   const int64_t yv = y / VEC;
-  if (yv < nvec ? (int)(yv % kRow) == tid : (int)(y - (int64_t)nvec * VEC) == tid) o[y] = from_f32<T>(at_y);
+  if (yv < nvec ? (int)(yv % NT) == tid : (int)(y - (int64_t)nvec * VEC) == tid) o[y] = from_f32<T>(at_y);
 }
 
 __global__ __launch_bounds__(1024) void lp_count_kernel(Rows a, int* counts) { count_tokens<1024>(a, counts); }
@@ -763,7 +765,7 @@ int vec_of(int dtype) { return (int)(16 / dtype_size(dtype)); }
 // less than a vector a thread.  512 rows of 32000 / 16 of 128256: 13.7 / 9.0 us;
 // with 2 on each CU 14.0 / 8.0, 8 14.9 / 9.0, 16 17.5 / 8.9.
 int splits_for(int64_t rows, int64_t v, int dtype) {
-  const int64_t most = v / ((int64_t)vec_of(dtype) * kBlock);
+  const int64_t most = v / ((int64_t)vec_of(dtype) * kBlock);  // (1 for the rows that a wave takes)
   int64_t s = rows ? (1024 + rows - 1) / rows : 1;
   if (s > most) s = most;
   if (s > kMaxSplits) s = kMaxSplits;
@@ -807,6 +809,17 @@ struct Layout {
   }
 };
 
+// Many rows of few vectors take a workgroup of one wave each.  Measured on
+// MI355X, bf16, log-probabilities / gradient / policy loss with 256 (512) threads
+// and with 64: 32768 (policy 16384) rows of 1003 77 / 73 / 87 us and 33 / 37 / 33;
+// of 4096 95 / 101 / 99 and 58 / 88 / 56; 16384 of 8192 68 / 89 / 118 and 56 / 86
+// / 106.  64 rows of 4000: 6.4 / 4.1 and 7.3 / 4.8.
+constexpr int kSmallVecs = 1024, kSmallRows = 512;
+
+bool small_rows(int dtype, const Rows& a) {
+  return a.v / vec_of(dtype) <= kSmallVecs && a.n * a.s >= kSmallRows;
+}
+
 unsigned capped(int64_t blocks) { return (unsigned)(blocks > kMaxGrid ? kMaxGrid : blocks); }
 
 int check_rows(const char* what, int dtype, const Rows& a, double temperature) {
@@ -842,7 +855,8 @@ int launch_partial(int dtype, const Rows& a, const Work& w, bool count, hipStrea
   const unsigned grid = capped(a.n * a.s * w.splits) + (count ? 1u : 0u);
   return by_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    lp_partial_kernel<T><<<grid, kBlock, 0, s>>>(a, w, count);
+    if (small_rows(dtype, a)) lp_partial_kernel<T, kWave><<<grid, kWave, 0, s>>>(a, w, count);
+    else lp_partial_kernel<T, kBlock><<<grid, kBlock, 0, s>>>(a, w, count);
   });
 }
 
@@ -857,13 +871,14 @@ int launch_rows(int dtype, const Rows& a, const Work& w, const Policy* p, hipStr
 }
 
 int launch_grad(int dtype, const Rows& a, const Grad& g, bool rows, hipStream_t s) {
-  const int64_t per = (int64_t)vec_of(dtype) * kBlock * kGradVec;
+  const bool small = small_rows(dtype, a);
+  const int64_t per = (int64_t)vec_of(dtype) * (small ? kWave : kBlock) * kGradVec;
   const int64_t chunks = (a.v + per - 1) / per;
-  Rows r = a;
   const unsigned grid = (rows ? capped(a.n * a.s * chunks) : 0u) + (g.sum ? 1u : 0u);
   return by_dtype(dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    lp_grad_kernel<T><<<grid, kBlock, 0, s>>>(r, g, chunks);
+    if (small) lp_grad_kernel<T, kWave><<<grid, kWave, 0, s>>>(a, g, chunks);
+    else lp_grad_kernel<T, kBlock><<<grid, kBlock, 0, s>>>(a, g, chunks);
   });
 }
 
@@ -878,17 +893,20 @@ constexpr int64_t kResidentRows = 256;
 template <class T>
 bool launch_policy(const Rows& a, const Work& w, const Policy& p, const Grad& g, hipStream_t s) {
   if constexpr (sizeof(T) == 2) {
-    const int64_t rows = a.n * a.s, per = (a.v / 8 + kRow - 1) / kRow;  // vectors of a thread
+    const int64_t rows = a.n * a.s, nvec = a.v / 8, per = (nvec + kRow - 1) / kRow;  // vectors of a thread
     if (rows < kResidentRows || rows > kMaxGrid || per > 32) return false;
     const bool aligned = aligned16(a.x) && a.xn % 8 == 0 && a.xs % 8 == 0;
     if (per > 16 && !aligned) return false;
     const unsigned grid = (unsigned)rows;
     lp_count_kernel<<<1, 1024, 0, s>>>(a, w.counts);
-    if (per <= 4) lp_policy_kernel<T, 0, 4><<<grid, kRow, 0, s>>>(a, w, p, g);
-    else if (per <= 8) lp_policy_kernel<T, 0, 8><<<grid, kRow, 0, s>>>(a, w, p, g);
-    else if (per <= 16) lp_policy_kernel<T, 0, 16><<<grid, kRow, 0, s>>>(a, w, p, g);
-    else if (per <= 24) lp_policy_kernel<T, 8, 16><<<grid, kRow, 0, s>>>(a, w, p, g);
-    else lp_policy_kernel<T, 8, 24><<<grid, kRow, 0, s>>>(a, w, p, g);
+    const bool small = nvec <= kSmallVecs && rows >= kSmallRows;
+    if (small && nvec <= 8 * kWave) lp_policy_kernel<T, kWave, 0, 8><<<grid, kWave, 0, s>>>(a, w, p, g);
+    else if (small) lp_policy_kernel<T, kWave, 0, 16><<<grid, kWave, 0, s>>>(a, w, p, g);
+    else if (per <= 4) lp_policy_kernel<T, kRow, 0, 4><<<grid, kRow, 0, s>>>(a, w, p, g);
+    else if (per <= 8) lp_policy_kernel<T, kRow, 0, 8><<<grid, kRow, 0, s>>>(a, w, p, g);
+    else if (per <= 16) lp_policy_kernel<T, kRow, 0, 16><<<grid, kRow, 0, s>>>(a, w, p, g);
+    else if (per <= 24) lp_policy_kernel<T, kRow, 8, 16><<<grid, kRow, 0, s>>>(a, w, p, g);
+    else lp_policy_kernel<T, kRow, 8, 24><<<grid, kRow, 0, s>>>(a, w, p, g);
     lp_sum_kernel<<<1, 1024, 0, s>>>(w.row64, rows, g.sum);
     return true;
   }
