@@ -18,6 +18,11 @@
 // heads of 128, nothing cached: forward 63 us (5.3 TB/s; a copy 5.8), backward
 // 92 us without and 102 us with the weights' gradients (5.5 and 4.9 TB/s).
 //
+// A head_dim whose half is no power of two of 16 bytes leaves lanes idle (96: 6 of
+// 8, 4.2 TB/s both ways; 80: 5 of 8, 3.4), one whose half is no multiple of 16
+// bytes (72: 2.1 TB/s), or a tensor off 16 bytes, takes 8 columns a lane at any
+// alignment and the last lane's one by one (all of them one by one: 0.6).
+//
 // Weight gradients: a workgroup adds up its heads in registers and writes one
 // row of partial sums, so there are few of them, each with the same share of
 // the heads: 768 (3 per CU, what the registers of two heads allow) 102 us; 1024
@@ -78,43 +83,50 @@ __device__ __forceinline__ float head_sum(float v, int lanes) {
   return v;
 }
 
-// A lane's values of one half of a head.  VEC: 16 bytes at column c * E;
-// otherwise (unaligned, or a half that is no multiple of 16 bytes) elements c,
-// c + L, ...
+// 16 bytes at an address that is a multiple of the element only (global memory
+// takes them at any)
+typedef unsigned int u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+
+// A lane's values of one half of a head: E columns at c * E.  VEC: 16 aligned
+// bytes, and every lane's columns are there.  Otherwise (tensors off 16 bytes, or
+// a half that is no multiple of 16 bytes) 8 columns, of which the last lane may
+// have fewer.
 template <class T, bool VEC>
 struct Lane {
   static constexpr int E = VEC ? 16 / (int)sizeof(T) : 8;
-  int c, lanes, half;
-  __device__ __forceinline__ int col(int j) const { return VEC ? c * E + j : c + j * lanes; }
-  __device__ __forceinline__ bool on(int j) const { return col(j) < half; }
+  int c, half;
+  __device__ __forceinline__ bool on(int j) const { return VEC || c * E + j < half; }
+  __device__ __forceinline__ bool full() const { return VEC || c * E + E <= half; }
 
   // The values as they are in memory (cos and sin may be of another type TC).
   template <class S, bool NT>
   struct Raw {
     static constexpr int PER = 16 / (int)sizeof(S);
-    Vec16<S> v[VEC ? E / PER : 1];
-    S e[VEC ? 1 : E];
+    Vec16<S> v[E / PER];
   };
   template <class S, bool NT>
   __device__ __forceinline__ void load(const S* p, Raw<S, NT>& r) const {
-    if constexpr (VEC) {
+    constexpr int PER = Raw<S, NT>::PER;
+    p += c * E;
+    if (full()) {
 #pragma unroll
-      for (int k = 0; k < E / Raw<S, NT>::PER; ++k) {
-        const S* q = p + c * E + k * Raw<S, NT>::PER;
-        r.v[k] = NT ? load16_nt(q) : load16(q);
+      for (int k = 0; k < E / PER; ++k) {
+        if constexpr (VEC) {
+          r.v[k] = NT ? load16_nt(p + k * PER) : load16(p + k * PER);
+        } else {
+          const u32x4_any w = *reinterpret_cast<const u32x4_any*>(p + k * PER);
+          r.v[k].raw = make_uint4(w.x, w.y, w.z, w.w);
+        }
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < E; ++j) r.e[j] = on(j) ? p[col(j)] : from_f32<S>(0.f);
+      for (int j = 0; j < E; ++j) r.v[j / PER].v[j % PER] = on(j) ? p[j] : from_f32<S>(0.f);
     }
   }
   template <class S, bool NT>
   __device__ __forceinline__ void values(const Raw<S, NT>& r, float (&v)[E]) const {
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      if constexpr (VEC) v[j] = to_f32(r.v[j / Raw<S, NT>::PER].v[j % Raw<S, NT>::PER]);
-      else v[j] = to_f32(r.e[j]);
-    }
+    for (int j = 0; j < E; ++j) v[j] = to_f32(r.v[j / Raw<S, NT>::PER].v[j % Raw<S, NT>::PER]);
   }
   template <class S>
   __device__ __forceinline__ void plus(const S* p, float offset, float (&v)[E]) const {
@@ -130,33 +142,43 @@ struct Lane {
     else plus((const float*)w + first, offset, v);
   }
   __device__ __forceinline__ void store(T* p, const float (&v)[E]) const {
-    if constexpr (VEC) {
-      Vec16<T> t;
+    constexpr int PER = 16 / (int)sizeof(T);
+    Vec16<T> t[E / PER];
 #pragma unroll
-      for (int j = 0; j < E; ++j) t.v[j] = from_f32<T>(v[j]);
-      store16_nt(p + c * E, t);
+    for (int j = 0; j < E; ++j) t[j / PER].v[j % PER] = from_f32<T>(v[j]);
+    p += c * E;
+    if (full()) {
+#pragma unroll
+      for (int k = 0; k < E / PER; ++k) {
+        if constexpr (VEC) {
+          store16_nt(p + k * PER, t[k]);
+        } else {
+          const u32x4_any w = {t[k].raw.x, t[k].raw.y, t[k].raw.z, t[k].raw.w};
+          *reinterpret_cast<u32x4_any*>(p + k * PER) = w;
+        }
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < E; ++j)
-        if (on(j)) p[col(j)] = from_f32<T>(v[j]);
+        if (on(j)) p[j] = t[j / PER].v[j % PER];
     }
   }
 };
 
-template <class T, class TC, bool VEC, bool BWD, bool DW, bool LATE>
+template <class T, class TC, bool VEC, bool SEQ, bool BWD, bool DW, bool LATE>
 __global__ __launch_bounds__(kBlock) void qk_norm_rope_kernel(Args a) {
   using LaneT = Lane<T, VEC>;
   using X = typename LaneT::template Raw<T, true>;
   using C = typename LaneT::template Raw<TC, false>;
   constexpr int E = LaneT::E;
-  constexpr int HEADS = VEC ? kHeads : 1;
+  constexpr int HEADS = kHeads;
   extern __shared__ float lds[];  // DW: [waves][D]
   const bool is_k = blockIdx.x >= a.q.blocks;
   const Side& s = is_k ? a.k : a.q;
   const uint32_t block = is_k ? blockIdx.x - a.q.blocks : blockIdx.x;
   const int lanes = a.lanes, half = a.half;
-  const LaneT lane{(int)threadIdx.x & (lanes - 1), lanes, half};
-  const bool active = VEC ? lane.c * E < half : lane.c < half;
+  const LaneT lane{(int)threadIdx.x & (lanes - 1), half};
+  const bool active = lane.c * E < half;
   const uint32_t per_block = kBlock / lanes, step = s.blocks * per_block;
   const uint32_t groups = (s.heads + HEADS - 1) / HEADS, items = s.tokens * groups;
 
@@ -170,8 +192,18 @@ __global__ __launch_bounds__(kBlock) void qk_norm_rope_kernel(Args a) {
   for (int j = 0; j < E; ++j) al[j] = ah[j] = 0.f;
 
   for (uint32_t item = block * per_block + threadIdx.x / lanes; item < items; item += step) {
-    const uint32_t t = item / groups, h0 = (item - t * groups) * HEADS;
-    const uint32_t b = t / a.seq_len, sq = t - b * a.seq_len;
+    uint32_t b, sq, h0;
+    if constexpr (SEQ) {
+      const uint32_t r = item / a.seq_len;
+      sq = item - r * a.seq_len;
+      b = r / groups;
+      h0 = (r - b * groups) * HEADS;
+    } else {
+      const uint32_t r = item / groups;
+      h0 = (item - r * groups) * HEADS;
+      b = r / a.seq_len;
+      sq = r - b * a.seq_len;
+    }
     X rl[HEADS] = {}, rh[HEADS] = {}, dl[HEADS] = {}, dh[HEADS] = {};
     C rc = {}, rs = {};
     const T* x = (const T*)s.x + ((int64_t)b * s.xv.sb + (int64_t)h0 * s.xv.sh + (int64_t)sq * s.xv.ss);
@@ -190,7 +222,7 @@ __global__ __launch_bounds__(kBlock) void qk_norm_rope_kernel(Args a) {
           lane.load(dy + u * s.dv.sh + half, dh[u]);
         }
     }
-    const int64_t pos = a.positions ? a.positions[t] : (int64_t)sq;
+    const int64_t pos = a.positions ? a.positions[(int64_t)b * a.seq_len + sq] : (int64_t)sq;
     const bool in_table = pos >= 0 && pos < a.table_rows;
     if (active && in_table) {
       lane.load((const TC*)a.cos + ((int64_t)b * a.cos_sb + pos * a.cos_ss), rc);
@@ -272,8 +304,8 @@ __global__ __launch_bounds__(kBlock) void qk_norm_rope_kernel(Args a) {
 #pragma unroll
       for (int j = 0; j < E; ++j)
         if (lane.on(j)) {
-          lds[wave * 2 * half + lane.col(j)] = al[j];
-          lds[wave * 2 * half + half + lane.col(j)] = ah[j];
+          lds[wave * 2 * half + lane.c * E + j] = al[j];
+          lds[wave * 2 * half + half + lane.c * E + j] = ah[j];
         }
     }
     __syncthreads();
@@ -314,10 +346,9 @@ __global__ __launch_bounds__(1024) void qk_dweight_kernel(const float* qp, uint3
   }
 }
 
-int lanes_for(int64_t half, bool vec, size_t es) {
-  const int64_t chunks = vec ? half * (int64_t)es / 16 : half;
+int lanes_for(int64_t half, int64_t each) {
   int lanes = 1;
-  while (lanes < chunks && lanes < 64) lanes <<= 1;
+  while (lanes * each < half) lanes <<= 1;
   return lanes;
 }
 
@@ -341,21 +372,22 @@ void split_blocks(Args& a, int heads_each, uint64_t cap) {
 // does not matter, and the test in the loop costs 3 us of 63 ([4, 4096]).
 constexpr uint32_t kFewBlocks = 1024;
 
-template <class T, class TC, bool VEC, bool BWD>
-void launch_vec(const Args& a, uint32_t blocks, size_t lds, hipStream_t s) {
+template <class T, class TC, bool VEC, bool SEQ, bool BWD>
+void launch_as(const Args& a, uint32_t blocks, size_t lds, hipStream_t s) {
   if constexpr (BWD) {
-    if (lds) qk_norm_rope_kernel<T, TC, VEC, true, true, true><<<blocks, kBlock, lds, s>>>(a);
-    else qk_norm_rope_kernel<T, TC, VEC, true, false, false><<<blocks, kBlock, 0, s>>>(a);
+    if (lds) qk_norm_rope_kernel<T, TC, VEC, SEQ, true, true, true><<<blocks, kBlock, lds, s>>>(a);
+    else qk_norm_rope_kernel<T, TC, VEC, SEQ, true, false, false><<<blocks, kBlock, 0, s>>>(a);
   } else {
-    if (blocks <= kFewBlocks) qk_norm_rope_kernel<T, TC, VEC, false, false, true><<<blocks, kBlock, 0, s>>>(a);
-    else qk_norm_rope_kernel<T, TC, VEC, false, false, false><<<blocks, kBlock, 0, s>>>(a);
+    if (blocks <= kFewBlocks) qk_norm_rope_kernel<T, TC, VEC, SEQ, false, false, true><<<blocks, kBlock, 0, s>>>(a);
+    else qk_norm_rope_kernel<T, TC, VEC, SEQ, false, false, false><<<blocks, kBlock, 0, s>>>(a);
   }
 }
 
 template <class T, class TC, bool BWD>
-void launch(const Args& a, bool vec, uint32_t blocks, size_t lds, hipStream_t s) {
-  if (vec) launch_vec<T, TC, true, BWD>(a, blocks, lds, s);
-  else launch_vec<T, TC, false, BWD>(a, blocks, lds, s);
+void launch(const Args& a, bool vec, bool seq_first, uint32_t blocks, size_t lds, hipStream_t s) {
+  if (!vec) launch_as<T, TC, false, false, BWD>(a, blocks, lds, s);
+  else if (seq_first) launch_as<T, TC, true, true, BWD>(a, blocks, lds, s);
+  else launch_as<T, TC, true, false, BWD>(a, blocks, lds, s);
 }
 
 template <bool BWD>
@@ -394,7 +426,7 @@ int run(int dtype, const char* what, Args& a, int w_dtype, int table_dtype, int6
       for (int64_t st : {s->dv.sb, s->dv.sh, s->dv.ss}) vec = vec && st % V == 0;
   }
   for (int64_t st : {a.cos_sb, a.cos_ss, a.sin_sb, a.sin_ss}) vec = vec && st % Vt == 0;
-  a.lanes = lanes_for(a.half, vec, es);
+  a.lanes = lanes_for(a.half, vec ? V : 8);
   a.seq_len = (uint32_t)seq_len;
   a.eps = (float)eps;
   a.offset = (float)offset;
@@ -402,10 +434,14 @@ int run(int dtype, const char* what, Args& a, int w_dtype, int table_dtype, int6
   a.w_dtype = w_dtype;
   a.q.heads = (uint32_t)n_q;
   a.k.heads = (uint32_t)n_kv;
+  // a wave's heads lie next to each other in memory: heads of a token in [B, S,
+  // H, D] memory, tokens of a head in [B, H, S, D] (bf16 [4, 32 + 8, 7324, 128],
+  // forward / backward: by tokens 105 / 176 us, by heads 128 / 202)
+  const bool seq_first = n_q > 1 && seq_len > 1 && a.q.xv.ss < a.q.xv.sh;
   a.q.tokens = a.k.tokens = (uint32_t)(batch * seq_len);
   hipStream_t s = (hipStream_t)stream;
   const bool dw = dqw || dkw;
-  split_blocks(a, vec ? kHeads : 1, dw ? kDwBlocks : kMaxBlocks);
+  split_blocks(a, kHeads, dw ? kDwBlocks : kMaxBlocks);
   if (dw) {  // both sides' partial sums, one after the other
     a.q.part = dqw ? work : nullptr;
     a.k.part = dkw ? work + (int64_t)a.q.blocks * head_dim : nullptr;
@@ -415,14 +451,14 @@ int run(int dtype, const char* what, Args& a, int w_dtype, int table_dtype, int6
     const size_t lds = dw ? (kBlock / 64) * (size_t)head_dim * sizeof(float) : 0;
     const bool f32_table = table_dtype != dtype;
     switch (dtype) {
-      case FORGE_DTYPE_F32: launch<float, float, BWD>(a, vec, blocks, lds, s); break;
+      case FORGE_DTYPE_F32: launch<float, float, BWD>(a, vec, seq_first, blocks, lds, s); break;
       case FORGE_DTYPE_BF16:
-        if (f32_table) launch<bf16_t, float, BWD>(a, vec, blocks, lds, s);
-        else launch<bf16_t, bf16_t, BWD>(a, vec, blocks, lds, s);
+        if (f32_table) launch<bf16_t, float, BWD>(a, vec, seq_first, blocks, lds, s);
+        else launch<bf16_t, bf16_t, BWD>(a, vec, seq_first, blocks, lds, s);
         break;
       default:
-        if (f32_table) launch<fp16_t, float, BWD>(a, vec, blocks, lds, s);
-        else launch<fp16_t, fp16_t, BWD>(a, vec, blocks, lds, s);
+        if (f32_table) launch<fp16_t, float, BWD>(a, vec, seq_first, blocks, lds, s);
+        else launch<fp16_t, fp16_t, BWD>(a, vec, seq_first, blocks, lds, s);
     }
     FORGE_CHECK_LAUNCH();
   }
