@@ -23,7 +23,7 @@
 // at any element's address.  Measured on MI355X, nothing cached, forward /
 // backward: bf16 [8192, 14336] silu 161 / 157 us (5.9 / 6.0 TB/s; a copy 5.8),
 // tanh 167 / 165; fp16 [4096, 14337] erf 85 / 89; fp32 [4096, 11008] silu 99 /
-// 99.  With 16 columns a thread the 16-bit backward took 235 us (two stores 32
+// 99.  With 16 columns a thread the 16-bit backward took 237 us (two stores 32
 // bytes apart in place of whole lines); one vector in flight 166 / 158, four
 // 165 / 159; two in fp32 103 / 107.  The forward's arithmetic (two activations'
 // worth) is close behind the memory: testing every value for infinities took

@@ -579,8 +579,9 @@ __global__ __launch_bounds__(NT) void lp_grad_kernel(Rows a, Grad g, int64_t chu
 //   D  the gradient, each exponential again (kept in 16 bits it would be rounded
 //      twice)
 // Measured on MI355X, bf16 [8, 1024, 128256], 66% of the rows kept, nothing
-// cached: 655 us, 5.3 TB/s of reads and writes (a copy 5.8), against 815 us for
-// the passes above, which read those rows twice at 6.0 TB/s.
+// cached, least of 24: 654 us, 5.3 TB/s of reads and writes (a copy 5.8), against
+// 818 us for the passes above, which read those rows twice at 5.9 TB/s (on
+// average 663 and 857).
 // One fma gives x k - m k: what rounding m k leaves is the same factor on every
 // exponential and on d, and the log-probability takes it into account.  Where m k
 // passes 2^29 (a row of a mask's lowest values) that factor could leave fp32;
