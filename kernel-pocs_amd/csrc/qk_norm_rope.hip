@@ -102,13 +102,16 @@ struct Lane {
   template <class S, bool NT>
   struct Raw {
     static constexpr int PER = 16 / (int)sizeof(S);
-    Vec16<S> v[E / PER];
+    Vec16<S> v[E < PER ? 1 : E / PER];
   };
   template <class S, bool NT>
   __device__ __forceinline__ void load(const S* p, Raw<S, NT>& r) const {
     constexpr int PER = Raw<S, NT>::PER;
     p += c * E;
-    if (full()) {
+    if constexpr (E < PER) {  // 16-bit weights of fp32 heads: less than 16 bytes
+#pragma unroll
+      for (int j = 0; j < E; ++j) r.v[0].v[j] = on(j) ? p[j] : from_f32<S>(0.f);
+    } else if (full()) {
 #pragma unroll
       for (int k = 0; k < E / PER; ++k) {
         if constexpr (VEC) {

@@ -188,6 +188,25 @@ def test_layouts(layout, b, nq, nk, s, d, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("wdtype", [BF16, FP16, FP32], ids=str)
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32], ids=str)
+@pytest.mark.parametrize("d", [64, 72, 128, 256])
+def test_weights_of_another_type(d, dtype, wdtype):
+    for layout in ("bshd", "bhsd"):
+        q, k = _make(2, 5, 3, 9, d, dtype, layout)
+        cos, sin = (t.cuda() for t in _cos_sin(9, d, dtype))
+        _check(q, k, *_weights(d, wdtype, 0.0), cos, sin, None, 0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wdtype", [BF16, FP16], ids=str)
+def test_narrow_weights_of_many_tokens(wdtype):
+    q, k = _make(2, 32, 8, 1100, 128, FP32)  # more workgroups than ask for the weights late
+    cos, sin = (t.cuda() for t in _cos_sin(1100, 128, FP32))
+    _check(q, k, *_weights(128, wdtype, 1.0), cos, sin, None, 1.0, train_weights=False)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("batched", [False, True])
 @pytest.mark.parametrize("tdtype", [BF16, FP32], ids=str)
 def test_positions_and_tables(batched, tdtype):
