@@ -923,8 +923,9 @@ Rows make_rows(const void* x, int64_t xn, int64_t xs, int64_t n, int64_t s, int6
 }  // namespace
 
 extern "C" int64_t forge_logp_workspace(int dtype, int64_t n, int64_t s, int64_t v) {
-  if (n <= 0 || s <= 0 || v <= 0 || dtype_size(dtype) == 0) return 16;
-  return Layout(dtype, n, s, v).bytes;
+  if (n <= 0 || dtype_size(dtype) == 0) return 16;
+  // sequences of no tokens have counts and sums all the same
+  return Layout(dtype, n, s > 0 ? s : 0, v > 0 ? v : 0).bytes;
 }
 
 extern "C" int forge_token_logps_fwd(int dtype, const void* logits, int64_t ld_n, int64_t ld_s, int64_t n, int64_t s,
