@@ -585,8 +585,10 @@ __global__ __launch_bounds__(NT) void lp_grad_kernel(Rows a, Grad g, int64_t chu
 // One fma gives x k - m k: what rounding m k leaves is the same factor on every
 // exponential and on d, and the log-probability takes it into account.  Where m k
 // passes 2^29 (a row of a mask's lowest values) that factor could leave fp32;
-// values that differ are then 2^18 apart or more in the exponent, so a power of
-// two in place of k, whose products are exact, gives the same 1 or 0.
+// values that differ are then 2^17 apart or more in the exponent, so a power of
+// two in place of k, whose products are exact, gives the same 1 or 0.  1 does
+// where that product leaves fp32 (bf16 near its largest, t up to 0.72): k is
+// below 2^21, so |m| is 2^107 or more and values that differ are 2^98 apart.
 // ---------------------------------------------------------------------------
 constexpr int kRow = 512;  // threads of a row
 
@@ -695,6 +697,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NR > 8 ? 4 :
   const bool far = fabsf(mk) >= 0x1p29f && fabsf(m) < INFINITY;
   if (far) {
     k = __uint_as_float(__float_as_uint(k) & 0x7f800000);
+    if (!(fabsf(m * k) < INFINITY)) k = 1.f;
     mk = m * k;
   }
 

@@ -45,3 +45,56 @@ def test_preference_of_empty_answers(pairs, normalized, reduction):
     assert ((o.rewards.double().cpu() - rewards).abs() <= rewards.abs() * 2.0 ** -23).all()
     (d,) = torch.autograd.grad(o.loss, x, torch.ones_like(o.loss))
     assert d.shape == x.shape
+
+
+# ---------------------------------------------------------------------------
+# policy rows at a type's extreme values
+# ---------------------------------------------------------------------------
+U = 2.0 ** -24
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("temperature", [1e-6, 0.01, 0.35, 0.7, 0.72, 0.73, 1.0, 3.0, 1e6])
+@pytest.mark.parametrize("s,v", [(4, 2052), (300, 515), (600, 515), (300, 20003), (300, 65544), (300, 131072)])
+def test_policy_rows_at_extreme_values(s, v, temperature, dtype):
+    """Rows of the lowest or the largest value, some with a few at the other end.
+    fp32 within (64 + V / 8192) U for the sum and the logarithm (the exponents
+    are 0 or far below but in fp16 at t = 1e6, where they reach 0.2), 4 U of logp
+    for its product with 1 / t and its rounding; a gradient is rounded to its
+    type once."""
+    from kernels.logprob import forge_policy_loss
+
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    x = torch.zeros(1, s, v, dtype=dtype)
+    y = torch.full((1, s), 3)
+    x[0, 0] = low
+    x[0, 1] = high
+    x[0, 2], x[0, 2, 3] = low, 0.5 * high      # the target is the one above
+    x[0, 3], x[0, 3, v - 1] = low, high        # the target is not
+    if s > 4:
+        x[0, 4], x[0, 4, :5] = low, high       # a few share it
+        x[0, 5], x[0, 5, v // 2:] = high, low
+        x[0, 6], x[0, 6, 9:] = low / 2, low
+        x[0, 7] = low / 4
+        y[0, 8:] = IGNORE
+    n = min(s, 8)
+    lp_all = (x[0, :n].double() / temperature).log_softmax(-1)
+    lp = lp_all[:, 3]
+    hot = torch.zeros_like(lp_all)
+    hot[:, 3] = 1.0
+    grad = lp_all.exp() - hot
+
+    xg = x.cuda().requires_grad_(True)
+    # with an advantage of t a row's gradient is p - onehot
+    o = forge_policy_loss(xg, y.cuda(), torch.full((1,), temperature, device="cuda"), temperature=temperature,
+                          reduction="sum")
+    (got,) = torch.autograd.grad(o.loss, xg)
+    assert (o.logps[0, n:] == 0).all() and (got[0, n:] == 0).all()
+    e = (64 + v / 8192 + 3 * 0.2) * U
+    # equal where a distance / t is past fp32's range
+    off = torch.where(o.logps[0, :n].cpu() == lp.float(), 0.0, (o.logps[0, :n].cpu().double() - lp).abs())
+    assert (off <= e + lp.abs() * 4 * U).all(), off
+    bound = grad.abs() * (torch.finfo(dtype).eps / 2 + 2 * e + 8 * U) + torch.finfo(dtype).smallest_normal
+    assert ((got[0, :n].double().cpu() - grad).abs() <= bound).all()
+    assert abs(o.loss.item() + temperature * n) <= temperature * n * 4 * U  # r = 1
