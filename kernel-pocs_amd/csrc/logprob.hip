@@ -344,9 +344,12 @@ __device__ __forceinline__ void policy_token(const Policy& p, int64_t n, int64_t
   kl = 0.f;
   if (p.ref) {
     const double f = (double)p.ref[n * p.rn + s * p.rs] - lp, e = expm1(f);
-    kl = (float)(e - f);
-    loss += p.beta * (e - f);
-    d -= p.beta * e;
+    const double far = f == INFINITY ? f : e - f;
+    kl = (float)far;
+    if (p.beta != 0.0) {  // (where it is only reported an infinite one may not reach the loss: 0 times it is NaN)
+      loss += p.beta * far;
+      d -= p.beta * e;
+    }
   }
 }
 

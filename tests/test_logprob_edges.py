@@ -98,3 +98,49 @@ def test_policy_rows_at_extreme_values(s, v, temperature, dtype):
     bound = grad.abs() * (torch.finfo(dtype).eps / 2 + 2 * e + 8 * U) + torch.finfo(dtype).smallest_normal
     assert ((got[0, :n].double().cpu() - grad).abs() <= bound).all()
     assert abs(o.loss.item() + temperature * n) <= temperature * n * 4 * U  # r = 1
+
+
+# ---------------------------------------------------------------------------
+# a divergence that is only reported
+# ---------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("s", [6, 300, 600])
+def test_divergence_without_a_weight(s, dtype):
+    """ref_logps with kl_coef = 0 report kl and change nothing else, infinite
+    as it may be: a token that the reference rules out (-inf), one that the
+    policy does, and one that the reference finds e^1000 times likelier."""
+    from kernels.logprob import forge_policy_loss
+
+    g = torch.Generator().manual_seed(s)
+    inf = float("inf")
+    x = torch.randn(1, s, 1000, generator=g).to(dtype)
+    y = torch.randint(0, 1000, (1, s), generator=g)
+    y[0, 5] = IGNORE
+    x[0, 1, y[0, 1]] = -inf
+    ref = torch.full((1, s), -7.0)
+    ref[0, 0], ref[0, 1], ref[0, 2], ref[0, 5] = -inf, -3.0, 1000.0, float("nan")
+    old = torch.full((1, s), -7.5)
+    adv = torch.randn(1, s, generator=g)
+    xg = x.cuda().requires_grad_(True)
+
+    def call(ref, kl_coef=0.0):
+        o = forge_policy_loss(xg, y.cuda(), adv.cuda(), old.cuda(), None if ref is None else ref.cuda(), kl_coef=kl_coef)
+        return o, torch.autograd.grad(o.loss, xg)[0]
+
+    want, dw = call(None)
+    got, d = call(ref)
+    assert want.loss.isfinite() and torch.equal(got.loss, want.loss) and torch.equal(got.logps, want.logps)
+    assert torch.equal(d, dw) and d.isfinite().all() and (want.kl == 0).all()
+    assert (got.kl[0, :3] == inf).all() and got.kl[0, 3:].isfinite().all() and got.kl[0, 5] == 0
+    f = ref[0, 3:5].double() - got.logps[0, 3:5].double().cpu()
+    kl = torch.expm1(f) - f
+    # logps come back rounded (U of themselves), which moves kl by its slope
+    off = (torch.expm1(f).abs() + f.exp() * 1e-6) * got.logps[0, 3:5].double().cpu().abs() * 2.0 ** -23 + kl * 2.0 ** -22
+    assert ((got.kl[0, 3:5].double().cpu() - kl).abs() <= off).all()
+    with torch.no_grad():
+        plain = forge_policy_loss(xg, y.cuda(), adv.cuda(), old.cuda(), ref.cuda())
+    assert plain.loss.isfinite() and (plain.kl[0, :3] == inf).all()
+    # with a weight the loss is infinite, not NaN; a token that the reference rules out keeps a finite gradient
+    weighted, d = call(ref, 0.1)
+    assert weighted.loss == inf and d[0, 0].isfinite().all() and torch.equal(weighted.kl, got.kl)
