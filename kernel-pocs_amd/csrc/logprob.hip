@@ -631,7 +631,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NR > 8 ? 4 :
     if (tid == 0) {
       w.logps[row] = f;
       w.row64[row] = f;
-      p.kl[row] = f;
+      p.kl[row] = p.ref ? f : 0.f;
     }
     fill(f);
     return;

@@ -144,3 +144,19 @@ def test_divergence_without_a_weight(s, dtype):
     # with a weight the loss is infinite, not NaN; a token that the reference rules out keeps a finite gradient
     weighted, d = call(ref, 0.1)
     assert weighted.loss == inf and d[0, 0].isfinite().all() and torch.equal(weighted.kl, got.kl)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("s", [6, 300, 600])
+def test_kl_of_targets_out_of_range(s):
+    """NaN where there is a reference, 0 where there is none, whatever the size
+    of the batch."""
+    from kernels.logprob import forge_policy_loss
+
+    x = torch.randn(1, s, 100).bfloat16().cuda().requires_grad_(True)
+    y = torch.randint(0, 100, (1, s)).cuda()
+    y[0, 1], y[0, 2] = 100, -5
+    ref = torch.full((1, s), -5.0, device="cuda")
+    none, some = (forge_policy_loss(x, y, torch.ones(1, device="cuda"), ref_logps=r) for r in (None, ref))
+    assert (none.kl == 0).all() and none.loss.isnan() and some.loss.isnan()
+    assert some.kl[0, 1:3].isnan().all() and not some.kl[0, 0].isnan() and not some.kl[0, 3:].isnan().any()
