@@ -446,7 +446,8 @@ __global__ __launch_bounds__(kBlock) void lp_pairs_kernel(Pairs p) {
     if (p.kind == FORGE_PREF_SIGMOID) {
       const double tail = log1p(exp(-fabs(h)));
       const double up = tail + (h < 0.0 ? -h : 0.0), down = tail + (h > 0.0 ? h : 0.0);  // -log s(h), -log s(-h)
-      loss = (1.0 - p.smoothing) * up + p.smoothing * down;
+      // (a term of weight 0 may be infinite)
+      loss = (p.smoothing < 1.0 ? (1.0 - p.smoothing) * up : 0.0) + (p.smoothing > 0.0 ? p.smoothing * down : 0.0);
       d = p.beta * (p.smoothing - 1.0 / (1.0 + exp(h)));
     } else if (p.kind == FORGE_PREF_HINGE) {
       loss = h >= 1.0 ? 0.0 : 1.0 - h;  // (a NaN stays)

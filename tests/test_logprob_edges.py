@@ -160,3 +160,33 @@ def test_kl_of_targets_out_of_range(s):
     none, some = (forge_policy_loss(x, y, torch.ones(1, device="cuda"), ref_logps=r) for r in (None, ref))
     assert (none.kl == 0).all() and none.loss.isnan() and some.loss.isnan()
     assert some.kl[0, 1:3].isnan().all() and not some.kl[0, 0].isnan() and not some.kl[0, 3:].isnan().any()
+
+
+# ---------------------------------------------------------------------------
+# answers that the policy rules out
+# ---------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("smoothing,chosen,want", [(0.0, False, 0.0), (0.0, True, float("inf")), (1.0, True, 0.0),
+                                                   (0.1, False, float("inf"))])
+def test_preference_of_answers_ruled_out(smoothing, chosen, want):
+    """A token at -inf makes its answer's log-probability -inf and h infinite:
+    the sigmoid loss of that pair is 0 or infinite (a term of weight 0 is left
+    out: 0 times infinity is NaN), and the other pair's is its own."""
+    from kernels.logprob import forge_preference_loss
+
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(4, 3, 40, generator=g)
+    y = torch.randint(0, 40, (4, 3), generator=g).cuda()
+    xg = x.cuda().requires_grad_(True)
+    clean = forge_preference_loss(xg, y, label_smoothing=smoothing, reduction="none")
+    x[0 if chosen else 2, 1, y[0 if chosen else 2, 1]] = -float("inf")
+    xg = x.cuda().requires_grad_(True)
+    o = forge_preference_loss(xg, y, label_smoothing=smoothing, reduction="none")
+    assert o.loss[0] == want and torch.equal(o.loss[1], clean.loss[1])
+    assert o.logps[0 if chosen else 2] == -float("inf")
+    (d,) = torch.autograd.grad(o.loss, xg, torch.ones_like(o.loss))
+    assert d.isfinite().all()
+    if want == 0.0:
+        assert (d[[0, 2]] == 0).all()
+        mean = forge_preference_loss(xg, y, label_smoothing=smoothing)
+        assert abs(mean.loss.item() - o.loss[1].item() / 2) <= 2.0 ** -23 * o.loss[1].item()
