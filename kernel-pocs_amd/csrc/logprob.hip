@@ -69,17 +69,17 @@ struct Work {
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // 2^(far k): the exponent p = far k is rounded; what that and k_lo leave is
-// added to first order as rest += 2^p (far k - p + far k_lo).
+// added to first order as rest += 2^p (far k - p + far k_lo).  Where 2^p is not
+// 0 that difference is below 2^-16; where p is infinite it is infinite or NaN,
+// and held between -1 and 1 (a NaN gives -1) 2^p = 0 times it is 0, so that
+// masked columns leave the others' rest as it is.
 __device__ __forceinline__ float exp2_rest(float far, float k, float k_lo, float& rest) {
   const float p = far * k, e = fast_exp2(p);
-  rest = fmaf(e, fmaf(far, k_lo, fmaf(far, k, -p)), rest);
+  rest = fmaf(e, __builtin_amdgcn_fmed3f(fmaf(far, k_lo, fmaf(far, k, -p)), -1.f, 1.f), rest);
   return e;
 }
 
-// (an infinite far leaves a NaN rest beside a sum that needs none)
-__device__ __forceinline__ float with_rest(float sum, float rest) {
-  return rest == rest ? fmaf(rest, (float)kLn2, sum) : sum;
-}
+__device__ __forceinline__ float with_rest(float sum, float rest) { return fmaf(rest, (float)kLn2, sum); }
 
 // Sum of 2^((v - at) k) over N values, which are overwritten.  16-bit logits
 // take few values near the maximum, and most rows of a batch have much the same

@@ -190,3 +190,36 @@ def test_preference_of_answers_ruled_out(smoothing, chosen, want):
         assert (d[[0, 2]] == 0).all()
         mean = forge_preference_loss(xg, y, label_smoothing=smoothing)
         assert abs(mean.loss.item() - o.loss[1].item() / 2) <= 2.0 ** -23 * o.loss[1].item()
+
+
+# ---------------------------------------------------------------------------
+# masked columns
+# ---------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=str)
+@pytest.mark.parametrize("rows,v,temperature", [(3, 30011, 1.0), (40, 128256, 0.7), (700, 1003, 1.0), (1100, 5000, 2.0)])
+def test_masked_columns_change_nothing_else(rows, v, temperature, dtype):
+    """Scattered columns at -infinity, at the type's lowest value or at -1e4
+    have no share: the sums over the others, with the corrections of their
+    rounding, are the same bit for bit.  (Targets near probability 1, where a
+    log-probability shows its row's sum to 1e-9.)"""
+    from kernels.logprob import forge_token_logps
+
+    g = torch.Generator().manual_seed(rows)
+    x = torch.randn(1, rows, v, generator=g) * 2
+    y = torch.randint(0, v, (1, rows), generator=g)
+    x.scatter_(-1, y.unsqueeze(-1), 14.0)
+    masked = torch.rand(1, rows, v, generator=g) < 0.1
+    masked.scatter_(-1, y.unsqueeze(-1), False)
+    results = []
+    for value in (-float("inf"), torch.finfo(dtype).min, -1e4):
+        xg = x.masked_fill(masked, value).to(dtype).cuda().requires_grad_(True)
+        lp = forge_token_logps(xg, y.cuda(), temperature=temperature)
+        (d,) = torch.autograd.grad(lp, xg, torch.ones_like(lp))
+        assert (d[masked.cuda()] == 0).all()
+        results.append((lp.detach(), d))
+    want = (x.masked_fill(masked, -float("inf")).to(dtype).double() / temperature).log_softmax(-1)
+    want = want.gather(-1, y.unsqueeze(-1)).squeeze(-1)
+    assert ((results[0][0].double().cpu() - want).abs() <= (64 + v / 8192 + 3 * 30) * U + want.abs() * U).all()
+    for lp, d in results[1:]:
+        assert torch.equal(lp, results[0][0]) and torch.equal(d, results[0][1])
