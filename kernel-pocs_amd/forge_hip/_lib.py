@@ -17,6 +17,7 @@ import os
 from pathlib import Path
 
 import torch  # loads the HIP runtime (libamdhip64.so.7) that the library links against
+import torch.autograd.forward_ad as forward_ad
 
 LIB_PATH = Path(os.environ.get("FORGE_HIP_LIB", Path(__file__).resolve().parent / "libforge_hip.so"))
 
@@ -275,6 +276,15 @@ def on_device(t: torch.Tensor):
     """Makes t's device the current one for a launch (its stream belongs to
     that device); nothing to do where it is already."""
     return _NO_SWITCH if torch._C._cuda_getDevice() == t.device.index else torch.cuda.device(t.device)
+
+
+def refuse_tangents(*tensors) -> None:
+    """For a launch that goes past its autograd Function (which refuses them by
+    itself): a result without its tangent would be a derivative of 0."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("forge_hip operators have no jvp: forward-mode differentiation is not supported")
 
 
 def ptr(t):

@@ -137,6 +137,7 @@ def glu_act8(gate: torch.Tensor, up: torch.Tensor, activation: str = "silu") -> 
     _check_pair(gate, up)
     if torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
         return ForgeGLUAct8Function.apply(gate, up, act)
+    L.refuse_tangents(gate, up)
     return _forward(gate, up, act, keep=False)[0].view(gate.shape)
 
 
@@ -149,6 +150,7 @@ def glu_act8_packed(gate_up: torch.Tensor, activation: str = "silu") -> torch.Te
     L.require_gpu(gate_up)
     if torch.is_grad_enabled() and gate_up.requires_grad:
         return ForgePackedGLUAct8Function.apply(gate_up, act)
+    L.refuse_tangents(gate_up)
     cols = gate_up.shape[-1] // 2
     out, _ = _forward(gate_up[..., :cols], gate_up[..., cols:], act, keep=False)
     return out.view(*gate_up.shape[:-1], cols)

@@ -136,6 +136,7 @@ def forge_policy_loss(logits: torch.Tensor, target: torch.Tensor, advantages: to
             _REDUCTIONS[reduction], int(ignore_index))
     if torch.is_grad_enabled() and logits.requires_grad:
         return PolicyLossOutput(*ForgePolicyLossFunction.apply(x, t, *args, bool(inplace)))
+    L.refuse_tangents(logits)
     return PolicyLossOutput(*_launch(x, t, *args, None))
 
 

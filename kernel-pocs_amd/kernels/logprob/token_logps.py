@@ -63,6 +63,7 @@ def forge_token_logps(logits: torch.Tensor, target: torch.Tensor, ignore_index: 
     if torch.is_grad_enabled() and logits.requires_grad:
         logps = ForgeTokenLogpsFunction.apply(x, t, int(ignore_index), float(temperature))
     else:
+        L.refuse_tangents(logits)
         logps, _ = _forward(x, t, int(ignore_index), float(temperature), keep=False)
     return logps.reshape(target.shape)
 

@@ -164,8 +164,8 @@ def apply_qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
     q, k, q_weight, k_weight = _unit_last(q), _unit_last(k), q_weight.contiguous(), k_weight.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or q_weight.requires_grad
                                     or k_weight.requires_grad):
-        return ForgeQKNormRoPEFunction.apply(q, k, q_weight, k_weight, cos.detach(), sin.detach(), positions, float(eps),
-                                             float(offset))
+        return ForgeQKNormRoPEFunction.apply(q, k, q_weight, k_weight, cos, sin, positions, float(eps), float(offset))
+    L.refuse_tangents(q, k, q_weight, k_weight, cos, sin)
     return _forward(q, k, q_weight, k_weight, cos, sin, positions, float(eps), float(offset))
 
 
