@@ -78,8 +78,9 @@ def target_2d(target: torch.Tensor, dim: int) -> torch.Tensor:
 def check_inplace(logits: torch.Tensor) -> None:
     """The gradient can be written over [N, S, V] logits only where they are an
     operation's result, columns are adjacent and no two elements share memory."""
-    if logits.requires_grad and logits.is_leaf:
-        raise ValueError("inplace needs logits that are not a leaf: their gradient would be themselves")
+    base = logits._base
+    if logits.requires_grad and (logits.is_leaf or base is not None and base.is_leaf and base.requires_grad):
+        raise ValueError("inplace needs logits that are not a leaf, nor a view of one: their gradient would be themselves")
     (n, s, v), (sn, ss, sv) = logits.shape, logits.stride()
     inner, outer = ((s, ss), (n, sn)) if ss <= sn else ((n, sn), (s, ss))
     ok = v <= 1 or sv == 1

@@ -223,3 +223,24 @@ def test_masked_columns_change_nothing_else(rows, v, temperature, dtype):
     assert ((results[0][0].double().cpu() - want).abs() <= (64 + v / 8192 + 3 * 30) * U + want.abs() * U).all()
     for lp, d in results[1:]:
         assert torch.equal(lp, results[0][0]) and torch.equal(d, results[0][1])
+
+
+# ---------------------------------------------------------------------------
+# in place
+# ---------------------------------------------------------------------------
+def test_inplace_of_a_leafs_view_is_refused():
+    """A view of a leaf is the leaf's data, which its gradient may not replace."""
+    from kernels.logprob import forge_policy_loss, forge_preference_loss
+    from kernels.logprob._rows import check_inplace
+
+    leaf, y = torch.zeros(4, 3, 8, requires_grad=True), torch.zeros(4, 3, dtype=torch.long)
+    for view in (leaf, leaf[:], leaf.view(4, 3, 8), leaf[:, :, :5], leaf.transpose(0, 1), leaf[1:].narrow(1, 0, 2),
+                 torch.zeros(5, 3, 8)[1:].requires_grad_(True)):
+        with pytest.raises(ValueError, match="not a leaf"):
+            check_inplace(view)
+    with pytest.raises(ValueError, match="not a leaf"):
+        forge_policy_loss(leaf[:], y, torch.zeros(4), inplace=True)
+    with pytest.raises(ValueError, match="not a leaf"):
+        forge_preference_loss(leaf.view(4, 3, 8), y, inplace=True)
+    for result in (leaf * 1.0, (leaf * 1.0)[:, 1:], leaf.detach(), leaf.detach()[1:], torch.zeros(2, 3, 8)[:, :2]):
+        check_inplace(result)
