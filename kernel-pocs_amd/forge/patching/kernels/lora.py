@@ -46,11 +46,13 @@ Fused paths:
 """
 from __future__ import annotations
 
+import copy
 import importlib
 from typing import NamedTuple, Optional
 
 import torch
 
+from .basic import make_rmsnorm_forward
 from .common import ForgeSkipPatch
 
 # ---------------------------------------------------------------------------
@@ -353,33 +355,86 @@ def _attention_interface(module, modeling, kwargs):
     return modeling.ALL_ATTENTION_FUNCTIONS[impl]
 
 
+def _probe_norm(norm, eps) -> Optional[float]:
+    """The offset o with which the class's forward, run on a CPU copy with
+    weights and inputs of this function's own, is x / sqrt(mean x^2 + eps) *
+    (weight + o), or None."""
+    if set(norm._parameters) != {"weight"} or norm._buffers or norm._modules:
+        return None
+    (dim,) = norm.weight.shape
+    at = torch.arange(dim, dtype=torch.float32, device="cpu")
+    weight = 0.75 + 0.5 * torch.sin(1.3 * at)
+    # a row that outweighs eps and one that does not
+    x = torch.stack([torch.cos(1.7 * at + 0.3), eps ** 0.5 * torch.cos(2.3 * at + 0.1)])
+    probe = copy.copy(norm)
+    probe.__dict__["_parameters"] = {"weight": torch.nn.Parameter(weight, requires_grad=False)}
+    try:
+        with torch.no_grad():
+            got = type(norm).forward(probe, x)
+    except Exception:  # a forward of other arguments, or one that needs a GPU
+        return None
+    if not isinstance(got, torch.Tensor) or got.shape != x.shape or got.device != x.device:
+        return None
+    normed = x.double() / (x.double().square().mean(-1, keepdim=True) + eps).sqrt()
+    for offset in (0.0, 1.0):
+        if torch.allclose(got.double(), normed * (weight.double() + offset), rtol=1e-4, atol=1e-5):
+            return offset
+    return None
+
+
+# by class and what its forward may read beside its weight: plain attributes
+_PROBED_NORMS: dict = {}
+
+
+def norm_offset(norm, eps: float) -> Optional[float]:
+    """What a norm module's forward adds to its weight (0.0 or 1.0), or None for
+    a forward that is not an RMS norm with this eps.  Names do not say it
+    (Gemma3's norms add one, Gemma3n's do not): the forward is run once.  A
+    class without a forward, which holds the weights only, is taken by its name
+    (Gemma...: 1.0)."""
+    own = vars(norm).get("forward")
+    if own is not None and getattr(own, "__module__", None) != make_rmsnorm_forward.__module__:
+        return None  # not the class's forward, nor this framework's adapter of it
+    if type(norm).forward is torch.nn.Module.forward:
+        return 1.0 if type(norm).__name__.startswith("Gemma") else 0.0
+    plain = sorted((k, v) for k, v in vars(norm).items() if isinstance(v, (bool, int, float, str)))
+    key = (type(norm), tuple(norm.weight.shape), eps, tuple(plain))
+    if key not in _PROBED_NORMS:
+        _PROBED_NORMS[key] = _probe_norm(norm, eps)
+    return _PROBED_NORMS[key]
+
+
 def qk_norm_args(module, Q, K, cos, sin, config):
     """(q weight, k weight, eps, offset) when the two norms and RoPE can run as
     one pass over Q, K [B, S, heads, D], else None: both norms plain RMS norms
-    over head_dim (class names end in RMSNorm) with one eps and no hooks, GPU
-    tensors, cos/sin [B or 1, S, D] of a half-split rotation.  The stored weight
-    is the difference from one (offset 1.0) in Gemma's classes;
-    config["qk_norm_offset"] overrides."""
+    over head_dim (class names end in RMSNorm, `norm_offset` knows their
+    forward) with one eps, one offset and no hooks, GPU tensors, cos/sin [B or
+    1, S, D] of a half-split rotation.  config["qk_norm_offset"] gives the
+    offset of a norm whose forward is not looked at."""
     q_norm, k_norm = getattr(module, "q_norm", None), getattr(module, "k_norm", None)
     if q_norm is None or k_norm is None or not Q.is_cuda or _is_dtensor(Q):
         return None
-    names, eps = [], []
+    eps = []
     for norm in (q_norm, k_norm):
         w = getattr(norm, "weight", None)
         if not type(norm).__name__.endswith("RMSNorm") or w is None or _is_dtensor(w) or w.shape != Q.shape[-1:]:
             return None
         if w.device != Q.device or norm._forward_hooks or norm._forward_pre_hooks:
             return None
-        names.append(type(norm).__name__)
         eps.append(getattr(norm, "variance_epsilon", getattr(norm, "eps", None)))
-    if eps[0] is None or eps[0] != eps[1] or names[0] != names[1] or q_norm.weight.dtype != k_norm.weight.dtype:
+    if eps[0] is None or eps[0] != eps[1] or type(q_norm) is not type(k_norm) or q_norm.weight.dtype != k_norm.weight.dtype:
         return None
     if cos.dim() != 3 or cos.shape != sin.shape or cos.shape[0] not in (1, Q.shape[0]):
         return None
     if tuple(cos.shape[1:]) != (Q.shape[1], Q.shape[-1]) or cos.device != Q.device:
         return None
-    offset = float(config.get("qk_norm_offset", 1.0 if names[0].startswith("Gemma") else 0.0))
-    return q_norm.weight, k_norm.weight, float(eps[0]), offset
+    eps = float(eps[0])
+    offset = config.get("qk_norm_offset")
+    if offset is None:
+        offset = norm_offset(q_norm, eps)
+        if offset is None or norm_offset(k_norm, eps) != offset:
+            return None
+    return q_norm.weight, k_norm.weight, eps, float(offset)
 
 
 def _qkv_states(module, modeling, hidden_states, cos, sin, config):
@@ -455,4 +510,4 @@ def make_lora_qkv_forward(module, config):
 
 
 __all__ = ["LiveLoRA", "live_lora", "make_lora_mlp_forward", "make_lora_qkv_forward", "mlp_fused_args",
-           "qk_norm_args", "qkv_fused_args", "rope_tables"]
+           "norm_offset", "qk_norm_args", "qkv_fused_args", "rope_tables"]
