@@ -404,6 +404,13 @@ def norm_offset(norm, eps: float) -> Optional[float]:
     return _PROBED_NORMS[key]
 
 
+def has_hooks(module) -> bool:
+    """Whether calling the module does more than its forward (its own hooks of
+    either pass, or global ones)."""
+    return bool(module._forward_hooks or module._forward_pre_hooks or module._backward_hooks
+                or module._backward_pre_hooks or torch.nn.modules.module._has_any_global_hook())
+
+
 def qk_norm_args(module, Q, K, cos, sin, config):
     """(q weight, k weight, eps, offset) when the two norms and RoPE can run as
     one pass over Q, K [B, S, heads, D], else None: both norms plain RMS norms
@@ -419,7 +426,7 @@ def qk_norm_args(module, Q, K, cos, sin, config):
         w = getattr(norm, "weight", None)
         if not type(norm).__name__.endswith("RMSNorm") or w is None or _is_dtensor(w) or w.shape != Q.shape[-1:]:
             return None
-        if w.device != Q.device or norm._forward_hooks or norm._forward_pre_hooks:
+        if w.device != Q.device or has_hooks(norm):
             return None
         eps.append(getattr(norm, "variance_epsilon", getattr(norm, "eps", None)))
     if eps[0] is None or eps[0] != eps[1] or type(q_norm) is not type(k_norm) or q_norm.weight.dtype != k_norm.weight.dtype:
@@ -509,5 +516,5 @@ def make_lora_qkv_forward(module, config):
     return forward
 
 
-__all__ = ["LiveLoRA", "live_lora", "make_lora_mlp_forward", "make_lora_qkv_forward", "mlp_fused_args",
+__all__ = ["LiveLoRA", "has_hooks", "live_lora", "make_lora_mlp_forward", "make_lora_qkv_forward", "mlp_fused_args",
            "norm_offset", "qk_norm_args", "qkv_fused_args", "rope_tables"]

@@ -139,3 +139,39 @@ def test_fused_attention_with_the_norms_of_other_models(model, name, offset, mon
     for n in ("q_norm", "k_norm"):
         a, b, c = (getattr(t, n).weight.grad for t in (m, plain, m32))
         _check(a, b, c, n)
+
+
+def test_hooks_of_a_norm():
+    from forge.patching.kernels.lora import has_hooks
+
+    for register in ("register_forward_hook", "register_forward_pre_hook", "register_full_backward_hook",
+                     "register_full_backward_pre_hook"):
+        norm = FlaggedRMSNorm(False)
+        assert not has_hooks(norm)
+        handle = getattr(norm, register)(lambda *a: None)
+        assert has_hooks(norm), register
+        handle.remove()
+        assert not has_hooks(norm)
+    handle = torch.nn.modules.module.register_module_full_backward_hook(lambda *a: None)
+    try:
+        assert has_hooks(FlaggedRMSNorm(False))
+    finally:
+        handle.remove()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("register", ["register_full_backward_hook", "register_full_backward_pre_hook"])
+def test_a_norm_with_backward_hooks_runs(register):
+    """A gradient observer on a norm sees its gradient, so the module runs."""
+    from test_patch_adapters import _run, build
+
+    from forge.patching import FORWARD_MAKERS
+
+    m, rot = build("qwen3", "attn", dtype=torch.bfloat16, device="cuda")
+    seen = []
+    getattr(m.k_norm, register)(lambda *a: seen.append(1))
+    m.forward = FORWARD_MAKERS["lora_qkv"](m, {"fuse_qk_norm": True})
+    x = torch.randn(2, 9, 512, device="cuda", dtype=torch.bfloat16)
+    cos, sin = rot(x, torch.arange(9, device="cuda")[None])
+    _run(m, x, ((cos, sin), None), "attn", torch.ones(2, 9, 512, device="cuda"))
+    assert seen == [1]
