@@ -47,6 +47,7 @@ Fused paths:
 from __future__ import annotations
 
 import copy
+import functools
 import importlib
 from typing import NamedTuple, Optional
 
@@ -404,6 +405,34 @@ def norm_offset(norm, eps: float) -> Optional[float]:
     return _PROBED_NORMS[key]
 
 
+@functools.lru_cache(maxsize=64)
+def rotates_halves(rotate, head_dim) -> bool:
+    """Whether a modeling module's apply_rotary_pos_emb(q, k, cos, sin) turns
+    column j with column j + head_dim / 2, as the kernels here do (others turn
+    neighbours, take one tensor, or a part of the head): it is run once on the
+    CPU, on angles of this function's own.  None, a module without such a
+    function, is taken for one that does."""
+    if rotate is None:
+        return True
+    from forge.kernels.rope import forge_apply_rotary_pos_emb
+
+    if rotate is forge_apply_rotary_pos_emb:
+        return True
+    half = head_dim // 2
+    at = torch.arange(half, dtype=torch.float32, device="cpu")
+    angle = torch.stack([0.2 + 0.7 * at, 1.1 + 0.3 * at]).unsqueeze(0)
+    c, s = angle.cos(), angle.sin()
+    q = torch.cos(0.9 * torch.arange(4 * head_dim, dtype=torch.float32, device="cpu")).view(1, 2, 2, head_dim)
+    try:
+        with torch.no_grad():
+            got = rotate(q, q[:, :1], torch.cat([c, c], -1), torch.cat([s, s], -1))
+        lo, hi = q[..., :half], q[..., half:]
+        want = torch.cat([lo * c - hi * s, hi * c + lo * s], -1)
+        return len(got) == 2 and all(torch.allclose(a, b, rtol=1e-4, atol=1e-5) for a, b in zip(got, (want, want[:, :1])))
+    except Exception:
+        return False
+
+
 def has_hooks(module) -> bool:
     """Whether calling the module does more than its forward (its own hooks of
     either pass, or global ones)."""
@@ -466,7 +495,9 @@ def _qkv_states(module, modeling, hidden_states, cos, sin, config):
     else:
         Q, K, V = module.q_proj(hidden_states), module.k_proj(hidden_states), module.v_proj(hidden_states)
     Q, K, V = Q.view(hidden_shape), K.view(hidden_shape), V.view(hidden_shape)
-    norm = qk_norm_args(module, Q, K, cos, sin, config) if config.get("fuse_qk_norm", False) else None
+    norm = None
+    if config.get("fuse_qk_norm", False) and rotates_halves(getattr(modeling, "apply_rotary_pos_emb", None), D):
+        norm = qk_norm_args(module, Q, K, cos, sin, config)
     if norm is not None:
         from kernels.rope.qk_norm_rope import apply_qk_norm_rope
 
@@ -517,4 +548,4 @@ def make_lora_qkv_forward(module, config):
 
 
 __all__ = ["LiveLoRA", "has_hooks", "live_lora", "make_lora_mlp_forward", "make_lora_qkv_forward", "mlp_fused_args",
-           "norm_offset", "qk_norm_args", "qkv_fused_args", "rope_tables"]
+           "norm_offset", "qk_norm_args", "qkv_fused_args", "rope_tables", "rotates_halves"]

@@ -113,6 +113,7 @@ def test_fused_attention_with_the_norms_of_other_models(model, name, offset, mon
 
     from forge.patching import FORWARD_MAKERS
 
+    import forge.kernels.rope  # noqa: F401  (takes the name before it is replaced)
     import kernels.rope.qk_norm_rope as qk
 
     calls, apply = [], qk.apply_qk_norm_rope
@@ -175,3 +176,40 @@ def test_a_norm_with_backward_hooks_runs(register):
     cos, sin = rot(x, torch.arange(9, device="cuda")[None])
     _run(m, x, ((cos, sin), None), "attn", torch.ones(2, 9, 512, device="cuda"))
     assert seen == [1]
+
+
+# ---------------------------------------------------------------------------
+# the rotation
+# ---------------------------------------------------------------------------
+def test_which_rotations_are_half_split():
+    from forge.kernels.rope import forge_apply_rotary_pos_emb
+    from forge.patching.kernels.lora import rotates_halves
+
+    def of(model):
+        return importlib.import_module(f"transformers.models.{model}.modeling_{model}").apply_rotary_pos_emb
+
+    for model in ("llama", "qwen3", "qwen2", "gemma2", "gemma3", "olmo2", "t5gemma2"):
+        assert rotates_halves(of(model), 128), model
+    # neighbours are rotated with each other; one tensor a call; a part of the head
+    for model in ("cohere", "ernie4_5", "gemma3n", "glm"):
+        assert not rotates_halves(of(model), 128), model
+    assert rotates_halves(forge_apply_rotary_pos_emb, 64)
+    assert not rotates_halves(lambda q, k, cos, sin: (q, k), 64)
+
+
+@pytest.mark.gpu
+def test_fused_norms_leave_another_rotation_to_the_model(monkeypatch):
+    from test_patch_adapters import MQ3, _run, build
+
+    from forge.patching import FORWARD_MAKERS
+
+    cohere = importlib.import_module("transformers.models.cohere.modeling_cohere")
+    monkeypatch.setattr(MQ3, "apply_rotary_pos_emb", cohere.apply_rotary_pos_emb)
+    m, rot = build("qwen3", "attn", dtype=torch.bfloat16, device="cuda")
+    x = torch.randn(2, 9, 512, device="cuda", dtype=torch.bfloat16)
+    cos, sin = rot(x, torch.arange(9, device="cuda")[None])
+    outs = []
+    for config in ({}, {"fuse_qk_norm": True}):
+        m.forward = FORWARD_MAKERS["lora_qkv"](m, config)
+        outs.append(_run(m, x, ((cos, sin), None), "attn", torch.ones(2, 9, 512, device="cuda"))[0])
+    assert torch.equal(*outs)
