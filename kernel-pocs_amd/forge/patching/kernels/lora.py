@@ -481,10 +481,13 @@ def _qkv_states(module, modeling, hidden_states, cos, sin, config):
     D = module.head_dim
     hidden_shape = (*hidden_states.shape[:-1], -1, D)
     has_norm = hasattr(module, "q_norm") or hasattr(module, "k_norm")
+    halves = rotates_halves(getattr(modeling, "apply_rotary_pos_emb", None), D)
     fused = qkv_fused_args(module, hidden_states)
     if fused is not None:
         q, k, v = fused
-        tables = None if has_norm else rope_tables(cos, sin, hidden_states, D, q.W.shape[0], k.W.shape[0])
+        tables = None
+        if not has_norm and halves:
+            tables = rope_tables(cos, sin, hidden_states, D, q.W.shape[0], k.W.shape[0])
         lora = (q.W, k.W, v.W, _bf16(q.A), _bf16(q.B), q.s, _bf16(k.A), _bf16(k.B), k.s,
                 _bf16(v.A), _bf16(v.B), v.s)
         if tables is not None:
@@ -496,7 +499,7 @@ def _qkv_states(module, modeling, hidden_states, cos, sin, config):
         Q, K, V = module.q_proj(hidden_states), module.k_proj(hidden_states), module.v_proj(hidden_states)
     Q, K, V = Q.view(hidden_shape), K.view(hidden_shape), V.view(hidden_shape)
     norm = None
-    if config.get("fuse_qk_norm", False) and rotates_halves(getattr(modeling, "apply_rotary_pos_emb", None), D):
+    if config.get("fuse_qk_norm", False) and halves:
         norm = qk_norm_args(module, Q, K, cos, sin, config)
     if norm is not None:
         from kernels.rope.qk_norm_rope import apply_qk_norm_rope

@@ -213,3 +213,28 @@ def test_fused_norms_leave_another_rotation_to_the_model(monkeypatch):
         m.forward = FORWARD_MAKERS["lora_qkv"](m, config)
         outs.append(_run(m, x, ((cos, sin), None), "attn", torch.ones(2, 9, 512, device="cuda"))[0])
     assert torch.equal(*outs)
+
+
+@pytest.mark.gpu
+def test_fused_projections_leave_another_rotation_to_the_model(monkeypatch):
+    """A LoRA attention without norms whose model turns neighbouring columns:
+    the RoPE epilogue of the fused projections is not used."""
+    import copy
+
+    from test_patch_adapters import ML, _check, _run, build
+
+    from forge.patching import FORWARD_MAKERS
+
+    cohere = importlib.import_module("transformers.models.cohere.modeling_cohere")
+    monkeypatch.setattr(ML, "apply_rotary_pos_emb", cohere.apply_rotary_pos_emb)
+    m, rot = build("llama", "attn", dtype=torch.bfloat16, device="cuda")
+    m32, plain = copy.deepcopy(m).float(), copy.deepcopy(m)
+    x, dy = (torch.randn(2, 9, 512, device="cuda") for _ in range(2))
+    cos, sin = rot(x, torch.arange(9, device="cuda")[None])
+    bf = torch.bfloat16
+    r32 = _run(m32, x, ((cos.float(), sin.float()), None), "attn", dy)
+    rp = _run(plain, x.to(bf), ((cos.to(bf), sin.to(bf)), None), "attn", dy)
+    m.forward = FORWARD_MAKERS["lora_qkv"](m, {})
+    rf = _run(m, x.to(bf), ((cos.to(bf), sin.to(bf)), None), "attn", dy)
+    _check(rf[0], rp[0], r32[0], "out")
+    _check(rf[1], rp[1], r32[1], "dx")
