@@ -28,7 +28,7 @@ _GELU_EXACT = {"gelu", "gelu_python"}
 _GELU_TANH = {"gelu_pytorch_tanh", "gelu_new"}
 
 
-def _saved_in_8_bits(config) -> bool:
+def saved_in_8_bits(config) -> bool:
     """config["saved_activations"]: None (gate and up are saved as they are) or
     "8bit" (glu_act8: an 8-bit copy of them is, on a GPU)."""
     saved = config.get("saved_activations")
@@ -60,7 +60,7 @@ def make_geglu_forward(module, config):
                 f"forge.patch: geglu kernel cannot infer GELU variant for hidden_activation={act!r}. "
                 f"Pass approximate='tanh' or approximate='none' via the mapping config to override.")
 
-    if _saved_in_8_bits(config):
+    if saved_in_8_bits(config):
         from forge.kernels.glu_act8 import glu_act8
 
         kind = "gelu_tanh" if approximate == "tanh" else "gelu_exact"
@@ -90,7 +90,7 @@ def make_swiglu_forward(module, config):
             f"Route this module to the 'geglu' kernel instead.")
     from forge.kernels.swiglu import swiglu
 
-    if _saved_in_8_bits(config):
+    if saved_in_8_bits(config):
         from forge.kernels.glu_act8 import glu_act8
 
         def forward8(x):

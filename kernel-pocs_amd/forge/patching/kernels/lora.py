@@ -53,7 +53,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from .basic import make_rmsnorm_forward
+from .basic import make_rmsnorm_forward, saved_in_8_bits
 from .common import ForgeSkipPatch
 
 # ---------------------------------------------------------------------------
@@ -290,6 +290,10 @@ def make_lora_mlp_forward(module, config):
     adapters (lora.py:189-191).  Call time: the fused kernel when
     `mlp_fused_args` accepts the live tensors, else the submodules (with the
     SwiGLU / GeGLU kernel for the activation, as in the reference)."""
+    if saved_in_8_bits(config):
+        raise NotImplementedError(
+            "forge.patch: the fused LoRA MLP saves gate and up as they are; saved_activations='8bit' belongs to the "
+            "'swiglu' or 'geglu' kernel, which take the same module.")
     activation = _detect_mlp_activation(module)
 
     if activation == "silu":
