@@ -385,6 +385,19 @@ int forge_policy_loss(int dtype, const void* logits, int64_t ld_n, int64_t ld_s,
                       float* loss, float* logps, float* kl,
                       void* dlogits, int64_t d_n, int64_t d_s, void* work, void* stream);
 
+/* The same with dlogits = grad_scale dloss/dlogits, rounded once: the scale of
+ * a loss that is scaled for fp16 gradients, one fp32 value on the device (NULL:
+ * 1).  The loss itself is not scaled. */
+int forge_policy_loss_scaled(int dtype, const void* logits, int64_t ld_n, int64_t ld_s,
+                             int64_t n, int64_t s, int64_t v,
+                             const int64_t* target, int64_t t_n, int64_t t_s, int64_t ignore_index,
+                             double temperature, const float* advantages, int64_t a_n, int64_t a_s,
+                             const float* old_logps, int64_t o_n, int64_t o_s,
+                             const float* ref_logps, int64_t r_n, int64_t r_s,
+                             double clip_low, double clip_high, double kl_coef, int reduction,
+                             const float* grad_scale, float* loss, float* logps, float* kl,
+                             void* dlogits, int64_t d_n, int64_t d_s, void* work, void* stream);
+
 /* ------------------------------------------------------------------------
  * RMSNorm (forward + backward, deterministic weight gradient)
  * ------------------------------------------------------------------------ */

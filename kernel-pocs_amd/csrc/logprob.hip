@@ -328,6 +328,7 @@ struct Policy {
   double low, high, beta;            // clip range, weight of the divergence
   int reduction;
   float* kl;                         // [N, S]
+  const float* scale;                // of the gradient, or nullptr (1)
 };
 
 // A token's loss -min(r A, clip(r) A) + beta (e^f - f - 1), with r = exp(logp -
@@ -377,6 +378,7 @@ __global__ __launch_bounds__(kBlock) void lp_rows_kernel(Rows a, Work w, Policy 
           const double weight = token_weight(a, w.counts, p.reduction, n);
           loss *= weight;
           d *= weight;
+          if (p.scale) d *= (double)*p.scale;
         }
         w.row64[row] = loss;
         w.coef[row] = (float)d;
@@ -731,7 +733,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(NR > 8 ? 4 :
     w.logps[row] = (float)lp;
     w.row64[row] = loss * weight;
     p.kl[row] = kl;
-    const float c = (float)(dl * weight) * g.inv_t;
+    const float c = (float)(p.scale ? dl * weight * (double)*p.scale : dl * weight) * g.inv_t;
     say[0] = c == 0.f ? 0.f : -c / d;
     say[1] = c == 0.f ? 0.f : -c * (float)expm1(lp);
   }
@@ -998,13 +1000,13 @@ extern "C" int forge_preference_fwd(int dtype, const void* logits, int64_t ld_n,
   return FORGE_OK;
 }
 
-extern "C" int forge_policy_loss(int dtype, const void* logits, int64_t ld_n, int64_t ld_s, int64_t n, int64_t s, int64_t v,
-                                 const int64_t* target, int64_t t_n, int64_t t_s, int64_t ignore_index,
-                                 double temperature, const float* advantages, int64_t a_n, int64_t a_s,
-                                 const float* old_logps, int64_t o_n, int64_t o_s, const float* ref_logps, int64_t r_n,
-                                 int64_t r_s, double clip_low, double clip_high, double kl_coef, int reduction,
-                                 float* loss, float* logps, float* kl, void* dlogits, int64_t d_n, int64_t d_s,
-                                 void* work, void* stream) {
+extern "C" int forge_policy_loss_scaled(int dtype, const void* logits, int64_t ld_n, int64_t ld_s, int64_t n, int64_t s,
+                                        int64_t v, const int64_t* target, int64_t t_n, int64_t t_s, int64_t ignore_index,
+                                        double temperature, const float* advantages, int64_t a_n, int64_t a_s,
+                                        const float* old_logps, int64_t o_n, int64_t o_s, const float* ref_logps,
+                                        int64_t r_n, int64_t r_s, double clip_low, double clip_high, double kl_coef,
+                                        int reduction, const float* grad_scale, float* loss, float* logps, float* kl,
+                                        void* dlogits, int64_t d_n, int64_t d_s, void* work, void* stream) {
   const Rows a = make_rows(logits, ld_n, ld_s, n, s, v, target, t_n, t_s, ignore_index, temperature);
   if (int rc = check_rows("policy_loss", dtype, a, temperature)) return rc;
   if (reduction != FORGE_REDUCE_MEAN && reduction != FORGE_REDUCE_SUM && reduction != FORGE_REDUCE_SEQUENCE)
@@ -1015,7 +1017,7 @@ extern "C" int forge_policy_loss(int dtype, const void* logits, int64_t ld_n, in
   const Layout l(dtype, n, s, v);
   const Work w = l.work(work, logps, (float2*)((char*)work + l.state));
   const Policy p = {advantages, a_n, a_s, old_logps, o_n, o_s, ref_logps, r_n, r_s, 1.0 - clip_low, 1.0 + clip_high,
-                    kl_coef, reduction, kl};
+                    kl_coef, reduction, kl, grad_scale};
   const Grad g = {dlogits, d_n, d_s, w.coef, s, 1, nullptr, 0, 1, w.state, logps, (float)(1.0 / temperature), w.row64, loss};
   hipStream_t st = (hipStream_t)stream;
   if (n * s > 0) {
@@ -1028,4 +1030,16 @@ extern "C" int forge_policy_loss(int dtype, const void* logits, int64_t ld_n, in
     if (int rc = launch_rows(dtype, a, w, &p, st)) return rc;
   }
   return launch_grad(dtype, a, g, dlogits != nullptr && n * s > 0, st);
+}
+
+extern "C" int forge_policy_loss(int dtype, const void* logits, int64_t ld_n, int64_t ld_s, int64_t n, int64_t s, int64_t v,
+                                 const int64_t* target, int64_t t_n, int64_t t_s, int64_t ignore_index,
+                                 double temperature, const float* advantages, int64_t a_n, int64_t a_s,
+                                 const float* old_logps, int64_t o_n, int64_t o_s, const float* ref_logps, int64_t r_n,
+                                 int64_t r_s, double clip_low, double clip_high, double kl_coef, int reduction,
+                                 float* loss, float* logps, float* kl, void* dlogits, int64_t d_n, int64_t d_s,
+                                 void* work, void* stream) {
+  return forge_policy_loss_scaled(dtype, logits, ld_n, ld_s, n, s, v, target, t_n, t_s, ignore_index, temperature,
+                                  advantages, a_n, a_s, old_logps, o_n, o_s, ref_logps, r_n, r_s, clip_low, clip_high,
+                                  kl_coef, reduction, nullptr, loss, logps, kl, dlogits, d_n, d_s, work, stream);
 }

@@ -184,6 +184,10 @@ forge_policy_loss = _decl(
     "forge_policy_loss",
     _LP_ROWS + [c_f64] + [c_vp, c_i64, c_i64] * 3 + [c_f64] * 3 + [c_int] + [c_vp] * 4 + [c_i64] * 2 + [c_vp] * 2
 )
+forge_policy_loss_scaled = _decl(
+    "forge_policy_loss_scaled",
+    _LP_ROWS + [c_f64] + [c_vp, c_i64, c_i64] * 3 + [c_f64] * 3 + [c_int] + [c_vp] * 5 + [c_i64] * 2 + [c_vp] * 2
+)
 forge_ce_target_prob = _decl(
     "forge_ce_target_prob", [c_int, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_f32, c_vp, c_vp]
 )
@@ -232,7 +236,7 @@ EXPORTED = [
     "forge_swiglu_fwd", "forge_swiglu_bwd", "forge_geglu_fwd", "forge_geglu_bwd", "forge_rope",
     "forge_qk_norm_rope_fwd", "forge_qk_norm_rope_bwd", "forge_qk_norm_rope_bwd_workspace",
     "forge_logp_workspace", "forge_token_logps_fwd", "forge_token_logps_bwd", "forge_preference_fwd",
-    "forge_policy_loss",
+    "forge_policy_loss", "forge_policy_loss_scaled",
     "forge_glu_act8_bytes", "forge_glu_act8_fwd", "forge_glu_act8_bwd",
     "forge_ce_fwd", "forge_ce_target_stats", "forge_ce_fwd_reduce", "forge_ce_stats_wait", "forge_ce_scale",
     "forge_sum_f32",

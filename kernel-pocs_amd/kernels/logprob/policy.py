@@ -3,7 +3,7 @@
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 
@@ -24,7 +24,8 @@ class PolicyLossOutput:
     kl: torch.Tensor
 
 
-def _launch(x, target, adv, old, ref, clip_low, clip_high, kl_coef, temperature, reduction, ignore_index, dlogits):
+def _launch(x, target, adv, old, ref, clip_low, clip_high, kl_coef, temperature, reduction, ignore_index, dlogits,
+            grad_scale=None):
     n, s, _ = x.shape
     f32 = {"dtype": torch.float32, "device": x.device}
     loss, logps, kl = torch.empty((), **f32), torch.empty((n, s), **f32), torch.empty((n, s), **f32)
@@ -35,10 +36,11 @@ def _launch(x, target, adv, old, ref, clip_low, clip_high, kl_coef, temperature,
 
     with L.on_device(x):
         L.check(
-            L.forge_policy_loss(*R.rows_args(x, target, ignore_index), temperature, *strided(adv), *strided(old),
-                                *strided(ref), clip_low, clip_high, kl_coef, reduction, loss.data_ptr(),
-                                logps.data_ptr(), kl.data_ptr(), L.ptr(dlogits),
-                                *((0, 0) if dlogits is None else dlogits.stride()[:2]), work.data_ptr(), L.stream_of(x)),
+            L.forge_policy_loss_scaled(*R.rows_args(x, target, ignore_index), temperature, *strided(adv), *strided(old),
+                                       *strided(ref), clip_low, clip_high, kl_coef, reduction, L.ptr(grad_scale),
+                                       loss.data_ptr(), logps.data_ptr(), kl.data_ptr(), L.ptr(dlogits),
+                                       *((0, 0) if dlogits is None else dlogits.stride()[:2]), work.data_ptr(),
+                                       L.stream_of(x)),
             "forge_policy_loss")
     return loss, logps, kl
 
@@ -46,16 +48,18 @@ def _launch(x, target, adv, old, ref, clip_low, clip_high, kl_coef, temperature,
 class ForgePolicyLossFunction(torch.autograd.Function):
     """forward(ctx, logits [N, S, V], target [N, S], advantages, old_logps,
     ref_logps [N, S] or None, clip_low, clip_high, kl_coef, temperature,
-    reduction, ignore_index, inplace) -> (loss, logps, kl).  The forward writes
-    dloss/dlogits, over the logits with inplace; the backward hands that out,
-    scaled by the incoming gradient where it is not 1."""
+    reduction, ignore_index, inplace, grad_scale) -> (loss, logps, kl).  The
+    forward writes dloss/dlogits times grad_scale (one fp32 element, or None),
+    over the logits with inplace; the backward hands that out, scaled by the
+    incoming gradient / grad_scale where that is not 1."""
 
     @staticmethod
     def forward(ctx, x, target, adv, old, ref, clip_low, clip_high, kl_coef, temperature, reduction, ignore_index,
-                inplace):
+                inplace, grad_scale=None):
         ctx.dlogits = x.detach() if inplace else torch.empty(x.shape, dtype=x.dtype, device=x.device)
         loss, logps, kl = _launch(x, target, adv, old, ref, clip_low, clip_high, kl_coef, temperature, reduction,
-                                  ignore_index, ctx.dlogits)
+                                  ignore_index, ctx.dlogits, grad_scale)
+        ctx.grad_scale = grad_scale
         if inplace:
             torch.autograd.graph.increment_version(x)  # what else has saved the logits must not use them
         ctx.mark_non_differentiable(logps, kl)
@@ -72,6 +76,8 @@ class ForgePolicyLossFunction(torch.autograd.Function):
             # scaled in place on the device where the scale is not 1: a 16-bit
             # gradient is rounded a second time then, as in forge_cross_entropy
             grad = grad.to(torch.float32).reshape(1)
+            if ctx.grad_scale is not None:
+                grad = grad / ctx.grad_scale
             sn, ss, _ = d.stride()
             if s == 1:
                 parts = [(d, n, sn)]
@@ -85,14 +91,30 @@ class ForgePolicyLossFunction(torch.autograd.Function):
                         L.forge_ce_scale(L.dtype_code(d.dtype), part.data_ptr(), max(ld, v), rows, v, grad.data_ptr(),
                                          L.DTYPE_F32, L.stream_of(d)),
                         "forge_ce_scale")
-        return (d,) + (None,) * 11
+        return (d,) + (None,) * 12
+
+
+def _scale(grad_scale, logits) -> torch.Tensor:
+    """One fp32 element of the call's own."""
+    if not isinstance(grad_scale, torch.Tensor):
+        if not 0.0 < grad_scale < float("inf"):
+            raise ValueError(f"grad_scale must be positive and finite, got {grad_scale}")
+        return torch.full((1,), float(grad_scale), dtype=torch.float32, device=logits.device)
+    if grad_scale.numel() != 1:
+        raise ValueError(f"grad_scale must have one element, got shape {tuple(grad_scale.shape)}")
+    if not grad_scale.is_floating_point():
+        raise TypeError(f"grad_scale must be floating point, got {grad_scale.dtype}")
+    if grad_scale.device != logits.device:
+        raise ValueError(f"grad_scale must be on the logits' device {logits.device}, got {grad_scale.device}")
+    return grad_scale.detach().reshape(1).to(torch.float32, copy=True)
 
 
 def forge_policy_loss(logits: torch.Tensor, target: torch.Tensor, advantages: torch.Tensor,
                       old_logps: Optional[torch.Tensor] = None, ref_logps: Optional[torch.Tensor] = None,
                       clip_low: float = 0.2, clip_high: float = 0.2, kl_coef: float = 0.0, temperature: float = 1.0,
                       reduction: str = "mean", ignore_index: int = -100, inplace: bool = False,
-                      validate_targets: bool = False) -> PolicyLossOutput:
+                      validate_targets: bool = False,
+                      grad_scale: Union[None, float, torch.Tensor] = None) -> PolicyLossOutput:
     """Policy-gradient loss of sampled tokens.  logits [N, S, V] (fp16, bf16,
     fp32), target [N, S] with ignore_index on prompts and padding (their rows
     are not read, and get zero gradients; nothing else of them is read either).
@@ -108,7 +130,11 @@ def forge_policy_loss(logits: torch.Tensor, target: torch.Tensor, advantages: to
 
     Where the logits want a gradient the forward computes it, over the logits'
     storage with inplace (forge_cross_entropy's contract) or into a new tensor,
-    and the backward runs once.  A target outside [0, V) makes the loss NaN;
+    and the backward runs once.  That gradient is rounded to the logits' type
+    before the incoming one is known: under loss scaling (fp16) pass the loss's
+    scale as grad_scale (a number, or one element on the device), and what is
+    rounded is the scaled gradient; the loss is returned unscaled, and a
+    backward from scale * loss hands the gradient out as it is.  A target outside [0, V) makes the loss NaN;
     validate_targets=True raises IndexError instead (one host sync)."""
     R.check_logits(logits, target, temperature)
     if logits.dim() != 3:
@@ -128,6 +154,8 @@ def forge_policy_loss(logits: torch.Tensor, target: torch.Tensor, advantages: to
         advantages = R.per_token(advantages, shape, "advantages", logits)
     old = None if old_logps is None else R.per_token(old_logps, shape, "old_logps", logits)
     ref = None if ref_logps is None else R.per_token(ref_logps, shape, "ref_logps", logits)
+    if grad_scale is not None:
+        grad_scale = _scale(grad_scale, logits)
     L.require_gpu(logits)
     if validate_targets:
         R.check_targets(target, ignore_index, logits.shape[-1])
@@ -135,7 +163,7 @@ def forge_policy_loss(logits: torch.Tensor, target: torch.Tensor, advantages: to
     args = (advantages, old, ref, float(clip_low), float(clip_high), float(kl_coef), float(temperature),
             _REDUCTIONS[reduction], int(ignore_index))
     if torch.is_grad_enabled() and logits.requires_grad:
-        return PolicyLossOutput(*ForgePolicyLossFunction.apply(x, t, *args, bool(inplace)))
+        return PolicyLossOutput(*ForgePolicyLossFunction.apply(x, t, *args, bool(inplace), grad_scale))
     L.refuse_tangents(logits)
     return PolicyLossOutput(*_launch(x, t, *args, None))
 

@@ -244,3 +244,88 @@ def test_inplace_of_a_leafs_view_is_refused():
         forge_preference_loss(leaf.view(4, 3, 8), y, inplace=True)
     for result in (leaf * 1.0, (leaf * 1.0)[:, 1:], leaf.detach(), leaf.detach()[1:], torch.zeros(2, 3, 8)[:, :2]):
         check_inplace(result)
+
+
+# ---------------------------------------------------------------------------
+# loss scaling
+# ---------------------------------------------------------------------------
+def _scaled_case(n, s, v, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(n, s, v, generator=g) * 2).to(dtype)
+    y = torch.randint(0, v, (n, s), generator=g)
+    y[:, 0] = IGNORE
+    return x, y, torch.randn(n, generator=g)
+
+
+def test_grad_scale_refusals():
+    from kernels.logprob import forge_policy_loss
+
+    x, y, adv = _scaled_case(2, 3, 8, torch.float16)
+    for bad in (0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="grad_scale must be positive"):
+            forge_policy_loss(x, y, adv, grad_scale=bad)
+    with pytest.raises(ValueError, match="one element"):
+        forge_policy_loss(x, y, adv, grad_scale=torch.ones(2))
+    with pytest.raises(TypeError, match="floating point"):
+        forge_policy_loss(x, y, adv, grad_scale=torch.ones(1, dtype=torch.long))
+    with pytest.raises(RuntimeError, match="ROCm GPU"):
+        forge_policy_loss(x, y, adv, grad_scale=torch.ones(()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("kind", ["float", "tensor", "scaler"])
+@pytest.mark.parametrize("n,s,v", [(8, 1024, 130), (2, 100, 3003), (4, 100, 20000)])
+def test_fp16_gradients_under_loss_scaling(n, s, v, kind, inplace):
+    """"mean" over the tokens puts a column's gradient far below fp16's least
+    (6e-8): with grad_scale what is rounded is the scaled gradient, to half a
+    step of fp16 (2^-11) or of its subnormals, over the fp32 error of p (2 e,
+    e = (64 + V / 8192 + 3 R) U with R the range of a row of logits, below 40)
+    and 8 U of the coefficient's products."""
+    from kernels.logprob import forge_policy_loss
+    from oracle import logprob as O
+
+    scale = 65536.0
+    x, y, adv = _scaled_case(n, s, v, torch.float16)
+    leaf = x.cuda().requires_grad_(True)
+    scaler = torch.amp.GradScaler("cuda", init_scale=scale)
+    given = {"float": scale, "tensor": torch.tensor(scale, device="cuda"), "scaler": scaler.get_scale()}[kind]
+    o = forge_policy_loss(leaf * 1.0, y.cuda(), adv.cuda(), grad_scale=given, inplace=inplace)
+    up = scaler.scale(o.loss) if kind == "scaler" else o.loss * scale
+    (d,) = torch.autograd.grad(up, leaf)
+    plain = forge_policy_loss(leaf, y.cuda(), adv.cuda())
+    assert torch.equal(plain.loss, o.loss) and torch.equal(plain.logps, o.logps)  # the loss is not scaled
+    kept = y != IGNORE
+    lp = O.token_logps(x, y)
+    _, _, coef = O.policy(lp, kept, adv.unsqueeze(1).expand(n, s), None, None, 0.2, 0.2, 0.0, "mean")
+    want = O.dlogits(x, y, coef * scale)
+    e = (64 + v / 8192 + 3 * 40) * U
+    bound = want.abs() * (2.0 ** -11 + 2 * e + 8 * U) + 2.0 ** -25
+    assert ((d.double().cpu() - want).abs() <= bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=str)
+def test_grad_scale_other_than_the_incoming_gradient(dtype):
+    """What arrives divided by grad_scale multiplies what is stored, which is
+    rounded once more; powers of two change nothing but subnormals."""
+    from kernels.logprob import forge_policy_loss
+
+    x, y, adv = (t.cuda() for t in _scaled_case(3, 40, 77, dtype))
+    x = x.requires_grad_(True)
+
+    def grad(grad_scale, up):
+        o = forge_policy_loss(x, y, adv, reduction="sum", grad_scale=grad_scale)
+        return torch.autograd.grad(o.loss, x, torch.tensor(up, device="cuda"))[0]
+
+    want = grad(None, 1.0)
+    least = torch.finfo(dtype).smallest_normal
+    for grad_scale, up in ((16.0, 16.0), (16.0, 1.0), (1.0, 1.0), (1.0, 16.0), (256.0, 4.0)):
+        got = grad(grad_scale, up).double() / up
+        assert ((got - want.double()).abs() <= least).all(), (grad_scale, up)
+    # the scale is the call's own: a buffer that changes afterwards does not count
+    s = torch.tensor(8.0, device="cuda")
+    o = forge_policy_loss(x, y, adv, reduction="sum", grad_scale=s)
+    s.mul_(2.0)
+    (got,) = torch.autograd.grad(o.loss, x, torch.tensor(8.0, device="cuda"))
+    assert ((got.double() / 8 - want.double()).abs() <= least).all()
