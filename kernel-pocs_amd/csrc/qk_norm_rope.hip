@@ -415,6 +415,12 @@ int run(int dtype, const char* what, Args& a, int w_dtype, int table_dtype, int6
   if (batch > lim || n_q > lim || n_kv > lim || seq_len > lim || batch * seq_len > lim ||
       batch * seq_len * (n_q > n_kv ? n_q : n_kv) > lim)
     return forge_set_error(FORGE_ERR_UNSUPPORTED, "%s: more than 2^30 heads in a call", what);
+  const int64_t tokens = batch * seq_len;
+  for (const Side* s : {&a.q, &a.k})
+    if (tokens * (s == &a.q ? n_q : n_kv) > 0 && (!s->x || !s->out || !s->w || (BWD && !s->dy)))
+      return forge_set_error(FORGE_ERR_INVALID, "%s: an array of q or k is NULL", what);
+  if (tokens * (n_q + n_kv) > 0 && (!a.cos || !a.sin))
+    return forge_set_error(FORGE_ERR_INVALID, "%s: cos or sin is NULL", what);
   if ((dqw || dkw) && !work) return forge_set_error(FORGE_ERR_INVALID, "%s: weight gradients need the workspace", what);
 
   const size_t es = dtype_size(dtype), ets = dtype_size(table_dtype);
