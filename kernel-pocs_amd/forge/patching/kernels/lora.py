@@ -444,6 +444,11 @@ def has_hooks(module) -> bool:
                 or module._backward_pre_hooks or torch.nn.modules.module._has_any_global_hook())
 
 
+# what apply_qk_norm_rope takes
+_NORM_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+_NORM_HEAD_DIM = 1024
+
+
 def qk_norm_args(module, Q, K, cos, sin, config):
     """(q weight, k weight, eps, offset) when the two norms and RoPE can run as
     one pass over Q, K [B, S, heads, D], else None: both norms plain RMS norms
@@ -454,12 +459,14 @@ def qk_norm_args(module, Q, K, cos, sin, config):
     q_norm, k_norm = getattr(module, "q_norm", None), getattr(module, "k_norm", None)
     if q_norm is None or k_norm is None or not Q.is_cuda or _is_dtensor(Q):
         return None
+    if Q.dtype not in _NORM_DTYPES or K.dtype != Q.dtype or Q.shape[-1] % 2 or Q.shape[-1] > _NORM_HEAD_DIM:
+        return None
     eps = []
     for norm in (q_norm, k_norm):
         w = getattr(norm, "weight", None)
         if not type(norm).__name__.endswith("RMSNorm") or w is None or _is_dtensor(w) or w.shape != Q.shape[-1:]:
             return None
-        if w.device != Q.device or has_hooks(norm):
+        if w.dtype not in _NORM_DTYPES or w.device != Q.device or has_hooks(norm):
             return None
         eps.append(getattr(norm, "variance_epsilon", getattr(norm, "eps", None)))
     if eps[0] is None or eps[0] != eps[1] or type(q_norm) is not type(k_norm) or q_norm.weight.dtype != k_norm.weight.dtype:

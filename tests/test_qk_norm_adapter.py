@@ -238,3 +238,20 @@ def test_fused_projections_leave_another_rotation_to_the_model(monkeypatch):
     rf = _run(m, x.to(bf), ((cos.to(bf), sin.to(bf)), None), "attn", dy)
     _check(rf[0], rp[0], r32[0], "out")
     _check(rf[1], rp[1], r32[1], "dx")
+
+
+@pytest.mark.gpu
+def test_fused_norms_leave_other_types_to_the_modules():
+    """A float64 attention runs with the option as it does without."""
+    from test_patch_adapters import _run, build
+
+    from forge.patching import FORWARD_MAKERS
+
+    m, rot = build("qwen3", "attn", dtype=torch.float64, device="cuda")
+    x = torch.randn(2, 9, 512, device="cuda", dtype=torch.float64)
+    cos, sin = rot(x, torch.arange(9, device="cuda")[None])
+    outs = []
+    for config in ({}, {"fuse_qk_norm": True}):
+        m.forward = FORWARD_MAKERS["lora_qkv"](m, config)
+        outs.append(_run(m, x, ((cos, sin), None), "attn", torch.ones(2, 9, 512, device="cuda"))[0])
+    assert outs[0].dtype == torch.float64 and torch.equal(*outs)
