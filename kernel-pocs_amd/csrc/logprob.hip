@@ -27,7 +27,12 @@
 // max of x and d = sum 2^((x_j - m) k) are fp32, and everything behind them (the
 // logarithm, ratios, divergences, sums over a sequence and over the batch) is in
 // 64 bits: a sum of thousands of log-probabilities less the reference model's is
-// a small difference of large numbers.  p_j is 2^((x_j - m) k) / d.  (One fma
+// a small difference of large numbers.  p_j is 2^((x_j - m) k) / d.  The rows
+// that lp_policy_kernel holds use the first part of k alone and no corrections:
+// there a log-probability belongs to its own token's ratio and is not summed.
+// Mean error over 4096 16-bit rows of 32000 and 128256 at t = 1 and 0.7, with and
+// without masked columns: up to 1.2e-8 from lp_partial_kernel, 4e-8 to 6e-8 held
+// (rms 1.3e-7 and 1.5e-7, most of it the rounding of the result to fp32).  (One fma
 // x_j k - m k would do where m is moderate, but its result at x_j = m is the
 // rounding error of m k, which is no longer small where every logit of a row is
 // a mask's -1e30.)  A row with a NaN or +infinity, or with nothing but
@@ -773,9 +778,10 @@ int vec_of(int dtype) { return (int)(16 / dtype_size(dtype)); }
 
 // Pieces of a row: enough workgroups for the card (4 on each CU), none with
 // less than a vector a thread.  512 rows of 32000 / 16 of 128256: 13.7 / 9.0 us;
-// with 2 on each CU 14.0 / 8.0, 8 14.9 / 9.0, 16 17.5 / 8.9.
+// with 2 on each CU 14.0 / 8.0, 8 14.9 / 9.0, 16 17.5 / 8.9.  (Rows that a wave
+// takes: 512 to 1023 of them in two pieces from 512 vectors on, else in one.)
 int splits_for(int64_t rows, int64_t v, int dtype) {
-  const int64_t most = v / ((int64_t)vec_of(dtype) * kBlock);  // (1 for the rows that a wave takes)
+  const int64_t most = v / ((int64_t)vec_of(dtype) * kBlock);
   int64_t s = rows ? (1024 + rows - 1) / rows : 1;
   if (s > most) s = most;
   if (s > kMaxSplits) s = kMaxSplits;
