@@ -267,7 +267,8 @@ def _run_own(case, t):
         out = _call("logps")(t["logits"], t["target"], temperature=case["temperature"])
         return (out, *torch.autograd.grad(out, leaves, t["dlogps"])) if case["train"] else (out,)
     if op == "preference":
-        o = _call("preference")(t["logits"], t["target"], t["ref_logps"], beta=0.1, label_smoothing=case["smoothing"],
+        smoothing = case["smoothing"] if case["kind"] == "sigmoid" else 0.0  # the other losses have none
+        o = _call("preference")(t["logits"], t["target"], t["ref_logps"], beta=0.1, label_smoothing=smoothing,
                                 loss_type=case["kind"], length_normalized=case["normalized"])
         return (o.loss, o.logps, o.rewards, *torch.autograd.grad(o.loss, leaves))
     if op == "policy":
