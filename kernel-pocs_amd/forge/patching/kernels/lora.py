@@ -23,7 +23,8 @@ tensors off the submodules (`linear.base_layer.weight`, `lora_A[adapter]`,
     cast);
   * the widths are ones the kernels take (multiples of 8; the fused RoPE
     epilogue needs head_dim 64 or 128 and projection widths that are
-    multiples of 256, with a full-width cos/sin table).
+    multiples of 256, with a full-width cos/sin table, and a model whose
+    apply_rotary_pos_emb turns column j with j + head_dim / 2).
 
 Otherwise the call takes the reference's submodule path, so a patched module
 is never less general than the reference's.
