@@ -374,7 +374,8 @@ int forge_preference_fwd(int dtype, const void* logits, int64_t ld_n, int64_t ld
  *   -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^f - f - 1),
  *   r = exp(logp - old) (old_logps NULL: 1), f = ref - logp (ref_logps NULL: no
  * such term), reduced to one fp32 value.  With kl_coef 0 ref_logps only reports
- * kl.  logps, kl (e^f - f - 1, infinite for an infinite f): dense fp32 [N, S].  dlogits (NULL: loss only) gets dloss/dlogits and may be the logits. */
+ * kl.  logps, kl (e^f - f - 1, infinite for an infinite f): dense fp32 [N, S].
+ * dlogits (NULL: loss only) gets dloss/dlogits and may be the logits. */
 int forge_policy_loss(int dtype, const void* logits, int64_t ld_n, int64_t ld_s,
                       int64_t n, int64_t s, int64_t v,
                       const int64_t* target, int64_t t_n, int64_t t_s, int64_t ignore_index,

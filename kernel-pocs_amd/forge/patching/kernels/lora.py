@@ -371,7 +371,7 @@ def _probe_norm(norm, eps) -> Optional[float]:
     at = torch.arange(dim, dtype=torch.float32, device="cpu")
     weight = 0.75 + 0.5 * torch.sin(1.3 * at)
     # a row that outweighs eps and one that does not
-    x = torch.stack([torch.cos(1.7 * at + 0.3), eps ** 0.5 * torch.cos(2.3 * at + 0.1)])
+    x = torch.stack([torch.cos(1.7 * at + 0.3), max(eps, 1e-8) ** 0.5 * torch.cos(2.3 * at + 0.1)])
     probe = copy.copy(norm)
     probe.__dict__["_parameters"] = {"weight": torch.nn.Parameter(weight, requires_grad=False)}
     try:

@@ -16,8 +16,8 @@ _REDUCTIONS = {"mean": L.REDUCE_MEAN, "sum": L.REDUCE_SUM, "sequence": L.REDUCE_
 @dataclass(frozen=True)
 class PolicyLossOutput:
     """loss: fp32 scalar.  logps: the tokens' log-probabilities; kl: e^f - f -
-    1 with f = ref_logps - logps (0 without ref_logps); fp32 in the target's
-    shape, 0 where it is ignored.  Only the loss carries a gradient."""
+    1 with f = ref_logps - logps (0 without ref_logps, infinite where f is);
+    fp32 in the target's shape, 0 where it is ignored.  Only the loss carries a gradient."""
 
     loss: torch.Tensor
     logps: torch.Tensor
@@ -97,8 +97,8 @@ class ForgePolicyLossFunction(torch.autograd.Function):
 def _scale(grad_scale, logits) -> torch.Tensor:
     """One fp32 element of the call's own."""
     if not isinstance(grad_scale, torch.Tensor):
-        if not 0.0 < grad_scale < float("inf"):
-            raise ValueError(f"grad_scale must be positive and finite, got {grad_scale}")
+        if not 2.0 ** -126 <= grad_scale < 2.0 ** 127:
+            raise ValueError(f"grad_scale must be positive and finite in fp32, got {grad_scale}")
         return torch.full((1,), float(grad_scale), dtype=torch.float32, device=logits.device)
     if grad_scale.numel() != 1:
         raise ValueError(f"grad_scale must have one element, got shape {tuple(grad_scale.shape)}")

@@ -261,7 +261,7 @@ def test_grad_scale_refusals():
     from kernels.logprob import forge_policy_loss
 
     x, y, adv = _scaled_case(2, 3, 8, torch.float16)
-    for bad in (0.0, -1.0, float("inf"), float("nan")):
+    for bad in (0.0, -1.0, 1e-60, 1e60, float("inf"), float("nan")):
         with pytest.raises(ValueError, match="grad_scale must be positive"):
             forge_policy_loss(x, y, adv, grad_scale=bad)
     with pytest.raises(ValueError, match="one element"):

@@ -90,6 +90,8 @@ def test_norms_that_are_something_else():
     flagged = FlaggedRMSNorm(False)
     flagged.plus_one = True
     assert norm_offset(flagged, 1e-6) == 1.0
+    flagged.eps = 0.0
+    assert norm_offset(flagged, 0.0) == 1.0 and norm_offset(flagged, 1e-6) is None
     # a forward of the instance's own: only the framework's adapter of the same norm is known
     patched = FlaggedRMSNorm(False)
     patched.forward = lambda x: x
