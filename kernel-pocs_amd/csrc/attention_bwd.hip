@@ -1,0 +1,332 @@
+// Attention backward for gfx950: three launches, no atomics (the sums have a
+// fixed order).
+//   delta_i = sum_d o_i dout_i, and lse in units of log2, by head and query;
+//   dq_i = scale sum_j ds_ij k_j,       a workgroup to 128 queries of a head;
+//   dv_j = sum_i p_ij dout_i, dk_j = scale sum_i ds_ij q_i over the queries of the
+//   group's heads,                      a workgroup to 128 keys of a kv head,
+// with p_ij = exp2(s_ij c - lse_i) computed again and ds_ij = p_ij (dout_i . v_j -
+// delta_i).  p and ds are rounded to 16 bits as operands; every sum is in fp32.
+// As in the forward, products are laid out so that p and ds stay in the
+// registers that they are computed in: keys x queries for dq, queries x keys for
+// dk and dv.
+#include "attention.h"
+
+namespace fattn {
+
+// rows [batch][row] of the query side, one wave to a (row, head) at a time
+template <class T>
+__global__ __launch_bounds__(256) void attn_delta_kernel(Args a, float* lse2, int64_t n_rows, int64_t pairs) {
+  const int lane = threadIdx.x % 64;
+  // 16 lanes to a (row, head), D / 8 chunks of 8
+  for (int64_t p = ((int64_t)blockIdx.x * 256 + threadIdx.x) / 16; p < pairs; p += (int64_t)gridDim.x * 16) {
+    const int64_t row = p / a.H;
+    const int head = (int)(p % a.H);
+    const int64_t batch = a.cu_q ? 0 : row / a.tq, r = a.cu_q ? row : row % a.tq;
+    const T* o = row_ptr<T>(a.o, batch, r, head);
+    const T* d = row_ptr<T>(a.dout, batch, r, head);
+    float sum = 0.f;
+    for (int c = 8 * (lane % 16); c < a.D; c += 128) {
+      const Vec16<T> x = load16(o + c), y = load16(d + c);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += to_f32(x.v[i]) * to_f32(y.v[i]);
+    }
+#pragma unroll
+    for (int off = 8; off >= 1; off /= 2) sum += __shfl_xor(sum, off, 64);
+    if (lane % 16 == 0) {
+      const float l = a.lse[row * a.H + head];
+      a.delta[head * n_rows + row] = sum;
+      // a query without keys: exp2(s - inf) = 0
+      lse2[head * n_rows + row] = l == -__builtin_inff() ? __builtin_inff() : l * LOG2E;
+    }
+  }
+}
+
+template <class T, int DP>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dq_kernel(Args a, const float* lse2, int64_t n_rows, int tiles) {
+  constexpr int BM = 128, BN = 64, KS = DP / 16, DB = DP / 32;
+  using Dma = TileDma<DP, BN, 4>;
+  __shared__ __attribute__((aligned(1024))) char smem[(DP == 256 ? 2 : 4) * Dma::BYTES];
+  constexpr int NST = DP == 256 ? 1 : 2;
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int G = a.H / a.Hkv, h = lane / 32;
+  const Item it = item_of(blockIdx.x, tiles, a.Hkv, G);
+  if (it.tile >= tiles) return;
+  const TileAt at = find_tile(a.cu_q, a.B, a.tq, BM, it.tile);
+  if (at.seq > a.B) return;
+  const Span sq = span_of(a.cu_q, a.B, a.tq, at.seq);
+  Span sk = span_of(a.cu_k, a.B, a.tk, at.seq);
+  if (at.seq < 0 || at.seq >= a.B) sk.len = 0;
+  const int head = it.kv * G + it.g;
+  const int q0 = ((sq.len + BM - 1) / BM - 1 - at.tile) * BM;
+  const int shift = sk.len - sq.len;
+  const int rows = min(BM, sq.len - q0);
+  const int k_end = a.causal ? min(sk.len, q0 + rows + shift) : sk.len;
+  const int n_t = k_end > 0 ? (k_end + BN - 1) / BN : 0;
+  const int wq = q0 + wave * 32, iq = wq + lane % 32;
+  const bool live = iq < sq.len;
+  bf16x8 qf[KS], df[KS];
+  {
+    const T* qp = row_ptr<T>(a.q, sq.batch, sq.start + (live ? iq : 0), head);
+    const T* dp = row_ptr<T>(a.dout, sq.batch, sq.start + (live ? iq : 0), head);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int d = 16 * ks + 8 * h;
+      uint4 v = make_uint4(0, 0, 0, 0), w = v;
+      if (live && d < a.D) {
+        v = *reinterpret_cast<const uint4*>(qp + d);
+        w = *reinterpret_cast<const uint4*>(dp + d);
+      }
+      qf[ks] = __builtin_bit_cast(bf16x8, v);
+      df[ks] = __builtin_bit_cast(bf16x8, w);
+    }
+  }
+  const int64_t row = a.cu_q ? sq.start + iq : sq.batch * a.tq + iq;
+  const float lse = live ? lse2[head * n_rows + row] : __builtin_inff();
+  const float delta = live ? a.delta[head * n_rows + row] : 0.f;
+
+  Dma kd, vd;
+  kd.setup(a.k.row, a.D, wave);
+  vd.setup(a.v.row, a.D, wave);
+  const T* kp = row_ptr<T>(a.k, sk.batch, sk.start, it.kv);
+  const T* vp = row_ptr<T>(a.v, sk.batch, sk.start, it.kv);
+  auto issue = [&](int t) {
+    char* st = smem + (t % NST) * 2 * Dma::BYTES;
+    kd.load(kp + (int64_t)t * BN * a.k.row, sk.len - t * BN, st, wave);
+    vd.load(vp + (int64_t)t * BN * a.v.row, sk.len - t * BN, st + Dma::BYTES, wave);
+  };
+  TrOff<DP> tr;
+  tr.setup(lane);
+  f32x16 acc[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[db][r] = 0.f;
+  const float c = a.scale * LOG2E;
+  const int sees = a.causal ? min(sk.len, iq + shift + 1) : sk.len;
+  const int all_see = a.causal ? min(sk.len, wq + shift + 1) : sk.len;
+  const int any_sees = a.causal ? min(sk.len, min(wq + 32, sq.len) + shift) : (wq < sq.len ? sk.len : 0);
+
+  if (n_t > 0) issue(0);
+  for (int t = 0; t < n_t; ++t) {
+    wait_dma<0>();
+    barrier();
+    if (NST == 2 && t + 1 < n_t) issue(t + 1);
+    const char* kt = smem + (t % NST) * 2 * Dma::BYTES;
+    const char* vt = kt + Dma::BYTES;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const int k0 = t * BN + 32 * kb;
+      if (k0 >= any_sees) continue;
+      f32x16 s, dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s = mfma32<T>(frag_rows<DP>(kt, 32 * kb, ks, lane), qf[ks], s);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) dp = mfma32<T>(frag_rows<DP>(vt, 32 * kb, ks, lane), df[ks], dp);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = exp2_hw(__builtin_fmaf(s[r], c, -lse)) * (dp[r] - delta);
+      if (k0 + 32 > all_see) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (k0 + 8 * (r / 4) + 4 * h + r % 4 >= sees) s[r] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const bf16x8 ds = pack_acc<T>(s, i);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[db] = mfma32<T>(frag_cols<DP>(kt, tr, 32 * kb + 16 * i, db), ds, acc[db]);
+      }
+    }
+    if (NST == 1 && t + 1 < n_t) {
+      wait_dma<0>();
+      barrier();  // every wave has read the tile
+      issue(t + 1);
+    }
+  }
+  if (!live) return;
+  T* op = row_ptr<T>(a.dq, sq.batch, sq.start + iq, head);
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = 32 * db + 8 * i + 4 * h;
+      if (d >= a.D) continue;
+      uint32_t w[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const T lo = (T)(acc[db][4 * i + 2 * j] * a.scale), hi = (T)(acc[db][4 * i + 2 * j + 1] * a.scale);
+        w[j] = (uint32_t)__builtin_bit_cast(uint16_t, lo) | ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
+      }
+      *reinterpret_cast<uint2*>(op + d) = make_uint2(w[0], w[1]);
+    }
+}
+
+// A wave keeps 32 keys and values (the products' second operands) and their
+// gradients in registers: one wave a SIMD.  At DP = 256 those take more registers
+// than there are, so dk and dv are a launch each (DK, DV).
+template <class T, int DP, bool DK, bool DV>
+__global__ __launch_bounds__(256, 1) void attn_dkv_kernel(Args a, const float* lse2, int64_t n_rows, int tiles) {
+  constexpr int BN = 128, BQ = DP == 256 ? 32 : 64, KS = DP / 16, DB = DP / 32;
+  using Dma = TileDma<DP, BQ, 4>;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * 2 * Dma::BYTES];
+  __shared__ __attribute__((aligned(256))) float stat[2][2][64];
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int G = a.H / a.Hkv, h = lane / 32;
+  const Item it = item_of(blockIdx.x, tiles, a.Hkv, 1);
+  if (it.tile >= tiles) return;
+  const TileAt at = find_tile(a.cu_k, a.B, a.tk, BN, it.tile);
+  if (at.seq > a.B) return;
+  const Span sk = span_of(a.cu_k, a.B, a.tk, at.seq);
+  Span sq = span_of(a.cu_q, a.B, a.tq, at.seq);
+  if (at.seq < 0 || at.seq >= a.B) sq.len = 0;
+  const int k0 = at.tile * BN, wk = k0 + wave * 32, jk = wk + lane % 32;
+  const bool live = jk < sk.len;
+  const int shift = sk.len - sq.len;
+  bf16x8 kf[KS], vf[KS];
+  {
+    const T* kp = row_ptr<T>(a.k, sk.batch, sk.start + (live ? jk : 0), it.kv);
+    const T* vp = row_ptr<T>(a.v, sk.batch, sk.start + (live ? jk : 0), it.kv);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int d = 16 * ks + 8 * h;
+      uint4 v = make_uint4(0, 0, 0, 0), w = v;
+      if (live && d < a.D) {
+        v = *reinterpret_cast<const uint4*>(kp + d);
+        w = *reinterpret_cast<const uint4*>(vp + d);
+      }
+      kf[ks] = __builtin_bit_cast(bf16x8, v);
+      vf[ks] = __builtin_bit_cast(bf16x8, w);
+    }
+  }
+  // the first query that sees a key of the tile, and tiles of queries from there
+  const int first = a.causal ? max(0, k0 - shift) / BQ * BQ : 0;
+  const int per = sq.len > first ? (sq.len - first + BQ - 1) / BQ : 0, n_t = per * G;
+  Dma qd, dd;
+  qd.setup(a.q.row, a.D, wave);
+  dd.setup(a.dout.row, a.D, wave);
+  auto issue = [&](int t) {
+    const int head = it.kv * G + t / per, i0 = first + t % per * BQ, left = sq.len - i0;
+    char* st = smem + (t % 2) * 2 * Dma::BYTES;
+    qd.load(row_ptr<T>(a.q, sq.batch, sq.start + i0, head), left, st, wave);
+    dd.load(row_ptr<T>(a.dout, sq.batch, sq.start + i0, head), left, st + Dma::BYTES, wave);
+    // (rows that do not exist: q = dout = 0, so p = exp2(0) and ds = 0 add zeros)
+    const int64_t row = a.cu_q ? sq.start + i0 : sq.batch * a.tq + i0;
+    if (wave < 2) {
+      const __amdgpu_buffer_rsrc_t r = make_rsrc((wave ? a.delta : lse2) + head * n_rows + row);
+      dma4(r, &stat[t % 2][wave][0], lane < left && lane < BQ ? lane * 4 : OOB);
+    }
+  };
+  TrOff<DP> tr;
+  tr.setup(lane);
+  f32x16 dk[DB], dv[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dk[db][r] = dv[db][r] = 0.f;
+  const float c = a.scale * LOG2E;
+
+  if (n_t > 0) issue(0);
+  for (int t = 0; t < n_t; ++t) {
+    wait_dma<0>();
+    barrier();
+    if (t + 1 < n_t) issue(t + 1);
+    const char* qt = smem + (t % 2) * 2 * Dma::BYTES;
+    const char* dt = qt + Dma::BYTES;
+#pragma unroll
+    for (int qb = 0; qb < BQ / 32; ++qb) {
+      const int i0 = first + t % per * BQ + 32 * qb;
+      // (causal: the last query of the block sees nothing of this wave's keys)
+      if (i0 >= sq.len || wk >= sk.len || (a.causal && i0 + 31 + shift < wk)) continue;
+      f32x16 s, dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s = mfma32<T>(frag_rows<DP>(qt, 32 * qb, ks, lane), kf[ks], s);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        if constexpr (DK) dp = mfma32<T>(frag_rows<DP>(dt, 32 * qb, ks, lane), vf[ks], dp);
+      const bool edge = a.causal && i0 + shift < wk + 31;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(&stat[t % 2][0][32 * qb + 8 * i + 4 * h]);
+        const f32x4 de = *reinterpret_cast<const f32x4*>(&stat[t % 2][1][32 * qb + 8 * i + 4 * h]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = 4 * i + j;
+          float p = exp2_hw(__builtin_fmaf(s[r], c, -ls[j]));
+          float d = p * (dp[r] - de[j]);
+          if (edge && i0 + 8 * i + 4 * h + j + shift < jk) p = d = 0.f;
+          s[r] = p;
+          dp[r] = d;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const bf16x8 p = pack_acc<T>(s, i), ds = pack_acc<T>(dp, i);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          if constexpr (DV) dv[db] = mfma32<T>(frag_cols<DP>(dt, tr, 32 * qb + 16 * i, db), p, dv[db]);
+          if constexpr (DK) dk[db] = mfma32<T>(frag_cols<DP>(qt, tr, 32 * qb + 16 * i, db), ds, dk[db]);
+        }
+      }
+    }
+  }
+  if (!live) return;
+  T* kp = row_ptr<T>(a.dk, sk.batch, sk.start + jk, it.kv);
+  T* vp = row_ptr<T>(a.dv, sk.batch, sk.start + jk, it.kv);
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = 32 * db + 8 * i + 4 * h;
+      if (d >= a.D) continue;
+      uint32_t w[2], x[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        T lo = (T)(dk[db][4 * i + 2 * j] * a.scale), hi = (T)(dk[db][4 * i + 2 * j + 1] * a.scale);
+        w[j] = (uint32_t)__builtin_bit_cast(uint16_t, lo) | ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
+        lo = (T)dv[db][4 * i + 2 * j];
+        hi = (T)dv[db][4 * i + 2 * j + 1];
+        x[j] = (uint32_t)__builtin_bit_cast(uint16_t, lo) | ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
+      }
+      if constexpr (DK) *reinterpret_cast<uint2*>(kp + d) = make_uint2(w[0], w[1]);
+      if constexpr (DV) *reinterpret_cast<uint2*>(vp + d) = make_uint2(x[0], x[1]);
+    }
+}
+
+template <class T, int DP, bool DK, bool DV>
+static int launch_dkv(const Args& a, const float* lse2, int64_t n_rows, int64_t n, int64_t tiles, hipStream_t s) {
+  attn_dkv_kernel<T, DP, DK, DV><<<(unsigned)n, 256, 0, s>>>(a, lse2, n_rows, (int)tiles);
+  FORGE_CHECK_LAUNCH();
+  return FORGE_OK;
+}
+
+template <class T, int DP>
+static int launch_bwd_dp(const Args& a, float* lse2, int64_t n_rows, hipStream_t s) {
+  const int64_t tq = most_tiles(a.cu_q, a.B, a.tq, 128), tk = most_tiles(a.cu_k, a.B, a.tk, 128);
+  const int64_t nq = items(tq, a.Hkv, a.H / a.Hkv), nk = items(tk, a.Hkv, 1);
+  if (nq > 0x7fffffffLL || nk > 0x7fffffffLL) return forge_set_error(FORGE_ERR_INVALID, "attention: too many tiles");
+  const int64_t pairs = n_rows * a.H;
+  if (pairs) attn_delta_kernel<T><<<grid_for(pairs * 16, 256, 256 * 64), 256, 0, s>>>(a, lse2, n_rows, pairs);
+  FORGE_CHECK_LAUNCH();
+  if (nq && n_rows) attn_dq_kernel<T, DP><<<(unsigned)nq, 256, 0, s>>>(a, lse2, n_rows, (int)tq);
+  FORGE_CHECK_LAUNCH();
+  if (nk == 0) return FORGE_OK;
+  if (DP < 256) return launch_dkv<T, DP, true, DP < 256>(a, lse2, n_rows, nk, tk, s);
+  if (int e = launch_dkv<T, DP, true, DP < 256>(a, lse2, n_rows, nk, tk, s)) return e;
+  return launch_dkv<T, DP, DP < 256, true>(a, lse2, n_rows, nk, tk, s);
+}
+
+template <class T>
+static int launch_bwd_t(const Args& a, float* lse2, int64_t n_rows, hipStream_t s) {
+  if (a.D <= 64) return launch_bwd_dp<T, 64>(a, lse2, n_rows, s);
+  if (a.D <= 128) return launch_bwd_dp<T, 128>(a, lse2, n_rows, s);
+  return launch_bwd_dp<T, 256>(a, lse2, n_rows, s);
+}
+
+int launch_bwd(int dtype, const Args& a, float* lse2, int64_t n_rows, hipStream_t s) {
+  return dtype == FORGE_DTYPE_F16 ? launch_bwd_t<fp16_t>(a, lse2, n_rows, s) : launch_bwd_t<bf16_t>(a, lse2, n_rows, s);
+}
+
+}  // namespace fattn

@@ -1,0 +1,182 @@
+// Attention forward for gfx950.
+//
+// One pass over the keys with a running maximum m and sum l a query:
+//   S^T = K Q^T (keys x queries), p = exp2(s c - m c) with c = scale log2(e),
+//   O^T += V^T P^T, and at the end o = O / l, lse = m scale + ln l.
+// Both products are formed transposed, so that a lane of v_mfma_f32_32x32x16
+// holds one query's scores (the maximum and the sum are in-lane, with one exchange
+// between the halves of the wave), and those registers, rounded to 16 bits,
+// are the second product's operand as they are: P never leaves registers.
+// Rounding p to 16 bits errs by half a step of each term at random, less than
+// the rounding of the result.
+//
+// A workgroup of 4 waves takes 128 queries of one head, 32 a wave; tiles of 64
+// keys and values come by LDS-DMA into a ring of two.
+#include "attention.h"
+
+namespace fattn {
+
+constexpr int BN = 64;
+
+template <class T, int DP>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a, int tiles) {
+  constexpr int BM = 128, KS = DP / 16, DB = DP / 32;
+  using Dma = TileDma<DP, BN, 4>;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * Dma::BYTES];
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int G = a.H / a.Hkv, h = lane / 32;
+  const Item it = item_of(blockIdx.x, tiles, a.Hkv, G);
+  if (it.tile >= tiles) return;
+  const TileAt at = find_tile(a.cu_q, a.B, a.tq, BM, it.tile);
+  if (at.seq > a.B) return;
+  const Span sq = span_of(a.cu_q, a.B, a.tq, at.seq);
+  Span sk = span_of(a.cu_k, a.B, a.tk, at.seq);
+  if (at.seq < 0 || at.seq >= a.B) sk.len = 0;
+  const int head = it.kv * G + it.g;
+  // the last tile of a sequence, which sees the most keys, first
+  const int q0 = ((sq.len + BM - 1) / BM - 1 - at.tile) * BM;
+  const int shift = sk.len - sq.len;
+  const int rows = min(BM, sq.len - q0);
+  const int k_end = a.causal ? min(sk.len, q0 + rows + shift) : sk.len;
+  const int n_t = k_end > 0 ? (k_end + BN - 1) / BN : 0;
+
+  const int wq = q0 + wave * 32, iq = wq + lane % 32;  // this wave's first query, this lane's
+  const bool live = iq < sq.len;
+  bf16x8 qf[KS];
+  {
+    const T* qp = row_ptr<T>(a.q, sq.batch, sq.start + (live ? iq : 0), head);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int d = 16 * ks + 8 * h;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (live && d < a.D) v = *reinterpret_cast<const uint4*>(qp + d);
+      qf[ks] = __builtin_bit_cast(bf16x8, v);
+    }
+  }
+  Dma kd, vd;
+  kd.setup(a.k.row, a.D, wave);
+  vd.setup(a.v.row, a.D, wave);
+  const T* kp = row_ptr<T>(a.k, sk.batch, sk.start, it.kv);
+  const T* vp = row_ptr<T>(a.v, sk.batch, sk.start, it.kv);
+  auto issue = [&](int t) {
+    char* st = smem + (t % 2) * 2 * Dma::BYTES;
+    kd.load(kp + (int64_t)t * BN * a.k.row, sk.len - t * BN, st, wave);
+    vd.load(vp + (int64_t)t * BN * a.v.row, sk.len - t * BN, st + Dma::BYTES, wave);
+  };
+  TrOff<DP> tr;
+  tr.setup(lane);
+
+  f32x16 o[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
+  const float c = a.scale * LOG2E;
+  float m = -__FLT_MAX__, l = 0.f;  // m: in units of log2; l: this half's sum
+
+  // keys that this lane's query sees, and those that every query of the wave does
+  const int sees = a.causal ? min(sk.len, iq + shift + 1) : sk.len;
+  const int all_see = a.causal ? min(sk.len, wq + shift + 1) : sk.len;
+  const int any_sees = a.causal ? min(sk.len, min(wq + 32, sq.len) + shift) : (wq < sq.len ? sk.len : 0);
+
+  if (n_t > 0) issue(0);
+  for (int t = 0; t < n_t; ++t) {
+    wait_dma<0>();
+    barrier();
+    if (t + 1 < n_t) issue(t + 1);
+    const int k0 = t * BN;
+    if (k0 >= any_sees) continue;
+    const char* kt = smem + (t % 2) * 2 * Dma::BYTES;
+    const char* vt = kt + Dma::BYTES;
+    f32x16 s[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s[kb] = mfma32<T>(frag_rows<DP>(kt, 32 * kb, ks, lane), qf[ks], s[kb]);
+    }
+    if (k0 + BN > all_see) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (k0 + 32 * kb + 8 * (r / 4) + 4 * h + r % 4 >= sees) s[kb][r] = -__builtin_inff();
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
+    top = fmaxf(top, other_half(top)) * c;
+    if (__any(top > m)) {
+      const float up = fmaxf(top, m), f = exp2_hw(m - up);
+      m = up;
+      l *= f;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[db][r] *= f;
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float p = exp2_hw(__builtin_fmaf(s[kb][r], c, -m));
+        l += p;
+        s[kb][r] = p;
+      }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bf16x8 p = pack_acc<T>(s[i / 2], i % 2);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) o[db] = mfma32<T>(frag_cols<DP>(vt, tr, 16 * i, db), p, o[db]);
+    }
+  }
+  l += other_half(l);
+  if (!live) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // (a row without keys)
+  T* op = row_ptr<T>(a.o, sq.batch, sq.start + iq, head);
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = 32 * db + 8 * i + 4 * h;
+      if (d >= a.D) continue;
+      uint32_t w[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const T lo = (T)(o[db][4 * i + 2 * j] * inv), hi = (T)(o[db][4 * i + 2 * j + 1] * inv);
+        w[j] = (uint32_t)__builtin_bit_cast(uint16_t, lo) | ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
+      }
+      *reinterpret_cast<uint2*>(op + d) = make_uint2(w[0], w[1]);
+    }
+  if (h == 0 && a.lse) {
+    const int64_t row = a.cu_q ? sq.start + iq : sq.batch * a.tq + iq;
+    a.lse[row * a.H + head] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * LN2;
+  }
+}
+
+template <class T, int DP>
+static int launch_fwd_dp(const Args& a, hipStream_t s) {
+  const int64_t tiles = most_tiles(a.cu_q, a.B, a.tq, 128);
+  const int64_t n = items(tiles, a.Hkv, a.H / a.Hkv);
+  if (n > 0x7fffffffLL) return forge_set_error(FORGE_ERR_INVALID, "attention: too many tiles");
+  if (n == 0) return FORGE_OK;
+  attn_fwd_kernel<T, DP><<<(unsigned)n, 256, 0, s>>>(a, (int)tiles);
+  FORGE_CHECK_LAUNCH();
+  return FORGE_OK;
+}
+
+template <class T>
+static int launch_fwd_t(const Args& a, hipStream_t s) {
+  if (a.D <= 64) return launch_fwd_dp<T, 64>(a, s);
+  if (a.D <= 128) return launch_fwd_dp<T, 128>(a, s);
+  return launch_fwd_dp<T, 256>(a, s);
+}
+
+int launch_fwd(int dtype, const Args& a, hipStream_t s) {
+  return dtype == FORGE_DTYPE_F16 ? launch_fwd_t<fp16_t>(a, s) : launch_fwd_t<bf16_t>(a, s);
+}
+
+}  // namespace fattn

@@ -230,6 +230,17 @@ forge_transpose_2b_batch = _decl("forge_transpose_2b_batch", [c_int, c_vp, c_vp,
 TRANSPOSE_BATCH_MAX = 8
 forge_cast_f32_bf16 = _decl("forge_cast_f32_bf16", [c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp])
 
+forge_attention_fwd_workspace = _decl("forge_attention_fwd_workspace", [c_int] + [c_i64] * 6, c_i64)
+forge_attention_fwd = _decl(
+    "forge_attention_fwd", [c_int] + [c_vp, c_i64, c_i64, c_i64] * 4 + [c_vp] * 3 + [c_i64] * 6 + [c_f32, c_int, c_vp, c_vp]
+)
+forge_attention_bwd_workspace = _decl("forge_attention_bwd_workspace", [c_int] + [c_i64] * 3, c_i64)
+forge_attention_bwd = _decl(
+    "forge_attention_bwd",
+    [c_int] + [c_vp, c_i64, c_i64, c_i64] * 5 + [c_vp] + [c_vp, c_i64, c_i64, c_i64] * 3 + [c_vp] * 2 + [c_i64] * 6
+    + [c_f32, c_int, c_vp, c_vp],
+)
+
 # Every symbol include/forge_hip.h declares (checked by the CPU test suite).
 EXPORTED = [
     "forge_version", "forge_last_error", "forge_arch_ok",
@@ -245,6 +256,7 @@ EXPORTED = [
     "forge_lora_a", "forge_lora_a_noalloc", "forge_zero", "forge_copy", "forge_cast_f32_bf16", "forge_splitk_reduce",
     "forge_ce_target_prob", "forge_row_scale", "forge_gemm_generic", "forge_transpose_2b", "forge_transpose_2b_batch",
     "forge_rmsnorm_fwd", "forge_rmsnorm_bwd", "forge_rmsnorm_bwd_workspace",
+    "forge_attention_fwd", "forge_attention_fwd_workspace", "forge_attention_bwd", "forge_attention_bwd_workspace",
 ]
 
 # Number of successful library calls (tests use it to prove the HIP path ran).

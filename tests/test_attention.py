@@ -1,0 +1,279 @@
+"""Attention over packed sequences and dense batches (`forge_varlen_attention`,
+`forge_attention`).
+
+Tolerances are derived in oracle/attention.py, before the first run: scores,
+statistics and sums in fp32, and one rounding to the 16-bit type (half a step:
+finfo.eps / 2 relative, half the spacing of its subnormals absolute) of each
+probability, each gradient of a score, and each result."""
+import math
+
+import pytest
+import torch
+
+from oracle.attention import head_fwd_bwd, packed_fwd_bwd
+
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def _unit(dtype):
+    f = torch.finfo(dtype)
+    return f.eps / 2, f.smallest_normal * f.eps / 2
+
+
+def _offsets(lens):
+    at = [0]
+    for n in lens:
+        at.append(at[-1] + n)
+    return at
+
+
+def _make(lens_q, lens_k, H, kv, D, dtype, seed=0, tail_q=0, tail_k=0, layout="plain", std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    T, Tk = sum(lens_q) + tail_q, sum(lens_k) + tail_k
+    if layout == "packed":  # columns of one projection's output
+        assert T == Tk
+        t = (torch.randn(T, H + 2 * kv, D, generator=g) * std).to(dtype)
+        q, k, v = t.split([H, kv, kv], 1)
+    elif layout == "heads":  # tokens of a head beside each other
+        q, k, v = ((torch.randn(h, n, D, generator=g) * std).to(dtype).transpose(0, 1)
+                   for h, n in ((H, T), (kv, Tk), (kv, Tk)))
+    else:
+        q, k, v = ((torch.randn(n, h, D, generator=g) * std).to(dtype) for h, n in ((H, T), (kv, Tk), (kv, Tk)))
+    do = torch.randn(T, H, D, generator=g).to(dtype)
+    return q, k, v, do
+
+
+def _within(got, ref, err, what):
+    got = got.detach().double().cpu()
+    assert got.shape == ref.shape, what
+    inf = torch.isinf(ref)
+    assert torch.equal(torch.isinf(got), inf), what
+    over = ((got - ref).abs() - err)[~inf]
+    worst = over.max().item() if over.numel() else -1.0
+    assert worst <= 0, f"{what}: off by {worst:.3e} more than the bound"
+
+
+def _check(lens_q, lens_k, H, kv, D, dtype, causal=True, train=True, scale=None, **kw):
+    from kernels.attention import forge_varlen_attention
+
+    q, k, v, do = _make(lens_q, lens_k, H, kv, D, dtype, **kw)
+    cu_q, cu_k = _offsets(lens_q), _offsets(lens_k)
+    ref = packed_fwd_bwd(q, k, v, do, cu_q, cu_k, scale or D ** -0.5, causal, *_unit(dtype))
+
+    def gpu(t):  # keeps the strides
+        base = t._base if t._base is not None else t
+        return torch.as_strided(base.cuda(), t.shape, t.stride(), t.storage_offset())
+
+    qg, kg, vg = (gpu(t).detach().requires_grad_(train) for t in (q, k, v))
+    out, lse = forge_varlen_attention(qg, kg, vg, torch.tensor(cu_q, device="cuda", dtype=torch.int32),
+                                      torch.tensor(cu_k, device="cuda", dtype=torch.int32), causal=causal, scale=scale,
+                                      return_lse=True)
+    assert out.dtype == dtype and lse.dtype == torch.float32
+    _within(out, ref.o, ref.o_err, "out")
+    _within(lse, ref.lse, ref.lse_err, "lse")
+    if train:
+        for n, x in zip(("dq", "dk", "dv"), torch.autograd.grad(out, (qg, kg, vg), do.cuda())):
+            _within(x, getattr(ref, n), getattr(ref, n + "_err"), n)
+
+
+# ---------------------------------------------------------------------------
+# the oracle and refusals (CPU)
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("n,m,causal", [(5, 5, True), (3, 7, True), (7, 3, True), (4, 6, False), (1, 1, True)])
+def test_oracle_against_autograd_and_differences(n, m, causal):
+    g = torch.Generator().manual_seed(n * 10 + m)
+    q, k, v, do = (torch.randn(r, 8, generator=g, dtype=torch.float64) for r in (n, m, m, n))
+    r = head_fwd_bwd(q, k, v, do, 0.3, causal, 0.0, 0.0)
+
+    def f(q, k, v):
+        s = 0.3 * q @ k.T
+        if causal:
+            s = s.masked_fill(~torch.ones(n, m, dtype=torch.bool).tril(m - n), float("-inf"))
+        p = torch.nan_to_num(torch.softmax(s, -1), nan=0.0)
+        return p @ v
+
+    torch.testing.assert_close(r.o, f(q, k, v))
+    assert torch.equal(torch.isinf(r.lse), torch.tensor([causal and i + m - n < 0 for i in range(n)]))
+    step = 1e-6
+    for name, x in (("dq", q), ("dk", k), ("dv", v)):
+        num = torch.zeros_like(x)
+        for i in range(x.numel()):
+            e = torch.zeros_like(x).view(-1)
+            e[i] = step
+            e = e.view_as(x)
+            args = {"dq": q, "dk": k, "dv": v}
+            hi, lo = ((f(*[t + s * e if key == name else t for key, t in args.items()]) * do).sum() for s in (1, -1))
+            num.view(-1)[i] = (hi - lo) / (2 * step)
+        torch.testing.assert_close(getattr(r, name), num, rtol=1e-6, atol=1e-7)
+
+
+def test_refusals():
+    from kernels.attention import forge_attention, forge_varlen_attention
+
+    cu = torch.tensor([0, 4], dtype=torch.int32)
+
+    def call(q=(4, 4, 64), k=(4, 2, 64), v=None, dtype=BF16, cu=cu, **kw):
+        return forge_varlen_attention(torch.zeros(q, dtype=dtype), torch.zeros(k, dtype=dtype),
+                                      torch.zeros(v or k, dtype=kw.pop("v_dtype", dtype)), cu, **kw)
+
+    for match, kw in (("dimensions", {"q": (4, 64)}), ("same shape", {"v": (4, 1, 64)}), ("head_dim", {"k": (4, 2, 32)}),
+                      ("multiple of 8", {"q": (4, 4, 20), "k": (4, 2, 20)}),
+                      ("multiple of 8", {"q": (4, 4, 264), "k": (4, 2, 264)}),
+                      ("divides", {"k": (4, 3, 64)}), ("positive", {"scale": 0.0}), ("positive", {"scale": float("nan")}),
+                      ("positive", {"scale": float("inf")}), ("positive", {"scale": -1.0})):
+        with pytest.raises(ValueError, match=match):
+            call(**kw)
+    with pytest.raises(TypeError, match="fp16 or bf16"):
+        call(dtype=torch.float32)
+    with pytest.raises(TypeError, match="same dtype"):
+        call(v_dtype=FP16)
+    with pytest.raises(RuntimeError, match="GPU"):
+        call()
+    with pytest.raises(ValueError, match="batch"):
+        forge_attention(*(torch.zeros(b, 2, 4, 64, dtype=BF16) for b in (1, 2, 2)))
+
+
+def test_entry_point_refusals():
+    from forge_hip import _lib as L
+
+    rows = [16, 0, 512, 64]
+
+    def fwd(dtype=2, q=rows, k=rows, v=rows, o=rows, cu=(16, 16), sizes=(1, 4, 4, 4, 2, 64), scale=0.1):
+        return L.forge_attention_fwd(dtype, *q, *k, *v, *o, None, *cu, *sizes, scale, 1, None, None)
+
+    assert fwd(dtype=0) == 2 and b"dtype" in L.forge_last_error()
+    assert fwd(sizes=(1, 4, 4, 4, 2, 60)) == 2 and b"head_dim" in L.forge_last_error()
+    assert fwd(sizes=(1, 4, 4, 4, 2, 512)) == 2
+    assert fwd(sizes=(1, 4, 4, 4, 3, 64)) == 1 and b"heads" in L.forge_last_error()
+    assert fwd(sizes=(-1, 4, 4, 4, 2, 64)) == 1
+    assert fwd(sizes=(1, -4, 4, 4, 2, 64)) == 1
+    assert fwd(sizes=(1, 1 << 40, 4, 4, 2, 64)) == 1
+    assert fwd(cu=(None, 16)) == 1 and b"one side" in L.forge_last_error()
+    assert fwd(scale=0.0) == 1 and fwd(scale=float("nan")) == 1
+    for name, at in (("q", "q"), ("k", "k"), ("v", "v"), ("out", "o")):
+        assert fwd(**{at: [None, 0, 512, 64]}) == 1 and f"{name} is NULL".encode() in L.forge_last_error()
+        assert fwd(**{at: [24, 0, 512, 64]}) == 1 and b"aligned" in L.forge_last_error()
+        assert fwd(**{at: [16, 0, 516, 64]}) == 1
+        assert fwd(**{at: [16, 0, 1 << 23, 64]}) == 1 and b"stride" in L.forge_last_error()
+    assert L.forge_attention_bwd(2, *(rows * 5), None, *(rows * 3), 16, 16, 1, 4, 4, 4, 2, 64, 0.1, 1, 16, None) == 1
+    assert b"lse or work" in L.forge_last_error()
+    assert L.forge_attention_fwd_workspace(1, 1, 4, 4, 4, 3, 64) == -1
+    # nothing to do
+    empty = [None, 0, 0, 0]
+    assert fwd(q=empty, o=empty, sizes=(1, 0, 4, 4, 2, 64)) == 0
+
+
+# ---------------------------------------------------------------------------
+# kernels
+# ---------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("H,kv,D", [(4, 2, 128), (2, 2, 64), (7, 1, 96), (4, 4, 8), (3, 1, 256), (2, 1, 200), (16, 8, 40)])
+def test_packed_sequences(H, kv, D, dtype):
+    lens = [1, 130, 64, 0, 257, 31]
+    _check(lens, lens, H, kv, D, dtype, layout="packed")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lens_q,lens_k", [([5], [700]), ([200, 3], [264, 3]), ([300, 40], [100, 40]), ([129, 7], [0, 65]),
+                                           ([64], [64]), ([128, 128], [128, 192]), ([1] * 70, list(range(70)))])
+def test_lengths(lens_q, lens_k, causal):
+    """Keys before the queries, fewer keys than queries, none, whole tiles, more sequences than lanes."""
+    _check(lens_q, lens_k, 4, 2, 64, BF16, causal=causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,H,kv,D", [(BF16, 32, 8, 128), (FP16, 8, 8, 64), (BF16, 16, 1, 256), (FP16, 14, 2, 72)])
+@pytest.mark.parametrize("lens_q,lens_k", [([1, 1, 1], [1000, 1, 129]), ([1, 0, 2, 1], [0, 5, 2049, 128]), ([3], [300]),
+                                           ([0, 4, 0, 0], [50, 2, 0, 33])])
+def test_few_queries(dtype, H, kv, D, lens_q, lens_k):
+    """One token a sequence and a few: the kernel that cuts the keys into chunks."""
+    _check(lens_q, lens_k, H, kv, D, dtype, train=False)
+
+
+@pytest.mark.gpu
+def test_few_queries_with_gradients_and_without_causality():
+    _check([1, 2], [500, 40], 8, 2, 64, BF16)
+    _check([1, 2], [500, 40], 8, 2, 64, BF16, causal=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens_q", [[70, 20], [1, 1]])
+def test_rows_outside_the_sequences_are_zeros(lens_q):
+    _check(lens_q, [90, 40], 4, 2, 64, BF16, tail_q=9, tail_k=150)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("std,scale", [(6.0, None), (1.0, 3.0), (1.0, 1e-4), (30.0, None)])
+def test_sharp_and_flat_scores(std, scale):
+    _check([150, 33], [150, 33], 2, 1, 64, FP16, std=std, scale=scale)
+    _check([150, 1], [150, 300], 2, 1, 128, BF16, std=std, scale=scale)
+
+
+@pytest.mark.gpu
+def test_tokens_of_a_head_beside_each_other():
+    _check([90, 40], [90, 40], 4, 2, 64, BF16, layout="heads")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,H,kv,S,Sk,D", [(2, 4, 2, 130, 130, 128), (3, 2, 1, 1, 200, 64), (2, 4, 4, 70, 200, 64)])
+@pytest.mark.parametrize("memory", ["bshd", "bhsd", "odd"])
+def test_dense_batches(B, H, kv, S, Sk, D, memory):
+    from kernels.attention import forge_attention
+
+    g = torch.Generator().manual_seed(1)
+
+    def make(h, s):
+        if memory == "bshd":
+            return torch.randn(B, s, h, D, generator=g).to(BF16).cuda().transpose(1, 2)
+        if memory == "bhsd":
+            return torch.randn(B, h, s, D, generator=g).to(BF16).cuda()
+        return torch.randn(B * h * s * D + 1, generator=g).to(BF16).cuda()[1:].view(B, h, s, D)  # unaligned rows
+
+    q, k, v = (make(h, s).requires_grad_(True) for h, s in ((H, S), (kv, Sk), (kv, Sk)))
+    out, lse = forge_attention(q, k, v, return_lse=True)
+    do = torch.randn(B, H, S, D, generator=g).to(BF16).cuda()
+    grads = torch.autograd.grad(out, (q, k, v), do)
+    flat = [t.detach().cpu().transpose(1, 2).reshape(-1, t.shape[1], D) for t in (q, k, v, do)]
+    ref = packed_fwd_bwd(*flat, _offsets([S] * B), _offsets([Sk] * B), D ** -0.5, True, *_unit(BF16))
+    _within(lse.reshape(B * S, H), ref.lse, ref.lse_err, "lse")
+    for n, x in zip(("o", "dq", "dk", "dv"), (out, *grads)):
+        _within(x.transpose(1, 2).reshape(-1, x.shape[1], D), getattr(ref, n), getattr(ref, n + "_err"), n)
+
+
+@pytest.mark.gpu
+def test_nothing_to_do():
+    from kernels.attention import forge_attention, forge_varlen_attention
+
+    z = torch.zeros(0, 2, 64, dtype=BF16, device="cuda", requires_grad=True)
+    k = torch.ones(5, 2, 64, dtype=BF16, device="cuda", requires_grad=True)
+    cu = torch.zeros(3, dtype=torch.int32, device="cuda")
+    out = forge_varlen_attention(z, k, k, cu, torch.tensor([0, 2, 5], dtype=torch.int32, device="cuda"))
+    assert out.shape == z.shape
+    (g,) = torch.autograd.grad(out, k, torch.zeros_like(out))
+    assert torch.equal(g, torch.zeros_like(k))
+    q = torch.ones(5, 2, 64, dtype=BF16, device="cuda", requires_grad=True)
+    out, lse = forge_varlen_attention(q, z, z, torch.tensor([0, 2, 5], device="cuda"), cu, return_lse=True)
+    assert torch.equal(out, torch.zeros_like(q)) and bool((lse == -math.inf).all())
+    assert torch.equal(torch.autograd.grad(out, q, torch.ones_like(q))[0], torch.zeros_like(q))
+    # no sequences at all
+    out = forge_varlen_attention(q, k, k, torch.zeros(1, dtype=torch.int32, device="cuda"))
+    assert torch.equal(out, torch.zeros_like(q))
+    e = torch.zeros(2, 2, 3, 64, dtype=BF16, device="cuda")
+    assert forge_attention(e, e[:, :, :0], e[:, :, :0]).abs().max() == 0
+    assert forge_attention(e[:0], e[:0], e[:0]).shape == (0, 2, 3, 64)
+
+
+@pytest.mark.gpu
+def test_offsets_are_checked_when_asked():
+    from kernels.attention import forge_varlen_attention
+
+    q = torch.ones(5, 2, 64, dtype=BF16, device="cuda")
+    for bad in ([1, 5], [0, 6], [0, 3, 2], [0, -1]):
+        with pytest.raises(ValueError, match="begin at 0"):
+            forge_varlen_attention(q, q, q, torch.tensor(bad, device="cuda"), validate_offsets=True)
+    with pytest.raises(ValueError, match="sequences"):
+        forge_varlen_attention(q, q, q, torch.tensor([0, 5], device="cuda"), torch.tensor([0, 2, 5], device="cuda"))
+    with pytest.raises(ValueError, match="cu_seqlens_k"):
+        forge_varlen_attention(q, q[:3], q[:3], torch.tensor([0, 5], device="cuda"))
