@@ -803,6 +803,54 @@ int forge_attention_bwd(int dtype, const void* dout, int64_t do_batch, int64_t d
                         const int32_t* cu_q, const int32_t* cu_k, int64_t B, int64_t tq, int64_t tk,
                         int64_t H, int64_t Hkv, int64_t D, float scale, int causal, void* work, void* stream);
 
+/* ------------------------------------------------------------------------
+ * RMS norm with the residual's addition, and rows in 8 bits (no reference
+ * counterpart)
+ * ------------------------------------------------------------------------ */
+
+/* h = x + residual rounded to dtype, y = h rstd (weight + offset) rounded once, rstd =
+ * 1 / sqrt(mean h^2 + eps).  x and residual: rows of H values, pitches ldx, ldr >= H,
+ * any element alignment; h, y [rows][H].  residual NULL: h = x, which is not written
+ * (h may be NULL).  rstd (fp32 [rows]) may be NULL.  fp32 / bf16 / fp16, the weight
+ * of any of them. */
+int forge_add_rmsnorm_fwd(int dtype, int w_dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                          const void* weight, void* h, void* y, float* rstd, int64_t rows, int64_t H, double eps,
+                          double offset, void* stream);
+
+/* The same with y in 8 bits: with t = h (weight + offset) and a = max |t| of a row, q =
+ * round_half_even(127 t / a) of exact arithmetic and scale = a rstd / 127, y = q scale.
+ * q [rows][ldq], 16-byte aligned, ldq >= H a multiple of 16, zeros behind H.  A row
+ * with an infinity or NaN: scale NaN. */
+int forge_add_rmsnorm_int8(int dtype, int w_dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                           const void* weight, void* h, int8_t* q, int64_t ldq, float* scale, int64_t rows,
+                           int64_t H, double eps, double offset, void* stream);
+
+/* d = dh + rstd g - h rstd^3 mean(g h), g = dy (weight + offset): the gradient of x and of
+ * the residual, from those of y and h (dh may be NULL); dw = sum over rows of dy h
+ * rstd in a fixed order, of the weight's type (dw NULL: not formed; with rows == 0 it is
+ * not written).  work: forge_add_rmsnorm_bwd_workspace bytes for dw. */
+int64_t forge_add_rmsnorm_bwd_workspace(int dtype, int64_t rows, int64_t H);
+int forge_add_rmsnorm_bwd(int dtype, int w_dtype, const void* dy, int64_t lddy, const void* dh, int64_t lddh,
+                          const void* h, int64_t ldh, const void* weight, const float* rstd, void* d, void* dw,
+                          void* work, int64_t rows, int64_t H, double offset, void* stream);
+
+/* Rows in 8 bits: t = x, or x times col_scale[column] (may be NULL); q and scale = a /
+ * 127 as above. */
+int forge_quantize_rows(int dtype, const void* x, int64_t ldx, const float* col_scale, int8_t* q, int64_t ldq,
+                        float* scale, int64_t rows, int64_t H, void* stream);
+
+/* C[m, n] = (sum_k a[m, k] b[n, k]) row_scale[m] col_scale[n] + bias[n]: the sum exact in
+ * 32-bit integers (K up to 2^17), C (fp32, bf16 or fp16, pitch ldc) rounded once.  a
+ * [M][lda], b [N][ldb]: 16-byte aligned, pitches multiples of 16 below 2^22, zeros from K
+ * to the next multiple of 16.  bias: C's type, or NULL. */
+int forge_int8_gemm(const int8_t* a, int64_t lda, const float* row_scale, const int8_t* b, int64_t ldb,
+                    const float* col_scale, const void* bias, void* c, int64_t ldc, int c_dtype, int64_t M,
+                    int64_t N, int64_t K, void* stream);
+
+/* dst[c, r] = src[r, c] of 8-bit values, zeros in dst's columns from `rows` to ld_dst. */
+int forge_transpose_1b(const int8_t* src, int64_t ld_src, int64_t rows, int64_t cols, int8_t* dst, int64_t ld_dst,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -45,13 +45,29 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 fp16x8 __attribute__((ext_vector_type(8)));
 
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+
+// Operands of 8-bit integers and a C of type O: two values to a 16-bit word, so
+// that K, pitches and fragments are those of 16-bit operands of half the K
+// (v_mfma_i32_32x32x32_i8 and 16x16x64_i8 take the same 16 bytes a lane, in the
+// same time).  The accumulators hold 32-bit integers, exact up to K = 2^17, until
+// the epilogue has scaled them (scale_i8).
+template <class O> struct I8 {};
+template <class T> struct OutOf { typedef T type; static constexpr bool i8 = false; };
+template <class O> struct OutOf<I8<O>> { typedef O type; static constexpr bool i8 = true; };
+template <class T> using out_t = typename OutOf<T>::type;
+
 // The engines move operands as 16-bit words (bf16x8 is their 16-byte
 // fragment); the element type T (bf16_t or fp16_t) decides the MFMA
 // instruction, which has one shape, lane layout and rate for both types, and
 // the conversions of a STORE epilogue's 16-bit C.  Both accumulate in fp32.
 template <class T>
 __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
-  if constexpr (std::is_same_v<T, fp16_t>)
+  if constexpr (OutOf<T>::i8)
+    return __builtin_bit_cast(f32x16, __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b),
+                                                                           __builtin_bit_cast(i32x16, c), 0, 0, 0));
+  else if constexpr (std::is_same_v<T, fp16_t>)
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(fp16x8, a), __builtin_bit_cast(fp16x8, b), c, 0, 0, 0);
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -65,7 +81,10 @@ enum Layout { ROW = 0, COL = 1 };
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 template <class T>
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
-  if constexpr (std::is_same_v<T, fp16_t>)
+  if constexpr (OutOf<T>::i8)
+    return __builtin_bit_cast(f32x4, __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b),
+                                                                         __builtin_bit_cast(i32x4, c), 0, 0, 0));
+  else if constexpr (std::is_same_v<T, fp16_t>)
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(fp16x8, a), __builtin_bit_cast(fp16x8, b), c, 0, 0, 0);
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -158,6 +177,11 @@ struct EpiArgs {
   int64_t wpart_stride;
   const __bf16* wxt[2];
   int64_t wxt_ld;
+  // 8-bit operands (I8): C = acc row_scale[m] col_scale[n] + bias[n] (bias of C's
+  // type, or nullptr; with split-K it is added to the first slice)
+  const float* row_scale;
+  const float* col_scale;
+  const void* bias;
 };
 
 // Activations of the STORE epilogues, applied to alpha * acc + beta * C.
@@ -219,8 +243,6 @@ __device__ __forceinline__ void transpose8x8(const uint4 (&in)[8], uint4 (&out)[
 // resource on k0 (scalar work) and masks k beyond the segment's end.
 constexpr uint32_t OOB = 0x80000000u;       // offset >= num_records -> reads 0
 constexpr int NUM_RECORDS = 0x7fffffff;
-
-typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // The base is wave-uniform by construction; readfirstlane makes that
 // visible to the compiler so the descriptor lives in SGPRs (a descriptor it
@@ -431,6 +453,15 @@ __device__ __forceinline__ void tile_coords(int64_t tiles_m, int64_t tiles_n, in
   const int64_t in = id % group_span;
   tm = (int)(first_m + in % gm);
   tn = (int)(in / gm);
+}
+
+// An accumulator of 8-bit products to its value in C.
+__device__ __forceinline__ float scale_i8(float acc, float row, float col, float bias) {
+  return __builtin_fmaf((float)__builtin_bit_cast(int, acc) * row, col, bias);
+}
+template <class O>
+__device__ __forceinline__ float bias_i8(const EpiArgs& ep, int64_t n) {
+  return ep.bias && blockIdx.z == 0 ? to_f32<O>(((const O*)ep.bias)[n]) : 0.f;
 }
 
 // Scheduling-group masks of __builtin_amdgcn_sched_group_barrier.
@@ -1260,7 +1291,21 @@ void gemm_dma_kernel(GemmArgs args) {
     static_assert(staged_ok(BM, BN, WAVES_M, WAVES_N, EPI), "staged epilogue: 256 x 256 tile, wave tiles of <= 128 rows");
     epilogue_staged<T, WAVES_M, WAVES_N, EPI>(args, acc, m0, n0, lane, wm, wn, reinterpret_cast<float*>(smem));
   } else {
-    epilogue<T, BM, BN, WAVES_M, WAVES_N, EPI>(args, acc, m0, n0, lane, wm, wn);
+    if constexpr (OutOf<T>::i8) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const int64_t n = min(n0 + wn * TN + j * 32 + lane % 32, args.N - 1);
+        const float col = args.ep.col_scale[n], bias = bias_i8<out_t<T>>(args.ep, n);
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int64_t m = min(m0 + wm * TM + i * 32 + 4 * (lane / 32) + 8 * (r / 4) + r % 4, M - 1);
+            acc[i][j][r] = scale_i8(acc[i][j][r], args.ep.row_scale[m], col, bias);
+          }
+      }
+    }
+    epilogue<out_t<T>, BM, BN, WAVES_M, WAVES_N, EPI>(args, acc, m0, n0, lane, wm, wn);
   }
 }
 

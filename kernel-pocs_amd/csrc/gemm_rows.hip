@@ -115,13 +115,22 @@ __global__ __launch_bounds__(NW * 64) void gemm_rows_kernel(GemmArgs args) {
     for (int d = 0; d < ND; ++d) {
       v[d] = red[0][c * ND + d][b][l];
 #pragma unroll
-      for (int w = 1; w < NW; ++w) v[d] += red[w][c * ND + d][b][l];
+      for (int w = 1; w < NW; ++w) {
+        if constexpr (OutOf<T>::i8)
+          v[d] = __builtin_bit_cast(f32x4, __builtin_bit_cast(i32x4, v[d]) + __builtin_bit_cast(i32x4, red[w][c * ND + d][b][l]));
+        else
+          v[d] += red[w][c * ND + d][b][l];
+      }
     }
     if (m >= M) continue;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       if (n + q >= N) break;
-      if constexpr (ND == 2) {
+      if constexpr (OutOf<T>::i8) {
+        typedef out_t<T> O;
+        ((O*)ep.c)[m * ep.ldc + n + q] =
+            from_f32<O>(scale_i8(v[0][q], ep.row_scale[m], ep.col_scale[n + q], bias_i8<O>(ep, n + q)));
+      } else if constexpr (ND == 2) {
         const float e = v[0][q], g = v[1][q];
         if (ep.e) {
           ep.e[m * ep.ld_eg + n + q] = (__bf16)e;
@@ -191,6 +200,21 @@ int launch_rows(int epi, const GemmArgs& a, hipStream_t s) {
     case EPI_GEGLU_ERF_FWD: return launch_glu<EPI_GEGLU_ERF_FWD>(a, s);
   }
   return forge_set_error(FORGE_ERR_UNSUPPORTED, "gemm: epilogue %d on %lld rows", epi, (long long)a.M);
+}
+
+// 8-bit operands.
+template <class O>
+static int launch_rows_i8_t(const GemmArgs& a, hipStream_t s) {
+  if (a.M <= 16) return a.N < 16 * 64 ? launch_one<I8<O>, 1, 1, 16, EPI_STORE_BF16>(a, s) : launch_one<I8<O>, 1, 1, 8, EPI_STORE_BF16>(a, s);
+  return a.N < 16 * 64 ? launch_one<I8<O>, 2, 1, 16, EPI_STORE_BF16>(a, s) : launch_one<I8<O>, 2, 1, 8, EPI_STORE_BF16>(a, s);
+}
+
+int launch_rows_i8(int out_dtype, const GemmArgs& a, hipStream_t s) {
+  switch (out_dtype) {
+    case FORGE_DTYPE_F32: return launch_rows_i8_t<float>(a, s);
+    case FORGE_DTYPE_F16: return launch_rows_i8_t<fp16_t>(a, s);
+    default: return launch_rows_i8_t<bf16_t>(a, s);
+  }
 }
 
 }  // namespace fgemm

@@ -459,6 +459,7 @@ void gemm_w4_kernel(GemmArgs args) {
   int elane = lane, ewave = wave;
   asm volatile("" : "+v"(elane), "+s"(ewave));
   const int ewm = ewave % WAVES_M, ewn = ewave / WAVES_M;
+  if constexpr (OutOf<T>::i8) w4_scale_i8<out_t<T>>(args, acc, m0, n0, elane, ewm, ewn);
   if constexpr (STAGED) {
     static_assert(w4_staged_epi(EPI), "staged epilogue: 16-bit or fp32 outputs");
     static_assert(RING >= W4_F32_BYTES, "the fp32 epilogue's slabs reuse the ring");
@@ -468,9 +469,9 @@ void gemm_w4_kernel(GemmArgs args) {
     else if constexpr (BMODE == B_DUAL)
       w4_epilogue_staged_dual<EPI>(args, acc, m0, n0, elane, ewm, ewn, lds);
     else  // (STORE_BF16 is launched staged at beta = 0 only)
-      w4_epilogue_staged<T, EPI>(args, acc, m0, n0, elane, ewm, ewn, lds);
+      w4_epilogue_staged<out_t<T>, EPI>(args, acc, m0, n0, elane, ewm, ewn, lds);
   } else {
-    w4_epilogue_direct<T, BMODE, EPI>(args, acc, m0, n0, elane, ewm, ewn);
+    w4_epilogue_direct<out_t<T>, BMODE, EPI>(args, acc, m0, n0, elane, ewm, ewn);
   }
 }
 

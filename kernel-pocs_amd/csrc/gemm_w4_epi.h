@@ -61,6 +61,25 @@ __device__ __forceinline__ float col_alpha(const EpiArgs& ep, int64_t n) {
   return ep.alpha;
 }
 
+// The accumulators of 8-bit products, scaled in place to their values in C.
+template <class O>
+__device__ __forceinline__ void w4_scale_i8(const GemmArgs& args, f32x4 (&acc)[8][8], int64_t m0, int64_t n0, int lane,
+                                            int wm, int wn) {
+  const EpiArgs& ep = args.ep;
+  float row[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) row[i] = ep.row_scale[min(m0 + wm * 128 + i * 16 + lane % 16, args.M - 1)];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int64_t n = min(n0 + wn * 128 + 16 * j + 4 * (lane / 16) + q, args.N - 1);
+      const float col = ep.col_scale[n], bias = bias_i8<O>(ep, n);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i][j][q] = scale_i8(acc[i][j][q], row[i], col, bias);
+    }
+}
+
 // ---------------------------------------------------------------------------
 // Direct epilogue: every element from registers, bounds-checked.
 // ---------------------------------------------------------------------------

@@ -1,0 +1,118 @@
+// Products of 8-bit integers with a scale for each token and each channel:
+//   C[m, n] = (sum_k a[m, k] b[n, k]) row_scale[m] col_scale[n] + bias[n]
+// a [M][K] and b [N][K], K-contiguous with pitches that are multiples of 16
+// bytes and zeros from K to the next multiple of 16.  The sum is exact in 32-bit
+// integers; C is rounded once, to fp32, bf16 or fp16.
+//
+// The engines are those of the 16-bit products (gemm_w4.h, gemm_core.h,
+// gemm_rows.hip), which see two values as one 16-bit word: the matrix
+// instructions take as many bytes a lane in the same time, so a product runs in
+// the time of a 16-bit one of half the K, less what the epilogue adds.
+#include "gemm_launch.h"
+
+namespace fgemm {
+
+int launch_rows_i8(int out_dtype, const GemmArgs& a, hipStream_t s);
+
+template <class O, int EPI>
+static int launch_i8_big(const GemmArgs& a, hipStream_t s) {
+  const int64_t tm = (a.M + 255) / 256, tn = (a.N + 255) / 256;
+  if (tm * tn > 0x7fffffffLL) return forge_set_error(FORGE_ERR_INVALID, "int8_gemm: too many tiles");
+  const dim3 grid((unsigned)(tm * tn), 1, (unsigned)a.split_k);
+  if (a.ep.vec_ok) gemm_w4_kernel<I8<O>, B_SINGLE, EPI, true><<<grid, 256, 0, s>>>(a);
+  else gemm_w4_kernel<I8<O>, B_SINGLE, EPI, false><<<grid, 256, 0, s>>>(a);
+  FORGE_CHECK_LAUNCH();
+  return FORGE_OK;
+}
+
+template <class O, int BM, int BN, int NS, int WPE>
+static int launch_i8_tile(const GemmArgs& a, hipStream_t s) {
+  constexpr int EPI = std::is_same_v<O, float> ? EPI_STORE_F32 : EPI_STORE_BF16;
+  const int64_t tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
+  if (tm * tn > 0x7fffffffLL) return forge_set_error(FORGE_ERR_INVALID, "int8_gemm: too many tiles");
+  gemm_dma_kernel<I8<O>, BM, BN, 2, 2, EPI, 64, NS, false, WPE><<<dim3((unsigned)(tm * tn), 1, (unsigned)a.split_k), 256, 0, s>>>(a);
+  FORGE_CHECK_LAUNCH();
+  return FORGE_OK;
+}
+
+template <class O>
+static int launch_i8(int out_dtype, const GemmArgs& a, hipStream_t s) {
+  constexpr int EPI = std::is_same_v<O, float> ? EPI_STORE_F32 : EPI_STORE_BF16;
+  if (a.M <= 32) return launch_rows_i8(out_dtype, a, s);
+  const int64_t big = ((a.M + 255) / 256) * ((a.N + 255) / 256);
+  if (big >= 128) return launch_i8_big<O, EPI>(a, s);
+  const int64_t mid = ((a.M + 127) / 128) * ((a.N + 127) / 128);
+  if (mid >= 256) return launch_i8_tile<O, 128, 128, 2, 2>(a, s);
+  return launch_i8_tile<O, 64, 64, 3, 3>(a, s);
+}
+
+}  // namespace fgemm
+
+using namespace fgemm;
+
+extern "C" int forge_int8_gemm(const int8_t* a, int64_t lda, const float* row_scale, const int8_t* b, int64_t ldb,
+                               const float* col_scale, const void* bias, void* c, int64_t ldc, int c_dtype, int64_t M,
+                               int64_t N, int64_t K, void* stream) {
+  if (M < 0 || N < 0 || K < 0 || K > (int64_t(1) << 17))
+    return forge_set_error(FORGE_ERR_INVALID, "int8_gemm: sizes (K up to 2^17, where a sum fits 32 bits)");
+  if (c_dtype != FORGE_DTYPE_F32 && c_dtype != FORGE_DTYPE_F16 && c_dtype != FORGE_DTYPE_BF16)
+    return forge_set_error(FORGE_ERR_UNSUPPORTED, "int8_gemm: C dtype %d", c_dtype);
+  if (M == 0 || N == 0) return FORGE_OK;
+  const int64_t kp = (K + 15) / 16 * 16;
+  if (!row_scale || !col_scale || !c || (K > 0 && (!a || !b))) return forge_set_error(FORGE_ERR_INVALID, "int8_gemm: an array is NULL");
+  if (lda < kp || ldb < kp || lda % 16 || ldb % 16 || lda >= (int64_t(1) << 22) || ldb >= (int64_t(1) << 22))
+    return forge_set_error(FORGE_ERR_INVALID, "int8_gemm: pitches are multiples of 16 from K to 2^22");
+  if (!aligned16(a) || !aligned16(b)) return forge_set_error(FORGE_ERR_INVALID, "int8_gemm: operands are 16-byte aligned");
+  if (ldc < N) return forge_set_error(FORGE_ERR_INVALID, "int8_gemm: ldc below N");
+  GemmArgs g = {};
+  g.M = M;
+  g.N = N;
+  g.n_segs = 1;
+  g.split_k = 1;
+  g.segs[0].a = (const __bf16*)a;
+  g.segs[0].lda = lda / 2;
+  g.segs[0].b = (const __bf16*)b;
+  g.segs[0].ldb = ldb / 2;
+  g.segs[0].k = kp / 2;
+  g.segs[0].n_hi = N;
+  g.ep.c = c;
+  g.ep.ldc = ldc;
+  g.ep.alpha = 1.f;
+  g.ep.row_scale = row_scale;
+  g.ep.col_scale = col_scale;
+  g.ep.bias = bias;
+  g.ep.vec_ok = aligned16(c) && ldc % 8 == 0;
+  const hipStream_t s = (hipStream_t)stream;
+  if (c_dtype == FORGE_DTYPE_F32) return launch_i8<float>(c_dtype, g, s);
+  if (c_dtype == FORGE_DTYPE_F16) return launch_i8<fp16_t>(c_dtype, g, s);
+  return launch_i8<bf16_t>(c_dtype, g, s);
+}
+
+// dst[c][r] = src[r][c] of 8-bit values, 64 x 64 tiles through LDS, zeros in the
+// columns of dst from `rows` to its pitch.
+__global__ __launch_bounds__(256) void transpose_1b_kernel(const int8_t* src, int64_t ld_src, int64_t rows, int64_t cols,
+                                                           int8_t* dst, int64_t ld_dst) {
+  __shared__ int8_t tile[64][68];
+  const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
+  for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+    const int64_t r = r0 + i / 64, c = c0 + i % 64;
+    tile[i / 64][i % 64] = r < rows && c < cols ? src[r * ld_src + c] : (int8_t)0;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+    const int64_t c = c0 + i / 64, r = r0 + i % 64;
+    if (c < cols && r < ld_dst) dst[c * ld_dst + r] = tile[i % 64][i / 64];
+  }
+}
+
+extern "C" int forge_transpose_1b(const int8_t* src, int64_t ld_src, int64_t rows, int64_t cols, int8_t* dst,
+                                  int64_t ld_dst, void* stream) {
+  if (rows < 0 || cols < 0 || ld_src < cols || ld_dst < rows) return forge_set_error(FORGE_ERR_INVALID, "transpose_1b: sizes");
+  if (rows == 0 || cols == 0) return FORGE_OK;
+  if (!src || !dst) return forge_set_error(FORGE_ERR_INVALID, "transpose_1b: an array is NULL");
+  const int64_t x = (ld_dst + 63) / 64, y = (cols + 63) / 64;
+  if (x > 0x7fffffff || y > 65535) return forge_set_error(FORGE_ERR_INVALID, "transpose_1b: too large");
+  transpose_1b_kernel<<<dim3((unsigned)x, (unsigned)y), 256, 0, (hipStream_t)stream>>>(src, ld_src, rows, cols, dst, ld_dst);
+  FORGE_CHECK_LAUNCH();
+  return FORGE_OK;
+}

@@ -1,6 +1,9 @@
 """RMSNorm re-export (reference forge/forge/kernels/rmsnorm.py)."""
 from kernels.rmsnorm import (
+    ForgeAddRMSNormFunction,
     ForgeRMSNormFunction,
+    add_rmsnorm,
+    add_rmsnorm_int8,
     apply_rmsnorm,
     rmsnorm,
     rmsnorm_backward,
@@ -9,7 +12,10 @@ from kernels.rmsnorm import (
 )
 
 __all__ = [
+    "ForgeAddRMSNormFunction",
     "ForgeRMSNormFunction",
+    "add_rmsnorm",
+    "add_rmsnorm_int8",
     "apply_rmsnorm",
     "rmsnorm",
     "rmsnorm_backward",

@@ -1,0 +1,221 @@
+"""Linear layers on frozen 8-bit weights (`int8_linear`).
+
+Tolerances, derived before the first run: the integers and their sum are exact, so a
+result has the rounding of the sum to fp32, three of the scales and their products,
+one of the bias's addition (6 roundings of 2^-24 of the terms), and that of its type."""
+import pytest
+import torch
+
+from oracle.int8 import linear, quantize
+
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+U = 2.0 ** -24
+
+
+def _within(got, ref, terms, k, what):
+    f = torch.finfo(got.dtype)
+    bound = ref.abs() * (f.eps / 2) + terms * (k * U * (1 + f.eps)) + f.smallest_normal * f.eps
+    over = (got.detach().double().cpu() - ref).abs() - bound
+    worst = over.max().item() if over.numel() else -1.0
+    assert worst <= 0, f"{what}: off by {worst:.3e} more than the bound"
+
+
+def _weight(n, k, seed=1):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randint(-127, 128, (n, k), generator=g).to(torch.int8), torch.rand(n, generator=g) * 0.02 + 0.001
+
+
+def _check(m, n, k, dtype, bias=False, train=True, out_dtype=None, seed=0):
+    from kernels.int8 import Int8Weight, int8_linear
+
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(m, k, generator=g).to(dtype)
+    w, ws = _weight(n, k)
+    b = torch.randn(n, generator=g).to(out_dtype or dtype) if bias else None
+    weight = Int8Weight(w.cuda(), ws.cuda(), backward=train)
+    xg = x.cuda().requires_grad_(train)
+    y = int8_linear(xg, weight, None if b is None else b.cuda(), out_dtype=out_dtype)
+    assert y.dtype == (out_dtype or dtype)
+    ref, terms = linear(*quantize(x), w, ws, b)
+    _within(y, ref, terms, 6, "y")
+    if train:
+        dy = torch.randn(m, n, generator=g).to(y.dtype)
+        (dx,) = torch.autograd.grad(y, xg, dy.cuda())
+        ref, terms = linear(*quantize(dy.double() * ws.double()), w.T, torch.ones(k))
+        _within(dx, ref, terms, 6, "dx")
+        # the gradient of the formula, up to the rounding of dy w_scale to 8 bits: at most half a unit each
+        full = (dy.double() * ws.double()) @ w.double()
+        unit = quantize(dy.double() * ws.double())[1]
+        slack = 0.5 * unit.unsqueeze(1) * w.double().abs().sum(0)
+        assert bool(((dx.double().cpu() - full).abs() <= slack + full.abs() * torch.finfo(dtype).eps + 1e-30).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 130, 500), (16, 1024, 512), (17, 33, 100), (32, 2017, 1003), (33, 70, 64),
+                                   (100, 1024, 4096), (333, 257, 130), (129, 640, 4101)])
+def test_sizes(m, n, k, dtype):
+    _check(m, n, k, dtype, bias=m % 2 == 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("m,n,k", [(2600, 3000, 300), (4096, 2048, 1024), (1500, 1504, 77), (2049, 4104, 48)])
+def test_large_tiles(m, n, k, dtype):
+    _check(m, n, k, dtype, bias=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_output_types(m):
+    for dtype in (BF16, FP16, FP32):
+        for out in (BF16, FP16, FP32):
+            _check(m, 96, 160, dtype, bias=True, out_dtype=out)
+
+
+@pytest.mark.gpu
+def test_the_largest_sum():
+    """K = 2^17 of the largest products: 2^31 - ..., just inside 32 bits."""
+    from kernels.int8 import Int8Weight, int8_linear
+
+    k = 1 << 17
+    w = torch.full((3, k), 127, dtype=torch.int8)
+    w[1] = -127
+    x = torch.ones(2, k, device="cuda")
+    y = int8_linear(x, Int8Weight(w.cuda(), torch.ones(3, device="cuda")), out_dtype=FP32)
+    ref = torch.tensor([127.0, -127.0, 127.0], dtype=torch.float64) * k
+    assert bool(((y.double().cpu() - ref).abs() <= ref.abs() * 6 * U).all())
+
+
+@pytest.mark.gpu
+def test_rows_from_the_norm_and_quantizer():
+    from kernels.int8 import Int8Weight, int8_linear, quantize_int8_rows
+    from kernels.rmsnorm import add_rmsnorm_int8
+
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(3, 7, 300, generator=g).to(BF16).cuda()
+    w, ws = _weight(96, 300)
+    weight = Int8Weight(w.cuda(), ws.cuda())
+    y = int8_linear(x, weight)
+    assert y.shape == (3, 7, 96) and torch.equal(y, int8_linear(quantize_int8_rows(x), weight))
+    assert torch.equal(quantize_int8_rows(x).values.cpu().long(), quantize(x.cpu())[0])
+    rows, h = add_rmsnorm_int8(x, x, torch.ones(300, device="cuda", dtype=BF16))
+    y = int8_linear(rows, weight, out_dtype=FP32)
+    assert y.shape == (3, 7, 96)
+    ref, terms = linear(rows.padded[:, :300].cpu(), rows.scale.cpu(), w, ws)
+    _within(y.view(21, 96), ref, terms, 6, "y")
+    one = x[0, 0]
+    assert torch.equal(int8_linear(one, weight), int8_linear(x, weight)[0, 0])
+    assert torch.equal(quantize_int8_rows(one).values, quantize_int8_rows(x).values[0, 0])
+
+
+@pytest.mark.gpu
+def test_weights_from_floats():
+    from kernels.int8 import Int8Weight
+
+    g = torch.Generator().manual_seed(6)
+    w = torch.randn(70, 130, generator=g).to(BF16)
+    q, s = quantize(w)
+    weight = Int8Weight.from_float(w.cuda(), backward=True)
+    assert torch.equal(weight.values.cpu().long(), q)
+    torch.testing.assert_close(weight.scale.cpu().double(), s, rtol=4 * U, atol=0)
+    assert torch.equal(weight.transposed[:, :70], weight.values.t()) and bool((weight.transposed[:, 70:] == 0).all())
+    torch.testing.assert_close(weight.dequantize().cpu().double(), q * s.unsqueeze(1), rtol=1e-6, atol=0)
+
+
+@pytest.mark.gpu
+def test_not_finite_rows_and_nothing_to_do():
+    from kernels.int8 import Int8Weight, int8_linear
+
+    w, ws = _weight(40, 64)
+    weight = Int8Weight(w.cuda(), ws.cuda(), backward=True)
+    x = torch.randn(5, 64, device="cuda")
+    x[1, 3] = float("nan")
+    x[2, 5] = float("-inf")
+    x[3] = 0
+    y = int8_linear(x, weight)
+    assert bool(torch.isnan(y[1:3]).all()) and bool((y[3] == 0).all()) and bool(torch.isfinite(y[[0, 3, 4]]).all())
+    z = torch.zeros(0, 64, device="cuda", requires_grad=True)
+    out = int8_linear(z, weight)
+    assert out.shape == (0, 40) and torch.autograd.grad(out, z, torch.zeros_like(out))[0].shape == (0, 64)
+    # no columns, no channels
+    empty = Int8Weight(torch.zeros(3, 0, dtype=torch.int8, device="cuda"), torch.ones(3, device="cuda"))
+    b = torch.arange(3.0, device="cuda")
+    assert torch.equal(int8_linear(torch.zeros(2, 0, device="cuda"), empty, b), b.expand(2, 3))
+    none = Int8Weight(torch.zeros(0, 64, dtype=torch.int8, device="cuda"), torch.ones(0, device="cuda"))
+    assert int8_linear(x, none).shape == (5, 0)
+
+
+@pytest.mark.gpu
+def test_strided_inputs():
+    from kernels.int8 import Int8Weight, int8_linear
+
+    w, ws = _weight(40, 64)
+    weight = Int8Weight(w.cuda(), ws.cuda(), backward=True)
+    wide = torch.randn(9, 131, device="cuda").to(BF16)
+    for x in (wide[:, 1:65], wide[:, ::2][:, :64], wide[0, :64].expand(9, 64), wide[:, :64].t().contiguous().t()):
+        y = int8_linear(x, weight)
+        assert torch.equal(y, int8_linear(x.contiguous(), weight))
+        xg = x.detach().requires_grad_(True)
+        dy = torch.randn(40, 9, device="cuda").to(BF16).t()
+        got = torch.autograd.grad(int8_linear(xg, weight), xg, dy)[0]
+        xc = x.contiguous().detach().requires_grad_(True)
+        assert torch.equal(got, torch.autograd.grad(int8_linear(xc, weight), xc, dy.contiguous())[0])
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_gpu():
+    from kernels.int8 import Int8Weight, int8_linear, quantize_int8_rows
+
+    w, ws = _weight(40, 64)
+    weight = Int8Weight(w.cuda(), ws.cuda())
+    x = torch.zeros(2, 64, device="cuda", requires_grad=True)
+    with pytest.raises(ValueError, match="backward=True"):
+        int8_linear(x, weight)
+    with pytest.raises(ValueError, match="no gradient"):
+        quantize_int8_rows(x)
+    x = x.detach()
+    with pytest.raises(ValueError, match="columns"):
+        int8_linear(x[:, :63], weight)
+    with pytest.raises(ValueError, match="frozen"):
+        int8_linear(x, weight, torch.zeros(40, device="cuda", requires_grad=True))
+    with pytest.raises(ValueError, match="bias"):
+        int8_linear(x, weight, torch.zeros(39, device="cuda"))
+    with pytest.raises(TypeError, match="out_dtype"):
+        int8_linear(x, weight, out_dtype=torch.float64)
+    with pytest.raises(TypeError, match="Int8Weight"):
+        int8_linear(x, w.cuda())
+    with pytest.raises(TypeError, match="fp16, bf16 or fp32"):
+        int8_linear(x.double(), weight)
+
+
+def test_refusals():
+    from kernels.int8 import Int8Weight, quantize_int8_rows
+
+    w, ws = _weight(4, 8)
+    with pytest.raises(ValueError, match="int8 matrix"):
+        Int8Weight(w.float(), ws)
+    with pytest.raises(ValueError, match="scale"):
+        Int8Weight(w, ws[:3])
+    with pytest.raises(ValueError, match="32 bits"):
+        Int8Weight(torch.zeros(1, (1 << 17) + 1, dtype=torch.int8), ws[:1])
+    with pytest.raises(RuntimeError, match="GPU"):
+        Int8Weight(w, ws)
+    with pytest.raises(RuntimeError, match="GPU"):
+        quantize_int8_rows(torch.zeros(2, 8))
+
+
+def test_entry_point_refusals():
+    from forge_hip import _lib as L
+
+    def gemm(a=16, lda=64, rs=16, b=16, ldb=64, cs=16, c=16, ldc=40, dtype=2, M=4, N=40, K=64):
+        return L.forge_int8_gemm(a, lda, rs, b, ldb, cs, None, c, ldc, dtype, M, N, K, None)
+
+    assert gemm(dtype=3) == 2
+    for kw in ({"M": -1}, {"K": (1 << 17) + 1}, {"lda": 48}, {"ldb": 72}, {"lda": 1 << 22}, {"a": 24}, {"b": 8}, {"ldc": 39},
+               {"a": None}, {"b": None}, {"rs": None}, {"cs": None}, {"c": None}):
+        assert gemm(**kw) == 1, kw
+    assert gemm(M=0, a=None, c=None) == 0
+    assert L.forge_transpose_1b(None, 8, 4, 8, 16, 16, None) == 1
+    assert L.forge_transpose_1b(16, 7, 4, 8, 16, 16, None) == 1
+    assert L.forge_quantize_rows(2, 16, 8, None, 16, 8, 16, 2, 8, None) == 1
