@@ -96,12 +96,80 @@ __device__ __forceinline__ TileAt find_tile(const int32_t* cu, int B, int64_t to
     const uint64_t past = __ballot(sum > t);
     if (past) {
       const int at = __builtin_ctzll(past);
-      const int before = __shfl(sum - n, at, 64);
-      return {__builtin_amdgcn_readfirstlane(base + at), __builtin_amdgcn_readfirstlane(t - before)};
+      return {base + at, t - __builtin_amdgcn_readlane(sum - n, at)};
     }
-    t -= __shfl(sum, 63, 64);
+    t -= __builtin_amdgcn_readlane(sum, 63);
   }
   return {B + 1, 0};
+}
+
+// The same tiles in the order of `level`, the number of the tile from its
+// sequence's other end: the first tile of n has level n for the keys, the last
+// one for the queries, so that (causal) the tiles with the most work come first
+// and the last workgroups to start are short ones.  With the sequences' order
+// the dk, dv kernel ran 1285 us instead of ORDERED_US (8 sequences of 700 to 3400
+// tokens, 32 heads on 8: the longest began in the last round).  More than 256
+// sequences go in their own order: there are many tiles then, and short ones.
+struct LevelAt {
+  int seq, level;  // level: 1 .. tiles of the sequence
+};
+
+__device__ __forceinline__ int wave_sum_int(int v) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+// (What follows from it is the same in all lanes, and has to be seen as that: a
+// sequence's length in vector registers drove the dk, dv kernel's others to
+// scratch memory.)
+__device__ __forceinline__ LevelAt find_level(const int32_t* cu, int B, int64_t total, int rows, int t) {
+  if (!cu) {
+    const int per = (int)((total + rows - 1) / rows);
+    if (per == 0 || t >= per * B) return {B + 1, 1};
+    return {t % B, per - t / B};
+  }
+  if (B > 254) {
+    const TileAt at = find_tile(cu, B, total, rows, t);
+    if (at.seq > B) return {B + 1, 1};
+    return {at.seq, (span_of(cu, B, total, at.seq).len + rows - 1) / rows - at.tile};
+  }
+  const int lane = threadIdx.x % 64;
+  int n[4], top = 0;  // tiles of sequences -1 + 64 c + lane
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int s = -1 + 64 * c + lane;
+    n[c] = s <= B ? (span_of(cu, B, total, s).len + rows - 1) / rows : 0;
+    top = max(top, n[c]);
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) top = max(top, __shfl_xor(top, off, 64));
+  top = __builtin_amdgcn_readfirstlane(top);
+  auto from = [&](int level) {  // tiles of this level and above
+    int sum = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) sum += max(0, n[c] - level + 1);
+    return wave_sum_int(sum);
+  };
+  if (from(1) <= t) return {B + 1, 1};
+  int lo = 1, hi = top;  // the largest level with more than t tiles from it on
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (from(mid) > t) lo = mid;
+    else hi = mid - 1;
+  }
+  int left = t - from(lo + 1);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const uint64_t has = __ballot(n[c] >= lo);
+    const int count = __builtin_popcountll(has);
+    if (left < count) {
+      const bool mine = (has >> lane & 1) && __builtin_popcountll(has & ((uint64_t(1) << lane) - 1)) == left;
+      return {-1 + 64 * c + (int)__builtin_ctzll(__ballot(mine)), lo};
+    }
+    left -= count;
+  }
+  return {B + 1, 1};
 }
 
 // At most this many tiles of `rows` rows (host).
@@ -111,26 +179,34 @@ inline int64_t most_tiles(const int32_t* cu, int B, int64_t total, int rows) {
 }
 
 // ---------------------------------------------------------------------------
-// LDS tiles: rows of DP 16-bit values (DP = 64, 128 or 256), unpadded, the
-// 16-byte chunks of a row exchanged by an XOR with a function of the row.  A
-// fragment is read either by rows (32 rows, one chunk each: 16 neighbouring
-// rows must lie in different chunks of the 256-byte bank cycle) or transposed
-// (four rows, 64 bytes each: those must lie in different quarters of it).
-// Both hold for
-//   256- and 512-byte rows: 4 (row % 4) + row / 4 % 4
-//   128-byte rows (two in a bank cycle): 4 (row / 2 % 2) + row / 4 % 4.
+// LDS tiles: rows of DP 16-bit values (DP = 64, 128 or 256) in units of 4 rows (8
+// of 128 bytes), 16 bytes between units; in a unit the 16-byte chunks of a row
+// are exchanged by an XOR with f(row).  A fragment is read either by rows (32
+// rows, one chunk each: 16 neighbouring rows must lie in different chunks of the
+// 256-byte bank cycle) or transposed (four rows, 64 bytes each: those must lie in
+// different quarters of it).  Both hold: f exchanges the quarters among the rows of a
+// unit, and the gaps shift the units by a chunk each.  As f changes few bits of a
+// chunk's number and nothing beyond a unit, most of a read's address is an
+// immediate: four bases a lane serve all reads of one kind (an XOR of all four
+// bits, without gaps, took 16, and the dk, dv kernel kept them in scratch memory).
 // ---------------------------------------------------------------------------
 template <int DP>
-__device__ __forceinline__ int swz_rows(int row) {
-  if constexpr (DP == 64) return 4 * ((row >> 1) & 1) + ((row >> 2) & 3);
-  else return 4 * (row & 3) + ((row >> 2) & 3);
-}
+struct Tile {
+  static constexpr int RB = DP * 2, CPR = RB / 16;  // bytes and chunks of a row
+  static constexpr int UNIT = DP == 64 ? 8 : 4;     // rows of a unit
+  static constexpr int UB = UNIT * RB + 16;         // bytes from unit to unit
+  static constexpr int bytes(int rows) { return rows / UNIT * UB; }
+  static __device__ __forceinline__ int f(int row) {
+    if constexpr (DP == 64) return 4 * ((row >> 1) & 1) + 2 * ((row >> 2) & 1);
+    else return 4 * (row & 3);
+  }
+};
 
 // One LDS-DMA instruction: 16 (4) bytes of each lane, from its offset to lds +
 // 16 (4) lane.  (The host's pass over this code does not know the 16-byte form.)
-__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t off) {
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t off, int scalar_off) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, off, 0, 0, 0);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, off, scalar_off, 0, 0);
 #endif
 }
 __device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t r, void* lds, uint32_t off) {
@@ -139,74 +215,101 @@ __device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t r, void* lds, uint32
 #endif
 }
 
-// LDS-DMA of ROWS rows by NW waves: instruction j of wave w fills 1 KB.
+// LDS-DMA of ROWS rows by NW waves: an instruction fills 1 KB (half a unit at DP = 256).
 template <int DP, int ROWS, int NW>
 struct TileDma {
-  static constexpr int RB = DP * 2, CPR = RB / 16, RPI = 64 / CPR, N = ROWS / RPI / NW;
-  static_assert(ROWS % (RPI * NW) == 0 && N >= 1, "whole instructions");
-  static constexpr int BYTES = ROWS * RB;
-  uint32_t off[N];  // byte offset of this lane's chunk from the tile's first row (OOB: past D)
-  int row[N];       // its row
+  typedef Tile<DP> L;
+  static constexpr int RPI = 64 / L::CPR, N = ROWS / RPI / NW;  // rows of an instruction, instructions of a wave
+  static_assert(ROWS % (RPI * NW) == 0 && N >= 1 && (DP < 256 || N % 2 == 0), "whole instructions and units");
+  static constexpr int BYTES = L::bytes(ROWS);
+  int step;             // bytes of RPI rows
+  uint32_t off[DP == 256 ? 2 : 1];  // this lane's chunk from the instruction's first row (OOB: past D), by parity
 
-  __device__ __forceinline__ void setup(int64_t row_stride, int D, int wave) {
+  __device__ __forceinline__ void setup(int64_t row_stride, int D) {
     const int lane = threadIdx.x % 64;
+    step = (int)(row_stride * 2) * RPI;
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      row[j] = (wave * N + j) * RPI + lane / CPR;
-      const int chunk = (lane % CPR) ^ swz_rows<DP>(row[j]);
-      off[j] = chunk * 8 < D ? (uint32_t)(row[j] * (int)(row_stride * 2) + chunk * 16) : OOB;
+    for (int p = 0; p < (DP == 256 ? 2 : 1); ++p) {
+      const int row = p * RPI + lane / L::CPR, chunk = (lane % L::CPR) ^ L::f(row);
+      off[p] = chunk * 8 < D ? (uint32_t)(lane / L::CPR * (int)(row_stride * 2) + chunk * 16) : OOB;
     }
   }
-  // rows from `left` on do not exist and read as zeros
+  // rows from `left` on do not exist and read as zeros, as do columns from D on
   __device__ __forceinline__ void load(const void* first, int left, char* dst, int wave) const {
     const __amdgpu_buffer_rsrc_t r = make_rsrc(first);
+    const int lane_row = threadIdx.x % 64 / L::CPR;
 #pragma unroll
-    for (int j = 0; j < N; ++j)
-      dma16(r, dst + (wave * N + j) * 1024, row[j] < left ? off[j] : OOB);
+    for (int j = 0; j < N; ++j) {
+      const int i = wave * N + j;
+      char* to = dst + (DP == 256 ? i / 2 * L::UB + i % 2 * 1024 : i * L::UB);
+      const uint32_t o = off[DP == 256 ? j % 2 : 0];
+      dma16(r, to, i * RPI + lane_row < left ? o : OOB, i * step);
+    }
   }
 };
 
-// Fragment by rows: rows r0 .. r0 + 31 (r0 a multiple of 32), columns 16 ks .. + 15:
+// Fragments by rows: rows r0 .. r0 + 31 (r0 a multiple of 32), columns 16 ks .. + 15:
 // lane l holds row l % 32, columns 16 ks + 8 (l / 32) .. + 7.
 template <int DP>
-__device__ __forceinline__ bf16x8 frag_rows(const char* tile, int r0, int ks, int lane) {
-  const int row = r0 + lane % 32;
-  return *reinterpret_cast<const bf16x8*>(tile + row * (DP * 2) + (((2 * ks + lane / 32) ^ swz_rows<DP>(lane % 32)) << 4));
-}
+struct RowFrag {
+  typedef Tile<DP> L;
+  int base[4];  // of the chunks whose bits that f changes are those of 0 .. 3
+  __device__ __forceinline__ void setup(int lane) {
+    const int row = lane % 32, h = lane / 32;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      base[i] = row / L::UNIT * L::UB + row % L::UNIT * L::RB + ((((DP == 64 ? 2 : 4) * i + h) ^ L::f(row)) << 4);
+  }
+  __device__ __forceinline__ bf16x8 read(const char* tile, int r0, int ks) const {
+    const int at = r0 / L::UNIT * L::UB + (DP == 64 ? 0 : ks % 2 * 32 + ks / 8 * 256);
+    return *reinterpret_cast<const bf16x8*>(tile + base[DP == 64 ? ks : ks / 2 % 4] + at);
+  }
+};
 
-// Fragment of the transposed tile: columns c0 .. c0 + 31 (lane l holds column c0
+// Fragments of the transposed tile: columns 32 db .. + 31 (lane l holds column 32 db
 // + l % 32), rows r0 + 4 h + {0 .. 3} and r0 + 8 + 4 h + {0 .. 3}, h = l / 32, r0 a
 // multiple of 16: the rows in the order in which an accumulator of 32 x 32
 // holds them, so that its registers 8 i .. 8 i + 7, rounded, are the other operand.
 template <int DP>
-struct TrOff {
-  int lo, hi;  // byte offsets of the two reads at r0 = c0 = 0
+struct ColFrag {
+  typedef Tile<DP> L;
+  static constexpr int NB = DP == 64 ? 2 : 4;
+  int base[NB];
   __device__ __forceinline__ void setup(int lane) {
-    const int h = lane / 32, q = 4 * h + (lane % 16) / 4, c = 16 * ((lane / 16) % 2) + 4 * (lane % 4);
-    lo = q * (DP * 2) + (((c / 8) ^ swz_rows<DP>(q)) << 4) + (c % 8) * 2;
-    const int q8 = q + 8;
-    hi = q8 * (DP * 2) + (((c / 8) ^ swz_rows<DP>(q8)) << 4) + (c % 8) * 2;
+    const int q = 4 * (lane / 32) + lane % 16 / 4, c = 16 * (lane / 16 % 2) + 4 * (lane % 4);
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+      base[i] = q / L::UNIT * L::UB + q % L::UNIT * L::RB + (((4 * i + c / 8) ^ L::f(q)) << 4) + c % 8 * 2;
+  }
+  __device__ __forceinline__ bf16x8 read(const char* tile, int r0, int db) const {
+    const char* p = tile + base[db % NB] + r0 / L::UNIT * L::UB + db / NB * 256;
+    return tr_frag(p, p + 8 / L::UNIT * L::UB);
   }
 };
-// columns 32 db: chunks 4 db, an XOR of bits 6 and up of the offset with the row's swizzle in place
-template <int DP>
-__device__ __forceinline__ bf16x8 frag_cols(const char* tile, const TrOff<DP>& t, int r0, int db) {
-  const char* p = tile + r0 * (DP * 2);
-  return tr_frag(p + (t.lo ^ (db << 6)), p + (t.hi ^ (db << 6)));
-}
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// two values rounded to 16 bits (nearest even), in one word
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef T t2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), t2));
+}
 
 // registers 8 i .. 8 i + 7 of an accumulator as an operand
 template <class T>
 __device__ __forceinline__ bf16x8 pack_acc(const f32x16& a, int i) {
   uint32_t w[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const T lo = (T)a[8 * i + 2 * j], hi = (T)a[8 * i + 2 * j + 1];
-    w[j] = (uint32_t)__builtin_bit_cast(uint16_t, lo) | ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
-  }
+  for (int j = 0; j < 4; ++j) w[j] = pack2<T>(a[8 * i + 2 * j], a[8 * i + 2 * j + 1]);
   return __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+}
+
+// four values rounded and stored
+template <class T>
+__device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(a, b), pack2<T>(c, d));
 }
 
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }

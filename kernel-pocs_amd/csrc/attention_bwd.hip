@@ -1,10 +1,10 @@
 // Attention backward for gfx950: three launches, no atomics (the sums have a
 // fixed order).
-//   delta_i = sum_d o_i dout_i, and lse in units of log2, by head and query;
+//   -delta_i, delta_i = sum_d o_i dout_i, and -lse_i / scale, by head and query;
 //   dq_i = scale sum_j ds_ij k_j,       a workgroup to 128 queries of a head;
 //   dv_j = sum_i p_ij dout_i, dk_j = scale sum_i ds_ij q_i over the queries of the
 //   group's heads,                      a workgroup to 128 keys of a kv head,
-// with p_ij = exp2(s_ij c - lse_i) computed again and ds_ij = p_ij (dout_i . v_j -
+// with p_ij = exp2((s_ij - lse_i / scale) c), c = scale log2(e), computed again and ds_ij = p_ij (dout_i . v_j -
 // delta_i).  p and ds are rounded to 16 bits as operands; every sum is in fp32.
 // As in the forward, products are laid out so that p and ds stay in the
 // registers that they are computed in: keys x queries for dq, queries x keys for
@@ -15,7 +15,7 @@ namespace fattn {
 
 // rows [batch][row] of the query side, one wave to a (row, head) at a time
 template <class T>
-__global__ __launch_bounds__(256) void attn_delta_kernel(Args a, float* lse2, int64_t n_rows, int64_t pairs) {
+__global__ __launch_bounds__(256) void attn_delta_kernel(Args a, float* shift, int64_t n_rows, int64_t pairs) {
   const int lane = threadIdx.x % 64;
   // 16 lanes to a (row, head), D / 8 chunks of 8
   for (int64_t p = ((int64_t)blockIdx.x * 256 + threadIdx.x) / 16; p < pairs; p += (int64_t)gridDim.x * 16) {
@@ -34,15 +34,15 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(Args a, float* lse2, in
     for (int off = 8; off >= 1; off /= 2) sum += __shfl_xor(sum, off, 64);
     if (lane % 16 == 0) {
       const float l = a.lse[row * a.H + head];
-      a.delta[head * n_rows + row] = sum;
-      // a query without keys: exp2(s - inf) = 0
-      lse2[head * n_rows + row] = l == -__builtin_inff() ? __builtin_inff() : l * LOG2E;
+      a.delta[head * n_rows + row] = -sum;
+      // a query without keys: exp(scale (s - inf)) = 0
+      shift[head * n_rows + row] = l == -__builtin_inff() ? -__builtin_inff() : -l / a.scale;
     }
   }
 }
 
 template <class T, int DP>
-__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dq_kernel(Args a, const float* lse2, int64_t n_rows, int tiles) {
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dq_kernel(Args a, const float* shift_of, int64_t n_rows, int tiles) {
   constexpr int BM = 128, BN = 64, KS = DP / 16, DB = DP / 32;
   using Dma = TileDma<DP, BN, 4>;
   __shared__ __attribute__((aligned(1024))) char smem[(DP == 256 ? 2 : 4) * Dma::BYTES];
@@ -51,13 +51,13 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dq_kernel(Args a,
   const int G = a.H / a.Hkv, h = lane / 32;
   const Item it = item_of(blockIdx.x, tiles, a.Hkv, G);
   if (it.tile >= tiles) return;
-  const TileAt at = find_tile(a.cu_q, a.B, a.tq, BM, it.tile);
+  const LevelAt at = find_level(a.cu_q, a.B, a.tq, BM, it.tile);
   if (at.seq > a.B) return;
   const Span sq = span_of(a.cu_q, a.B, a.tq, at.seq);
   Span sk = span_of(a.cu_k, a.B, a.tk, at.seq);
   if (at.seq < 0 || at.seq >= a.B) sk.len = 0;
   const int head = it.kv * G + it.g;
-  const int q0 = ((sq.len + BM - 1) / BM - 1 - at.tile) * BM;
+  const int q0 = (at.level - 1) * BM;
   const int shift = sk.len - sq.len;
   const int rows = min(BM, sq.len - q0);
   const int k_end = a.causal ? min(sk.len, q0 + rows + shift) : sk.len;
@@ -81,37 +81,38 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dq_kernel(Args a,
     }
   }
   const int64_t row = a.cu_q ? sq.start + iq : sq.batch * a.tq + iq;
-  const float lse = live ? lse2[head * n_rows + row] : __builtin_inff();
+  const float c = a.scale * LOG2E;
+  const float below = live ? shift_of[head * n_rows + row] * c : -__builtin_inff();
   const float delta = live ? a.delta[head * n_rows + row] : 0.f;
 
   Dma kd, vd;
-  kd.setup(a.k.row, a.D, wave);
-  vd.setup(a.v.row, a.D, wave);
+  kd.setup(a.k.row, a.D);
+  vd.setup(a.v.row, a.D);
   const T* kp = row_ptr<T>(a.k, sk.batch, sk.start, it.kv);
   const T* vp = row_ptr<T>(a.v, sk.batch, sk.start, it.kv);
-  auto issue = [&](int t) {
-    char* st = smem + (t % NST) * 2 * Dma::BYTES;
+  auto issue = [&](int t, int slot) {
+    char* st = smem + slot * 2 * Dma::BYTES;
     kd.load(kp + (int64_t)t * BN * a.k.row, sk.len - t * BN, st, wave);
     vd.load(vp + (int64_t)t * BN * a.v.row, sk.len - t * BN, st + Dma::BYTES, wave);
   };
-  TrOff<DP> tr;
-  tr.setup(lane);
+  RowFrag<DP> fr;
+  ColFrag<DP> fc;
+  fr.setup(lane);
+  fc.setup(lane);
   f32x16 acc[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[db][r] = 0.f;
-  const float c = a.scale * LOG2E;
   const int sees = a.causal ? min(sk.len, iq + shift + 1) : sk.len;
   const int all_see = a.causal ? min(sk.len, wq + shift + 1) : sk.len;
   const int any_sees = a.causal ? min(sk.len, min(wq + 32, sq.len) + shift) : (wq < sq.len ? sk.len : 0);
 
-  if (n_t > 0) issue(0);
-  for (int t = 0; t < n_t; ++t) {
+  auto step = [&](int t, int slot) __attribute__((always_inline)) {
     wait_dma<0>();
     barrier();
-    if (NST == 2 && t + 1 < n_t) issue(t + 1);
-    const char* kt = smem + (t % NST) * 2 * Dma::BYTES;
+    if (NST == 2 && t + 1 < n_t) issue(t + 1, 1 - slot);
+    const char* kt = smem + slot * 2 * Dma::BYTES;
     const char* vt = kt + Dma::BYTES;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
@@ -121,11 +122,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dq_kernel(Args a,
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s = mfma32<T>(frag_rows<DP>(kt, 32 * kb, ks, lane), qf[ks], s);
+      for (int ks = 0; ks < KS; ++ks) s = mfma32<T>(fr.read(kt, 32 * kb, ks), qf[ks], s);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) dp = mfma32<T>(frag_rows<DP>(vt, 32 * kb, ks, lane), df[ks], dp);
+      for (int ks = 0; ks < KS; ++ks) dp = mfma32<T>(fr.read(vt, 32 * kb, ks), df[ks], dp);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = exp2_hw(__builtin_fmaf(s[r], c, -lse)) * (dp[r] - delta);
+      for (int r = 0; r < 16; ++r) s[r] = exp2_hw(__builtin_fmaf(s[r], c, below)) * (dp[r] + delta);
       if (k0 + 32 > all_see) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -135,14 +136,19 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dq_kernel(Args a,
       for (int i = 0; i < 2; ++i) {
         const bf16x8 ds = pack_acc<T>(s, i);
 #pragma unroll
-        for (int db = 0; db < DB; ++db) acc[db] = mfma32<T>(frag_cols<DP>(kt, tr, 32 * kb + 16 * i, db), ds, acc[db]);
+        for (int db = 0; db < DB; ++db) acc[db] = mfma32<T>(fc.read(kt, 32 * kb + 16 * i, db), ds, acc[db]);
       }
     }
     if (NST == 1 && t + 1 < n_t) {
       wait_dma<0>();
       barrier();  // every wave has read the tile
-      issue(t + 1);
+      issue(t + 1, 0);
     }
+  };
+  if (n_t > 0) issue(0, 0);
+  for (int t = 0; t < n_t; t += NST) {
+    step(t, 0);
+    if (NST == 2 && t + 1 < n_t) step(t + 1, 1);
   }
   if (!live) return;
   T* op = row_ptr<T>(a.dq, sq.batch, sq.start + iq, head);
@@ -152,13 +158,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dq_kernel(Args a,
     for (int i = 0; i < 4; ++i) {
       const int d = 32 * db + 8 * i + 4 * h;
       if (d >= a.D) continue;
-      uint32_t w[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const T lo = (T)(acc[db][4 * i + 2 * j] * a.scale), hi = (T)(acc[db][4 * i + 2 * j + 1] * a.scale);
-        w[j] = (uint32_t)__builtin_bit_cast(uint16_t, lo) | ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
-      }
-      *reinterpret_cast<uint2*>(op + d) = make_uint2(w[0], w[1]);
+      store4(op + d, acc[db][4 * i] * a.scale, acc[db][4 * i + 1] * a.scale, acc[db][4 * i + 2] * a.scale,
+             acc[db][4 * i + 3] * a.scale);
     }
 }
 
@@ -166,7 +167,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dq_kernel(Args a,
 // gradients in registers: one wave a SIMD.  At DP = 256 those take more registers
 // than there are, so dk and dv are a launch each (DK, DV).
 template <class T, int DP, bool DK, bool DV>
-__global__ __launch_bounds__(256, 1) void attn_dkv_kernel(Args a, const float* lse2, int64_t n_rows, int tiles) {
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a, const float* shift_of, int64_t n_rows, int tiles) {
   constexpr int BN = 128, BQ = DP == 256 ? 32 : 64, KS = DP / 16, DB = DP / 32;
   using Dma = TileDma<DP, BQ, 4>;
   __shared__ __attribute__((aligned(1024))) char smem[2 * 2 * Dma::BYTES];
@@ -175,12 +176,12 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(Args a, const float* l
   const int G = a.H / a.Hkv, h = lane / 32;
   const Item it = item_of(blockIdx.x, tiles, a.Hkv, 1);
   if (it.tile >= tiles) return;
-  const TileAt at = find_tile(a.cu_k, a.B, a.tk, BN, it.tile);
+  const LevelAt at = find_level(a.cu_k, a.B, a.tk, BN, it.tile);
   if (at.seq > a.B) return;
   const Span sk = span_of(a.cu_k, a.B, a.tk, at.seq);
   Span sq = span_of(a.cu_q, a.B, a.tq, at.seq);
   if (at.seq < 0 || at.seq >= a.B) sq.len = 0;
-  const int k0 = at.tile * BN, wk = k0 + wave * 32, jk = wk + lane % 32;
+  const int k0 = ((sk.len + BN - 1) / BN - at.level) * BN, wk = k0 + wave * 32, jk = wk + lane % 32;
   const bool live = jk < sk.len;
   const int shift = sk.len - sq.len;
   bf16x8 kf[KS], vf[KS];
@@ -199,26 +200,35 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(Args a, const float* l
       vf[ks] = __builtin_bit_cast(bf16x8, w);
     }
   }
-  // the first query that sees a key of the tile, and tiles of queries from there
+  // the first query that sees a key of the tile, and tiles of queries from there, of
+  // each of the group's heads in turn
   const int first = a.causal ? max(0, k0 - shift) / BQ * BQ : 0;
-  const int per = sq.len > first ? (sq.len - first + BQ - 1) / BQ : 0, n_t = per * G;
+  const int n_t = sq.len > first ? (sq.len - first + BQ - 1) / BQ * G : 0;
   Dma qd, dd;
-  qd.setup(a.q.row, a.D, wave);
-  dd.setup(a.dout.row, a.D, wave);
-  auto issue = [&](int t) {
-    const int head = it.kv * G + t / per, i0 = first + t % per * BQ, left = sq.len - i0;
-    char* st = smem + (t % 2) * 2 * Dma::BYTES;
-    qd.load(row_ptr<T>(a.q, sq.batch, sq.start + i0, head), left, st, wave);
-    dd.load(row_ptr<T>(a.dout, sq.batch, sq.start + i0, head), left, st + Dma::BYTES, wave);
+  qd.setup(a.q.row, a.D);
+  dd.setup(a.dout.row, a.D);
+  int next_i = first, next_head = it.kv * G;  // of the tile that is issued next
+  auto issue = [&](int slot) {
+    const int left = sq.len - next_i;
+    char* st = smem + slot * 2 * Dma::BYTES;
+    qd.load(row_ptr<T>(a.q, sq.batch, sq.start + next_i, next_head), left, st, wave);
+    dd.load(row_ptr<T>(a.dout, sq.batch, sq.start + next_i, next_head), left, st + Dma::BYTES, wave);
     // (rows that do not exist: q = dout = 0, so p = exp2(0) and ds = 0 add zeros)
-    const int64_t row = a.cu_q ? sq.start + i0 : sq.batch * a.tq + i0;
+    const int64_t row = (a.cu_q ? sq.start : sq.batch * a.tq) + next_i;
     if (wave < 2) {
-      const __amdgpu_buffer_rsrc_t r = make_rsrc((wave ? a.delta : lse2) + head * n_rows + row);
-      dma4(r, &stat[t % 2][wave][0], lane < left && lane < BQ ? lane * 4 : OOB);
+      const __amdgpu_buffer_rsrc_t r = make_rsrc((wave ? a.delta : shift_of) + next_head * n_rows + row);
+      dma4(r, &stat[slot][wave][0], lane < left && lane < BQ ? lane * 4 : OOB);
+    }
+    next_i += BQ;
+    if (next_i >= sq.len) {
+      next_i = first;
+      ++next_head;
     }
   };
-  TrOff<DP> tr;
-  tr.setup(lane);
+  RowFrag<DP> fr;
+  ColFrag<DP> fc;
+  fr.setup(lane);
+  fc.setup(lane);
   f32x16 dk[DB], dv[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db)
@@ -226,51 +236,63 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(Args a, const float* l
     for (int r = 0; r < 16; ++r) dk[db][r] = dv[db][r] = 0.f;
   const float c = a.scale * LOG2E;
 
-  if (n_t > 0) issue(0);
-  for (int t = 0; t < n_t; ++t) {
+  int tile_i = first;
+  auto step = [&](bool more, int slot) __attribute__((always_inline)) {
     wait_dma<0>();
     barrier();
-    if (t + 1 < n_t) issue(t + 1);
-    const char* qt = smem + (t % 2) * 2 * Dma::BYTES;
+    if (more) issue(1 - slot);
+    const int t_i = tile_i;
+    tile_i = tile_i + BQ < sq.len ? tile_i + BQ : first;
+    const char* qt = smem + slot * 2 * Dma::BYTES;
     const char* dt = qt + Dma::BYTES;
 #pragma unroll
     for (int qb = 0; qb < BQ / 32; ++qb) {
-      const int i0 = first + t % per * BQ + 32 * qb;
+      __builtin_amdgcn_sched_barrier(0);
+      const int i0 = t_i + 32 * qb;
       // (causal: the last query of the block sees nothing of this wave's keys)
       if (i0 >= sq.len || wk >= sk.len || (a.causal && i0 + 31 + shift < wk)) continue;
-      f32x16 s, dp;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s = mfma32<T>(frag_rows<DP>(qt, 32 * qb, ks, lane), kf[ks], s);
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        if constexpr (DK) dp = mfma32<T>(frag_rows<DP>(dt, 32 * qb, ks, lane), vf[ks], dp);
-      const bool edge = a.causal && i0 + shift < wk + 31;
+      f32x16 s, dp;  // begin with -lse / scale and -delta of their queries
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const f32x4 ls = *reinterpret_cast<const f32x4*>(&stat[t % 2][0][32 * qb + 8 * i + 4 * h]);
-        const f32x4 de = *reinterpret_cast<const f32x4*>(&stat[t % 2][1][32 * qb + 8 * i + 4 * h]);
+        const f32x4 x = *reinterpret_cast<const f32x4*>(&stat[slot][0][32 * qb + 8 * i + 4 * h]);
+        const f32x4 y = *reinterpret_cast<const f32x4*>(&stat[slot][1][32 * qb + 8 * i + 4 * h]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int r = 4 * i + j;
-          float p = exp2_hw(__builtin_fmaf(s[r], c, -ls[j]));
-          float d = p * (dp[r] - de[j]);
-          if (edge && i0 + 8 * i + 4 * h + j + shift < jk) p = d = 0.f;
-          s[r] = p;
-          dp[r] = d;
+          s[4 * i + j] = x[j];
+          dp[4 * i + j] = y[j];
         }
       }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s = mfma32<T>(fr.read(qt, 32 * qb, ks), kf[ks], s);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        if constexpr (DK) dp = mfma32<T>(fr.read(dt, 32 * qb, ks), vf[ks], dp);
+      if (a.causal && i0 + shift < wk + 31) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (i0 + 8 * (r / 4) + 4 * h + r % 4 + shift < jk) s[r] = -__builtin_inff();
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[r] = exp2_hw(s[r] * c);
+        dp[r] *= s[r];
+      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const bf16x8 p = pack_acc<T>(s, i), ds = pack_acc<T>(dp, i);
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
-          if constexpr (DV) dv[db] = mfma32<T>(frag_cols<DP>(dt, tr, 32 * qb + 16 * i, db), p, dv[db]);
-          if constexpr (DK) dk[db] = mfma32<T>(frag_cols<DP>(qt, tr, 32 * qb + 16 * i, db), ds, dk[db]);
+          if constexpr (DV) dv[db] = mfma32<T>(fc.read(dt, 32 * qb + 16 * i, db), p, dv[db]);
+          if constexpr (DK) dk[db] = mfma32<T>(fc.read(qt, 32 * qb + 16 * i, db), ds, dk[db]);
         }
       }
     }
+  };
+  if (n_t > 0) issue(0);
+  for (int t = 0; t < n_t; t += 2) {
+    step(t + 1 < n_t, 0);
+    if (t + 1 < n_t) step(t + 2 < n_t, 1);
   }
   if (!live) return;
   T* kp = row_ptr<T>(a.dk, sk.batch, sk.start + jk, it.kv);
@@ -281,52 +303,45 @@ __global__ __launch_bounds__(256, 1) void attn_dkv_kernel(Args a, const float* l
     for (int i = 0; i < 4; ++i) {
       const int d = 32 * db + 8 * i + 4 * h;
       if (d >= a.D) continue;
-      uint32_t w[2], x[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        T lo = (T)(dk[db][4 * i + 2 * j] * a.scale), hi = (T)(dk[db][4 * i + 2 * j + 1] * a.scale);
-        w[j] = (uint32_t)__builtin_bit_cast(uint16_t, lo) | ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
-        lo = (T)dv[db][4 * i + 2 * j];
-        hi = (T)dv[db][4 * i + 2 * j + 1];
-        x[j] = (uint32_t)__builtin_bit_cast(uint16_t, lo) | ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
-      }
-      if constexpr (DK) *reinterpret_cast<uint2*>(kp + d) = make_uint2(w[0], w[1]);
-      if constexpr (DV) *reinterpret_cast<uint2*>(vp + d) = make_uint2(x[0], x[1]);
+      if constexpr (DK)
+        store4(kp + d, dk[db][4 * i] * a.scale, dk[db][4 * i + 1] * a.scale, dk[db][4 * i + 2] * a.scale,
+               dk[db][4 * i + 3] * a.scale);
+      if constexpr (DV) store4(vp + d, dv[db][4 * i], dv[db][4 * i + 1], dv[db][4 * i + 2], dv[db][4 * i + 3]);
     }
 }
 
 template <class T, int DP, bool DK, bool DV>
-static int launch_dkv(const Args& a, const float* lse2, int64_t n_rows, int64_t n, int64_t tiles, hipStream_t s) {
-  attn_dkv_kernel<T, DP, DK, DV><<<(unsigned)n, 256, 0, s>>>(a, lse2, n_rows, (int)tiles);
+static int launch_dkv(const Args& a, const float* shift, int64_t n_rows, int64_t n, int64_t tiles, hipStream_t s) {
+  attn_dkv_kernel<T, DP, DK, DV><<<(unsigned)n, 256, 0, s>>>(a, shift, n_rows, (int)tiles);
   FORGE_CHECK_LAUNCH();
   return FORGE_OK;
 }
 
 template <class T, int DP>
-static int launch_bwd_dp(const Args& a, float* lse2, int64_t n_rows, hipStream_t s) {
+static int launch_bwd_dp(const Args& a, float* shift, int64_t n_rows, hipStream_t s) {
   const int64_t tq = most_tiles(a.cu_q, a.B, a.tq, 128), tk = most_tiles(a.cu_k, a.B, a.tk, 128);
   const int64_t nq = items(tq, a.Hkv, a.H / a.Hkv), nk = items(tk, a.Hkv, 1);
   if (nq > 0x7fffffffLL || nk > 0x7fffffffLL) return forge_set_error(FORGE_ERR_INVALID, "attention: too many tiles");
   const int64_t pairs = n_rows * a.H;
-  if (pairs) attn_delta_kernel<T><<<grid_for(pairs * 16, 256, 256 * 64), 256, 0, s>>>(a, lse2, n_rows, pairs);
+  if (pairs) attn_delta_kernel<T><<<grid_for(pairs * 16, 256, 256 * 64), 256, 0, s>>>(a, shift, n_rows, pairs);
   FORGE_CHECK_LAUNCH();
-  if (nq && n_rows) attn_dq_kernel<T, DP><<<(unsigned)nq, 256, 0, s>>>(a, lse2, n_rows, (int)tq);
+  if (nq && n_rows) attn_dq_kernel<T, DP><<<(unsigned)nq, 256, 0, s>>>(a, shift, n_rows, (int)tq);
   FORGE_CHECK_LAUNCH();
   if (nk == 0) return FORGE_OK;
-  if (DP < 256) return launch_dkv<T, DP, true, DP < 256>(a, lse2, n_rows, nk, tk, s);
-  if (int e = launch_dkv<T, DP, true, DP < 256>(a, lse2, n_rows, nk, tk, s)) return e;
-  return launch_dkv<T, DP, DP < 256, true>(a, lse2, n_rows, nk, tk, s);
+  if (DP < 256) return launch_dkv<T, DP, true, DP < 256>(a, shift, n_rows, nk, tk, s);
+  if (int e = launch_dkv<T, DP, true, DP < 256>(a, shift, n_rows, nk, tk, s)) return e;
+  return launch_dkv<T, DP, DP < 256, true>(a, shift, n_rows, nk, tk, s);
 }
 
 template <class T>
-static int launch_bwd_t(const Args& a, float* lse2, int64_t n_rows, hipStream_t s) {
-  if (a.D <= 64) return launch_bwd_dp<T, 64>(a, lse2, n_rows, s);
-  if (a.D <= 128) return launch_bwd_dp<T, 128>(a, lse2, n_rows, s);
-  return launch_bwd_dp<T, 256>(a, lse2, n_rows, s);
+static int launch_bwd_t(const Args& a, float* shift, int64_t n_rows, hipStream_t s) {
+  if (a.D <= 64) return launch_bwd_dp<T, 64>(a, shift, n_rows, s);
+  if (a.D <= 128) return launch_bwd_dp<T, 128>(a, shift, n_rows, s);
+  return launch_bwd_dp<T, 256>(a, shift, n_rows, s);
 }
 
-int launch_bwd(int dtype, const Args& a, float* lse2, int64_t n_rows, hipStream_t s) {
-  return dtype == FORGE_DTYPE_F16 ? launch_bwd_t<fp16_t>(a, lse2, n_rows, s) : launch_bwd_t<bf16_t>(a, lse2, n_rows, s);
+int launch_bwd(int dtype, const Args& a, float* shift, int64_t n_rows, hipStream_t s) {
+  return dtype == FORGE_DTYPE_F16 ? launch_bwd_t<fp16_t>(a, shift, n_rows, s) : launch_bwd_t<bf16_t>(a, shift, n_rows, s);
 }
 
 }  // namespace fattn

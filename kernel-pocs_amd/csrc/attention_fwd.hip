@@ -17,6 +17,7 @@
 namespace fattn {
 
 constexpr int BN = 64;
+constexpr float SLACK = 6.f;
 
 template <class T, int DP>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a, int tiles) {
@@ -27,14 +28,13 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a
   const int G = a.H / a.Hkv, h = lane / 32;
   const Item it = item_of(blockIdx.x, tiles, a.Hkv, G);
   if (it.tile >= tiles) return;
-  const TileAt at = find_tile(a.cu_q, a.B, a.tq, BM, it.tile);
+  const LevelAt at = find_level(a.cu_q, a.B, a.tq, BM, it.tile);
   if (at.seq > a.B) return;
   const Span sq = span_of(a.cu_q, a.B, a.tq, at.seq);
   Span sk = span_of(a.cu_k, a.B, a.tk, at.seq);
   if (at.seq < 0 || at.seq >= a.B) sk.len = 0;
   const int head = it.kv * G + it.g;
-  // the last tile of a sequence, which sees the most keys, first
-  const int q0 = ((sq.len + BM - 1) / BM - 1 - at.tile) * BM;
+  const int q0 = (at.level - 1) * BM;
   const int shift = sk.len - sq.len;
   const int rows = min(BM, sq.len - q0);
   const int k_end = a.causal ? min(sk.len, q0 + rows + shift) : sk.len;
@@ -54,17 +54,19 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a
     }
   }
   Dma kd, vd;
-  kd.setup(a.k.row, a.D, wave);
-  vd.setup(a.v.row, a.D, wave);
+  kd.setup(a.k.row, a.D);
+  vd.setup(a.v.row, a.D);
   const T* kp = row_ptr<T>(a.k, sk.batch, sk.start, it.kv);
   const T* vp = row_ptr<T>(a.v, sk.batch, sk.start, it.kv);
-  auto issue = [&](int t) {
-    char* st = smem + (t % 2) * 2 * Dma::BYTES;
+  auto issue = [&](int t, int slot) {
+    char* st = smem + slot * 2 * Dma::BYTES;
     kd.load(kp + (int64_t)t * BN * a.k.row, sk.len - t * BN, st, wave);
     vd.load(vp + (int64_t)t * BN * a.v.row, sk.len - t * BN, st + Dma::BYTES, wave);
   };
-  TrOff<DP> tr;
-  tr.setup(lane);
+  RowFrag<DP> fr;
+  ColFrag<DP> fc;
+  fr.setup(lane);
+  fc.setup(lane);
 
   f32x16 o[DB];
 #pragma unroll
@@ -79,14 +81,14 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a
   const int all_see = a.causal ? min(sk.len, wq + shift + 1) : sk.len;
   const int any_sees = a.causal ? min(sk.len, min(wq + 32, sq.len) + shift) : (wq < sq.len ? sk.len : 0);
 
-  if (n_t > 0) issue(0);
-  for (int t = 0; t < n_t; ++t) {
+  // (slot: a constant where the call is, so that it is part of the reads' immediates)
+  auto step = [&](int t, int slot) __attribute__((always_inline)) {
     wait_dma<0>();
     barrier();
-    if (t + 1 < n_t) issue(t + 1);
+    if (t + 1 < n_t) issue(t + 1, 1 - slot);
     const int k0 = t * BN;
-    if (k0 >= any_sees) continue;
-    const char* kt = smem + (t % 2) * 2 * Dma::BYTES;
+    if (k0 >= any_sees) return;
+    const char* kt = smem + slot * 2 * Dma::BYTES;
     const char* vt = kt + Dma::BYTES;
     f32x16 s[2];
 #pragma unroll
@@ -94,7 +96,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s[kb] = mfma32<T>(frag_rows<DP>(kt, 32 * kb, ks, lane), qf[ks], s[kb]);
+      for (int ks = 0; ks < KS; ++ks) s[kb] = mfma32<T>(fr.read(kt, 32 * kb, ks), qf[ks], s[kb]);
     }
     if (k0 + BN > all_see) {
 #pragma unroll
@@ -109,8 +111,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
     top = fmaxf(top, other_half(top)) * c;
-    if (__any(top > m)) {
-      const float up = fmaxf(top, m), f = exp2_hw(m - up);
+    // m follows the maximum by steps of SLACK at least: p stays below 2^SLACK, and
+    // the sums are seldom scaled (a new maximum, however small, comes up in one of
+    // 32 queries at almost every tile)
+    if (__any(top > m + SLACK)) {
+      const float up = top > m + SLACK ? top : m, f = exp2_hw(m - up);
       m = up;
       l *= f;
 #pragma unroll
@@ -130,8 +135,13 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a
     for (int i = 0; i < 4; ++i) {
       const bf16x8 p = pack_acc<T>(s[i / 2], i % 2);
 #pragma unroll
-      for (int db = 0; db < DB; ++db) o[db] = mfma32<T>(frag_cols<DP>(vt, tr, 16 * i, db), p, o[db]);
+      for (int db = 0; db < DB; ++db) o[db] = mfma32<T>(fc.read(vt, 16 * i, db), p, o[db]);
     }
+  };
+  if (n_t > 0) issue(0, 0);
+  for (int t = 0; t < n_t; t += 2) {
+    step(t, 0);
+    if (t + 1 < n_t) step(t + 1, 1);
   }
   l += other_half(l);
   if (!live) return;
@@ -143,13 +153,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a
     for (int i = 0; i < 4; ++i) {
       const int d = 32 * db + 8 * i + 4 * h;
       if (d >= a.D) continue;
-      uint32_t w[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const T lo = (T)(o[db][4 * i + 2 * j] * inv), hi = (T)(o[db][4 * i + 2 * j + 1] * inv);
-        w[j] = (uint32_t)__builtin_bit_cast(uint16_t, lo) | ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
-      }
-      *reinterpret_cast<uint2*>(op + d) = make_uint2(w[0], w[1]);
+      store4(op + d, o[db][4 * i] * inv, o[db][4 * i + 1] * inv, o[db][4 * i + 2] * inv, o[db][4 * i + 3] * inv);
     }
   if (h == 0 && a.lse) {
     const int64_t row = a.cu_q ? sq.start + iq : sq.batch * a.tq + iq;

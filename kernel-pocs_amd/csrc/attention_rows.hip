@@ -20,17 +20,6 @@ struct Parts {      // sums of a chunk: [chunk of its sequence][query * H + head
   int C;            // keys a chunk
 };
 
-template <class T>
-__device__ __forceinline__ void store4(T* p, const float (&f)[4]) {
-  uint32_t w[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const T lo = (T)f[2 * j], hi = (T)f[2 * j + 1];
-    w[j] = (uint32_t)__builtin_bit_cast(uint16_t, lo) | ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
-  }
-  *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-}
-
 __device__ __forceinline__ int chunks_of(int len, int C) { return max(1, (len + C - 1) / C); }
 
 template <class T, int DP, int NW>
@@ -56,13 +45,15 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_rows_kernel(Args a, Parts par
   const int n_rows = sq.len * G, shift = sk.len - sq.len;
   const float c = a.scale * LOG2E;
   Dma kd, vd;
-  kd.setup(a.k.row, a.D, 0);
-  vd.setup(a.v.row, a.D, 0);
+  kd.setup(a.k.row, a.D);
+  vd.setup(a.v.row, a.D);
   const T* kp = row_ptr<T>(a.k, sk.batch, sk.start, kv);
   const T* vp = row_ptr<T>(a.v, sk.batch, sk.start, kv);
   char* ring = smem + wave * 2 * 2 * Dma::BYTES;
-  TrOff<DP> tr;
-  tr.setup(lane);
+  RowFrag<DP> fr;
+  ColFrag<DP> fc;
+  fr.setup(lane);
+  fc.setup(lane);
   const int n_t = hi > lo ? (hi - lo + 31) / 32 : 0, mine = n_t > wave ? (n_t - wave + NW - 1) / NW : 0;
   auto issue = [&](int i) {
     const int k0 = lo + 32 * (wave + i * NW);
@@ -102,7 +93,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_rows_kernel(Args a, Parts par
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s = mfma32<T>(frag_rows<DP>(kt, 0, ks, lane), qf[ks], s);
+      for (int ks = 0; ks < KS; ++ks) s = mfma32<T>(fr.read(kt, 0, ks), qf[ks], s);
       float top = -__builtin_inff();
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -126,7 +117,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_rows_kernel(Args a, Parts par
       for (int j = 0; j < 2; ++j) {
         const bf16x8 p = pack_acc<T>(s, j);
 #pragma unroll
-        for (int db = 0; db < DB; ++db) o[db] = mfma32<T>(frag_cols<DP>(vt, tr, 16 * j, db), p, o[db]);
+        for (int db = 0; db < DB; ++db) o[db] = mfma32<T>(fc.read(vt, 16 * j, db), p, o[db]);
       }
       wait_dma<2 * Dma::N>();  // (the reads of this slot are done; the other slot's DMA may be under way)
       if (i + 2 < mine) issue(i + 2);
@@ -166,7 +157,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_rows_kernel(Args a, Parts par
         const float inv = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] *= inv;
-        store4(row_ptr<T>(a.o, sq.batch, sq.start + t, hd) + d, v);
+        store4(row_ptr<T>(a.o, sq.batch, sq.start + t, hd) + d, v[0], v[1], v[2], v[3]);
         if (d == 0 && a.lse) a.lse[q * a.H + hd] = total == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(total)) * LN2;
       } else {
         const int64_t at_part = at.tile * parts.n + q * a.H + hd;
@@ -232,7 +223,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(Args a, Parts parts) {
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] *= inv;
-    store4(op + 4 * lane, v);
+    store4(op + 4 * lane, v[0], v[1], v[2], v[3]);
   }
   if (lane == 0 && a.lse) a.lse[p] = total == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(total)) * LN2;
 }
