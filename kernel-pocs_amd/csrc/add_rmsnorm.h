@@ -4,8 +4,7 @@
 // TPR threads (64: a wave, 256: a workgroup) take a row of H values in vectors of
 // V = 16 bytes: thread t the vectors t, t + TPR, ... (NV of them, held in registers;
 // NV = 0: any number, read again where they are needed).  Rows may begin at any
-// element: global memory takes 16-byte accesses at any address, and they
-// measured as fast as aligned ones.  The last vector of a row may be short.
+// element: global memory takes 16-byte accesses at any address.  The last vector of a row may be short.
 #pragma once
 
 #include <type_traits>
@@ -19,44 +18,108 @@ typedef unsigned int u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
 
 template <class T> constexpr int V = 16 / (int)sizeof(T);
 
-// 16 bytes of a row, of which `n` values exist (the rest are zeros)
+// V values of a row, held as words (a 16-bit value in a register of its own
+// would take all of it)
 template <class T>
-__device__ __forceinline__ Vec16<T> load_part(const T* p, int n) {
-  Vec16<T> r;
+struct Vec {
+  uint32_t w[4];
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (std::is_same_v<T, float>) return __uint_as_float(w[i]);
+    else if constexpr (std::is_same_v<T, bf16_t>) return __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    else return (float)__builtin_bit_cast(fp16_t, (uint16_t)(i % 2 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu));
+  }
+  __device__ __forceinline__ void set(const float* f) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef T t2 __attribute__((ext_vector_type(2)));
+    if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(f[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{f[2 * i], f[2 * i + 1]}), t2));
+    }
+  }
+  // values widened before this point are not kept behind it: they are widened again
+  __device__ __forceinline__ void keep() {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(w[i]));
+  }
+  __device__ __forceinline__ void clear() { w[0] = w[1] = w[2] = w[3] = 0; }
+};
+
+template <class T> struct Raw { typedef uint16_t type; };
+template <> struct Raw<float> { typedef uint32_t type; };
+
+// 16 bytes of a row, of which `n` values exist (the rest are zeros).  A row is
+// read once: nontemporal.
+template <class T>
+__device__ __forceinline__ Vec<T> load_part(const T* p, int n) {
+  Vec<T> r;
   if (n >= V<T>) {
-    const u32x4_any w = *reinterpret_cast<const u32x4_any*>(p);
-    r.raw = make_uint4(w.x, w.y, w.z, w.w);
+    const u32x4_any w = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p));
+    r.w[0] = w.x; r.w[1] = w.y; r.w[2] = w.z; r.w[3] = w.w;
   } else {
-    r.raw = make_uint4(0, 0, 0, 0);
+    typedef typename Raw<T>::type R;
+    const R* e = reinterpret_cast<const R*>(p);
+    r.clear();
 #pragma unroll
     for (int i = 0; i < V<T>; ++i)
-      if (i < n) r.v[i] = p[i];
+      if (i < n) r.w[i * sizeof(R) / 4] |= (uint32_t)e[i] << (sizeof(R) == 2 ? 16 * (i % 2) : 0);
   }
   return r;
 }
 
 template <class T>
-__device__ __forceinline__ void store_part(T* p, const Vec16<T>& r, int n) {
+__device__ __forceinline__ void store_part(T* p, const Vec<T>& r, int n) {
   if (n >= V<T>) {
-    const u32x4_any w = {r.raw.x, r.raw.y, r.raw.z, r.raw.w};
+    const u32x4_any w = {r.w[0], r.w[1], r.w[2], r.w[3]};
     *reinterpret_cast<u32x4_any*>(p) = w;
   } else {
+    typedef typename Raw<T>::type R;
+    R* e = reinterpret_cast<R*>(p);
 #pragma unroll
     for (int i = 0; i < V<T>; ++i)
-      if (i < n) p[i] = r.v[i];
+      if (i < n) e[i] = (R)(r.w[i * sizeof(R) / 4] >> (sizeof(R) == 2 ? 16 * (i % 2) : 0));
   }
 }
 
-// V values of a weight of any type, widened
+// N values of type S at any element, widened
+template <class S, int N>
+__device__ __forceinline__ void load_wide(const S* p, float* o) {
+  constexpr int PER = 16 / (int)sizeof(S);
+  if constexpr (N >= PER) {
+#pragma unroll
+    for (int k = 0; k < N / PER; ++k) {
+      Vec16<S> v;
+      const u32x4_any w = *reinterpret_cast<const u32x4_any*>(p + k * PER);
+      v.raw = make_uint4(w.x, w.y, w.z, w.w);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) o[k * PER + i] = to_f32(v.v[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = to_f32(p[i]);
+  }
+}
+
+// V values of a weight of any type, widened (NULL: ones)
 template <class T>
 __device__ __forceinline__ void load_weight(const void* w, int w_dtype, int64_t c, int n, float (&o)[V<T>]) {
+  if (!w) {
 #pragma unroll
-  for (int i = 0; i < V<T>; ++i) {
-    if (i >= n) o[i] = 0.f;
-    else if (!w) o[i] = 1.f;
-    else if (w_dtype == FORGE_DTYPE_F32) o[i] = ((const float*)w)[c + i];
-    else if (w_dtype == FORGE_DTYPE_F16) o[i] = (float)((const fp16_t*)w)[c + i];
-    else o[i] = (float)((const bf16_t*)w)[c + i];
+    for (int i = 0; i < V<T>; ++i) o[i] = 1.f;
+  } else if (n >= V<T>) {
+    if (w_dtype == FORGE_DTYPE_F32) load_wide<float, V<T>>((const float*)w + c, o);
+    else if (w_dtype == FORGE_DTYPE_F16) load_wide<fp16_t, V<T>>((const fp16_t*)w + c, o);
+    else load_wide<bf16_t, V<T>>((const bf16_t*)w + c, o);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V<T>; ++i) {
+      if (i >= n) o[i] = 0.f;
+      else if (w_dtype == FORGE_DTYPE_F32) o[i] = ((const float*)w)[c + i];
+      else if (w_dtype == FORGE_DTYPE_F16) o[i] = (float)((const fp16_t*)w)[c + i];
+      else o[i] = (float)((const bf16_t*)w)[c + i];
+    }
   }
 }
 
@@ -78,17 +141,17 @@ __device__ __forceinline__ A row_sum(A v, A* buf) {
 template <int TPR>
 constexpr int rows_per_block = 256 / TPR;
 
-// Launches f<TPR, NV> for rows of H values.
-#define FROWS_PICK(T, H, F)                                     \
+// The kernel F<T, TPR, NV, ...> for rows of H values.
+#define FROWS_PICK(T, H, F, ...)                                \
   do {                                                          \
     const int64_t nv_ = ((H) + frows::V<T> - 1) / frows::V<T>;  \
-    if (nv_ <= 64) return F<T, 64, 1>;                          \
-    if (nv_ <= 128) return F<T, 64, 2>;                         \
-    if (nv_ <= 256) return F<T, 256, 1>;                        \
-    if (nv_ <= 512) return F<T, 256, 2>;                        \
-    if (nv_ <= 1024) return F<T, 256, 4>;                       \
-    if (nv_ <= 2048) return F<T, 256, 8>;                       \
-    return F<T, 256, 0>;                                        \
+    if (nv_ <= 64) return F<T, 64, 1, __VA_ARGS__>;             \
+    if (nv_ <= 128) return F<T, 64, 2, __VA_ARGS__>;            \
+    if (nv_ <= 256) return F<T, 256, 1, __VA_ARGS__>;           \
+    if (nv_ <= 512) return F<T, 256, 2, __VA_ARGS__>;           \
+    if (nv_ <= 1024) return F<T, 256, 4, __VA_ARGS__>;          \
+    if (nv_ <= 2048) return F<T, 256, 8, __VA_ARGS__>;          \
+    return F<T, 256, 0, __VA_ARGS__>;                           \
   } while (0)
 
 }  // namespace frows

@@ -9,8 +9,8 @@
 //
 // The integers are those of exact arithmetic.  t of two 16-bit factors is exact in
 // fp32; otherwise the largest is found in 64 bits.  127 t / a errs by less than
-// 1e-4 in fp32 (127 times a few roundings of 2^-24), so only values that close
-// to a border between two integers are divided again, in 64 bits.
+// 6e-5 in fp32, so only values that close to a border between two integers are
+// divided again, in 64 bits (one vector of 8 in 130).
 //
 // Bound by HBM: x and the residual are read once, h and y written once.
 #include "add_rmsnorm.h"
@@ -20,7 +20,7 @@ namespace frows {
 struct FwdArgs {
   const void* x; int64_t ldx;
   const void* res; int64_t ldr;  // or NULL
-  const void* w; int w_dtype;    // or NULL: ones
+  const void* w; int w_dtype;
   void* h;                       // [rows][H], or NULL where there is no residual
   void* y;                       // [rows][H]
   int8_t* q; int64_t ldq;        // [rows][ldq], zeros from H on
@@ -28,143 +28,184 @@ struct FwdArgs {
   float* rstd;                   // [rows], or NULL
   int64_t rows, H;
   float eps, offset;
-  int exact;                     // t is exact in fp32
 };
 
-enum Mode { NORM, NORM8, ROWS8 };
+// What becomes of a row: its norm, its norm in 8 bits (the products exact in fp32, or
+// not), the row itself in 8 bits, or times a scale a column.
+enum Mode { NORM, NORM8, NORM8_WIDE, ROWS8, ROWS8_SCALED };
 
-template <class T, int MODE>
-struct Elem {
-  // the stored sum
-  static __device__ __forceinline__ Vec16<T> add(const Vec16<T>& x, const Vec16<T>& r) {
-    Vec16<T> h;
+// The integers of V values of a row with factors w, as bytes.  inv = 127 / a.
+template <class T, bool UNIT>
+__device__ __forceinline__ void quantize(const Vec<T>& v, const float* w, double offset, float inv, double a, bool tiny,
+                                         uint32_t (&word)[V<T> / 4]) {
+  int k[V<T>];
+  bool near = tiny;
 #pragma unroll
-    for (int i = 0; i < V<T>; ++i) h.v[i] = from_f32<T>(to_f32(x.v[i]) + to_f32(r.v[i]));
-    return h;
+  for (int i = 0; i < V<T>; ++i) {
+    const float t = (UNIT ? v.get(i) : v.get(i) * (w[i] + (float)offset)) * inv, r = rintf(t);
+    near = near || fabsf(t - r) > 0.5f - 6e-5f;
+    k[i] = (int)r;
   }
-};
-
-__device__ __forceinline__ int quantize(float v, float w, float offset, float inv, double a, bool tiny) {
-  const float t = v * (w + offset) * inv;
-  const float k = rintf(t);
-  if (tiny || fabsf(fabsf(t - k) - 0.5f) < 1e-3f) return (int)rint(127.0 * ((double)v * ((double)w + (double)offset)) / a);
-  return (int)k;
+  if (near) {  // (6e-5: 127 times 8 roundings of 2^-24)
+#pragma unroll
+    for (int i = 0; i < V<T>; ++i) {
+      const double t = UNIT ? (double)v.get(i) : (double)v.get(i) * ((double)w[i] + offset);
+      k[i] = (int)rint(127.0 * t / a);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V<T>; ++i) {
+    const uint32_t byte = (uint32_t)(k[i] & 255) << (8 * (i % 4));
+    word[i / 4] = i % 4 ? word[i / 4] | byte : byte;
+  }
 }
 
 template <class T, int TPR, int NV, int MODE>
 __global__ __launch_bounds__(256) void add_rmsnorm_kernel(FwdArgs a) {
   constexpr int VN = V<T>, RPB = rows_per_block<TPR>, N = NV ? NV : 1;
+  constexpr bool SUMS = MODE == NORM || MODE == NORM8 || MODE == NORM8_WIDE, EIGHT = MODE != NORM;
+  constexpr bool WIDE = MODE == NORM8_WIDE || MODE == ROWS8_SCALED, UNIT = MODE == ROWS8;
+  // a thread's weights are held, or read again for every row where they are too many
+  constexpr bool HELD = !UNIT && NV > 0 && NV <= 4, RELOAD = !UNIT && NV > 4;
+  constexpr bool AHEAD = NV > 0 && NV <= 4;  // the next row's loads are in flight while a row is worked on
   __shared__ float sums[2][4];
   __shared__ uint32_t tops[2][4];
   __shared__ double tops64[2][4];
   const int tid = threadIdx.x % TPR, slot = threadIdx.x / TPR;
   const int n_vec = (int)((a.H + VN - 1) / VN);
   const T* xp = (const T*)a.x;
-  const T* rp = (const T*)a.res;
-  float w[N][VN];
-  if constexpr (NV > 0) {
+  const T* rp = SUMS ? (const T*)a.res : nullptr;
+  // the factors of t: weight + offset, of which WIDE adds the offset in 64 bits
+  const float add = WIDE ? 0.f : a.offset;
+  const double add64 = WIDE ? (double)a.offset : 0.0;
+  float w[HELD ? N : 1][VN];
+  auto load_w = [&](int c, float (&o)[VN]) {
+    load_weight<T>(a.w, a.w_dtype, c, (int)min((int64_t)VN, a.H - c), o);
+#pragma unroll
+    for (int i = 0; i < VN; ++i) o[i] += add;
+  };
+  if constexpr (HELD) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (tid + j * TPR) * VN;
-      load_weight<T>(a.w, a.w_dtype, c, (int)(a.H - c), w[j]);
+      const int vec = tid + j * TPR;
+      if (vec < n_vec) load_w(vec * VN, w[j]);
     }
   }
-  int flip = 0;
-  // (every thread of a workgroup goes through the same rounds: row_sum has barriers)
-  for (int64_t first = (int64_t)blockIdx.x * RPB; first < a.rows; first += (int64_t)gridDim.x * RPB, flip ^= 1) {
-    const int64_t row = first + slot;
-    if (TPR == 64 && row >= a.rows) return;
-    Vec16<T> h[N];
+  Vec<T> x[2][N], r[2][N];
+  auto fetch = [&](int64_t row, int set) {
+    if constexpr (NV > 0) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int vec = tid + j * TPR, c = vec * VN, n = (int)min((int64_t)VN, a.H - c);
+        if (vec < n_vec && row < a.rows) {
+          x[set][j] = load_part(xp + row * a.ldx + c, n);
+          if (SUMS && rp) r[set][j] = load_part(rp + row * a.ldr + c, n);
+        }
+      }
+    }
+  };
+  auto sum = [&](const Vec<T>& u, const Vec<T>& v) {
+    Vec<T> h;
+    float f[VN];
+#pragma unroll
+    for (int i = 0; i < VN; ++i) f[i] = u.get(i) + v.get(i);
+    h.set(f);
+    return h;
+  };
+
+  auto work = [&](int64_t row, int set, int flip) __attribute__((always_inline)) {
     float ss = 0.f;
     uint32_t top = 0;
     double top64 = 0.0;
-    auto see = [&](const Vec16<T>& v, const float (&wv)[VN]) {
+    auto see = [&](const Vec<T>& v, const float* wv) {
 #pragma unroll
       for (int i = 0; i < VN; ++i) {
-        const float f = to_f32(v.v[i]);
-        if (MODE != ROWS8) ss += f * f;
-        if (MODE != NORM) {
-          top = max(top, __float_as_uint(f * (wv[i] + a.offset)) & 0x7fffffffu);
-          if (!a.exact) top64 = fmax(top64, fabs((double)f * ((double)wv[i] + (double)a.offset)));
-        }
+        const float f = v.get(i);
+        if (SUMS) ss += f * f;
+        if (EIGHT) top = max(top, __float_as_uint(UNIT ? f : f * (wv[i] + (float)add64)) & 0x7fffffffu);
+        if (WIDE) top64 = fmax(top64, fabs((double)f * ((double)wv[i] + add64)));
       }
-    };
-    auto read = [&](int vec) {
-      const int c = vec * VN, n = (int)min((int64_t)VN, a.H - c);
-      Vec16<T> v = load_part(xp + row * a.ldx + c, n);
-      if (MODE != ROWS8 && rp) {
-        v = Elem<T, MODE>::add(v, load_part(rp + row * a.ldr + c, n));
-        store_part((T*)a.h + row * a.H + c, v, n);
-      }
-      return v;
     };
     if constexpr (NV > 0) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int vec = tid + j * TPR;
         if (vec < n_vec) {
-          h[j] = read(vec);
-          see(h[j], w[j]);
+          if (SUMS && rp) {
+            x[set][j] = sum(x[set][j], r[set][j]);
+            store_part((T*)a.h + row * a.H + vec * VN, x[set][j], (int)min((int64_t)VN, a.H - vec * VN));
+          }
+          if (RELOAD) load_w(vec * VN, w[0]);
+          see(x[set][j], w[HELD ? j : 0]);
         }
       }
     } else {
       for (int vec = tid; vec < n_vec; vec += TPR) {
-        load_weight<T>(a.w, a.w_dtype, vec * VN, (int)(a.H - vec * VN), w[0]);
-        see(read(vec), w[0]);
+        const int c = vec * VN, n = (int)min((int64_t)VN, a.H - c);
+        Vec<T> v = load_part(xp + row * a.ldx + c, n);
+        if (SUMS && rp) {
+          v = sum(v, load_part(rp + row * a.ldr + c, n));
+          store_part((T*)a.h + row * a.H + c, v, n);
+        }
+        if (!UNIT) load_w(c, w[0]);
+        see(v, w[0]);
       }
     }
     float rstd = 1.f;
-    if constexpr (MODE != NORM) {
+    if constexpr (EIGHT) {
 #pragma unroll
       for (int off = 32; off >= 1; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
-      if (!a.exact) {
+      if constexpr (WIDE) {
 #pragma unroll
         for (int off = 32; off >= 1; off >>= 1) top64 = fmax(top64, __shfl_xor(top64, off, 64));
       }
       if constexpr (TPR > 64) {
         if (threadIdx.x % 64 == 0) {
           tops[flip][threadIdx.x / 64] = top;
-          tops64[flip][threadIdx.x / 64] = top64;
+          if (WIDE) tops64[flip][threadIdx.x / 64] = top64;
         }
-        if (MODE == ROWS8) __syncthreads();
+        if (!SUMS) __syncthreads();
       }
     }
-    if constexpr (MODE != ROWS8) {
+    if constexpr (SUMS) {
       ss = row_sum<TPR>(ss, sums[flip]);
       rstd = rsqrtf(ss / (float)a.H + a.eps);
       if (tid == 0 && a.rstd) a.rstd[row] = rstd;
     }
     float inv = 0.f;
     bool tiny = false, bad = false;
-    if constexpr (MODE != NORM) {
+    if constexpr (EIGHT) {
       if constexpr (TPR > 64) {
 #pragma unroll
         for (int k = 0; k < TPR / 64; ++k) {
           top = max(top, tops[flip][k]);
-          top64 = fmax(top64, tops64[flip][k]);
+          if (WIDE) top64 = fmax(top64, tops64[flip][k]);
         }
       }
-      if (a.exact) top64 = (double)__uint_as_float(top);
+      if (!WIDE) top64 = (double)__uint_as_float(top);
       // infinities and NaN: the row's scale is NaN, and so is all that is computed of it
       bad = top >= 0x7f800000u;
       tiny = top64 < 1e-30;
       inv = tiny || bad ? 0.f : 127.f / (float)top64;
       if (tid == 0) a.scale[row] = bad ? __builtin_nanf("") : (float)top64 * rstd / 127.f;
     }
-    auto write = [&](const Vec16<T>& v, const float (&wv)[VN], int vec) {
-      const int c = vec * VN, n = (int)min((int64_t)VN, a.H - c);
-      if constexpr (MODE == NORM) {
-        Vec16<T> y;
+    auto write = [&](const Vec<T>& v, const float* wv, int vec) {
+      const int c = vec * VN;
+      if constexpr (!EIGHT) {
+        Vec<T> y;
+        float f[VN];
 #pragma unroll
-        for (int i = 0; i < VN; ++i) y.v[i] = from_f32<T>(to_f32(v.v[i]) * rstd * (wv[i] + a.offset));
-        store_part((T*)a.y + row * a.H + c, y, n);
+        for (int i = 0; i < VN; ++i) f[i] = v.get(i) * rstd * wv[i];
+        y.set(f);
+        store_part((T*)a.y + row * a.H + c, y, (int)min((int64_t)VN, a.H - c));
       } else {
         uint32_t word[VN / 4];
+        if (bad || top64 == 0.0) {
 #pragma unroll
-        for (int i = 0; i < VN; ++i) {
-          const int k = bad || top64 == 0.0 || i >= n ? 0 : quantize(to_f32(v.v[i]), wv[i], a.offset, inv, top64, tiny);
-          const uint32_t byte = (uint32_t)(k & 255) << (8 * (i % 4));
-          word[i / 4] = i % 4 ? word[i / 4] | byte : byte;
+          for (int k = 0; k < VN / 4; ++k) word[k] = 0;
+        } else {
+          // (values behind the row's end are zeros)
+          quantize<T, UNIT>(v, wv, add64, inv, top64, tiny, word);
         }
         int8_t* p = a.q + row * a.ldq + c;  // (ldq is a multiple of 16)
         if constexpr (VN == 8) *reinterpret_cast<uint2*>(p) = make_uint2(word[0], word[1]);
@@ -175,35 +216,60 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(FwdArgs a) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int vec = tid + j * TPR;
-        if (vec < n_vec) write(h[j], w[j], vec);
+        if (vec < n_vec) {
+          x[set][j].keep();
+          if (RELOAD) load_w(vec * VN, w[0]);
+          write(x[set][j], w[HELD ? j : 0], vec);
+        }
       }
     } else {
       for (int vec = tid; vec < n_vec; vec += TPR) {
         const int c = vec * VN, n = (int)min((int64_t)VN, a.H - c);
-        load_weight<T>(a.w, a.w_dtype, c, n, w[0]);
+        if (!UNIT) load_w(c, w[0]);
         // (this thread wrote these values of h itself)
-        const T* src = MODE != ROWS8 && rp ? (const T*)a.h + row * a.H : xp + row * a.ldx;
+        const T* src = SUMS && rp ? (const T*)a.h + row * a.H : xp + row * a.ldx;
         write(load_part(src + c, n), w[0], vec);
       }
     }
-    if constexpr (MODE != NORM) {
+    if constexpr (EIGHT) {
       for (int64_t c = (int64_t)n_vec * VN + tid; c < a.ldq; c += TPR) a.q[row * a.ldq + c] = 0;
+    }
+  };
+
+  // (every thread of a workgroup goes through the same rounds: sums over a row have barriers)
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t row = (int64_t)blockIdx.x * RPB + slot;
+  if constexpr (AHEAD) {
+    fetch(row, 0);
+    for (; row < a.rows; row += 2 * step) {
+      fetch(row + step, 1);
+      work(row, 0, 0);
+      if (row + step >= a.rows) break;
+      fetch(row + 2 * step, 0);
+      work(row + step, 1, 1);
+    }
+  } else {
+    for (int flip = 0; row < a.rows; row += step, flip ^= 1) {
+      fetch(row, 0);
+      work(row, 0, flip);
     }
   }
 }
 
 typedef void (*Kernel)(FwdArgs);
-template <class T, int TPR, int NV> constexpr Kernel norm_k = add_rmsnorm_kernel<T, TPR, NV, NORM>;
-template <class T, int TPR, int NV> constexpr Kernel norm8_k = add_rmsnorm_kernel<T, TPR, NV, NORM8>;
-template <class T, int TPR, int NV> constexpr Kernel rows8_k = add_rmsnorm_kernel<T, TPR, NV, ROWS8>;
-
-template <class T> Kernel pick_norm(int64_t H) { FROWS_PICK(T, H, norm_k); }
-template <class T> Kernel pick_norm8(int64_t H) { FROWS_PICK(T, H, norm8_k); }
-template <class T> Kernel pick_rows8(int64_t H) { FROWS_PICK(T, H, rows8_k); }
+template <class T, int TPR, int NV, int MODE> constexpr Kernel fwd_k = add_rmsnorm_kernel<T, TPR, NV, MODE>;
+template <class T, int MODE> static Kernel pick_mode(int64_t H) { FROWS_PICK(T, H, fwd_k, MODE); }
 
 template <class T>
 static Kernel pick(int mode, int64_t H) {
-  return mode == NORM ? pick_norm<T>(H) : mode == NORM8 ? pick_norm8<T>(H) : pick_rows8<T>(H);
+  switch (mode) {
+    case NORM: return pick_mode<T, NORM>(H);
+    case NORM8:
+      if constexpr (sizeof(T) == 2) return pick_mode<T, NORM8>(H);
+    case NORM8_WIDE: return pick_mode<T, NORM8_WIDE>(H);
+    case ROWS8: return pick_mode<T, ROWS8>(H);
+    default: return pick_mode<T, ROWS8_SCALED>(H);
+  }
 }
 
 static int launch(const char* what, int dtype, int mode, const FwdArgs& a, hipStream_t s) {
@@ -266,9 +332,10 @@ extern "C" int forge_add_rmsnorm_int8(int dtype, int w_dtype, const void* x, int
   a.q = q;
   a.ldq = ldq;
   a.scale = scale;
-  a.exact = narrow(dtype) && narrow(w_dtype) && offset == 0.0;
+  // (a product of two 16-bit values is exact in fp32)
+  const int mode = narrow(dtype) && narrow(w_dtype) && offset == 0.0 ? NORM8 : NORM8_WIDE;
   if (rows > 0 && H > 0 && (!weight || (residual && !h))) return forge_set_error(FORGE_ERR_INVALID, "add_rmsnorm: an array is NULL");
-  return launch("add_rmsnorm", dtype, NORM8, a, (hipStream_t)stream);
+  return launch("add_rmsnorm", dtype, mode, a, (hipStream_t)stream);
 }
 
 extern "C" int forge_quantize_rows(int dtype, const void* x, int64_t ldx, const float* col_scale, int8_t* q, int64_t ldq,
@@ -283,6 +350,5 @@ extern "C" int forge_quantize_rows(int dtype, const void* x, int64_t ldx, const 
   a.scale = scale;
   a.rows = rows;
   a.H = H;
-  a.exact = col_scale == nullptr;
-  return launch("quantize_rows", dtype, ROWS8, a, (hipStream_t)stream);
+  return launch("quantize_rows", dtype, col_scale ? ROWS8_SCALED : ROWS8, a, (hipStream_t)stream);
 }

@@ -16,151 +16,207 @@ struct BwdArgs {
   const void* w; int w_dtype;
   const float* rstd;
   void* d;                       // [rows][H]
-  float* part;                   // [blocks][H], or NULL
+  float* part;                   // [blocks][ld_part]
+  int64_t ld_part;
   int64_t rows, H;
   float offset;
 };
 
-template <class T, int TPR, int NV>
+template <class T, int TPR, int NV, bool DW>
 __global__ __launch_bounds__(256) void add_rmsnorm_bwd_kernel(BwdArgs a) {
   constexpr int VN = V<T>, RPB = rows_per_block<TPR>, N = NV ? NV : 1;
+  constexpr bool AHEAD = NV > 0 && NV <= 2;  // the next row's loads are in flight while a row is worked on
   __shared__ float sums[2][4];
-  __shared__ float cols[TPR == 64 ? 4 * 64 * N * VN : 1];
+  __shared__ float cols[TPR == 64 && DW ? 4 * 64 * N * VN : 1];
   const int tid = threadIdx.x % TPR, slot = threadIdx.x / TPR;
   const int n_vec = (int)((a.H + VN - 1) / VN);
   const float inv_h = 1.f / (float)a.H;
-  float w[N][VN], dw[N][VN];
+  constexpr bool HELD = NV <= 4;  // a thread's weights are held, or read again for every row
+  float w[HELD ? N : 1][VN], dw[N][VN];
+  auto load_w = [&](int c, float (&o)[VN]) {
+    load_weight<T>(a.w, a.w_dtype, c, (int)min((int64_t)VN, a.H - c), o);
+#pragma unroll
+    for (int i = 0; i < VN; ++i) o[i] += a.offset;
+  };
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int c = (tid + j * TPR) * VN;
-    load_weight<T>(a.w, a.w_dtype, c, (int)(a.H - c), w[j]);
+    const int vec = tid + j * TPR;
+    if (HELD && vec < n_vec) load_w(vec * VN, w[j]);
 #pragma unroll
     for (int i = 0; i < VN; ++i) dw[j][i] = 0.f;
   }
-  int flip = 0;
-  for (int64_t first = (int64_t)blockIdx.x * RPB; first < a.rows; first += (int64_t)gridDim.x * RPB, flip ^= 1) {
-    const int64_t row = first + slot;
-    const bool on = row < a.rows;
-    const float rstd = on ? a.rstd[row] : 0.f;
-    Vec16<T> h[N], dy[N], dh[N];
-    const T* hp = (const T*)a.h + row * a.ldh;
-    const T* yp = (const T*)a.dy + row * a.lddy;
-    const T* sp = (const T*)a.dh + row * a.lddh;
-    float dot = 0.f;
+  struct Set {
+    Vec<T> h[N], dy[N], dh[N];
+    float rstd;
+  } sets[2];
+  auto fetch = [&](int64_t row, Set& s) {
+    if (row >= a.rows) return;
+    s.rstd = a.rstd[row];
     if constexpr (NV > 0) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int vec = tid + j * TPR, c = vec * VN, n = (int)min((int64_t)VN, a.H - c);
-        if (on && vec < n_vec) {
-          h[j] = load_part(hp + c, n);
-          dy[j] = load_part(yp + c, n);
-          if (a.dh) dh[j] = load_part(sp + c, n);
-          else dh[j].raw = make_uint4(0, 0, 0, 0);
-#pragma unroll
-          for (int i = 0; i < VN; ++i) dot += to_f32(dy[j].v[i]) * (w[j][i] + a.offset) * to_f32(h[j].v[i]);
+        if (vec < n_vec) {
+          s.h[j] = load_part((const T*)a.h + row * a.ldh + c, n);
+          s.dy[j] = load_part((const T*)a.dy + row * a.lddy + c, n);
+          if (a.dh) s.dh[j] = load_part((const T*)a.dh + row * a.lddh + c, n);
+          else s.dh[j].clear();
         }
       }
+    }
+  };
+  bool started = false;  // NV = 0: this workgroup's partial row has been written
+  auto work = [&](int64_t row, Set& s, int flip) __attribute__((always_inline)) {
+    const bool on = row < a.rows;
+    float dot = 0.f;
+    auto add_dot = [&](const Vec<T>& x, const Vec<T>& y, const float (&wv)[VN]) {
+#pragma unroll
+      for (int i = 0; i < VN; ++i) dot += y.get(i) * wv[i] * x.get(i);
+    };
+    const T* hp = (const T*)a.h + row * a.ldh;
+    const T* yp = (const T*)a.dy + row * a.lddy;
+    if constexpr (NV > 0) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (on && tid + j * TPR < n_vec) {
+          if (!HELD) load_w((tid + j * TPR) * VN, w[0]);
+          add_dot(s.h[j], s.dy[j], w[HELD ? j : 0]);
+        }
     } else if (on) {
       for (int vec = tid; vec < n_vec; vec += TPR) {
         const int c = vec * VN, n = (int)min((int64_t)VN, a.H - c);
-        load_weight<T>(a.w, a.w_dtype, c, n, w[0]);
-        const Vec16<T> x = load_part(hp + c, n), y = load_part(yp + c, n);
-#pragma unroll
-        for (int i = 0; i < VN; ++i) dot += to_f32(y.v[i]) * (w[0][i] + a.offset) * to_f32(x.v[i]);
+        load_w(c, w[0]);
+        add_dot(load_part(hp + c, n), load_part(yp + c, n), w[0]);
       }
     }
     dot = row_sum<TPR>(dot, sums[flip]);
-    const float k = rstd * rstd * rstd * dot * inv_h;
-    auto finish = [&](const Vec16<T>& x, const Vec16<T>& y, const Vec16<T>& s, const float (&wv)[VN], int vec) {
-      Vec16<T> d;
+    if (!on) return;
+    const float rstd = s.rstd, k = rstd * rstd * rstd * dot * inv_h;
+    auto finish = [&](const Vec<T>& x, const Vec<T>& y, const Vec<T>& g, const float (&wv)[VN], int vec) {
+      Vec<T> d;
+      float f[VN];
 #pragma unroll
-      for (int i = 0; i < VN; ++i)
-        d.v[i] = from_f32<T>(to_f32(s.v[i]) + (rstd * (to_f32(y.v[i]) * (wv[i] + a.offset)) - to_f32(x.v[i]) * k));
+      for (int i = 0; i < VN; ++i) f[i] = g.get(i) + (rstd * (y.get(i) * wv[i]) - x.get(i) * k);
+      d.set(f);
       const int c = vec * VN;
       store_part((T*)a.d + row * a.H + c, d, (int)min((int64_t)VN, a.H - c));
     };
-    if (!on) continue;
     if constexpr (NV > 0) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int vec = tid + j * TPR;
         if (vec < n_vec) {
-          finish(h[j], dy[j], dh[j], w[j], vec);
+          s.h[j].keep();
+          s.dy[j].keep();
+          if (!HELD) load_w(vec * VN, w[0]);
+          finish(s.h[j], s.dy[j], s.dh[j], w[HELD ? j : 0], vec);
+          if constexpr (DW)
 #pragma unroll
-          for (int i = 0; i < VN; ++i) dw[j][i] += to_f32(dy[j].v[i]) * (to_f32(h[j].v[i]) * rstd);
+            for (int i = 0; i < VN; ++i) dw[j][i] += s.dy[j].get(i) * (s.h[j].get(i) * rstd);
         }
       }
     } else {
       for (int vec = tid; vec < n_vec; vec += TPR) {
         const int c = vec * VN, n = (int)min((int64_t)VN, a.H - c);
-        load_weight<T>(a.w, a.w_dtype, c, n, w[0]);
-        Vec16<T> s;
-        s.raw = make_uint4(0, 0, 0, 0);
-        if (a.dh) s = load_part(sp + c, n);
-        const Vec16<T> x = load_part(hp + c, n), y = load_part(yp + c, n);
-        finish(x, y, s, w[0], vec);
-        if (a.part) {  // (this thread's own columns of the workgroup's partial row)
-          float* p = a.part + blockIdx.x * a.H + c;
+        load_w(c, w[0]);
+        Vec<T> g;
+        g.clear();
+        if (a.dh) g = load_part((const T*)a.dh + row * a.lddh + c, n);
+        const Vec<T> x = load_part(hp + c, n), y = load_part(yp + c, n);
+        finish(x, y, g, w[0], vec);
+        if constexpr (DW) {  // (this thread's own columns of the workgroup's partial row)
+          float* p = a.part + blockIdx.x * a.ld_part + c;
 #pragma unroll
           for (int i = 0; i < VN; ++i)
             if (i < n) {
-              const float t = to_f32(y.v[i]) * (to_f32(x.v[i]) * rstd);
-              p[i] = first == (int64_t)blockIdx.x * RPB ? t : p[i] + t;
+              const float t = y.get(i) * (x.get(i) * rstd);
+              p[i] = started ? p[i] + t : t;
             }
         }
       }
+      started = true;
     }
-  }
-  if (!a.part || NV == 0) return;
-  float* part = a.part + blockIdx.x * a.H;
-  if constexpr (TPR == 64) {  // the four waves' sums, in wave order
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-#pragma unroll
-      for (int i = 0; i < VN; ++i) cols[slot * 64 * N * VN + (tid + j * 64) * VN + i] = dw[j][i];
-    __syncthreads();
-    for (int c = threadIdx.x; c < a.H; c += 256) {
-      float s = cols[c];
-#pragma unroll
-      for (int k = 1; k < 4; ++k) s += cols[k * 64 * N * VN + c];
-      part[c] = s;
+  };
+  // (every thread of a workgroup goes through the same rounds)
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t first = (int64_t)blockIdx.x * RPB;
+  if constexpr (AHEAD) {
+    fetch(first + slot, sets[0]);
+    for (; first < a.rows; first += 2 * step) {
+      fetch(first + step + slot, sets[1]);
+      work(first + slot, sets[0], 0);
+      if (first + step >= a.rows) break;
+      fetch(first + 2 * step + slot, sets[0]);
+      work(first + step + slot, sets[1], 1);
     }
   } else {
+    for (int flip = 0; first < a.rows; first += step, flip ^= 1) {
+      fetch(first + slot, sets[0]);
+      work(first + slot, sets[0], flip);
+    }
+  }
+  if constexpr (DW && NV > 0) {
+    float* part = a.part + blockIdx.x * a.ld_part;
+    if constexpr (TPR == 64) {  // the four waves' sums, in wave order
 #pragma unroll
-    for (int j = 0; j < N; ++j)
+      for (int j = 0; j < N; ++j)
 #pragma unroll
-      for (int i = 0; i < VN; ++i) {
-        const int c = (tid + j * TPR) * VN + i;
-        if (c < a.H) part[c] = dw[j][i];
+        for (int i = 0; i < VN; ++i) cols[slot * 64 * N * VN + (tid + j * 64) * VN + i] = dw[j][i];
+      __syncthreads();
+      for (int c = threadIdx.x; c < a.H; c += 256) {
+        float s = cols[c];
+#pragma unroll
+        for (int k = 1; k < 4; ++k) s += cols[k * 64 * N * VN + c];
+        part[c] = s;
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int c = (tid + j * TPR) * VN;
+#pragma unroll
+        for (int i = 0; i < VN; i += 4)  // (the pitch is a multiple of 4)
+          if (c + i < a.H) *reinterpret_cast<float4*>(part + c + i) = make_float4(dw[j][i], dw[j][i + 1], dw[j][i + 2], dw[j][i + 3]);
+      }
+    }
   }
 }
 
-// dw[c] = sum of the partial rows: 32 columns a workgroup, 8 groups of threads
-// add consecutive blocks of rows, one of them the groups' sums, in order.
-__global__ __launch_bounds__(256) void sum_parts_kernel(const float* part, int n, int64_t H, void* dw, int w_dtype) {
-  __shared__ float red[8][32];
-  const int c = threadIdx.x % 32, g = threadIdx.x / 32;
-  const int64_t col = (int64_t)blockIdx.x * 32 + c;
-  const int per = (n + 7) / 8, lo = g * per, hi = min(n, lo + per);
-  float s = 0.f;
-  if (col < H)
-    for (int r = lo; r < hi; ++r) s += part[r * H + col];
-  red[g][c] = s;
-  __syncthreads();
-  if (g == 0 && col < H) {
-#pragma unroll
-    for (int k = 1; k < 8; ++k) s += red[k][c];
-    if (w_dtype == FORGE_DTYPE_F32) ((float*)dw)[col] = s;
-    else if (w_dtype == FORGE_DTYPE_F16) ((fp16_t*)dw)[col] = (fp16_t)s;
-    else ((bf16_t*)dw)[col] = (bf16_t)s;
+// dw[c] = sum of the partial rows.  32 columns a workgroup, 4 a thread: 32 groups of
+// 8 threads add consecutive blocks of rows, and one of them the groups' sums, in
+// order.
+__global__ __launch_bounds__(256) void sum_parts_kernel(const float* part, int64_t ld, int n, int64_t H, void* dw, int w_dtype) {
+  __shared__ float4 red[32][8];
+  const int c4 = threadIdx.x % 8, g = threadIdx.x / 8;
+  const int64_t col = (int64_t)blockIdx.x * 32 + 4 * c4;
+  const int per = (n + 31) / 32, lo = g * per, hi = min(n, lo + per);
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (col < H) {
+#pragma unroll 8
+    for (int r = lo; r < hi; ++r) {
+      const float4 v = *reinterpret_cast<const float4*>(part + r * ld + col);
+      s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+    }
   }
+  red[g][c4] = s;
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
+  if (c >= H) return;
+  const float* f = reinterpret_cast<const float*>(&red[0][0]) + threadIdx.x;
+  float t = f[0];
+#pragma unroll
+  for (int k = 1; k < 32; ++k) t += f[32 * k];
+  if (w_dtype == FORGE_DTYPE_F32) ((float*)dw)[c] = t;
+  else if (w_dtype == FORGE_DTYPE_F16) ((fp16_t*)dw)[c] = (fp16_t)t;
+  else ((bf16_t*)dw)[c] = (bf16_t)t;
 }
 
 typedef void (*BwdKernel)(BwdArgs);
-template <class T, int TPR, int NV> constexpr BwdKernel bwd_k = add_rmsnorm_bwd_kernel<T, TPR, NV>;
-template <class T> BwdKernel pick_bwd(int64_t H) { FROWS_PICK(T, H, bwd_k); }
+template <class T, int TPR, int NV, bool DW> constexpr BwdKernel bwd_k = add_rmsnorm_bwd_kernel<T, TPR, NV, DW>;
+template <class T, bool DW> static BwdKernel pick_dw(int64_t H) { FROWS_PICK(T, H, bwd_k, DW); }
+template <class T> static BwdKernel pick_bwd(int64_t H, bool dw) { return dw ? pick_dw<T, true>(H) : pick_dw<T, false>(H); }
+
+static int64_t part_pitch(int64_t H) { return (H + 3) / 4 * 4; }
 
 // Workgroups: one partial row each.
 static int64_t bwd_blocks(int dtype, int64_t rows, int64_t H) {
@@ -175,7 +231,7 @@ using namespace frows;
 
 extern "C" int64_t forge_add_rmsnorm_bwd_workspace(int dtype, int64_t rows, int64_t H) {
   if (rows < 0 || H < 0 || dtype_size(dtype) == 0) return -1;
-  return bwd_blocks(dtype, rows, H) * H * 4;
+  return bwd_blocks(dtype, rows, H) * part_pitch(H) * 4;
 }
 
 extern "C" int forge_add_rmsnorm_bwd(int dtype, int w_dtype, const void* dy, int64_t lddy, const void* dh, int64_t lddh,
@@ -189,13 +245,13 @@ extern "C" int forge_add_rmsnorm_bwd(int dtype, int w_dtype, const void* dy, int
   if (lddy < H || ldh < H || (dh && lddh < H)) return forge_set_error(FORGE_ERR_INVALID, "add_rmsnorm: row pitch below %lld", (long long)H);
   if (rows == 0 || H == 0) return FORGE_OK;  // (the caller clears dw)
   if (!dy || !h || !weight || !rstd || !d || (dw && !work)) return forge_set_error(FORGE_ERR_INVALID, "add_rmsnorm: an array is NULL");
-  BwdArgs a = {dy, lddy, dh, lddh, h, ldh, weight, w_dtype, rstd, d, dw ? (float*)work : nullptr, rows, H, (float)offset};
-  const BwdKernel k = dtype == FORGE_DTYPE_F32 ? pick_bwd<float>(H) : dtype == FORGE_DTYPE_F16 ? pick_bwd<fp16_t>(H) : pick_bwd<bf16_t>(H);
+  BwdArgs a = {dy, lddy, dh, lddh, h, ldh, weight, w_dtype, rstd, d, (float*)work, part_pitch(H), rows, H, (float)offset};
+  const BwdKernel k = dtype == FORGE_DTYPE_F32 ? pick_bwd<float>(H, dw) : dtype == FORGE_DTYPE_F16 ? pick_bwd<fp16_t>(H, dw) : pick_bwd<bf16_t>(H, dw);
   const int64_t blocks = bwd_blocks(dtype, rows, H);
   k<<<(unsigned)blocks, 256, 0, (hipStream_t)stream>>>(a);
   FORGE_CHECK_LAUNCH();
   if (dw) {
-    sum_parts_kernel<<<(unsigned)((H + 31) / 32), 256, 0, (hipStream_t)stream>>>((const float*)work, (int)blocks, H, dw, w_dtype);
+    sum_parts_kernel<<<(unsigned)((H + 31) / 32), 256, 0, (hipStream_t)stream>>>((const float*)work, part_pitch(H), (int)blocks, H, dw, w_dtype);
     FORGE_CHECK_LAUNCH();
   }
   return FORGE_OK;
