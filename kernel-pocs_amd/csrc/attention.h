@@ -106,9 +106,8 @@ __device__ __forceinline__ TileAt find_tile(const int32_t* cu, int B, int64_t to
 // The same tiles in the order of `level`, the number of the tile from its
 // sequence's other end: the first tile of n has level n for the keys, the last
 // one for the queries, so that (causal) the tiles with the most work come first
-// and the last workgroups to start are short ones.  With the sequences' order
-// the dk, dv kernel ran 1285 us instead of ORDERED_US (8 sequences of 700 to 3400
-// tokens, 32 heads on 8: the longest began in the last round).  More than 256
+// and the last workgroups to start are short ones (13 sequences of 70 to 420
+// tokens, 14 heads of 64 on 2: the dk, dv kernel 113 -> 90 us).  More than 254
 // sequences go in their own order: there are many tiles then, and short ones.
 struct LevelAt {
   int seq, level;  // level: 1 .. tiles of the sequence

@@ -79,11 +79,11 @@ constexpr int LDS_PITCH = BK + 8;  // bf16 elements per LDS row
 enum Layout { ROW = 0, COL = 1 };
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+template <class T> using acc4_t = std::conditional_t<OutOf<T>::i8, i32x4, f32x4>;
 template <class T>
-__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
+__device__ __forceinline__ acc4_t<T> mfma16(bf16x8 a, bf16x8 b, acc4_t<T> c) {
   if constexpr (OutOf<T>::i8)
-    return __builtin_bit_cast(f32x4, __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b),
-                                                                         __builtin_bit_cast(i32x4, c), 0, 0, 0));
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
   else if constexpr (std::is_same_v<T, fp16_t>)
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(fp16x8, a), __builtin_bit_cast(fp16x8, b), c, 0, 0, 0);
   else
@@ -456,8 +456,8 @@ __device__ __forceinline__ void tile_coords(int64_t tiles_m, int64_t tiles_n, in
 }
 
 // An accumulator of 8-bit products to its value in C.
-__device__ __forceinline__ float scale_i8(float acc, float row, float col, float bias) {
-  return __builtin_fmaf((float)__builtin_bit_cast(int, acc) * row, col, bias);
+__device__ __forceinline__ float scale_i8(int acc, float row, float col, float bias) {
+  return __builtin_fmaf((float)acc * row, col, bias);
 }
 template <class O>
 __device__ __forceinline__ float bias_i8(const EpiArgs& ep, int64_t n) {
@@ -1301,7 +1301,7 @@ void gemm_dma_kernel(GemmArgs args) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int64_t m = min(m0 + wm * TM + i * 32 + 4 * (lane / 32) + 8 * (r / 4) + r % 4, M - 1);
-            acc[i][j][r] = scale_i8(acc[i][j][r], args.ep.row_scale[m], col, bias);
+            acc[i][j][r] = scale_i8(__float_as_int(acc[i][j][r]), args.ep.row_scale[m], col, bias);
           }
       }
     }

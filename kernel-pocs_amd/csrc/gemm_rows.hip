@@ -28,15 +28,15 @@ template <class T, int MB, int CB, int NW, int EPI>
 __global__ __launch_bounds__(NW * 64) void gemm_rows_kernel(GemmArgs args) {
   constexpr int ND = glu_fwd_epi(EPI) ? 2 : 1;
   constexpr int U = MB <= 2 ? 8 : 4;  // k-steps whose loads are in flight
-  __shared__ __attribute__((aligned(16))) f32x4 red[NW][CB * ND][MB][64];
+  __shared__ __attribute__((aligned(16))) acc4_t<T> red[NW][CB * ND][MB][64];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int64_t M = args.M, N = args.N, n0 = (int64_t)blockIdx.x * (16 * CB);
   const int r16 = lane % 16, kg = 16 * (lane / 16);
-  f32x4 acc[CB * ND][MB];
+  acc4_t<T> acc[CB * ND][MB];
 #pragma unroll
   for (int d = 0; d < CB * ND; ++d)
 #pragma unroll
-    for (int b = 0; b < MB; ++b) acc[d][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int b = 0; b < MB; ++b) acc[d][b] = acc4_t<T>{0, 0, 0, 0};
 
   int turn = 0;  // chunks dealt out so far, over all segments
   for (int s = 0; s < args.n_segs; ++s) {
@@ -110,17 +110,12 @@ __global__ __launch_bounds__(NW * 64) void gemm_rows_kernel(GemmArgs args) {
   for (int i = threadIdx.x; i < CB * MB * 64; i += NW * 64) {
     const int c = i / (MB * 64), b = i / 64 % MB, l = i % 64;
     const int64_t m = 16 * b + l % 16, n = n0 + 16 * c + 4 * (l / 16);
-    f32x4 v[ND];
+    acc4_t<T> v[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       v[d] = red[0][c * ND + d][b][l];
 #pragma unroll
-      for (int w = 1; w < NW; ++w) {
-        if constexpr (OutOf<T>::i8)
-          v[d] = __builtin_bit_cast(f32x4, __builtin_bit_cast(i32x4, v[d]) + __builtin_bit_cast(i32x4, red[w][c * ND + d][b][l]));
-        else
-          v[d] += red[w][c * ND + d][b][l];
-      }
+      for (int w = 1; w < NW; ++w) v[d] += red[w][c * ND + d][b][l];
     }
     if (m >= M) continue;
 #pragma unroll

@@ -59,6 +59,29 @@ __device__ __forceinline__ void bare_barrier() {
   asm volatile("" ::: "memory");
 }
 
+// acc += a b for accumulators that fill the AGPR file.  The compiler's 8-bit
+// instruction does not tie its result to its addend: it moved 270 accumulators a K
+// tile between the register files ([8192, 4096], K = 14336 467 -> 336 us, [8192, 14336], K =
+// 4096 532 -> 389).  Here
+// it is tied.  What the compiler would have waited for: the fragments' LDS reads (it
+// does: they are operands), and results that are read by anything but the same
+// accumulator's next product, 64 instructions on (settle, behind the loop).
+template <class T>
+__device__ __forceinline__ void mfma16_acc(bf16x8 a, bf16x8 b, acc4_t<T>& c) {
+  if constexpr (OutOf<T>::i8) asm("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  else c = mfma16<T>(a, b, c);
+}
+template <class T, int N, int K>
+__device__ __forceinline__ void settle(acc4_t<T> (&acc)[N][K]) {
+  if constexpr (OutOf<T>::i8) {
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");  // 32 cycles: the last results are written (8 passes and their latency)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int j = 0; j < K; ++j) asm volatile("" : "+a"(acc[i][j]));
+  }
+}
+
 // LDS-DMA loader of one 256-row K-contiguous operand tile for the 4-wave
 // engine.  As DmaLoader (XOR-swizzled 16-byte chunks, OOB offsets read
 // zeros), but the segment-tail mask is a per-lane select instead of a
@@ -263,11 +286,11 @@ void gemm_w4_kernel(GemmArgs args) {
   const int t_begin = blockIdx.z * per;
   const int t_end = min(total_tiles, t_begin + per);
 
-  f32x4 acc[FM][FN];
+  acc4_t<T> acc[FM][FN];
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < FN; ++j) acc[i][j] = acc4_t<T>{0, 0, 0, 0};
 
   static_assert(!(BT && BMODE == B_DUAL), "dual B operands are K-contiguous");
   using LoaderA = std::conditional_t<AT, W4LoaderT<BKT>, W4Loader<BKT, false>>;
@@ -366,7 +389,7 @@ void gemm_w4_kernel(GemmArgs args) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int m = 4 * p + u, i = m / FN, j = m % FN;
-      acc[i][j] = mfma16<T>(bfr[ks][j], af[ks][i], acc[i][j]);
+      mfma16_acc<T>(bfr[ks][j], af[ks][i], acc[i][j]);
     }
   };
   constexpr int NGRP = FM * FN / 4;  // 16 groups of four MFMAs per k-step ...
@@ -454,13 +477,16 @@ void gemm_w4_kernel(GemmArgs args) {
     }
     wait_vmcnt<0>();  // no zero-fill DMA may land in the staged epilogue's LDS
   }
+  settle<T>(acc);
   // The epilogue's per-lane addresses are formed here: hoisted above the main
   // loop (which holds 128 VGPRs of fragments), they spill inside it.
   int elane = lane, ewave = wave;
   asm volatile("" : "+v"(elane), "+s"(ewave));
   const int ewm = ewave % WAVES_M, ewn = ewave / WAVES_M;
-  if constexpr (OutOf<T>::i8) w4_scale_i8<out_t<T>>(args, acc, m0, n0, elane, ewm, ewn);
-  if constexpr (STAGED) {
+  if constexpr (OutOf<T>::i8) {
+    static_assert(RING == 160 * 1024, "the scales' place in the ring");
+    w4_epilogue_i8<out_t<T>, STAGED>(args, acc, m0, n0, elane, ewm, ewn, smem);
+  } else if constexpr (STAGED) {
     static_assert(w4_staged_epi(EPI), "staged epilogue: 16-bit or fp32 outputs");
     static_assert(RING >= W4_F32_BYTES, "the fp32 epilogue's slabs reuse the ring");
     __bf16* lds = reinterpret_cast<__bf16*>(smem);
@@ -469,9 +495,9 @@ void gemm_w4_kernel(GemmArgs args) {
     else if constexpr (BMODE == B_DUAL)
       w4_epilogue_staged_dual<EPI>(args, acc, m0, n0, elane, ewm, ewn, lds);
     else  // (STORE_BF16 is launched staged at beta = 0 only)
-      w4_epilogue_staged<out_t<T>, EPI>(args, acc, m0, n0, elane, ewm, ewn, lds);
+      w4_epilogue_staged<T, EPI>(args, acc, m0, n0, elane, ewm, ewn, lds);
   } else {
-    w4_epilogue_direct<out_t<T>, BMODE, EPI>(args, acc, m0, n0, elane, ewm, ewn);
+    w4_epilogue_direct<T, BMODE, EPI>(args, acc, m0, n0, elane, ewm, ewn);
   }
 }
 

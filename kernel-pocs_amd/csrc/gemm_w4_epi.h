@@ -61,25 +61,6 @@ __device__ __forceinline__ float col_alpha(const EpiArgs& ep, int64_t n) {
   return ep.alpha;
 }
 
-// The accumulators of 8-bit products, scaled in place to their values in C.
-template <class O>
-__device__ __forceinline__ void w4_scale_i8(const GemmArgs& args, f32x4 (&acc)[8][8], int64_t m0, int64_t n0, int lane,
-                                            int wm, int wn) {
-  const EpiArgs& ep = args.ep;
-  float row[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) row[i] = ep.row_scale[min(m0 + wm * 128 + i * 16 + lane % 16, args.M - 1)];
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int64_t n = min(n0 + wn * 128 + 16 * j + 4 * (lane / 16) + q, args.N - 1);
-      const float col = ep.col_scale[n], bias = bias_i8<O>(ep, n);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i][j][q] = scale_i8(acc[i][j][q], row[i], col, bias);
-    }
-}
-
 // ---------------------------------------------------------------------------
 // Direct epilogue: every element from registers, bounds-checked.
 // ---------------------------------------------------------------------------
@@ -801,6 +782,119 @@ __device__ __forceinline__ void w4_epilogue_staged_dual(const GemmArgs& args, f3
           hp[q] = lh[o + q];
         }
       }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// 8-bit products: C = acc row_scale[m] col_scale[n] + bias[n].  The tile's scales
+// go to LDS behind the main loop and are read a block of columns at a time:
+// held in registers (72 a lane), they left the allocator too few for the main
+// loop, which then moved 270 accumulators a K tile between the register files.
+// VEC: C's rows are 16-byte vectors.
+// ---------------------------------------------------------------------------
+constexpr int W4_SCALES = 160 * 1024 - 3 * 256 * 4;  // byte offset in the ring: row, column scales, bias
+
+template <class O, bool VEC>
+__device__ __forceinline__ void w4_epilogue_i8(const GemmArgs& args, const i32x4 (&acc)[8][8], int64_t m0, int64_t n0, int lane,
+                                               int wm, int wn, char* smem) {
+  static_assert(W4_STAGE_BYTES <= W4_SCALES && W4_F32_BYTES <= W4_SCALES, "scales behind the staged tile");
+  const EpiArgs& ep = args.ep;
+  const int64_t M = args.M, N = args.N;
+  const int tid = threadIdx.x, cl = 4 * (lane / 16);
+  float* scales = reinterpret_cast<float*>(smem + W4_SCALES);
+  const int64_t sm = min(m0 + tid, M - 1), sn = min(n0 + tid, N - 1);
+  const float row_scale = ep.row_scale[sm], col_scale = ep.col_scale[sn], col_bias = bias_i8<O>(ep, sn);
+  lds_barrier();  // the main loop's LDS reads are done in every wave
+  scales[tid] = row_scale;
+  scales[256 + tid] = col_scale;
+  scales[512 + tid] = col_bias;
+  lds_barrier();
+  float row[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) row[i] = scales[wm * 128 + i * 16 + lane % 16];
+  const float* cs = scales + 256 + wn * 128 + cl;
+  auto value = [&](int i, int j, const f32x4& col, const f32x4& bias, float (&v)[4]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = scale_i8(acc[i][j][q], row[i], col[q], bias[q]);
+  };
+  O* c0 = (O*)ep.c + (int64_t)blockIdx.z * ep.split_stride;
+  if constexpr (!VEC) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const f32x4 col = *reinterpret_cast<const f32x4*>(cs + 16 * j), bias = *reinterpret_cast<const f32x4*>(cs + 256 + 16 * j);
+      const int64_t n = n0 + wn * 128 + 16 * j + cl;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t m = m0 + wm * 128 + i * 16 + lane % 16;
+        float v[4];
+        value(i, j, col, bias, v);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (m < M && n + q < N) c0[m * ep.ldc + n + q] = from_f32<O>(v[q]);
+      }
+    }
+  } else if constexpr (sizeof(O) == 2) {  // the whole tile through LDS, as in w4_epilogue_staged
+    __bf16* lds = reinterpret_cast<__bf16*>(smem);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const f32x4 col = *reinterpret_cast<const f32x4*>(cs + 16 * j), bias = *reinterpret_cast<const f32x4*>(cs + 256 + 16 * j);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float v[4];
+        value(i, j, col, bias, v);
+        *reinterpret_cast<uint2*>(lds + (wm * 128 + i * 16 + lane % 16) * W4_SP + wn * 128 + 16 * j + cl) = pack4<O>(v);
+      }
+    }
+    lds_barrier();
+    const int c = (tid % 32) * 8;
+    const int64_t n = n0 + c;
+    const bool full = n + 8 <= N;
+#pragma unroll 4
+    for (int it = 0; it < 32; ++it) {
+      const int rr = it * 8 + tid / 32;
+      const int64_t m = m0 + rr;
+      if (m >= M || n >= N) continue;
+      O* cp = c0 + m * ep.ldc + n;
+      if (full) {
+        st16(cp, *reinterpret_cast<const uint4*>(lds + rr * W4_SP + c));
+      } else {
+        const O* pv = reinterpret_cast<const O*>(lds + rr * W4_SP + c);
+        for (int q = 0; q < 8 && n + q < N; ++q) cp[q] = pv[q];
+      }
+    }
+  } else {  // fp32: 64 rows of each wave's block at a time through a slab of its own
+    constexpr int SLAB = 64 * W4_FP;
+    static_assert(4 * SLAB * 4 <= W4_F32_BYTES, "four slabs");
+    float* slab = reinterpret_cast<float*>(smem) + (wn * 2 + wm) * SLAB;
+    const int c = (lane % 32) * 4;
+    const int64_t n = n0 + wn * 128 + c;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const f32x4 col = *reinterpret_cast<const f32x4*>(cs + 16 * j), bias = *reinterpret_cast<const f32x4*>(cs + 256 + 16 * j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float v[4];
+          value(4 * half + i, j, col, bias, v);
+          *reinterpret_cast<f32x4*>(slab + (16 * i + lane % 16) * W4_FP + 16 * j + cl) = f32x4{v[0], v[1], v[2], v[3]};
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave's slab is written
+      const int64_t mb = m0 + wm * 128 + 64 * half;
+#pragma unroll 4
+      for (int it = 0; it < 32; ++it) {
+        const int rr = it * 2 + lane / 32;
+        if (mb + rr >= M || n >= N) continue;
+        float* cp = (float*)c0 + (mb + rr) * ep.ldc + n;
+        if (n + 4 <= N) {
+          *reinterpret_cast<f32x4*>(cp) = *reinterpret_cast<const f32x4*>(slab + rr * W4_FP + c);
+        } else {
+          for (int q = 0; q < 4 && n + q < N; ++q) cp[q] = slab[rr * W4_FP + c + q];
+        }
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (and read, before the other half is written)
     }
   }
 }
