@@ -178,7 +178,7 @@ struct EpiArgs {
   const __bf16* wxt[2];
   int64_t wxt_ld;
   // 8-bit operands (I8): C = acc row_scale[m] col_scale[n] + bias[n] (bias of C's
-  // type, or nullptr; with split-K it is added to the first slice)
+  // type, or nullptr)
   const float* row_scale;
   const float* col_scale;
   const void* bias;
@@ -461,7 +461,7 @@ __device__ __forceinline__ float scale_i8(int acc, float row, float col, float b
 }
 template <class O>
 __device__ __forceinline__ float bias_i8(const EpiArgs& ep, int64_t n) {
-  return ep.bias && blockIdx.z == 0 ? to_f32<O>(((const O*)ep.bias)[n]) : 0.f;
+  return ep.bias ? to_f32<O>(((const O*)ep.bias)[n]) : 0.f;
 }
 
 // Scheduling-group masks of __builtin_amdgcn_sched_group_barrier.
@@ -1291,7 +1291,21 @@ void gemm_dma_kernel(GemmArgs args) {
     static_assert(staged_ok(BM, BN, WAVES_M, WAVES_N, EPI), "staged epilogue: 256 x 256 tile, wave tiles of <= 128 rows");
     epilogue_staged<T, WAVES_M, WAVES_N, EPI>(args, acc, m0, n0, lane, wm, wn, reinterpret_cast<float*>(smem));
   } else {
-    if constexpr (OutOf<T>::i8) {
+    if constexpr (std::is_same_v<T, I8<int>>) {  // a part of K: the integers as they are
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const int64_t n = n0 + wn * TN + j * 32 + lane % 32;
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int64_t m = m0 + wm * TM + i * 32 + 4 * (lane / 32) + 8 * (r / 4) + r % 4;
+            if (m < M && n < args.N)
+              ((int*)args.ep.c)[(int64_t)blockIdx.z * args.ep.split_stride + m * args.ep.ldc + n] = __float_as_int(acc[i][j][r]);
+          }
+      }
+      return;
+    } else if constexpr (OutOf<T>::i8) {
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
         const int64_t n = min(n0 + wn * TN + j * 32 + lane % 32, args.N - 1);
@@ -1305,6 +1319,7 @@ void gemm_dma_kernel(GemmArgs args) {
           }
       }
     }
+    if constexpr (!std::is_same_v<T, I8<int>>)
     epilogue<out_t<T>, BM, BN, WAVES_M, WAVES_N, EPI>(args, acc, m0, n0, lane, wm, wn);
   }
 }

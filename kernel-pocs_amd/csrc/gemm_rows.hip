@@ -197,11 +197,22 @@ int launch_rows(int epi, const GemmArgs& a, hipStream_t s) {
   return forge_set_error(FORGE_ERR_UNSUPPORTED, "gemm: epilogue %d on %lld rows", epi, (long long)a.M);
 }
 
-// 8-bit operands.
+// 8-bit operands.  Columns and waves a workgroup: measured on MI355X, weights not
+// cached, us with 16 x 8 / 32 x 4 / 32 x 2 / 64 x 2: [16, 4096], K = 14336 17 / 23 / 23 / 36;
+// [16, 6144], K = 4096 11.1 / 9.7 / 9.9 / 14.1, [16, 14336] 21 / 17 / 16 / 17, [16, 28672] 38 /
+// 30 / 29 / 29, [32, 28672] 50 / 38 / 35 / 32.
+template <class O, int MB>
+static int launch_rows_i8_mb(const GemmArgs& a, hipStream_t s) {
+  if (a.N <= 4096) return launch_one<I8<O>, MB, 1, 8, EPI_STORE_BF16>(a, s);
+  if (a.N <= 8192) return launch_one<I8<O>, MB, 2, 4, EPI_STORE_BF16>(a, s);
+  return launch_one<I8<O>, MB, 2, 2, EPI_STORE_BF16>(a, s);
+}
+
 template <class O>
 static int launch_rows_i8_t(const GemmArgs& a, hipStream_t s) {
-  if (a.M <= 16) return a.N < 16 * 64 ? launch_one<I8<O>, 1, 1, 16, EPI_STORE_BF16>(a, s) : launch_one<I8<O>, 1, 1, 8, EPI_STORE_BF16>(a, s);
-  return a.N < 16 * 64 ? launch_one<I8<O>, 2, 1, 16, EPI_STORE_BF16>(a, s) : launch_one<I8<O>, 2, 1, 8, EPI_STORE_BF16>(a, s);
+  if (a.M <= 16) return launch_rows_i8_mb<O, 1>(a, s);
+  if (a.M <= 32) return launch_rows_i8_mb<O, 2>(a, s);
+  return launch_one<I8<O>, 4, 1, 8, EPI_STORE_BF16>(a, s);  // (up to 4096 columns)
 }
 
 int launch_rows_i8(int out_dtype, const GemmArgs& a, hipStream_t s) {

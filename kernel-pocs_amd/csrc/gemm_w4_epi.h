@@ -818,7 +818,7 @@ __device__ __forceinline__ void w4_epilogue_i8(const GemmArgs& args, const i32x4
 #pragma unroll
     for (int q = 0; q < 4; ++q) v[q] = scale_i8(acc[i][j][q], row[i], col[q], bias[q]);
   };
-  O* c0 = (O*)ep.c + (int64_t)blockIdx.z * ep.split_stride;
+  O* c0 = (O*)ep.c;
   if constexpr (!VEC) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {

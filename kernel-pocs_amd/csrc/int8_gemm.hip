@@ -35,24 +35,79 @@ static int launch_i8_tile(const GemmArgs& a, hipStream_t s) {
   return FORGE_OK;
 }
 
+// The engine by the product's size.  Measured on MI355X, weights not cached, us:
+//   rows (gemm_rows.hip): up to 32 rows; up to 64 of [4096] x K = 4096 and less, [33,
+//     1024] 9.7, [64, 4096] 14.4 against 12.0 and 14.7 with 64 x 64 tiles split 4 ways;
+//   256 x 256 tiles from 128 of them on: [2000, 14336], K = 4096 114, 128 x 128 tiles 184;
+//   64 x 128 tiles where they fill the chip: [1000, 4096], K = 4096 34, 64 x 64 tiles 43,
+//     256 x 256 49; [4000, 1024] 30 / 38 / 47;
+//   64 x 64 tiles, split over K where they are few and K is long: [100, 1024], K =
+//     14336 48 -> 16 in 8 parts, [128, 4096], K = 14336 50 -> 30 in 4, [100, 4096], K = 4096
+//     18.8 -> 16.7; not [333, 1008], K = 2016: 10.9, 12.5 in 2.
+enum Engine { ROWS, BIG, TILE_128, TILE_64 };
+struct Plan {
+  int engine, split;
+};
+
+static Plan plan_i8(int64_t M, int64_t N, int64_t K) {
+  auto tiles = [&](int64_t bm, int64_t bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
+  if (M <= 32 || (M <= 64 && N <= 4096 && K <= 4096)) return {ROWS, 1};
+  if (tiles(256, 256) >= 128) return {BIG, 1};
+  if (tiles(64, 128) >= 256) return {TILE_128, 1};
+  const int64_t t = tiles(64, 64), steps = (K + 127) / 128;
+  int64_t split = steps < 32 ? 1 : 512 / t < steps / 8 ? 512 / t : steps / 8;
+  return {TILE_64, (int)(split < 1 ? 1 : split > 8 ? 8 : split)};
+}
+
+static int64_t part_pitch(int64_t N) { return (N + 3) / 4 * 4; }
+
+// C from the integers of the parts of K: still exact, and rounded once.
 template <class O>
-static int launch_i8(int out_dtype, const GemmArgs& a, hipStream_t s) {
+__global__ __launch_bounds__(256) void join_i8_kernel(const int* parts, int64_t stride, int n, int64_t M, int64_t N, int64_t vecs,
+                                                      EpiArgs ep) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / vecs, c = i % vecs * 4;
+  if (m >= M) return;
+  i32x4 sum = {0, 0, 0, 0};
+  for (int z = 0; z < n; ++z) sum += *reinterpret_cast<const i32x4*>(parts + z * stride + m * vecs * 4 + c);
+  const float row = ep.row_scale[m];
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    if (c + q < N) ((O*)ep.c)[m * ep.ldc + c + q] = from_f32<O>(scale_i8(sum[q], row, ep.col_scale[c + q], bias_i8<O>(ep, c + q)));
+}
+
+template <class O>
+static int launch_i8(int out_dtype, const GemmArgs& a, const Plan& p, int* work, hipStream_t s) {
   constexpr int EPI = std::is_same_v<O, float> ? EPI_STORE_F32 : EPI_STORE_BF16;
-  if (a.M <= 32) return launch_rows_i8(out_dtype, a, s);
-  const int64_t big = ((a.M + 255) / 256) * ((a.N + 255) / 256);
-  if (big >= 128) return launch_i8_big<O, EPI>(a, s);
-  const int64_t mid = ((a.M + 127) / 128) * ((a.N + 127) / 128);
-  if (mid >= 256) return launch_i8_tile<O, 128, 128, 2, 2>(a, s);
-  return launch_i8_tile<O, 64, 64, 3, 3>(a, s);
+  if (p.engine == ROWS) return launch_rows_i8(out_dtype, a, s);
+  if (p.engine == BIG) return launch_i8_big<O, EPI>(a, s);
+  if (p.engine == TILE_128) return launch_i8_tile<O, 64, 128, 3, 2>(a, s);
+  if (p.split == 1) return launch_i8_tile<O, 64, 64, 3, 3>(a, s);
+  GemmArgs g = a;  // the parts' integers
+  g.ep.c = work;
+  g.ep.ldc = part_pitch(a.N);
+  g.ep.split_stride = a.M * g.ep.ldc;
+  g.split_k = p.split;
+  if (int e = launch_i8_tile<int, 64, 64, 3, 3>(g, s)) return e;
+  const int64_t items = a.M * (g.ep.ldc / 4);
+  join_i8_kernel<O><<<(unsigned)((items + 255) / 256), 256, 0, s>>>(work, g.ep.split_stride, p.split, a.M, a.N, g.ep.ldc / 4, a.ep);
+  FORGE_CHECK_LAUNCH();
+  return FORGE_OK;
 }
 
 }  // namespace fgemm
 
 using namespace fgemm;
 
+extern "C" int64_t forge_int8_gemm_workspace(int64_t M, int64_t N, int64_t K) {
+  if (M < 0 || N < 0 || K < 0) return -1;
+  if (M == 0 || N == 0) return 0;
+  const Plan p = plan_i8(M, N, (K + 15) / 16 * 16);
+  return p.split > 1 ? p.split * M * part_pitch(N) * 4 : 0;
+}
+
 extern "C" int forge_int8_gemm(const int8_t* a, int64_t lda, const float* row_scale, const int8_t* b, int64_t ldb,
                                const float* col_scale, const void* bias, void* c, int64_t ldc, int c_dtype, int64_t M,
-                               int64_t N, int64_t K, void* stream) {
+                               int64_t N, int64_t K, void* work, void* stream) {
   if (M < 0 || N < 0 || K < 0 || K > (int64_t(1) << 17))
     return forge_set_error(FORGE_ERR_INVALID, "int8_gemm: sizes (K up to 2^17, where a sum fits 32 bits)");
   if (c_dtype != FORGE_DTYPE_F32 && c_dtype != FORGE_DTYPE_F16 && c_dtype != FORGE_DTYPE_BF16)
@@ -82,10 +137,12 @@ extern "C" int forge_int8_gemm(const int8_t* a, int64_t lda, const float* row_sc
   g.ep.col_scale = col_scale;
   g.ep.bias = bias;
   g.ep.vec_ok = aligned16(c) && ldc % 8 == 0;
+  const Plan p = plan_i8(M, N, kp);
+  if (p.split > 1 && (!work || !aligned16(work))) return forge_set_error(FORGE_ERR_INVALID, "int8_gemm: work is NULL or not aligned");
   const hipStream_t s = (hipStream_t)stream;
-  if (c_dtype == FORGE_DTYPE_F32) return launch_i8<float>(c_dtype, g, s);
-  if (c_dtype == FORGE_DTYPE_F16) return launch_i8<fp16_t>(c_dtype, g, s);
-  return launch_i8<bf16_t>(c_dtype, g, s);
+  if (c_dtype == FORGE_DTYPE_F32) return launch_i8<float>(c_dtype, g, p, (int*)work, s);
+  if (c_dtype == FORGE_DTYPE_F16) return launch_i8<fp16_t>(c_dtype, g, p, (int*)work, s);
+  return launch_i8<bf16_t>(c_dtype, g, p, (int*)work, s);
 }
 
 // dst[c][r] = src[r][c] of 8-bit values, 64 x 64 tiles through LDS, zeros in the

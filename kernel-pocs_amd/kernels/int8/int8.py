@@ -153,10 +153,12 @@ class Int8Weight:
 def _product(q, scale, w, w_scale, bias, dtype, n, k):
     out = torch.empty(q.shape[0], n, dtype=dtype, device=q.device)
     if out.numel():
+        nbytes = L.forge_int8_gemm_workspace(q.shape[0], n, k)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
         with L.on_device(q):
             L.check(L.forge_int8_gemm(q.data_ptr(), q.shape[1], scale.data_ptr(), w.data_ptr(), w.shape[1],
                                       w_scale.data_ptr(), L.ptr(bias), out.data_ptr(), n, L.dtype_code(dtype), q.shape[0],
-                                      n, k, L.stream_of(q)), "forge_int8_gemm")
+                                      n, k, L.ptr(work), L.stream_of(q)), "forge_int8_gemm")
     return out
 
 

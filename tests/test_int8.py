@@ -53,7 +53,8 @@ def _check(m, n, k, dtype, bias=False, train=True, out_dtype=None, seed=0):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 130, 500), (16, 1024, 512), (17, 33, 100), (32, 2017, 1003), (33, 70, 64),
-                                   (100, 1024, 4096), (333, 257, 130), (129, 640, 4101)])
+                                   (100, 1024, 4096), (333, 257, 130), (129, 640, 4101), (64, 4096, 300), (20, 9001, 200),
+                                   (70, 70, 14336)])
 def test_sizes(m, n, k, dtype):
     _check(m, n, k, dtype, bias=m % 2 == 1)
 
@@ -209,13 +210,17 @@ def test_entry_point_refusals():
     from forge_hip import _lib as L
 
     def gemm(a=16, lda=64, rs=16, b=16, ldb=64, cs=16, c=16, ldc=40, dtype=2, M=4, N=40, K=64):
-        return L.forge_int8_gemm(a, lda, rs, b, ldb, cs, None, c, ldc, dtype, M, N, K, None)
+        return L.forge_int8_gemm(a, lda, rs, b, ldb, cs, None, c, ldc, dtype, M, N, K, None, None)
 
     assert gemm(dtype=3) == 2
     for kw in ({"M": -1}, {"K": (1 << 17) + 1}, {"lda": 48}, {"ldb": 72}, {"lda": 1 << 22}, {"a": 24}, {"b": 8}, {"ldc": 39},
                {"a": None}, {"b": None}, {"rs": None}, {"cs": None}, {"c": None}):
         assert gemm(**kw) == 1, kw
     assert gemm(M=0, a=None, c=None) == 0
+    # a product that is split over K needs its workspace
+    assert L.forge_int8_gemm_workspace(4, 40, 64) == 0 and L.forge_int8_gemm_workspace(100, 1024, 14336) == 8 * 100 * 1024 * 4
+    assert gemm(M=100, N=1024, K=14336, lda=14336, ldb=14336, ldc=1024) == 1 and b"work" in L.forge_last_error()
+    assert L.forge_int8_gemm_workspace(-1, 40, 64) == -1
     assert L.forge_transpose_1b(None, 8, 4, 8, 16, 16, None) == 1
     assert L.forge_transpose_1b(16, 7, 4, 8, 16, 16, None) == 1
     assert L.forge_quantize_rows(2, 16, 8, None, 16, 8, 16, 2, 8, None) == 1
