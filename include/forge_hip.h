@@ -849,6 +849,14 @@ int forge_int8_gemm(const int8_t* a, int64_t lda, const float* row_scale, const 
                     const float* col_scale, const void* bias, void* c, int64_t ldc, int c_dtype, int64_t M,
                     int64_t N, int64_t K, void* work, void* stream);
 
+/* forge_quantize_rows and forge_int8_gemm of the result in one call: C = x w^T with
+ * the rows of x (times x_col_scale, or NULL) in 8 bits.  work:
+ * forge_int8_linear_workspace bytes, 16-byte aligned. */
+int64_t forge_int8_linear_workspace(int64_t M, int64_t N, int64_t K);
+int forge_int8_linear(int x_dtype, const void* x, int64_t ldx, const float* x_col_scale, const int8_t* w,
+                      int64_t ldw, const float* w_scale, const void* bias, void* c, int64_t ldc, int c_dtype,
+                      int64_t M, int64_t N, int64_t K, void* work, void* stream);
+
 /* dst[c, r] = src[r, c] of 8-bit values, zeros in dst's columns from `rows` to ld_dst. */
 int forge_transpose_1b(const int8_t* src, int64_t ld_src, int64_t rows, int64_t cols, int8_t* dst, int64_t ld_dst,
                        void* stream);

@@ -145,6 +145,32 @@ extern "C" int forge_int8_gemm(const int8_t* a, int64_t lda, const float* row_sc
   return launch_i8<bf16_t>(c_dtype, g, p, (int*)work, s);
 }
 
+// The rows of x in 8 bits and their product in one call: work holds the integers,
+// their scales, and the product's own workspace.
+static int64_t rows8_bytes(int64_t M, int64_t kp) { return M * kp + (M * 4 + 15) / 16 * 16; }
+
+extern "C" int64_t forge_int8_linear_workspace(int64_t M, int64_t N, int64_t K) {
+  const int64_t own = forge_int8_gemm_workspace(M, N, K);
+  return own < 0 ? -1 : rows8_bytes(M, (K + 15) / 16 * 16) + own;
+}
+
+extern "C" int forge_int8_linear(int x_dtype, const void* x, int64_t ldx, const float* x_col_scale, const int8_t* w, int64_t ldw,
+                                 const float* w_scale, const void* bias, void* c, int64_t ldc, int c_dtype, int64_t M, int64_t N,
+                                 int64_t K, void* work, void* stream) {
+  if (M < 0 || N < 0 || K < 0) return forge_set_error(FORGE_ERR_INVALID, "int8_linear: sizes");
+  if (M == 0 || N == 0) return FORGE_OK;
+  if (!work || !aligned16(work)) return forge_set_error(FORGE_ERR_INVALID, "int8_linear: work is NULL or not aligned");
+  const int64_t kp = (K + 15) / 16 * 16;
+  int8_t* q = (int8_t*)work;
+  float* scale = (float*)(q + M * kp);
+  // (no columns: every sum is 0, whatever the scales; they are not written)
+  if (K > 0)
+    if (int e = forge_quantize_rows(x_dtype, x, ldx, x_col_scale, q, kp, scale, M, K, stream)) return e;
+  if (K == 0)
+    if (int e = forge_zero(scale, M * 4, stream)) return e;
+  return forge_int8_gemm(q, kp, scale, w, ldw, w_scale, bias, c, ldc, c_dtype, M, N, K, q + rows8_bytes(M, kp), stream);
+}
+
 // dst[c][r] = src[r][c] of 8-bit values, 64 x 64 tiles through LDS, zeros in the
 // columns of dst from `rows` to its pitch.
 __global__ __launch_bounds__(256) void transpose_1b_kernel(const int8_t* src, int64_t ld_src, int64_t rows, int64_t cols,

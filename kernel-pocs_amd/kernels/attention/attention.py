@@ -31,8 +31,8 @@ _MAX_ROW = 1 << 23  # elements from one token to the next
 
 
 def _rows_ok(t, strides):
-    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and strides[1] < _MAX_ROW
-            and all(s % 8 == 0 for s in strides))
+    batch, row, head = strides
+    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and row < _MAX_ROW and (batch | row | head) % 8 == 0
 
 
 class _Layout:

@@ -33,7 +33,9 @@ def _pitch(k: int) -> int:
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """x as [rows, K] with a unit stride in K."""
-    x2 = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if x2.is_contiguous():
+        return x2
     if x2.stride(-1) != 1 and x2.shape[-1] > 1 or (x2.shape[0] > 1 and x2.stride(0) < x2.shape[-1]):
         x2 = x2.contiguous()
     return x2
@@ -162,6 +164,20 @@ def _product(q, scale, w, w_scale, bias, dtype, n, k):
     return out
 
 
+def _linear(x2, col_scale, w, w_scale, bias, dtype, n, k):
+    """The rows of x2 [M, k] (times col_scale) rounded to 8 bits, times w [n, k]: [M, n]."""
+    rows, device = x2.shape[0], x2.device
+    out = torch.empty(rows, n, dtype=dtype, device=device)
+    if rows and n:
+        work = torch.empty(L.forge_int8_linear_workspace(rows, n, k), dtype=torch.uint8, device=device)
+        with L.on_device(x2):
+            L.check(L.forge_int8_linear(L.dtype_code(x2.dtype), x2.data_ptr(), _ld(x2), L.ptr(col_scale), w.data_ptr(),
+                                        w.shape[1], w_scale.data_ptr(), L.ptr(bias), out.data_ptr(), n,
+                                        L.dtype_code(dtype), rows, n, k, work.data_ptr(), L.stream_of(x2)),
+                    "forge_int8_linear")
+    return out
+
+
 class Int8LinearFunction(torch.autograd.Function):
     """forward(ctx, x, weight, bias, dtype) on checked arguments; keeps nothing of x."""
 
@@ -169,15 +185,15 @@ class Int8LinearFunction(torch.autograd.Function):
     def forward(ctx, x, weight, bias, dtype):
         ctx.weight, ctx.x_shape, ctx.x_dtype = weight, x.shape, x.dtype
         n, k = weight.shape
-        return _product(*_quantize(_rows(x)), weight.padded, weight.scale, bias, dtype, n, k).view(*x.shape[:-1], n)
+        return _linear(_rows(x), None, weight.padded, weight.scale, bias, dtype, n, k).view(*x.shape[:-1], n)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         w = ctx.weight
         n, k = w.shape
-        q, scale = _quantize(_rows(dy), w.scale)
-        return _product(q, scale, w.transposed, w.ones, None, ctx.x_dtype, k, n).view(ctx.x_shape), None, None, None
+        dx = _linear(_rows(dy), w.scale, w.transposed, w.ones, None, ctx.x_dtype, k, n)
+        return dx.view(ctx.x_shape), None, None, None
 
 
 def int8_linear(x: Union[torch.Tensor, Int8Rows], weight: Int8Weight, bias: Optional[torch.Tensor] = None, *,
@@ -215,7 +231,7 @@ def int8_linear(x: Union[torch.Tensor, Int8Rows], weight: Int8Weight, bias: Opti
             raise ValueError("the gradient of x needs a weight made with backward=True")
         return Int8LinearFunction.apply(x, weight, bias, dtype)
     L.refuse_tangents(x)
-    return _product(*_quantize(_rows(x)), weight.padded, weight.scale, bias, dtype, n, k).view(*x.shape[:-1], n)
+    return _linear(_rows(x), None, weight.padded, weight.scale, bias, dtype, n, k).view(*x.shape[:-1], n)
 
 
 __all__ = ["Int8LinearFunction", "Int8Rows", "Int8Weight", "int8_linear", "quantize_int8_rows"]

@@ -221,6 +221,12 @@ def test_entry_point_refusals():
     assert L.forge_int8_gemm_workspace(4, 40, 64) == 0 and L.forge_int8_gemm_workspace(100, 1024, 14336) == 8 * 100 * 1024 * 4
     assert gemm(M=100, N=1024, K=14336, lda=14336, ldb=14336, ldc=1024) == 1 and b"work" in L.forge_last_error()
     assert L.forge_int8_gemm_workspace(-1, 40, 64) == -1
+    def linear(x=16, ldx=64, w=16, c=16, work=16, M=4, N=40, K=64):
+        return L.forge_int8_linear(2, x, ldx, None, w, 64, 16, None, c, N, 2, M, N, K, work, None)
+
+    assert L.forge_int8_linear_workspace(4, 40, 60) == 4 * 64 + 16 and L.forge_int8_linear_workspace(-1, 40, 64) == -1
+    assert linear(M=0, x=None, work=None) == 0 and linear(work=None) == 1 and linear(work=24) == 1
+    assert linear(M=-1) == 1 and linear(ldx=63) == 1 and linear(x=None) == 1
     assert L.forge_transpose_1b(None, 8, 4, 8, 16, 16, None) == 1
     assert L.forge_transpose_1b(16, 7, 4, 8, 16, 16, None) == 1
     assert L.forge_quantize_rows(2, 16, 8, None, 16, 8, 16, 2, 8, None) == 1
