@@ -6,12 +6,42 @@
 //   group's heads,                      a workgroup to 128 keys of a kv head,
 // with p_ij = exp2((s_ij - lse_i / scale) c), c = scale log2(e), computed again and ds_ij = p_ij (dout_i . v_j -
 // delta_i).  p and ds are rounded to 16 bits as operands; every sum is in fp32.
+// fp16 has few small values (2^-14 is the last with 11 bits), so there p is 2^14
+// times as large, and ds times a power of two from 2^14 down to 1, a wave's choice that
+// falls, with its sums, when one of its ds would pass fp16's largest value.  The sums
+// are taken back at the end.  All of that is exact.
 // As in the forward, products are laid out so that p and ds stay in the
 // registers that they are computed in: keys x queries for dq, queries x keys for
 // dk and dv.
+#include <type_traits>
+
 #include "attention.h"
 
 namespace fattn {
+
+template <class T>
+constexpr float P_BITS = std::is_same_v<T, fp16_t> ? 14.f : 0.f;
+
+// The wave's ds, 2^14 unit times what they are, within fp16's range as far as unit
+// can fall; the sums follow.
+template <class T, int DB>
+__device__ __forceinline__ void keep_in_range(f32x16& ds, float& unit, f32x16 (&sums)[DB]) {
+  if constexpr (std::is_same_v<T, fp16_t>) {
+    while (true) {
+      float top = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(ds[r]));
+      if (unit < 0x1p-13f || !__any(top > 65504.f)) return;
+      unit *= 0.25f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) ds[r] *= 0.25f;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sums[db][r] *= 0.25f;
+    }
+  }
+}
 
 // rows [batch][row] of the query side, one wave to a (row, head) at a time
 template <class T>
@@ -82,7 +112,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dq_kernel(Args a,
   }
   const int64_t row = a.cu_q ? sq.start + iq : sq.batch * a.tq + iq;
   const float c = a.scale * LOG2E;
-  const float below = live ? shift_of[head * n_rows + row] * c : -__builtin_inff();
+  const float below = live ? shift_of[head * n_rows + row] * c + P_BITS<T> : -__builtin_inff();
+  float unit = 1.f;
   const float delta = live ? a.delta[head * n_rows + row] : 0.f;
 
   Dma kd, vd;
@@ -126,12 +157,13 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dq_kernel(Args a,
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) dp = mfma32<T>(fr.read(vt, 32 * kb, ks), df[ks], dp);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = exp2_hw(__builtin_fmaf(s[r], c, below)) * (dp[r] + delta);
+      for (int r = 0; r < 16; ++r) s[r] = exp2_hw(__builtin_fmaf(s[r], c, below)) * ((dp[r] + delta) * unit);
       if (k0 + 32 > all_see) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (k0 + 8 * (r / 4) + 4 * h + r % 4 >= sees) s[r] = 0.f;
       }
+      keep_in_range<T>(s, unit, acc);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const bf16x8 ds = pack_acc<T>(s, i);
@@ -151,6 +183,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dq_kernel(Args a,
     if (NST == 2 && t + 1 < n_t) step(t + 1, 1);
   }
   if (!live) return;
+  const float back = a.scale * exp2f(-P_BITS<T>) / unit;
   T* op = row_ptr<T>(a.dq, sq.batch, sq.start + iq, head);
 #pragma unroll
   for (int db = 0; db < DB; ++db)
@@ -158,8 +191,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dq_kernel(Args a,
     for (int i = 0; i < 4; ++i) {
       const int d = 32 * db + 8 * i + 4 * h;
       if (d >= a.D) continue;
-      store4(op + d, acc[db][4 * i] * a.scale, acc[db][4 * i + 1] * a.scale, acc[db][4 * i + 2] * a.scale,
-             acc[db][4 * i + 3] * a.scale);
+      store4(op + d, acc[db][4 * i] * back, acc[db][4 * i + 1] * back, acc[db][4 * i + 2] * back,
+             acc[db][4 * i + 3] * back);
     }
 }
 
@@ -235,6 +268,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[db][r] = dv[db][r] = 0.f;
   const float c = a.scale * LOG2E;
+  float unit = 1.f;
 
   int tile_i = first;
   auto step = [&](bool more, int slot) __attribute__((always_inline)) {
@@ -274,9 +308,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[r] = exp2_hw(s[r] * c);
-        dp[r] *= s[r];
+        s[r] = exp2_hw(P_BITS<T> ? __builtin_fmaf(s[r], c, P_BITS<T>) : s[r] * c);
+        dp[r] *= s[r] * unit;
       }
+      if constexpr (DK) keep_in_range<T>(dp, unit, dk);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -295,6 +330,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
     if (t + 1 < n_t) step(t + 2 < n_t, 1);
   }
   if (!live) return;
+  const float p_one = exp2f(-P_BITS<T>), back = a.scale * p_one / unit;
   T* kp = row_ptr<T>(a.dk, sk.batch, sk.start + jk, it.kv);
   T* vp = row_ptr<T>(a.dv, sk.batch, sk.start + jk, it.kv);
 #pragma unroll
@@ -304,9 +340,9 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
       const int d = 32 * db + 8 * i + 4 * h;
       if (d >= a.D) continue;
       if constexpr (DK)
-        store4(kp + d, dk[db][4 * i] * a.scale, dk[db][4 * i + 1] * a.scale, dk[db][4 * i + 2] * a.scale,
-               dk[db][4 * i + 3] * a.scale);
-      if constexpr (DV) store4(vp + d, dv[db][4 * i], dv[db][4 * i + 1], dv[db][4 * i + 2], dv[db][4 * i + 3]);
+        store4(kp + d, dk[db][4 * i] * back, dk[db][4 * i + 1] * back, dk[db][4 * i + 2] * back,
+               dk[db][4 * i + 3] * back);
+      if constexpr (DV) store4(vp + d, dv[db][4 * i] * p_one, dv[db][4 * i + 1] * p_one, dv[db][4 * i + 2] * p_one, dv[db][4 * i + 3] * p_one);
     }
 }
 

@@ -15,16 +15,18 @@ import torch
 FLUSH = 2.0 ** -126  # v_exp_f32 returns 0 where the result is below it
 
 
-def head_fwd_bwd(q, k, v, do, scale, causal, unit, tiny):
+def head_fwd_bwd(q, k, v, do, scale, causal, unit, tiny, tiny_bwd=None):
     """q, do [n, D]; k, v [m, D] (any floating type).  unit: the largest relative
     error of rounding to the kernels' operand type, tiny: its largest absolute one
-    (half the spacing of its subnormals).
+    (half the spacing of its subnormals); tiny_bwd: that of the gradients' p and ds,
+    where they are held as multiples.
 
     Returns o, lse, dq, dk, dv and for each x an x_err: how far a computation may be
     that keeps s, sums and statistics in fp32, and rounds p, ds and o to that type."""
     q, k, v, do = (t.double() for t in (q, k, v, do))
     n, m = q.shape[0], k.shape[0]
     u32 = 2.0 ** -24
+    tiny_bwd = tiny if tiny_bwd is None else tiny_bwd
     sees = torch.ones(n, m, dtype=torch.bool)
     if causal:
         sees = sees.tril(m - n)
@@ -46,8 +48,8 @@ def head_fwd_bwd(q, k, v, do, scale, causal, unit, tiny):
     # delta is formed from the rounded o
     delta_err = (do.abs() * (o_err + depth * u32 * o.abs())).sum(-1, keepdim=True)
     # (a probability below the smallest normal of fp32 is 0: off by FLUSH, and ds by that times its other factor)
-    ds_err = p * (delta_err + dp_mag * depth * u32) + ds.abs() * (unit + 3 * rel) + (tiny + FLUSH * (dp - delta).abs()) * sees
-    pv_err = p * (unit + 3 * rel) + (tiny + FLUSH) * sees
+    ds_err = p * (delta_err + dp_mag * depth * u32) + ds.abs() * (unit + 3 * rel) + (tiny_bwd + FLUSH * (dp - delta).abs()) * sees
+    pv_err = p * (unit + 3 * rel) + (tiny_bwd + FLUSH) * sees
     # fp32 sums over up to n or m terms
     acc_n, acc_m = (n + 16) * u32, (m + 16) * u32
     dq, dk, dv = scale * ds @ k, scale * ds.T @ q, p.T @ do
@@ -58,7 +60,7 @@ def head_fwd_bwd(q, k, v, do, scale, causal, unit, tiny):
                            dk_err=dk_err, dv_err=dv_err)
 
 
-def packed_fwd_bwd(q, k, v, do, cu_q, cu_k, scale, causal, unit, tiny):
+def packed_fwd_bwd(q, k, v, do, cu_q, cu_k, scale, causal, unit, tiny, tiny_bwd=None):
     """The same of packed sequences: q, do [T, H, D], k, v [T_k, Hkv, D] on the CPU, offsets as
     lists; rows outside the sequences are zeros (lse -inf)."""
     T, H, D = q.shape
@@ -71,7 +73,7 @@ def packed_fwd_bwd(q, k, v, do, cu_q, cu_k, scale, causal, unit, tiny):
         a, b = slice(cu_q[i], cu_q[i + 1]), slice(cu_k[i], cu_k[i + 1])
         for h in range(H):
             g = h * kv // H
-            x = head_fwd_bwd(q[a, h], k[b, g], v[b, g], do[a, h], scale, causal, unit, tiny)
+            x = head_fwd_bwd(q[a, h], k[b, g], v[b, g], do[a, h], scale, causal, unit, tiny, tiny_bwd)
             for n in ("o", "lse", "dq"):
                 getattr(r, n)[a, h] = getattr(x, n)
                 err[n + "_err"][a, h] = getattr(x, n + "_err")

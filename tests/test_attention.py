@@ -212,6 +212,28 @@ def test_sharp_and_flat_scores(std, scale):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D,kv", [(64, 2), (128, 1), (256, 4)])
+@pytest.mark.parametrize("size", [2.0 ** -10, 2.0 ** 9])
+def test_gradients_of_fp16_over_its_range(size, D, kv):
+    """Small gradients: p and ds are held as multiples (2^-14 of the type's smallest steps).  Large ones, where
+    those multiples would pass its largest value (|do . v| over 2^13): as they come."""
+    from kernels.attention import forge_varlen_attention
+
+    lens = [300, 1, 77]
+    q, k, v, do = _make(lens, lens, 4, kv, D, FP16)
+    do = (do * size).half()
+    at = _offsets(lens)
+    unit, tiny = _unit(FP16)
+    ref = packed_fwd_bwd(q, k, v, do, at, at, D ** -0.5, True, unit, tiny, tiny * 2.0 ** -14 if size < 1 else tiny)
+    assert ref.dq.abs().max() < 60000
+    leaves = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    cu = torch.tensor(at, device="cuda", dtype=torch.int32)
+    grads = torch.autograd.grad(forge_varlen_attention(*leaves, cu, cu), leaves, do.cuda())
+    for n, x in zip(("dq", "dk", "dv"), grads):
+        _within(x, getattr(ref, n), getattr(ref, n + "_err"), n)
+
+
+@pytest.mark.gpu
 def test_tokens_of_a_head_beside_each_other():
     _check([90, 40], [90, 40], 4, 2, 64, BF16, layout="heads")
 
