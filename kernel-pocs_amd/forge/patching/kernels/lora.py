@@ -44,6 +44,9 @@ Fused paths:
     RoPE and the model's own norm and apply_rotary_pos_emb follow; with
     config["fuse_qk_norm"] both norms and RoPE are one pass instead
     (apply_qk_norm_rope, which rounds once where the modules round four times).
+    With config["attention"] = "forge" the attention itself is forge_attention, or
+    forge_varlen_attention for sequences packed into one row, on calls whose
+    attention is that (`attention_args`).
 """
 from __future__ import annotations
 
@@ -361,6 +364,62 @@ def _attention_interface(module, modeling, kwargs):
     return modeling.ALL_ATTENTION_FUNCTIONS[impl]
 
 
+# keyword arguments of a call that change nothing of its attention
+_NEUTRAL = {"position_ids", "position_embeddings", "cache_position", "use_cache", "return_dict", "output_hidden_states",
+            "num_items_in_batch", "logits_to_keep", "max_length_q", "max_length_k", "cu_seq_lens_q", "cu_seq_lens_k"}
+
+
+def attention_args(module, query, key, value, attention_mask, kwargs):
+    """(causal, offsets of the packed queries, of their keys, or None and None) when
+    forge_attention or forge_varlen_attention is the attention that this call asks
+    for, else None.  Taken: fp16 and bf16 GPU tensors without a mask, dropout, soft
+    cap or weights to return, and without a window that hides a key; one token
+    against its cache, or as many queries as keys.  As in the model's own
+    implementations "eager" without a mask sees every key and the others are causal
+    where module.is_causal says so; cu_seq_lens_q and cu_seq_lens_k (the "flash_attention"
+    implementations' arguments) give sequences packed into one row, and such an
+    implementation may find them in position_ids instead, so then it runs itself.
+    Implementations of other names run themselves."""
+    if attention_mask is not None or not query.is_cuda or any(_is_dtensor(t) for t in (query, key, value)):
+        return None
+    if query.dtype not in (torch.float16, torch.bfloat16) or key.dtype != query.dtype or value.dtype != query.dtype:
+        return None
+    D, queries, keys = query.shape[-1], query.shape[2], key.shape[2]
+    if D < 8 or D % 8 or D > 256 or key.shape != value.shape or key.shape[-1] != D or query.shape[1] % key.shape[1]:
+        return None
+    if module.training and float(getattr(module, "attention_dropout", 0.0)) != 0.0 or not module.scaling > 0.0:
+        return None
+    if getattr(module, "attn_logit_softcapping", None) is not None:
+        return None
+    if any(v is not None and v is not False and n not in _NEUTRAL for n, v in kwargs.items()):
+        return None
+    window = _sliding_window(module)
+    if window is not None and window < keys:
+        return None
+    impl = module.config._attn_implementation or "eager"
+    flash = impl.startswith("flash_attention")
+    if not flash and impl not in ("eager", "sdpa"):
+        return None
+    causal = impl != "eager" and bool(getattr(module, "is_causal", True))
+    at_q, at_k = kwargs.get("cu_seq_lens_q"), kwargs.get("cu_seq_lens_k")
+    if at_q is not None or at_k is not None:
+        if at_q is None or at_k is None or query.shape[0] != 1 or not flash:
+            return None
+        return causal, at_q, at_k
+    if flash and kwargs.get("position_ids") is not None or queries not in (1, keys):
+        return None
+    return causal and queries > 1, None, None
+
+
+def _forge_attention(query, key, value, scale, causal, at_q, at_k):
+    from forge.kernels.attention import forge_attention, forge_varlen_attention
+
+    if at_q is None:
+        return forge_attention(query, key, value, causal=causal, scale=scale).transpose(1, 2)
+    q, k, v = (t[0].transpose(0, 1) for t in (query, key, value))
+    return forge_varlen_attention(q, k, v, at_q, at_k, causal=causal, scale=scale).unsqueeze(0)
+
+
 def _probe_norm(norm, eps) -> Optional[float]:
     """The offset o with which the class's forward, run on a CPU copy with
     weights and inputs of this function's own, is x / sqrt(mean x^2 + eps) *
@@ -534,7 +593,10 @@ def make_lora_qkv_forward(module, config):
     cache_position, **kwargs), KV-cache update, sliding window, attention
     interface selection, Gemma2's softcap, o_proj through its submodule.
     config["fuse_qk_norm"] (default False): q/k norms and RoPE in one pass where
-    `qk_norm_args` allows."""
+    `qk_norm_args` allows.  config["attention"] (default None: the model's
+    implementation): "forge", forge_attention where `attention_args` allows."""
+    if config.get("attention") not in (None, "forge"):
+        raise ValueError(f"forge.patch: attention must be None or 'forge', got {config['attention']!r}")
     for proj in (module.q_proj, module.k_proj, module.v_proj):
         _check_lora_active(proj)
     modeling = importlib.import_module(module.__class__.__module__)
@@ -548,6 +610,10 @@ def make_lora_qkv_forward(module, config):
         if kv_cache is not None:
             key, value = kv_cache.update(key, value, module.layer_idx,
                                          {"sin": sin, "cos": cos, "cache_position": cache_position})
+        taken = attention_args(module, query, key, value, attention_mask, kwargs) if config.get("attention") else None
+        if taken is not None:
+            attn_output = _forge_attention(query, key, value, float(module.scaling), *taken)
+            return module.o_proj(attn_output.reshape(*input_shape, -1)), None
         extra = {}
         softcap = getattr(module, "attn_logit_softcapping", None)
         if softcap is not None:
@@ -562,5 +628,5 @@ def make_lora_qkv_forward(module, config):
     return forward
 
 
-__all__ = ["LiveLoRA", "has_hooks", "live_lora", "make_lora_mlp_forward", "make_lora_qkv_forward", "mlp_fused_args",
-           "norm_offset", "qk_norm_args", "qkv_fused_args", "rope_tables", "rotates_halves"]
+__all__ = ["LiveLoRA", "attention_args", "has_hooks", "live_lora", "make_lora_mlp_forward", "make_lora_qkv_forward",
+           "mlp_fused_args", "norm_offset", "qk_norm_args", "qkv_fused_args", "rope_tables", "rotates_halves"]

@@ -299,3 +299,42 @@ def test_offsets_are_checked_when_asked():
         forge_varlen_attention(q, q, q, torch.tensor([0, 5], device="cuda"), torch.tensor([0, 2, 5], device="cuda"))
     with pytest.raises(ValueError, match="cu_seqlens_k"):
         forge_varlen_attention(q, q[:3], q[:3], torch.tensor([0, 5], device="cuda"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("train", [False, True])
+def test_many_sequences(train):
+    """More than a workgroup looks at in one step (256), of 0 to 3 tokens, one long among them."""
+    lens = [i % 4 for i in range(600)]
+    lens[300] = 200
+    _check(lens, lens, 2, 1, 64, BF16, train=train)
+
+
+@pytest.mark.gpu
+def test_more_tiles_than_one_level_holds():
+    _check([700, 1, 300], [700, 1, 300], 3, 1, 64, BF16)
+    _check([1, 1500], [1, 1500], 1, 1, 8, FP16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("queries", [1, 300])
+def test_offsets_past_32_bits(queries):
+    """A cache whose last sequence begins 2^31 elements from its first: the same bits as from a small one."""
+    from kernels.attention import forge_varlen_attention
+
+    row = 4096  # elements from token to token: a layer's slice of a wider cache
+    tokens = (1 << 31) // row + 700
+    cache = torch.empty(tokens, row, device="cuda", dtype=BF16)
+    g = torch.Generator().manual_seed(0)
+    k, v = (torch.randn(500, 2, 64, generator=g).to(BF16).cuda() for _ in range(2))
+    q = torch.randn(queries, 4, 64, generator=g).to(BF16).cuda()
+    kc, vc = (cache[:, i * 128:(i + 1) * 128].view(tokens, 2, 64) for i in (0, 1))
+    at = tokens - 600
+    kc[at:at + 500], vc[at:at + 500] = k, v
+    cu_q = torch.tensor([0, 0, queries], device="cuda", dtype=torch.int32)
+    far = forge_varlen_attention(q, kc, vc, cu_q, torch.tensor([0, at, at + 500], device="cuda", dtype=torch.int32))
+    near = forge_varlen_attention(q, k, v, cu_q, torch.tensor([0, 0, 500], device="cuda", dtype=torch.int32))
+    if queries > 1:
+        assert torch.equal(far, near)
+    else:  # (a token's keys are cut by the number of all the cache's keys: other sums)
+        assert (far.float() - near.float()).abs().max() <= 2.0 ** -7 * v.float().abs().max()
