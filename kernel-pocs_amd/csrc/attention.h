@@ -16,6 +16,8 @@
 // predecessor, so wrong ones give wrong results, never an access outside it.
 #pragma once
 
+#include <type_traits>
+
 #include "gemm_core.h"
 
 namespace fattn {
@@ -285,6 +287,84 @@ struct ColFrag {
     return tr_frag(p, p + 8 / L::UNIT * L::UB);
   }
 };
+
+// Keys that a query does not see have p = 0, but 0 times an infinity or NaN is NaN,
+// and a product takes 16 keys at once.  Kernels run as if there were none; where
+// a causal sum comes out as NaN they run again with such values apart: added to the
+// sums of the queries that see them, and zeros in the tile.  (Seldom runs: few
+// registers, not speed.  No value of a finite tile passes through any of this.)
+template <class T, int DP>
+struct Special {
+  typedef Tile<DP> L;
+  static constexpr uint32_t EX = std::is_same_v<T, fp16_t> ? 0x7c00 : 0x7f80;
+  static __device__ __forceinline__ char* row_at(char* tile, int row) { return tile + row / L::UNIT * L::UB + row % L::UNIT * L::RB; }
+  static __device__ __forceinline__ bool is(uint32_t half) { return (half & EX) == EX; }
+
+  static __device__ __forceinline__ bool in_row(char* tile, int row) {
+    bool any = false;
+    for (int w = threadIdx.x % 64; w < DP / 2; w += 64) {
+      const uint32_t x = reinterpret_cast<const uint32_t*>(row_at(tile, row))[w];
+      any |= is(x) || is(x >> 16);
+    }
+    return __any(any);
+  }
+  // those of rows r0 .. r0 + n - 1, the keys from key0, of the keys before `sees`; as
+  // they are (times a p above 0) or as NaN
+  static __device__ __forceinline__ void add(f32x16 (&sums)[DP / 32], char* tile, int r0, int n, int key0, int sees, bool as_nan) {
+    const int h = threadIdx.x % 64 / 32;
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
+      const int row = r0 + j;
+      if (!in_row(tile, row)) continue;
+      const char* p = row_at(tile, row);
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          if (r % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+          const int d = 32 * db + 8 * (r / 4) + 4 * h + r % 4;
+          const uint16_t x = *reinterpret_cast<const uint16_t*>(p + ((d / 8 ^ L::f(row)) << 4) + d % 8 * 2);
+          const float v = as_nan ? __builtin_nanf("") : to_f32(__builtin_bit_cast(T, x));
+          sums[db][r] += is(x) && key0 + j < sees ? v : 0.f;
+        }
+    }
+  }
+  // zeros in their places, by waves `wave` of `waves`
+  static __device__ __forceinline__ void clear(char* tile, int r0, int n, int wave, int waves) {
+#pragma unroll 1
+    for (int row = r0 + wave; row < r0 + n; row += waves)
+      for (int w = threadIdx.x % 64; w < DP / 2; w += 64) {
+        uint32_t* p = reinterpret_cast<uint32_t*>(row_at(tile, row)) + w;
+        const uint32_t x = *p;
+        if (is(x) || is(x >> 16)) *p = (is(x) ? 0 : x & 0xffff) | (is(x >> 16) ? 0 : x & 0xffff0000u);
+      }
+  }
+};
+
+template <int N>
+__device__ __forceinline__ bool any_nan(const f32x16 (&sums)[N]) {
+  float t = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) t = __builtin_fmaf(sums[i][r], 0.f, t);
+  return t != t;
+}
+
+// Whether any of the workgroup's 4 waves has it; through 16 bytes of LDS that no wave
+// reads any more after the first barrier.  (__syncthreads_or has an array of its own,
+// beside which the compiler no longer tells the tiles that are read from those
+// under way: it waited for the LDS-DMA before each tile's first read, 396 -> 430 us
+// for 329 GFLOP.)
+__device__ __forceinline__ bool any_of_4_waves(char* lds, int wave, bool has) {
+  const bool mine = __any(has);
+  __syncthreads();
+  if (threadIdx.x % 64 == 0) reinterpret_cast<int*>(lds)[wave] = mine;
+  __syncthreads();
+  const int4 v = *reinterpret_cast<const int4*>(lds);
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(v.x | v.y | v.z | v.w) != 0;
+}
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 

@@ -13,8 +13,6 @@
 // As in the forward, products are laid out so that p and ds stay in the
 // registers that they are computed in: keys x queries for dq, queries x keys for
 // dk and dv.
-#include <type_traits>
-
 #include "attention.h"
 
 namespace fattn {
@@ -113,7 +111,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dq_kernel(Args a,
   const int64_t row = a.cu_q ? sq.start + iq : sq.batch * a.tq + iq;
   const float c = a.scale * LOG2E;
   const float below = live ? shift_of[head * n_rows + row] * c + P_BITS<T> : -__builtin_inff();
-  float unit = 1.f;
+  float unit;
   const float delta = live ? a.delta[head * n_rows + row] : 0.f;
 
   Dma kd, vd;
@@ -131,24 +129,20 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dq_kernel(Args a,
   fr.setup(lane);
   fc.setup(lane);
   f32x16 acc[DB];
-#pragma unroll
-  for (int db = 0; db < DB; ++db)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[db][r] = 0.f;
   const int sees = a.causal ? min(sk.len, iq + shift + 1) : sk.len;
   const int all_see = a.causal ? min(sk.len, wq + shift + 1) : sk.len;
   const int any_sees = a.causal ? min(sk.len, min(wq + 32, sq.len) + shift) : (wq < sq.len ? sk.len : 0);
 
-  auto step = [&](int t, int slot) __attribute__((always_inline)) {
+  auto step = [&](int t, int slot, auto apart) __attribute__((always_inline)) {
     wait_dma<0>();
     barrier();
     if (NST == 2 && t + 1 < n_t) issue(t + 1, 1 - slot);
-    const char* kt = smem + slot * 2 * Dma::BYTES;
+    char* kt = smem + slot * 2 * Dma::BYTES;
     const char* vt = kt + Dma::BYTES;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       const int k0 = t * BN + 32 * kb;
-      if (k0 >= any_sees) continue;
+      if (!apart && k0 >= any_sees) continue;
       f32x16 s, dp;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
@@ -164,6 +158,13 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dq_kernel(Args a,
           if (k0 + 8 * (r / 4) + 4 * h + r % 4 >= sees) s[r] = 0.f;
       }
       keep_in_range<T>(s, unit, acc);
+      if constexpr (apart) {  // (the sign of ds is not known: NaN)
+        __syncthreads();        // every wave has its scores of these keys
+        Special<T, DP>::add(acc, kt, 32 * kb, 32, k0, sees, true);
+        __syncthreads();
+        Special<T, DP>::clear(kt, 32 * kb, 32, wave, 4);
+        __syncthreads();
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const bf16x8 ds = pack_acc<T>(s, i);
@@ -177,11 +178,20 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dq_kernel(Args a,
       issue(t + 1, 0);
     }
   };
-  if (n_t > 0) issue(0, 0);
-  for (int t = 0; t < n_t; t += NST) {
-    step(t, 0);
-    if (NST == 2 && t + 1 < n_t) step(t + 1, 1);
-  }
+  auto run = [&](auto apart) __attribute__((always_inline)) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[db][r] = 0.f;
+    unit = 1.f;
+    if (n_t > 0) issue(0, 0);
+    for (int t = 0; t < n_t; t += NST) {
+      step(t, 0, apart);
+      if (NST == 2 && t + 1 < n_t) step(t + 1, 1, apart);
+    }
+  };
+  run(std::false_type());
+  if (a.causal && any_of_4_waves(smem, wave, any_nan(acc))) run(std::true_type());
   if (!live) return;
   const float back = a.scale * exp2f(-P_BITS<T>) / unit;
   T* op = row_ptr<T>(a.dq, sq.batch, sq.start + iq, head);
@@ -203,8 +213,12 @@ template <class T, int DP, bool DK, bool DV>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a, const float* shift_of, int64_t n_rows, int tiles) {
   constexpr int BN = 128, BQ = DP == 256 ? 32 : 64, KS = DP / 16, DB = DP / 32;
   using Dma = TileDma<DP, BQ, 4>;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * 2 * Dma::BYTES];
-  __shared__ __attribute__((aligned(256))) float stat[2][2][64];
+  // One array: beside a second one the compiler waits for all LDS-DMA before it
+  // reads.  -lse / scale and -delta of two slots come first, the tiles TILES behind
+  // them, which is part of the fragments' bases: their immediates reach 64 KB.
+  constexpr int TILES = 1024;
+  __shared__ __attribute__((aligned(1024))) char smem[TILES + 2 * 2 * Dma::BYTES];
+  auto stat = [&](int slot, int i) __attribute__((always_inline)) { return reinterpret_cast<float*>(smem) + (slot * 2 + i) * 64; };
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int G = a.H / a.Hkv, h = lane / 32;
   const Item it = item_of(blockIdx.x, tiles, a.Hkv, 1);
@@ -243,14 +257,14 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
   int next_i = first, next_head = it.kv * G;  // of the tile that is issued next
   auto issue = [&](int slot) {
     const int left = sq.len - next_i;
-    char* st = smem + slot * 2 * Dma::BYTES;
+    char* st = smem + TILES + slot * 2 * Dma::BYTES;
     qd.load(row_ptr<T>(a.q, sq.batch, sq.start + next_i, next_head), left, st, wave);
     dd.load(row_ptr<T>(a.dout, sq.batch, sq.start + next_i, next_head), left, st + Dma::BYTES, wave);
     // (rows that do not exist: q = dout = 0, so p = exp2(0) and ds = 0 add zeros)
     const int64_t row = (a.cu_q ? sq.start : sq.batch * a.tq) + next_i;
     if (wave < 2) {
       const __amdgpu_buffer_rsrc_t r = make_rsrc((wave ? a.delta : shift_of) + next_head * n_rows + row);
-      dma4(r, &stat[slot][wave][0], lane < left && lane < BQ ? lane * 4 : OOB);
+      dma4(r, stat(slot, wave), lane < left && lane < BQ ? lane * 4 : OOB);
     }
     next_i += BQ;
     if (next_i >= sq.len) {
@@ -262,6 +276,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
   ColFrag<DP> fc;
   fr.setup(lane);
   fc.setup(lane);
+  for (int& x : fr.base) asm("" : "+v"(x += TILES));
+  for (int& x : fc.base) asm("" : "+v"(x += TILES));
   f32x16 dk[DB], dv[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db)
@@ -288,8 +304,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
       f32x16 s, dp;  // begin with -lse / scale and -delta of their queries
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(&stat[slot][0][32 * qb + 8 * i + 4 * h]);
-        const f32x4 y = *reinterpret_cast<const f32x4*>(&stat[slot][1][32 * qb + 8 * i + 4 * h]);
+        const f32x4 x = *reinterpret_cast<const f32x4*>(stat(slot, 0) + 32 * qb + 8 * i + 4 * h);
+        const f32x4 y = *reinterpret_cast<const f32x4*>(stat(slot, 1) + 32 * qb + 8 * i + 4 * h);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           s[4 * i + j] = x[j];
@@ -304,7 +320,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
       if (a.causal && i0 + shift < wk + 31) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (i0 + 8 * (r / 4) + 4 * h + r % 4 + shift < jk) s[r] = -__builtin_inff();
+          if (i0 + 8 * (r / 4) + 4 * h + r % 4 + shift < jk) {
+            s[r] = -__builtin_inff();
+            dp[r] = 0.f;
+          }
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {

@@ -69,12 +69,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a
   fc.setup(lane);
 
   f32x16 o[DB];
-#pragma unroll
-  for (int db = 0; db < DB; ++db)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
   const float c = a.scale * LOG2E;
-  float m = -__FLT_MAX__, l = 0.f;  // m: in units of log2; l: this half's sum
+  float m, l;  // m: in units of log2; l: this half's sum
 
   // keys that this lane's query sees, and those that every query of the wave does
   const int sees = a.causal ? min(sk.len, iq + shift + 1) : sk.len;
@@ -82,14 +78,14 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a
   const int any_sees = a.causal ? min(sk.len, min(wq + 32, sq.len) + shift) : (wq < sq.len ? sk.len : 0);
 
   // (slot: a constant where the call is, so that it is part of the reads' immediates)
-  auto step = [&](int t, int slot) __attribute__((always_inline)) {
+  auto step = [&](int t, int slot, auto apart) __attribute__((always_inline)) {
     wait_dma<0>();
     barrier();
     if (t + 1 < n_t) issue(t + 1, 1 - slot);
     const int k0 = t * BN;
-    if (k0 >= any_sees) return;
+    if (!apart && k0 >= any_sees) return;
     const char* kt = smem + slot * 2 * Dma::BYTES;
-    const char* vt = kt + Dma::BYTES;
+    char* vt = smem + slot * 2 * Dma::BYTES + Dma::BYTES;
     f32x16 s[2];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
@@ -131,6 +127,12 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a
         l += p;
         s[kb][r] = p;
       }
+    if constexpr (apart) {
+      Special<T, DP>::add(o, vt, 0, BN, k0, sees, false);
+      __syncthreads();
+      Special<T, DP>::clear(vt, 0, BN, wave, 4);
+      __syncthreads();
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const bf16x8 p = pack_acc<T>(s[i / 2], i % 2);
@@ -138,11 +140,21 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a
       for (int db = 0; db < DB; ++db) o[db] = mfma32<T>(fc.read(vt, 16 * i, db), p, o[db]);
     }
   };
-  if (n_t > 0) issue(0, 0);
-  for (int t = 0; t < n_t; t += 2) {
-    step(t, 0);
-    if (t + 1 < n_t) step(t + 1, 1);
-  }
+  auto run = [&](auto apart) __attribute__((always_inline)) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
+    m = -__FLT_MAX__;
+    l = 0.f;
+    if (n_t > 0) issue(0, 0);
+    for (int t = 0; t < n_t; t += 2) {
+      step(t, 0, apart);
+      if (t + 1 < n_t) step(t + 1, 1, apart);
+    }
+  };
+  run(std::false_type());
+  if (a.causal && any_of_4_waves(smem, wave, any_nan(o))) run(std::true_type());
   l += other_half(l);
   if (!live) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;  // (a row without keys)

@@ -27,8 +27,10 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_rows_kernel(Args a, Parts par
   constexpr int KS = DP / 16, DB = DP / 32, PITCH = DP + 4;
   using Dma = TileDma<DP, 32, 1>;
   constexpr int RING = NW * 2 * 2 * Dma::BYTES, SUMS = NW * 32 * PITCH * 4;
-  __shared__ __attribute__((aligned(1024))) char smem[RING > SUMS ? RING : SUMS];
-  __shared__ float stat[2][NW][32];
+  // (one array: beside a second one the compiler waits for all LDS-DMA before it reads)
+  constexpr int STAT = RING > SUMS ? RING : SUMS;
+  __shared__ __attribute__((aligned(1024))) char smem[STAT + 2 * NW * 32 * 4];
+  float* const stat = reinterpret_cast<float*>(smem + STAT);  // [2][NW][32]: maxima and sums
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), h = lane / 32;
   const int G = a.H / a.Hkv, kv = blockIdx.y;
   const TileAt at = find_tile(a.cu_k, a.B, a.tk, parts.C, blockIdx.x, 1);
@@ -77,50 +79,66 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_rows_kernel(Args a, Parts par
       qf[ks] = __builtin_bit_cast(bf16x8, v);
     }
     f32x16 o[DB];
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
-    float m = -__FLT_MAX__, l = 0.f;
+    float m, l;
     const int sees = a.causal ? min(sk.len, token + shift + 1) : sk.len;
-    for (int i = 0; i < mine; ++i) {
-      if (i + 1 < mine) wait_dma<2 * Dma::N>();
-      else wait_dma<0>();
-      const int k0 = lo + 32 * (wave + i * NW);
-      const char* kt = ring + (i % 2) * 2 * Dma::BYTES;
-      const char* vt = kt + Dma::BYTES;
-      f32x16 s;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s = mfma32<T>(fr.read(kt, 0, ks), qf[ks], s);
-      float top = -__builtin_inff();
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        if (k0 + 8 * (r / 4) + 4 * h + r % 4 >= sees) s[r] = -__builtin_inff();
-        top = fmaxf(top, s[r]);
-      }
-      top = fmaxf(top, other_half(top)) * c;
-      const float up = fmaxf(top, m), f = exp2_hw(m - up);
-      m = up;
-      l *= f;
+    auto run = [&](auto apart) __attribute__((always_inline)) {
 #pragma unroll
       for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[db][r] *= f;
+        for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
+      m = -__FLT_MAX__;
+      l = 0.f;
+      for (int i = 0; i < mine; ++i) {
+        if (i + 1 < mine) wait_dma<2 * Dma::N>();
+        else wait_dma<0>();
+        const int k0 = lo + 32 * (wave + i * NW);
+        const char* kt = ring + (i % 2) * 2 * Dma::BYTES;
+        char* vt = ring + (i % 2) * 2 * Dma::BYTES + Dma::BYTES;
+        f32x16 s;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[r] = exp2_hw(__builtin_fmaf(s[r], c, -m));
-        l += s[r];
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) s = mfma32<T>(fr.read(kt, 0, ks), qf[ks], s);
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          if (k0 + 8 * (r / 4) + 4 * h + r % 4 >= sees) s[r] = -__builtin_inff();
+          top = fmaxf(top, s[r]);
+        }
+        top = fmaxf(top, other_half(top)) * c;
+        const float up = fmaxf(top, m), f = exp2_hw(m - up);
+        m = up;
+        l *= f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[db][r] *= f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[r] = exp2_hw(__builtin_fmaf(s[r], c, -m));
+          l += s[r];
+        }
+        if constexpr (apart) {  // (the wave's own ring; its LDS accesses keep their order)
+          Special<T, DP>::add(o, vt, 0, 32, k0, sees, false);
+          Special<T, DP>::clear(vt, 0, 32, 0, 1);
+          wait_dma<0>();
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const bf16x8 p = pack_acc<T>(s, j);
+#pragma unroll
+          for (int db = 0; db < DB; ++db) o[db] = mfma32<T>(fc.read(vt, 16 * j, db), p, o[db]);
+        }
+        wait_dma<2 * Dma::N>();  // (the reads of this slot are done; the other slot's DMA may be under way)
+        if (i + 2 < mine) issue(i + 2);
       }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const bf16x8 p = pack_acc<T>(s, j);
-#pragma unroll
-        for (int db = 0; db < DB; ++db) o[db] = mfma32<T>(fc.read(vt, 16 * j, db), p, o[db]);
-      }
-      wait_dma<2 * Dma::N>();  // (the reads of this slot are done; the other slot's DMA may be under way)
-      if (i + 2 < mine) issue(i + 2);
+    };
+    run(std::false_type());
+    if (a.causal && sq.len > 1 && mine > 0 && __any(any_nan(o))) {  // (a token alone sees every key)
+      wait_dma<0>();  // the reads of the ring are done
+      issue(0);
+      if (mine > 1) issue(1);
+      run(std::true_type());
     }
     l += other_half(l);
     wait_dma<0>();
@@ -133,21 +151,21 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_rows_kernel(Args a, Parts par
         *reinterpret_cast<f32x4*>(sums + 32 * db + 8 * i + 4 * h) =
             f32x4{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]};
     if (h == 0) {
-      stat[0][wave][lane] = m;
-      stat[1][wave][lane] = l;
+      stat[wave * 32 + lane] = m;
+      stat[(NW + wave) * 32 + lane] = l;
     }
     __syncthreads();
     const int rows = min(32, n_rows - r0), vecs = a.D / 4;
     for (int x = threadIdx.x; x < rows * vecs; x += NW * 64) {
       const int r = x / vecs, d = x % vecs * 4, t = (r0 + r) / G, hd = kv * G + (r0 + r) % G;
-      float top = stat[0][0][r];
+      float top = stat[r];
 #pragma unroll
-      for (int w = 1; w < NW; ++w) top = fmaxf(top, stat[0][w][r]);
+      for (int w = 1; w < NW; ++w) top = fmaxf(top, stat[w * 32 + r]);
       float total = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        const float f = exp2_hw(stat[0][w][r] - top);
-        total += stat[1][w][r] * f;
+        const float f = exp2_hw(stat[w * 32 + r] - top);
+        total += stat[(NW + w) * 32 + r] * f;
         const f32x4 y = *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(smem) + (w * 32 + r) * PITCH + d);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] += y[j] * f;

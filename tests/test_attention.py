@@ -338,3 +338,53 @@ def test_offsets_past_32_bits(queries):
         assert torch.equal(far, near)
     else:  # (a token's keys are cut by the number of all the cache's keys: other sums)
         assert (far.float() - near.float()).abs().max() <= 2.0 ** -7 * v.float().abs().max()
+
+
+def _special(t, rows, values):
+    """t with values at some columns of the rows."""
+    t = t.clone()
+    for n, row in enumerate(rows):
+        for j, x in enumerate(values):
+            t[row, n % t.shape[1], (11 * j + 5 * n) % t.shape[2]] = x
+    return t
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("H,kv,D", [(2, 1, 64), (4, 2, 128), (2, 2, 256), (3, 1, 40)])
+@pytest.mark.parametrize("lens_q,lens_k", [([200, 90], [200, 90]), ([3, 7], [330, 40]), ([100], [300])])
+@pytest.mark.parametrize("train", [False, True])
+def test_values_that_are_not_finite_where_they_are_not_seen(lens_q, lens_k, H, kv, D, dtype, train):
+    """NaN and infinities in keys and values: the queries that do not see them are as they are without."""
+    from kernels.attention import forge_varlen_attention
+
+    q, k, v, do = _make(lens_q, lens_k, H, kv, D, dtype)
+    at_q, at_k = _offsets(lens_q), _offsets(lens_k)
+    # of the first sequence: from its key `first` on, next to the last queries' borders
+    first = lens_k[0] - lens_q[0] + lens_q[0] // 2
+    rows = list(range(first, lens_k[0], 2))
+    inf, nan = float("inf"), float("nan")
+    cu_q, cu_k = (torch.tensor(x, device="cuda", dtype=torch.int32) for x in (at_q, at_k))
+
+    def run(k, v):
+        leaves = [t.cuda().requires_grad_(train) for t in (q, k, v)]
+        out, lse = forge_varlen_attention(*leaves, cu_q, cu_k, return_lse=True)
+        return [out.detach(), lse.detach(), *(torch.autograd.grad(out, leaves, do.cuda())[:1] if train else ())]
+
+    plain = run(k, v)
+    clean = [i for i in range(at_q[-1]) if not lens_q[0] // 2 <= i < lens_q[0]]
+    for bad_k, bad_v in ((k, _special(v, rows, [nan, inf, -inf])), (_special(k, rows, [nan]), _special(v, rows, [nan])),
+                         (_special(k, rows, [inf, -inf]), v)):
+        for a, b in zip(run(bad_k, bad_v), plain):
+            assert torch.equal(a[clean], b[clean])
+    # where they are seen: infinities of a value in the columns that have them, with their sign
+    out = run(k, _special(v, rows[:1], [inf, -inf]))[0].double().cpu()
+    seen = slice(lens_q[0] // 2, lens_q[0])
+    want = [head_fwd_bwd(q[:at_q[1], h], k[:at_k[1], h * kv // H], _special(v, rows[:1], [inf, -inf])[:at_k[1], h * kv // H],
+                         do[:at_q[1], h], D ** -0.5, True, *_unit(dtype)).o for h in range(H)]
+    for h in range(H):
+        for x in (inf, -inf):
+            hit = want[h][seen] == x
+            assert torch.equal(out[seen, h] == x, hit) and (h * kv // H > 0 or hit.any())
+    # and a NaN of a key makes all of a query that sees it NaN
+    assert run(_special(k, rows[:1], [nan]), v)[0][seen][:, :H // kv].isnan().all()
