@@ -7,10 +7,13 @@
 // The integers do not depend on rstd, and both sums of a row are taken in one
 // pass.  Rows as they are (no norm): t = x, or x times a scale a column.
 //
-// The integers are those of exact arithmetic.  t of two 16-bit factors is exact in
-// fp32; otherwise the largest is found in 64 bits.  127 t / a errs by less than
-// 6e-5 in fp32, so only values that close to a border between two integers are
-// divided again, in 64 bits (one vector of 8 in 130).
+// The integers are those of exact arithmetic.  127 / a lies between two neighbours
+// below and above its value in fp32, t times each is rounded to an integer once (an fma
+// with 1.5 2^23, whose last byte it is), and as rounding keeps the order the
+// integer is that of t's exact quotient where both agree.  They differ where a border
+// between two integers lies within some 2^-23 of the quotient: those vectors are
+// divided again, in 64 bits.  t of two 16-bit factors is exact in fp32; otherwise the
+// largest is found in 64 bits and the two are 6 steps off, for the roundings of t.
 //
 // Bound by HBM: x and the residual are read once, h and y written once.
 #include "add_rmsnorm.h"
@@ -34,47 +37,43 @@ struct FwdArgs {
 // not), the row itself in 8 bits, or times a scale a column.
 enum Mode { NORM, NORM8, NORM8_WIDE, ROWS8, ROWS8_SCALED };
 
-// The integers of V values of a row with factors w, as bytes.  inv = 127 / a.
+// The integers of V values of a row with factors w, as bytes; below and above: of 127 / a.
 template <class T, bool UNIT>
-__device__ __forceinline__ void quantize(const Vec<T>& v, const float* w, double offset, float inv, double a, bool tiny,
-                                         uint32_t (&word)[V<T> / 4]) {
-  int k[V<T>];
-  bool near = tiny;
+__device__ __forceinline__ void quantize(const Vec<T>& v, const float* w, double offset, float below, float above, double a,
+                                         bool tiny, uint32_t (&word)[V<T> / 4]) {
+  uint32_t k[V<T>], differ = tiny;
 #pragma unroll
   for (int i = 0; i < V<T>; ++i) {
-    const float t = (UNIT ? v.get(i) : v.get(i) * (w[i] + (float)offset)) * inv, r = rintf(t);
-    near = near || fabsf(t - r) > 0.5f - 6e-5f;
-    k[i] = (int)r;
+    const float t = UNIT ? v.get(i) : v.get(i) * (w[i] + (float)offset);
+    k[i] = __float_as_uint(__builtin_fmaf(t, below, 0x1.8p23f));
+    differ |= k[i] ^ __float_as_uint(__builtin_fmaf(t, above, 0x1.8p23f));
   }
-  if (near) {  // (6e-5: 127 times 8 roundings of 2^-24)
+  if (differ) {
 #pragma unroll
     for (int i = 0; i < V<T>; ++i) {
       const double t = UNIT ? (double)v.get(i) : (double)v.get(i) * ((double)w[i] + offset);
-      k[i] = (int)rint(127.0 * t / a);
+      k[i] = (uint32_t)(int)rint(127.0 * t / a);
     }
   }
 #pragma unroll
-  for (int i = 0; i < V<T>; ++i) {
-    const uint32_t byte = (uint32_t)(k[i] & 255) << (8 * (i % 4));
-    word[i / 4] = i % 4 ? word[i / 4] | byte : byte;
-  }
+  for (int i = 0; i < V<T>; i += 4)
+    word[i / 4] = __builtin_amdgcn_perm(k[i + 1], k[i], 0x0c0c0400) | __builtin_amdgcn_perm(k[i + 3], k[i + 2], 0x04000c0c);
 }
 
-template <class T, int TPR, int NV, int MODE>
-__global__ __launch_bounds__(256) void add_rmsnorm_kernel(FwdArgs a) {
+template <class T, int TPR, int NV, int MODE, bool RES>
+__global__ __launch_bounds__(threads_of<TPR>) void add_rmsnorm_kernel(FwdArgs a) {
   constexpr int VN = V<T>, RPB = rows_per_block<TPR>, N = NV ? NV : 1;
   constexpr bool SUMS = MODE == NORM || MODE == NORM8 || MODE == NORM8_WIDE, EIGHT = MODE != NORM;
   constexpr bool WIDE = MODE == NORM8_WIDE || MODE == ROWS8_SCALED, UNIT = MODE == ROWS8;
-  // a thread's weights are held, or read again for every row where they are too many
-  constexpr bool HELD = !UNIT && NV > 0 && NV <= 4, RELOAD = !UNIT && NV > 4;
-  constexpr bool AHEAD = NV > 0 && NV <= 4;  // the next row's loads are in flight while a row is worked on
-  __shared__ float sums[2][4];
-  __shared__ uint32_t tops[2][4];
-  __shared__ double tops64[2][4];
+  constexpr bool HELD = !UNIT && NV > 0;  // a thread's weights
+  constexpr int WAVES = threads_of<TPR> / 64;
+  __shared__ float sums[2][WAVES];
+  __shared__ uint32_t tops[2][WAVES];
+  __shared__ double tops64[2][WAVES];
   const int tid = threadIdx.x % TPR, slot = threadIdx.x / TPR;
   const int n_vec = (int)((a.H + VN - 1) / VN);
   const T* xp = (const T*)a.x;
-  const T* rp = SUMS ? (const T*)a.res : nullptr;
+  const T* rp = (const T*)a.res;
   // the factors of t: weight + offset, of which WIDE adds the offset in 64 bits
   const float add = WIDE ? 0.f : a.offset;
   const double add64 = WIDE ? (double)a.offset : 0.0;
@@ -93,15 +92,12 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(FwdArgs a) {
   }
   Vec<T> x[2][N], r[2][N];
   auto fetch = [&](int64_t row, int set) {
-    if constexpr (NV > 0) {
+    row = min(row, a.rows - 1);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int vec = tid + j * TPR, c = vec * VN, n = (int)min((int64_t)VN, a.H - c);
-        if (vec < n_vec && row < a.rows) {
-          x[set][j] = load_part(xp + row * a.ldx + c, n);
-          if (SUMS && rp) r[set][j] = load_part(rp + row * a.ldr + c, n);
-        }
-      }
+    for (int j = 0; j < NV; ++j) {
+      const int c = (tid + j * TPR) * VN;
+      x[set][j] = load_held(xp + row * a.ldx, c, a.H);
+      if constexpr (RES) r[set][j] = load_held(rp + row * a.ldr, c, a.H);
     }
   };
   auto sum = [&](const Vec<T>& u, const Vec<T>& v) {
@@ -118,6 +114,14 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(FwdArgs a) {
     uint32_t top = 0;
     double top64 = 0.0;
     auto see = [&](const Vec<T>& v, const float* wv) {
+      if constexpr (UNIT && sizeof(T) == 2) {  // magnitudes of two values at once
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top),
+                                                                       __builtin_bit_cast(u16x2, v.w[i] & 0x7fff7fffu)));
+        return;
+      }
 #pragma unroll
       for (int i = 0; i < VN; ++i) {
         const float f = v.get(i);
@@ -131,11 +135,13 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(FwdArgs a) {
       for (int j = 0; j < NV; ++j) {
         const int vec = tid + j * TPR;
         if (vec < n_vec) {
-          if (SUMS && rp) {
+          const int n = (int)min((int64_t)VN, a.H - vec * VN);
+          fit(x[set][j], n);
+          if constexpr (RES) {
+            fit(r[set][j], n);
             x[set][j] = sum(x[set][j], r[set][j]);
-            store_part((T*)a.h + row * a.H + vec * VN, x[set][j], (int)min((int64_t)VN, a.H - vec * VN));
+            store_part((T*)a.h + row * a.H + vec * VN, x[set][j], n);
           }
-          if (RELOAD) load_w(vec * VN, w[0]);
           see(x[set][j], w[HELD ? j : 0]);
         }
       }
@@ -143,7 +149,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(FwdArgs a) {
       for (int vec = tid; vec < n_vec; vec += TPR) {
         const int c = vec * VN, n = (int)min((int64_t)VN, a.H - c);
         Vec<T> v = load_part(xp + row * a.ldx + c, n);
-        if (SUMS && rp) {
+        if (RES) {
           v = sum(v, load_part(rp + row * a.ldr + c, n));
           store_part((T*)a.h + row * a.H + c, v, n);
         }
@@ -153,12 +159,13 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(FwdArgs a) {
     }
     float rstd = 1.f;
     if constexpr (EIGHT) {
-#pragma unroll
-      for (int off = 32; off >= 1; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off, 64));
-      if constexpr (WIDE) {
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) top64 = fmax(top64, __shfl_xor(top64, off, 64));
+      if constexpr (UNIT && sizeof(T) == 2) {  // (their order is that of what they stand for)
+        Vec<T> m;
+        m.w[0] = max(top & 0xffffu, top >> 16);
+        top = __float_as_uint(m.get(0));
       }
+      top = over_wave(top, [](uint32_t p, uint32_t q) { return max(p, q); });
+      if constexpr (WIDE) top64 = over_wave(top64, [](double p, double q) { return fmax(p, q); });
       if constexpr (TPR > 64) {
         if (threadIdx.x % 64 == 0) {
           tops[flip][threadIdx.x / 64] = top;
@@ -172,7 +179,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(FwdArgs a) {
       rstd = rsqrtf(ss / (float)a.H + a.eps);
       if (tid == 0 && a.rstd) a.rstd[row] = rstd;
     }
-    float inv = 0.f;
+    float below = 0.f, above = 0.f;
     bool tiny = false, bad = false;
     if constexpr (EIGHT) {
       if constexpr (TPR > 64) {
@@ -186,7 +193,11 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(FwdArgs a) {
       // infinities and NaN: the row's scale is NaN, and so is all that is computed of it
       bad = top >= 0x7f800000u;
       tiny = top64 < 1e-30;
-      inv = tiny || bad ? 0.f : 127.f / (float)top64;
+      if (!tiny && !bad) {
+        const uint32_t inv = __float_as_uint(127.f / (float)top64);
+        below = __uint_as_float(inv - (WIDE ? 6 : 1));
+        above = __uint_as_float(inv + (WIDE ? 6 : 1));
+      }
       if (tid == 0) a.scale[row] = bad ? __builtin_nanf("") : (float)top64 * rstd / 127.f;
     }
     auto write = [&](const Vec<T>& v, const float* wv, int vec) {
@@ -205,7 +216,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(FwdArgs a) {
           for (int k = 0; k < VN / 4; ++k) word[k] = 0;
         } else {
           // (values behind the row's end are zeros)
-          quantize<T, UNIT>(v, wv, add64, inv, top64, tiny, word);
+          quantize<T, UNIT>(v, wv, add64, below, above, top64, tiny, word);
         }
         int8_t* p = a.q + row * a.ldq + c;  // (ldq is a multiple of 16)
         if constexpr (VN == 8) *reinterpret_cast<uint2*>(p) = make_uint2(word[0], word[1]);
@@ -218,7 +229,6 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(FwdArgs a) {
         const int vec = tid + j * TPR;
         if (vec < n_vec) {
           x[set][j].keep();
-          if (RELOAD) load_w(vec * VN, w[0]);
           write(x[set][j], w[HELD ? j : 0], vec);
         }
       }
@@ -227,7 +237,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(FwdArgs a) {
         const int c = vec * VN, n = (int)min((int64_t)VN, a.H - c);
         if (!UNIT) load_w(c, w[0]);
         // (this thread wrote these values of h itself)
-        const T* src = SUMS && rp ? (const T*)a.h + row * a.H : xp + row * a.ldx;
+        const T* src = RES ? (const T*)a.h + row * a.H : xp + row * a.ldx;
         write(load_part(src + c, n), w[0], vec);
       }
     }
@@ -239,7 +249,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(FwdArgs a) {
   // (every thread of a workgroup goes through the same rounds: sums over a row have barriers)
   const int64_t step = (int64_t)gridDim.x * RPB;
   int64_t row = (int64_t)blockIdx.x * RPB + slot;
-  if constexpr (AHEAD) {
+  if constexpr (NV > 0) {  // the next row's loads are in flight while a row is worked on
     fetch(row, 0);
     for (; row < a.rows; row += 2 * step) {
       fetch(row + step, 1);
@@ -249,26 +259,23 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(FwdArgs a) {
       work(row + step, 1, 1);
     }
   } else {
-    for (int flip = 0; row < a.rows; row += step, flip ^= 1) {
-      fetch(row, 0);
-      work(row, 0, flip);
-    }
+    for (int flip = 0; row < a.rows; row += step, flip ^= 1) work(row, 0, flip);
   }
 }
 
 typedef void (*Kernel)(FwdArgs);
-template <class T, int TPR, int NV, int MODE> constexpr Kernel fwd_k = add_rmsnorm_kernel<T, TPR, NV, MODE>;
-template <class T, int MODE> static Kernel pick_mode(int64_t H) { FROWS_PICK(T, H, fwd_k, MODE); }
+template <class T, int TPR, int NV, int MODE, bool RES> constexpr Kernel fwd_k = add_rmsnorm_kernel<T, TPR, NV, MODE, RES>;
+template <class T, int MODE, bool RES> static Kernel pick_mode(int64_t H) { FROWS_PICK(T, H, fwd_k, MODE, RES); }
 
 template <class T>
-static Kernel pick(int mode, int64_t H) {
+static Kernel pick(int mode, int64_t H, bool res) {
   switch (mode) {
-    case NORM: return pick_mode<T, NORM>(H);
+    case NORM: return res ? pick_mode<T, NORM, true>(H) : pick_mode<T, NORM, false>(H);
     case NORM8:
-      if constexpr (sizeof(T) == 2) return pick_mode<T, NORM8>(H);
-    case NORM8_WIDE: return pick_mode<T, NORM8_WIDE>(H);
-    case ROWS8: return pick_mode<T, ROWS8>(H);
-    default: return pick_mode<T, ROWS8_SCALED>(H);
+      if constexpr (sizeof(T) == 2) return res ? pick_mode<T, NORM8, true>(H) : pick_mode<T, NORM8, false>(H);
+    case NORM8_WIDE: return res ? pick_mode<T, NORM8_WIDE, true>(H) : pick_mode<T, NORM8_WIDE, false>(H);
+    case ROWS8: return pick_mode<T, ROWS8, false>(H);
+    default: return pick_mode<T, ROWS8_SCALED, false>(H);
   }
 }
 
@@ -283,11 +290,17 @@ static int launch(const char* what, int dtype, int mode, const FwdArgs& a, hipSt
     return forge_set_error(FORGE_ERR_INVALID, "%s: 8-bit rows need a pitch that is a multiple of 16, and 16-byte alignment", what);
   if (a.rows == 0 || a.H == 0) return FORGE_OK;
   if (!a.x || (mode == NORM ? !a.y : !a.q || !a.scale)) return forge_set_error(FORGE_ERR_INVALID, "%s: an array is NULL", what);
-  const Kernel k = dtype == FORGE_DTYPE_F32 ? pick<float>(mode, a.H)
-                   : dtype == FORGE_DTYPE_F16 ? pick<fp16_t>(mode, a.H) : pick<bf16_t>(mode, a.H);
-  const int64_t nv = (a.H * (int64_t)dtype_size(dtype) + 15) / 16, rpb = nv <= 128 ? 4 : 1;
-  const int64_t blocks = (a.rows + rpb - 1) / rpb;
-  k<<<(unsigned)(blocks < 2048 ? blocks : 2048), 256, 0, s>>>(a);
+  const bool res = a.res != nullptr;
+  const Kernel k = dtype == FORGE_DTYPE_F32 ? pick<float>(mode, a.H, res)
+                   : dtype == FORGE_DTYPE_F16 ? pick<fp16_t>(mode, a.H, res) : pick<bf16_t>(mode, a.H, res);
+  const int size = dtype_size(dtype), at_once = rows_at_once(a.H, size);
+  const int64_t blocks = (a.rows + at_once - 1) / at_once;
+  // Workgroups that stay while the rows go by, the next row of each in flight: few where
+  // a row is long or gives much to do, more where its loads are most of it (16-bit
+  // [8192, 4096]: norm 51 us by 2048, 48 by 1024, 45 by 512; a row times scales 27, 27, 32;
+  // a row as it is 27, 30, 36; [8192, 14336]: 86, 84, 84).
+  const int threads = threads_for(a.H, size), most = at_once > 1 ? 2048 : threads > 256 || mode == NORM ? 512 : mode == ROWS8 ? 2048 : 1024;
+  k<<<(unsigned)(blocks < most ? blocks : most), threads, 0, s>>>(a);
   FORGE_CHECK_LAUNCH();
   return FORGE_OK;
 }

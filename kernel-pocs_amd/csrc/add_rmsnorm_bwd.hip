@@ -22,17 +22,15 @@ struct BwdArgs {
   float offset;
 };
 
-template <class T, int TPR, int NV, bool DW>
-__global__ __launch_bounds__(256) void add_rmsnorm_bwd_kernel(BwdArgs a) {
+template <class T, int TPR, int NV, bool DW, bool DH>
+__global__ __launch_bounds__(threads_of<TPR>) void add_rmsnorm_bwd_kernel(BwdArgs a) {
   constexpr int VN = V<T>, RPB = rows_per_block<TPR>, N = NV ? NV : 1;
-  constexpr bool AHEAD = NV > 0 && NV <= 2;  // the next row's loads are in flight while a row is worked on
-  __shared__ float sums[2][4];
+  __shared__ float sums[2][threads_of<TPR> / 64];
   __shared__ float cols[TPR == 64 && DW ? 4 * 64 * N * VN : 1];
   const int tid = threadIdx.x % TPR, slot = threadIdx.x / TPR;
   const int n_vec = (int)((a.H + VN - 1) / VN);
   const float inv_h = 1.f / (float)a.H;
-  constexpr bool HELD = NV <= 4;  // a thread's weights are held, or read again for every row
-  float w[HELD ? N : 1][VN], dw[N][VN];
+  float w[N][VN], dw[N][VN];
   auto load_w = [&](int c, float (&o)[VN]) {
     load_weight<T>(a.w, a.w_dtype, c, (int)min((int64_t)VN, a.H - c), o);
 #pragma unroll
@@ -41,7 +39,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_bwd_kernel(BwdArgs a) {
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const int vec = tid + j * TPR;
-    if (HELD && vec < n_vec) load_w(vec * VN, w[j]);
+    if (NV > 0 && vec < n_vec) load_w(vec * VN, w[j]);
 #pragma unroll
     for (int i = 0; i < VN; ++i) dw[j][i] = 0.f;
   }
@@ -50,19 +48,15 @@ __global__ __launch_bounds__(256) void add_rmsnorm_bwd_kernel(BwdArgs a) {
     float rstd;
   } sets[2];
   auto fetch = [&](int64_t row, Set& s) {
-    if (row >= a.rows) return;
+    row = min(row, a.rows - 1);
     s.rstd = a.rstd[row];
-    if constexpr (NV > 0) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int vec = tid + j * TPR, c = vec * VN, n = (int)min((int64_t)VN, a.H - c);
-        if (vec < n_vec) {
-          s.h[j] = load_part((const T*)a.h + row * a.ldh + c, n);
-          s.dy[j] = load_part((const T*)a.dy + row * a.lddy + c, n);
-          if (a.dh) s.dh[j] = load_part((const T*)a.dh + row * a.lddh + c, n);
-          else s.dh[j].clear();
-        }
-      }
+    for (int j = 0; j < NV; ++j) {
+      const int c = (tid + j * TPR) * VN;
+      s.h[j] = load_held((const T*)a.h + row * a.ldh, c, a.H);
+      s.dy[j] = load_held((const T*)a.dy + row * a.lddy, c, a.H);
+      if constexpr (DH) s.dh[j] = load_held((const T*)a.dh + row * a.lddh, c, a.H);
+      else s.dh[j].clear();
     }
   };
   bool started = false;  // NV = 0: this workgroup's partial row has been written
@@ -79,8 +73,11 @@ __global__ __launch_bounds__(256) void add_rmsnorm_bwd_kernel(BwdArgs a) {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
         if (on && tid + j * TPR < n_vec) {
-          if (!HELD) load_w((tid + j * TPR) * VN, w[0]);
-          add_dot(s.h[j], s.dy[j], w[HELD ? j : 0]);
+          const int n = (int)min((int64_t)VN, a.H - (tid + j * TPR) * VN);
+          fit(s.h[j], n);
+          fit(s.dy[j], n);
+          if constexpr (DH) fit(s.dh[j], n);
+          add_dot(s.h[j], s.dy[j], w[j]);
         }
     } else if (on) {
       for (int vec = tid; vec < n_vec; vec += TPR) {
@@ -91,7 +88,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_bwd_kernel(BwdArgs a) {
     }
     dot = row_sum<TPR>(dot, sums[flip]);
     if (!on) return;
-    const float rstd = s.rstd, k = rstd * rstd * rstd * dot * inv_h;
+    const float rstd = NV > 0 ? s.rstd : a.rstd[row], k = rstd * rstd * rstd * dot * inv_h;
     auto finish = [&](const Vec<T>& x, const Vec<T>& y, const Vec<T>& g, const float (&wv)[VN], int vec) {
       Vec<T> d;
       float f[VN];
@@ -108,8 +105,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_bwd_kernel(BwdArgs a) {
         if (vec < n_vec) {
           s.h[j].keep();
           s.dy[j].keep();
-          if (!HELD) load_w(vec * VN, w[0]);
-          finish(s.h[j], s.dy[j], s.dh[j], w[HELD ? j : 0], vec);
+          finish(s.h[j], s.dy[j], s.dh[j], w[j], vec);
           if constexpr (DW)
 #pragma unroll
             for (int i = 0; i < VN; ++i) dw[j][i] += s.dy[j].get(i) * (s.h[j].get(i) * rstd);
@@ -121,7 +117,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_bwd_kernel(BwdArgs a) {
         load_w(c, w[0]);
         Vec<T> g;
         g.clear();
-        if (a.dh) g = load_part((const T*)a.dh + row * a.lddh + c, n);
+        if constexpr (DH) g = load_part((const T*)a.dh + row * a.lddh + c, n);
         const Vec<T> x = load_part(hp + c, n), y = load_part(yp + c, n);
         finish(x, y, g, w[0], vec);
         if constexpr (DW) {  // (this thread's own columns of the workgroup's partial row)
@@ -140,7 +136,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_bwd_kernel(BwdArgs a) {
   // (every thread of a workgroup goes through the same rounds)
   const int64_t step = (int64_t)gridDim.x * RPB;
   int64_t first = (int64_t)blockIdx.x * RPB;
-  if constexpr (AHEAD) {
+  if constexpr (NV > 0) {  // the next row's loads are in flight while a row is worked on
     fetch(first + slot, sets[0]);
     for (; first < a.rows; first += 2 * step) {
       fetch(first + step + slot, sets[1]);
@@ -150,10 +146,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_bwd_kernel(BwdArgs a) {
       work(first + step + slot, sets[1], 1);
     }
   } else {
-    for (int flip = 0; first < a.rows; first += step, flip ^= 1) {
-      fetch(first + slot, sets[0]);
-      work(first + slot, sets[0], flip);
-    }
+    for (int flip = 0; first < a.rows; first += step, flip ^= 1) work(first + slot, sets[0], flip);
   }
   if constexpr (DW && NV > 0) {
     float* part = a.part + blockIdx.x * a.ld_part;
@@ -212,16 +205,18 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(const float* part, int64
 }
 
 typedef void (*BwdKernel)(BwdArgs);
-template <class T, int TPR, int NV, bool DW> constexpr BwdKernel bwd_k = add_rmsnorm_bwd_kernel<T, TPR, NV, DW>;
-template <class T, bool DW> static BwdKernel pick_dw(int64_t H) { FROWS_PICK(T, H, bwd_k, DW); }
-template <class T> static BwdKernel pick_bwd(int64_t H, bool dw) { return dw ? pick_dw<T, true>(H) : pick_dw<T, false>(H); }
+template <class T, int TPR, int NV, bool DW, bool DH> constexpr BwdKernel bwd_k = add_rmsnorm_bwd_kernel<T, TPR, NV, DW, DH>;
+template <class T, bool DW, bool DH> static BwdKernel pick_one(int64_t H) { FROWS_PICK(T, H, bwd_k, DW, DH); }
+template <class T> static BwdKernel pick_bwd(int64_t H, bool dw, bool dh) {
+  return dw ? (dh ? pick_one<T, true, true>(H) : pick_one<T, true, false>(H)) : dh ? pick_one<T, false, true>(H) : pick_one<T, false, false>(H);
+}
 
 static int64_t part_pitch(int64_t H) { return (H + 3) / 4 * 4; }
 
 // Workgroups: one partial row each.
 static int64_t bwd_blocks(int dtype, int64_t rows, int64_t H) {
-  const int64_t nv = (H * (int64_t)dtype_size(dtype) + 15) / 16, rpb = nv <= 128 ? 4 : 1;
-  const int64_t blocks = (rows + rpb - 1) / rpb;
+  const int at_once = rows_at_once(H, dtype_size(dtype));
+  const int64_t blocks = (rows + at_once - 1) / at_once;
   return blocks < 512 ? blocks : 512;
 }
 
@@ -246,9 +241,9 @@ extern "C" int forge_add_rmsnorm_bwd(int dtype, int w_dtype, const void* dy, int
   if (rows == 0 || H == 0) return FORGE_OK;  // (the caller clears dw)
   if (!dy || !h || !weight || !rstd || !d || (dw && !work)) return forge_set_error(FORGE_ERR_INVALID, "add_rmsnorm: an array is NULL");
   BwdArgs a = {dy, lddy, dh, lddh, h, ldh, weight, w_dtype, rstd, d, (float*)work, part_pitch(H), rows, H, (float)offset};
-  const BwdKernel k = dtype == FORGE_DTYPE_F32 ? pick_bwd<float>(H, dw) : dtype == FORGE_DTYPE_F16 ? pick_bwd<fp16_t>(H, dw) : pick_bwd<bf16_t>(H, dw);
+  const BwdKernel k = dtype == FORGE_DTYPE_F32 ? pick_bwd<float>(H, dw, dh) : dtype == FORGE_DTYPE_F16 ? pick_bwd<fp16_t>(H, dw, dh) : pick_bwd<bf16_t>(H, dw, dh);
   const int64_t blocks = bwd_blocks(dtype, rows, H);
-  k<<<(unsigned)blocks, 256, 0, (hipStream_t)stream>>>(a);
+  k<<<(unsigned)blocks, threads_for(H, dtype_size(dtype)), 0, (hipStream_t)stream>>>(a);
   FORGE_CHECK_LAUNCH();
   if (dw) {
     sum_parts_kernel<<<(unsigned)((H + 31) / 32), 256, 0, (hipStream_t)stream>>>((const float*)work, part_pitch(H), (int)blocks, H, dw, w_dtype);
