@@ -791,7 +791,7 @@ int forge_attention_fwd(int dtype, const void* q, int64_t q_batch, int64_t q_row
 /* Gradients of q, k and v from that of out, with out and lse as the forward
  * left them; dk and dv are summed over a group's heads.  Sums have a fixed
  * order.  work: forge_attention_bwd_workspace bytes. */
-int64_t forge_attention_bwd_workspace(int varlen, int64_t B, int64_t tq, int64_t H);
+int64_t forge_attention_bwd_workspace(int varlen, int64_t B, int64_t tq, int64_t tk, int64_t H, int64_t Hkv, int64_t D);
 int forge_attention_bwd(int dtype, const void* dout, int64_t do_batch, int64_t do_row, int64_t do_head,
                         const void* q, int64_t q_batch, int64_t q_row, int64_t q_head,
                         const void* k, int64_t k_batch, int64_t k_row, int64_t k_head,

@@ -51,6 +51,8 @@ struct Args {
   int H, Hkv, D;
   float scale;
   int causal;
+  float* part;                        // dk and dv of `parts` parts of a group's heads, [part][row][Hkv][2][D]
+  int parts;                          // 1: dk and dv are written as they are
 };
 
 template <class T> __device__ __forceinline__ T* row_ptr(const Rows& r, int64_t batch, int64_t row, int head) {

@@ -6,7 +6,8 @@ namespace fattn {
 int launch_fwd(int dtype, const Args& a, hipStream_t s);
 int launch_rows(int dtype, const Args& a, int64_t n_queries, void* work, hipStream_t s);
 int64_t rows_workspace(const Args& a, int64_t n_queries);
-int launch_bwd(int dtype, const Args& a, float* lse2, int64_t n_rows, hipStream_t s);
+int launch_bwd(int dtype, const Args& a, float* shift, int64_t n_rows, hipStream_t s);
+int dkv_parts(const Args& a);
 
 // Few queries a sequence: the kernel that reads keys by chunks.  The lengths are
 // on the device, so the rule goes by their mean: at most 4 queries a sequence
@@ -95,9 +96,17 @@ extern "C" int forge_attention_fwd(int dtype, const void* q, int64_t q_batch, in
   return launch_fwd(dtype, a, (hipStream_t)stream);
 }
 
-extern "C" int64_t forge_attention_bwd_workspace(int varlen, int64_t B, int64_t tq, int64_t H) {
-  if (B < 0 || tq < 0 || H < 0) return -1;
-  return (varlen ? tq : B * tq) * H * 2 * 4;
+// -delta and -lse / scale by head and query, and dk and dv of parts of a group's heads
+static int64_t stat_bytes(int64_t n_queries, int64_t H) { return (n_queries * H * 2 * 4 + 15) / 16 * 16; }
+
+extern "C" int64_t forge_attention_bwd_workspace(int varlen, int64_t B, int64_t tq, int64_t tk, int64_t H, int64_t Hkv,
+                                                 int64_t D) {
+  static const int32_t none = 0;
+  const int32_t* cu = varlen ? &none : nullptr;  // (only whether it is NULL is looked at)
+  const Args a = make_args(cu, cu, B, tq, tk, H, Hkv, D, 1.f, 1);
+  if (check_sizes(FORGE_DTYPE_BF16, a)) return -1;
+  const int parts = dkv_parts(a);
+  return stat_bytes(varlen ? tq : B * tq, H) + (parts > 1 ? (int64_t)parts * (varlen ? tk : B * tk) * Hkv * 2 * D * 4 : 0);
 }
 
 extern "C" int forge_attention_bwd(int dtype, const void* dout, int64_t do_batch, int64_t do_row, int64_t do_head,
@@ -131,6 +140,9 @@ extern "C" int forge_attention_bwd(int dtype, const void* dout, int64_t do_batch
   if (int e = check_rows("dk", a.dk, nb, tk, Hkv)) return e;
   if (int e = check_rows("dv", a.dv, nb, tk, Hkv)) return e;
   if (n > 0 && (!lse || !work)) return forge_set_error(FORGE_ERR_INVALID, "attention: lse or work is NULL");
+  if (!aligned16(work)) return forge_set_error(FORGE_ERR_INVALID, "attention: work is not aligned");
   a.delta = (float*)work;
+  a.parts = n > 0 ? dkv_parts(a) : 1;
+  a.part = (float*)((char*)work + stat_bytes(n, H));
   return launch_bwd(dtype, a, (float*)work + n * H, n, (hipStream_t)stream);
 }

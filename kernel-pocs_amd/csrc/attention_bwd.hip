@@ -1,5 +1,5 @@
-// Attention backward for gfx950: three launches, no atomics (the sums have a
-// fixed order).
+// Attention backward for gfx950: three launches (four where there are few keys), no
+// atomics (the sums have a fixed order).
 //   -delta_i, delta_i = sum_d o_i dout_i, and -lse_i / scale, by head and query;
 //   dq_i = scale sum_j ds_ij k_j,       a workgroup to 128 queries of a head;
 //   dv_j = sum_i p_ij dout_i, dk_j = scale sum_i ds_ij q_i over the queries of the
@@ -221,7 +221,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
   auto stat = [&](int slot, int i) __attribute__((always_inline)) { return reinterpret_cast<float*>(smem) + (slot * 2 + i) * 64; };
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int G = a.H / a.Hkv, h = lane / 32;
-  const Item it = item_of(blockIdx.x, tiles, a.Hkv, 1);
+  const Item it = item_of(blockIdx.x, tiles, a.Hkv, a.parts);
   if (it.tile >= tiles) return;
   const LevelAt at = find_level(a.cu_k, a.B, a.tk, BN, it.tile);
   if (at.seq > a.B) return;
@@ -250,11 +250,12 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
   // the first query that sees a key of the tile, and tiles of queries from there, of
   // each of the group's heads in turn
   const int first = a.causal ? max(0, k0 - shift) / BQ * BQ : 0;
-  const int n_t = sq.len > first ? (sq.len - first + BQ - 1) / BQ * G : 0;
+  const int g_lo = G * it.g / a.parts, g_hi = G * (it.g + 1) / a.parts;  // of this part
+  const int n_t = sq.len > first ? (sq.len - first + BQ - 1) / BQ * (g_hi - g_lo) : 0;
   Dma qd, dd;
   qd.setup(a.q.row, a.D);
   dd.setup(a.dout.row, a.D);
-  int next_i = first, next_head = it.kv * G;  // of the tile that is issued next
+  int next_i = first, next_head = it.kv * G + g_lo;  // of the tile that is issued next
   auto issue = [&](int slot) {
     const int left = sq.len - next_i;
     char* st = smem + TILES + slot * 2 * Dma::BYTES;
@@ -350,6 +351,22 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
   }
   if (!live) return;
   const float p_one = exp2f(-P_BITS<T>), back = a.scale * p_one / unit;
+  if (a.parts > 1) {
+    const int64_t n_k = a.cu_k ? a.tk : a.tk * a.B, row = (a.cu_k ? sk.start : sk.batch * a.tk) + jk;
+    float* p = a.part + ((it.g * n_k + row) * a.Hkv + it.kv) * 2 * a.D;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 32 * db + 8 * i + 4 * h;
+        if (d >= a.D) continue;
+        if constexpr (DK)
+          *reinterpret_cast<f32x4*>(p + d) = f32x4{dk[db][4 * i], dk[db][4 * i + 1], dk[db][4 * i + 2], dk[db][4 * i + 3]} * back;
+        if constexpr (DV)
+          *reinterpret_cast<f32x4*>(p + a.D + d) = f32x4{dv[db][4 * i], dv[db][4 * i + 1], dv[db][4 * i + 2], dv[db][4 * i + 3]} * p_one;
+      }
+    return;
+  }
   T* kp = row_ptr<T>(a.dk, sk.batch, sk.start + jk, it.kv);
   T* vp = row_ptr<T>(a.dv, sk.batch, sk.start + jk, it.kv);
 #pragma unroll
@@ -365,6 +382,32 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
     }
 }
 
+// dk and dv: the sums of the parts, in order.  4 values a thread.
+template <class T>
+__global__ __launch_bounds__(256) void attn_dkv_join_kernel(Args a, int64_t n_k) {
+  const int vecs = a.D / 4;
+  const int64_t n = n_k * a.Hkv * 2 * vecs;
+  for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < n; x += (int64_t)gridDim.x * 256) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int p = 0; p < a.parts; ++p) v += *reinterpret_cast<const f32x4*>(a.part + (p * n + x) * 4);
+    const int d = (int)(x % vecs) * 4, which = (int)(x / vecs % 2), head = (int)(x / vecs / 2 % a.Hkv);
+    const int64_t row = x / vecs / 2 / a.Hkv, batch = a.cu_k ? 0 : row / a.tk;
+    store4(row_ptr<T>(which ? a.dv : a.dk, batch, a.cu_k ? row : row % a.tk, head) + d, v[0], v[1], v[2], v[3]);
+  }
+}
+
+// Parts of a group's heads, a workgroup each: where the tiles of keys alone would
+// leave CUs without work (two workgroups a CU are resident), and where a
+// workgroup has at least 16 tiles of queries to go through (a tile takes longer than
+// its share of the join).
+int dkv_parts(const Args& a) {
+  const int64_t G = a.H / a.Hkv, wgs = most_tiles(a.cu_k, a.B, a.tk, 128) * a.Hkv;
+  const int64_t queries = a.cu_q ? a.tq / (a.B > 0 ? a.B : 1) : a.tq;  // of a sequence
+  if (wgs == 0 || G * queries < 16 * 64) return 1;
+  const int64_t parts = 512 / wgs;
+  return (int)(parts < 1 ? 1 : parts > G ? G : parts);
+}
+
 template <class T, int DP, bool DK, bool DV>
 static int launch_dkv(const Args& a, const float* shift, int64_t n_rows, int64_t n, int64_t tiles, hipStream_t s) {
   attn_dkv_kernel<T, DP, DK, DV><<<(unsigned)n, 256, 0, s>>>(a, shift, n_rows, (int)tiles);
@@ -375,7 +418,7 @@ static int launch_dkv(const Args& a, const float* shift, int64_t n_rows, int64_t
 template <class T, int DP>
 static int launch_bwd_dp(const Args& a, float* shift, int64_t n_rows, hipStream_t s) {
   const int64_t tq = most_tiles(a.cu_q, a.B, a.tq, 128), tk = most_tiles(a.cu_k, a.B, a.tk, 128);
-  const int64_t nq = items(tq, a.Hkv, a.H / a.Hkv), nk = items(tk, a.Hkv, 1);
+  const int64_t nq = items(tq, a.Hkv, a.H / a.Hkv), nk = items(tk, a.Hkv, a.parts);
   if (nq > 0x7fffffffLL || nk > 0x7fffffffLL) return forge_set_error(FORGE_ERR_INVALID, "attention: too many tiles");
   const int64_t pairs = n_rows * a.H;
   if (pairs) attn_delta_kernel<T><<<grid_for(pairs * 16, 256, 256 * 64), 256, 0, s>>>(a, shift, n_rows, pairs);
@@ -383,9 +426,15 @@ static int launch_bwd_dp(const Args& a, float* shift, int64_t n_rows, hipStream_
   if (nq && n_rows) attn_dq_kernel<T, DP><<<(unsigned)nq, 256, 0, s>>>(a, shift, n_rows, (int)tq);
   FORGE_CHECK_LAUNCH();
   if (nk == 0) return FORGE_OK;
-  if (DP < 256) return launch_dkv<T, DP, true, DP < 256>(a, shift, n_rows, nk, tk, s);
   if (int e = launch_dkv<T, DP, true, DP < 256>(a, shift, n_rows, nk, tk, s)) return e;
-  return launch_dkv<T, DP, DP < 256, true>(a, shift, n_rows, nk, tk, s);
+  if (DP == 256)
+    if (int e = launch_dkv<T, DP, DP < 256, true>(a, shift, n_rows, nk, tk, s)) return e;
+  if (a.parts > 1) {
+    const int64_t n_k = a.cu_k ? a.tk : a.tk * a.B;
+    attn_dkv_join_kernel<T><<<grid_for(n_k * a.Hkv * 2 * (a.D / 4), 256, 256 * 16), 256, 0, s>>>(a, n_k);
+    FORGE_CHECK_LAUNCH();
+  }
+  return FORGE_OK;
 }
 
 template <class T>

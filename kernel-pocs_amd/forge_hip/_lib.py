@@ -234,7 +234,7 @@ forge_attention_fwd_workspace = _decl("forge_attention_fwd_workspace", [c_int] +
 forge_attention_fwd = _decl(
     "forge_attention_fwd", [c_int] + [c_vp, c_i64, c_i64, c_i64] * 4 + [c_vp] * 3 + [c_i64] * 6 + [c_f32, c_int, c_vp, c_vp]
 )
-forge_attention_bwd_workspace = _decl("forge_attention_bwd_workspace", [c_int] + [c_i64] * 3, c_i64)
+forge_attention_bwd_workspace = _decl("forge_attention_bwd_workspace", [c_int] + [c_i64] * 6, c_i64)
 forge_attention_bwd = _decl(
     "forge_attention_bwd",
     [c_int] + [c_vp, c_i64, c_i64, c_i64] * 5 + [c_vp] + [c_vp, c_i64, c_i64, c_i64] * 3 + [c_vp] * 2 + [c_i64] * 6

@@ -100,8 +100,7 @@ def _backward(dout, q, k, v, out, lse, cu_q, cu_k, scale, causal, layout):
     varlen = layout is _Layout.packed
     if q.numel() == 0:
         return dq, dk.zero_(), dv.zero_()
-    work = torch.empty(L.forge_attention_bwd_workspace(varlen, sizes[0], sizes[1], sizes[3]), dtype=torch.uint8,
-                       device=q.device)
+    work = torch.empty(L.forge_attention_bwd_workspace(varlen, *sizes), dtype=torch.uint8, device=q.device)
     with L.on_device(q):
         L.check(
             L.forge_attention_bwd(

@@ -388,3 +388,11 @@ def test_values_that_are_not_finite_where_they_are_not_seen(lens_q, lens_k, H, k
             assert torch.equal(out[seen, h] == x, hit) and (h * kv // H > 0 or hit.any())
     # and a NaN of a key makes all of a query that sees it NaN
     assert run(_special(k, rows[:1], [nan]), v)[0][seen][:, :H // kv].isnan().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens_q,lens_k", [([600], [600]), ([300, 0, 5, 400], [300, 9, 0, 700])])
+@pytest.mark.parametrize("H,kv,D,dtype", [(16, 1, 64, FP16), (12, 2, 128, BF16), (7, 1, 256, BF16), (40, 1, 8, BF16)])
+def test_few_keys_and_many_heads(lens_q, lens_k, H, kv, D, dtype):
+    """Gradients of keys whose heads go to several workgroups (heads that the parts do not divide)."""
+    _check(lens_q, lens_k, H, kv, D, dtype, tail_q=3, tail_k=40)
