@@ -76,7 +76,7 @@ extern "C" int64_t forge_attention_fwd_workspace(int varlen, int64_t B, int64_t 
 extern "C" int forge_attention_fwd(int dtype, const void* q, int64_t q_batch, int64_t q_row, int64_t q_head,
                                    const void* k, int64_t k_batch, int64_t k_row, int64_t k_head,
                                    const void* v, int64_t v_batch, int64_t v_row, int64_t v_head,
-                                   void* out, int64_t o_batch, int64_t o_row, int64_t o_head, float* lse,
+                                   void* out, int64_t o_batch, int64_t o_row, int64_t o_head, float* lse, int8_t* low,
                                    const int32_t* cu_q, const int32_t* cu_k, int64_t B, int64_t tq, int64_t tk,
                                    int64_t H, int64_t Hkv, int64_t D, float scale, int causal, void* work, void* stream) {
   Args a = make_args(cu_q, cu_k, B, tq, tk, H, Hkv, D, scale, causal);
@@ -86,6 +86,8 @@ extern "C" int forge_attention_fwd(int dtype, const void* q, int64_t q_batch, in
   a.v = {v, v_batch, v_row, v_head};
   a.o = {out, o_batch, o_row, o_head};
   a.lse = lse;
+  a.low = low;
+  if (low && (dtype != FORGE_DTYPE_F16 || !aligned16(low))) return forge_set_error(FORGE_ERR_INVALID, "attention: low is kept of fp16 only, 16-byte aligned");
   const int64_t nb = cu_q ? 1 : B, n = nb * tq;
   if (int e = check_rows("q", a.q, nb, tq, H)) return e;
   if (int e = check_rows("k", a.k, nb, tk, Hkv)) return e;
@@ -114,7 +116,7 @@ extern "C" int forge_attention_bwd(int dtype, const void* dout, int64_t do_batch
                                    const void* k, int64_t k_batch, int64_t k_row, int64_t k_head,
                                    const void* v, int64_t v_batch, int64_t v_row, int64_t v_head,
                                    const void* out, int64_t o_batch, int64_t o_row, int64_t o_head, const float* lse,
-                                   void* dq, int64_t dq_batch, int64_t dq_row, int64_t dq_head,
+                                   const int8_t* low, void* dq, int64_t dq_batch, int64_t dq_row, int64_t dq_head,
                                    void* dk, int64_t dk_batch, int64_t dk_row, int64_t dk_head,
                                    void* dv, int64_t dv_batch, int64_t dv_row, int64_t dv_head,
                                    const int32_t* cu_q, const int32_t* cu_k, int64_t B, int64_t tq, int64_t tk,
@@ -130,6 +132,7 @@ extern "C" int forge_attention_bwd(int dtype, const void* dout, int64_t do_batch
   a.dk = {dk, dk_batch, dk_row, dk_head};
   a.dv = {dv, dv_batch, dv_row, dv_head};
   a.lse = const_cast<float*>(lse);
+  a.low = const_cast<int8_t*>(low);
   const int64_t nb = cu_q ? 1 : B, n = nb * tq;
   if (int e = check_rows("dout", a.dout, nb, tq, H)) return e;
   if (int e = check_rows("q", a.q, nb, tq, H)) return e;
@@ -140,7 +143,8 @@ extern "C" int forge_attention_bwd(int dtype, const void* dout, int64_t do_batch
   if (int e = check_rows("dk", a.dk, nb, tk, Hkv)) return e;
   if (int e = check_rows("dv", a.dv, nb, tk, Hkv)) return e;
   if (n > 0 && (!lse || !work)) return forge_set_error(FORGE_ERR_INVALID, "attention: lse or work is NULL");
-  if (!aligned16(work)) return forge_set_error(FORGE_ERR_INVALID, "attention: work is not aligned");
+  if (n > 0 && dtype == FORGE_DTYPE_F16 && !low) return forge_set_error(FORGE_ERR_INVALID, "attention: fp16 needs low");
+  if (!aligned16(work) || !aligned16(low)) return forge_set_error(FORGE_ERR_INVALID, "attention: work or low is not aligned");
   a.delta = (float*)work;
   a.parts = n > 0 ? dkv_parts(a) : 1;
   a.part = (float*)((char*)work + stat_bytes(n, H));

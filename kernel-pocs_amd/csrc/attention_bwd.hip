@@ -55,8 +55,15 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(Args a, float* shift, i
     float sum = 0.f;
     for (int c = 8 * (lane % 16); c < a.D; c += 128) {
       const Vec16<T> x = load16(o + c), y = load16(d + c);
+      uint2 low = make_uint2(0, 0);
+      if constexpr (std::is_same_v<T, fp16_t>) low = *reinterpret_cast<const uint2*>(a.low + p * a.D + c);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += to_f32(x.v[i]) * to_f32(y.v[i]);
+      for (int i = 0; i < 8; ++i) {
+        float f = to_f32(x.v[i]);
+        if constexpr (std::is_same_v<T, fp16_t>)
+          f = __builtin_fmaf((float)(int8_t)((i < 4 ? low.x : low.y) >> (8 * (i % 4))), low_step(f), f);
+        sum += f * to_f32(y.v[i]);
+      }
     }
 #pragma unroll
     for (int off = 8; off >= 1; off /= 2) sum += __shfl_xor(sum, off, 64);

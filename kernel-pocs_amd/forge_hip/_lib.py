@@ -232,12 +232,12 @@ forge_cast_f32_bf16 = _decl("forge_cast_f32_bf16", [c_vp, c_i64, c_vp, c_i64, c_
 
 forge_attention_fwd_workspace = _decl("forge_attention_fwd_workspace", [c_int] + [c_i64] * 6, c_i64)
 forge_attention_fwd = _decl(
-    "forge_attention_fwd", [c_int] + [c_vp, c_i64, c_i64, c_i64] * 4 + [c_vp] * 3 + [c_i64] * 6 + [c_f32, c_int, c_vp, c_vp]
+    "forge_attention_fwd", [c_int] + [c_vp, c_i64, c_i64, c_i64] * 4 + [c_vp] * 4 + [c_i64] * 6 + [c_f32, c_int, c_vp, c_vp]
 )
 forge_attention_bwd_workspace = _decl("forge_attention_bwd_workspace", [c_int] + [c_i64] * 6, c_i64)
 forge_attention_bwd = _decl(
     "forge_attention_bwd",
-    [c_int] + [c_vp, c_i64, c_i64, c_i64] * 5 + [c_vp] + [c_vp, c_i64, c_i64, c_i64] * 3 + [c_vp] * 2 + [c_i64] * 6
+    [c_int] + [c_vp, c_i64, c_i64, c_i64] * 5 + [c_vp] * 2 + [c_vp, c_i64, c_i64, c_i64] * 3 + [c_vp] * 2 + [c_i64] * 6
     + [c_f32, c_int, c_vp, c_vp],
 )
 _ADD_NORM = [c_int, c_int, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp]

@@ -72,11 +72,13 @@ def _sizes(q, k, cu_q, layout):
     return q.shape[0], q.shape[2], k.shape[2], q.shape[1], k.shape[1], q.shape[3]
 
 
-def _forward(q, k, v, cu_q, cu_k, scale, causal, layout, want_lse):
+def _forward(q, k, v, cu_q, cu_k, scale, causal, layout, want_lse, train=False):
     sizes = _sizes(q, k, cu_q, layout)
     out = _new(q.shape, q, layout)
     varlen = layout is _Layout.packed
-    lse = None
+    lse = low = None
+    if train and q.dtype == torch.float16:  # what out's rounding took, for the gradients
+        low = torch.empty(out.numel(), dtype=torch.int8, device=q.device)
     if want_lse:
         lse = torch.empty((q.shape[0], q.shape[1]) if varlen else (q.shape[0], q.shape[2], q.shape[1]),
                           dtype=torch.float32, device=q.device)
@@ -87,13 +89,13 @@ def _forward(q, k, v, cu_q, cu_k, scale, causal, layout, want_lse):
             L.check(
                 L.forge_attention_fwd(
                     L.dtype_code(q.dtype), q.data_ptr(), *layout(q), k.data_ptr(), *layout(k), v.data_ptr(), *layout(v),
-                    out.data_ptr(), *layout(out), L.ptr(lse), L.ptr(cu_q), L.ptr(cu_k), *sizes, scale, causal,
-                    L.ptr(work), L.stream_of(q)),
+                    out.data_ptr(), *layout(out), L.ptr(lse), L.ptr(low), L.ptr(cu_q), L.ptr(cu_k), *sizes,
+                    scale, causal, L.ptr(work), L.stream_of(q)),
                 "forge_attention_fwd")
-    return out, lse
+    return out, lse, low
 
 
-def _backward(dout, q, k, v, out, lse, cu_q, cu_k, scale, causal, layout):
+def _backward(dout, q, k, v, out, lse, low, cu_q, cu_k, scale, causal, layout):
     dout = _readable(dout, layout)
     sizes = _sizes(q, k, cu_q, layout)
     dq, dk, dv = _new(q.shape, q, layout), _new(k.shape, k, layout), _new(v.shape, v, layout)
@@ -105,7 +107,7 @@ def _backward(dout, q, k, v, out, lse, cu_q, cu_k, scale, causal, layout):
         L.check(
             L.forge_attention_bwd(
                 L.dtype_code(q.dtype), dout.data_ptr(), *layout(dout), q.data_ptr(), *layout(q), k.data_ptr(), *layout(k),
-                v.data_ptr(), *layout(v), out.data_ptr(), *layout(out), lse.data_ptr(), dq.data_ptr(), *layout(dq),
+                v.data_ptr(), *layout(v), out.data_ptr(), *layout(out), lse.data_ptr(), L.ptr(low), dq.data_ptr(), *layout(dq),
                 dk.data_ptr(), *layout(dk), dv.data_ptr(), *layout(dv), L.ptr(cu_q), L.ptr(cu_k), *sizes, scale, causal,
                 work.data_ptr(), L.stream_of(q)),
             "forge_attention_bwd")
@@ -115,13 +117,14 @@ def _backward(dout, q, k, v, out, lse, cu_q, cu_k, scale, causal, layout):
 class ForgeAttentionFunction(torch.autograd.Function):
     """forward(ctx, q, k, v, cu_q, cu_k, scale, causal, packed) -> (out, lse) on
     arguments that the entry points have checked and laid out; saves them with
-    out and lse, and the backward computes the probabilities again."""
+    out and lse (fp16: and a byte a value of what out's rounding took), and the
+    backward computes the probabilities again."""
 
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, scale, causal, packed):
         layout = _Layout.packed if packed else _Layout.dense
-        out, lse = _forward(q, k, v, cu_q, cu_k, scale, causal, layout, True)
-        ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k)
+        out, lse, low = _forward(q, k, v, cu_q, cu_k, scale, causal, layout, True, True)
+        ctx.save_for_backward(q, k, v, out, lse, low, cu_q, cu_k)
         ctx.args = (scale, causal, layout)
         ctx.mark_non_differentiable(lse)
         return out, lse
@@ -179,7 +182,7 @@ def _apply(q, k, v, cu_q, cu_k, scale, causal, layout, return_lse):
         out, lse = ForgeAttentionFunction.apply(q, k, v, cu_q, cu_k, scale, bool(causal), layout is _Layout.packed)
     else:
         L.refuse_tangents(q, k, v)
-        out, lse = _forward(q, k, v, cu_q, cu_k, scale, bool(causal), layout, return_lse)
+        out, lse, _ = _forward(q, k, v, cu_q, cu_k, scale, bool(causal), layout, return_lse)
     return (out, lse) if return_lse else out
 
 

@@ -138,8 +138,8 @@ def test_entry_point_refusals():
 
     rows = [16, 0, 512, 64]
 
-    def fwd(dtype=2, q=rows, k=rows, v=rows, o=rows, cu=(16, 16), sizes=(1, 4, 4, 4, 2, 64), scale=0.1):
-        return L.forge_attention_fwd(dtype, *q, *k, *v, *o, None, *cu, *sizes, scale, 1, None, None)
+    def fwd(dtype=2, q=rows, k=rows, v=rows, o=rows, cu=(16, 16), sizes=(1, 4, 4, 4, 2, 64), scale=0.1, low=None):
+        return L.forge_attention_fwd(dtype, *q, *k, *v, *o, None, low, *cu, *sizes, scale, 1, None, None)
 
     assert fwd(dtype=0) == 2 and b"dtype" in L.forge_last_error()
     assert fwd(sizes=(1, 4, 4, 4, 2, 60)) == 2 and b"head_dim" in L.forge_last_error()
@@ -155,8 +155,18 @@ def test_entry_point_refusals():
         assert fwd(**{at: [24, 0, 512, 64]}) == 1 and b"aligned" in L.forge_last_error()
         assert fwd(**{at: [16, 0, 516, 64]}) == 1
         assert fwd(**{at: [16, 0, 1 << 23, 64]}) == 1 and b"stride" in L.forge_last_error()
-    assert L.forge_attention_bwd(2, *(rows * 5), None, *(rows * 3), 16, 16, 1, 4, 4, 4, 2, 64, 0.1, 1, 16, None) == 1
-    assert b"lse or work" in L.forge_last_error()
+    assert fwd(low=16) == 1 and fwd(dtype=1, low=24) == 1 and b"low" in L.forge_last_error()
+
+    def bwd(dtype=2, lse=16, low=None, work=16):
+        return L.forge_attention_bwd(dtype, *(rows * 5), lse, low, *(rows * 3), 16, 16, 1, 4, 4, 4, 2, 64, 0.1, 1, work, None)
+
+    assert bwd(lse=None) == 1 and b"lse or work" in L.forge_last_error()
+    assert bwd(work=None) == 1 and bwd(work=24) == 1
+    assert bwd(dtype=1) == 1 and bwd(dtype=1, low=24) == 1 and b"low" in L.forge_last_error()
+    assert L.forge_attention_bwd_workspace(1, 1, 4, 4, 4, 2, 64) == 4 * 4 * 2 * 4
+    # few keys, many heads: 16 parts of 300 keys
+    assert L.forge_attention_bwd_workspace(0, 1, 300, 300, 16, 1, 64) == 300 * 16 * 2 * 4 + 16 * 300 * 2 * 64 * 4
+    assert L.forge_attention_bwd_workspace(1, 1, 4, 4, 4, 3, 64) == -1
     assert L.forge_attention_fwd_workspace(1, 1, 4, 4, 4, 3, 64) == -1
     # nothing to do
     empty = [None, 0, 0, 0]
