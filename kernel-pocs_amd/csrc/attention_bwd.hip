@@ -10,6 +10,8 @@
 // times as large, and ds times a power of two from 2^14 down to 1, a wave's choice that
 // falls, with its sums, when one of its ds would pass fp16's largest value.  The sums
 // are taken back at the end.  All of that is exact.
+// 8 causal sequences of 16384 tokens, 32 heads of 128 on 8: 50 us (5.4 TB/s), 520 and 690
+// (both 950 TFLOP/s: matrix pipes and power, as in the forward).
 // As in the forward, products are laid out so that p and ds stay in the
 // registers that they are computed in: keys x queries for dq, queries x keys for
 // dk and dv.
@@ -403,7 +405,8 @@ __global__ __launch_bounds__(256) void attn_dkv_join_kernel(Args a, int64_t n_k)
   }
 }
 
-// Parts of a group's heads, a workgroup each: where the tiles of keys alone would
+// Parts of a group's heads, a workgroup each (13 sequences of 3001 tokens, 14 heads of 64
+// on 2: 80 workgroups 84 us, 480 33 and 5 for the join): where the tiles of keys alone would
 // leave CUs without work (two workgroups a CU are resident), and where a
 // workgroup has at least 16 tiles of queries to go through (a tile takes longer than
 // its share of the join).

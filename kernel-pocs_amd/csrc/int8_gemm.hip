@@ -7,7 +7,9 @@
 // The engines are those of the 16-bit products (gemm_w4.h, gemm_core.h,
 // gemm_rows.hip), which see two values as one 16-bit word: the matrix
 // instructions take as many bytes a lane in the same time, so a product runs in
-// the time of a 16-bit one of half the K, less what the epilogue adds.
+// the time of a 16-bit one of half the K, less what the epilogue adds.  [8192, 4096], K =
+// 14336 340 us (2830 TOP/s), [8192, 14336], K = 4096 390 (2470: its epilogue converts and writes
+// 235 MB); 16 rows by 28672, K = 4096 26 us (weights at 4.5 TB/s).
 #include "gemm_launch.h"
 
 namespace fgemm {
