@@ -241,6 +241,7 @@ extern "C" int forge_add_rmsnorm_bwd(int dtype, int w_dtype, const void* dy, int
   if (lddy < H || ldh < H || (dh && lddh < H)) return forge_set_error(FORGE_ERR_INVALID, "add_rmsnorm: row pitch below %lld", (long long)H);
   if (rows == 0 || H == 0) return FORGE_OK;  // (the caller clears dw)
   if (!dy || !h || !weight || !rstd || !d || (dw && !work)) return forge_set_error(FORGE_ERR_INVALID, "add_rmsnorm: an array is NULL");
+  if (dw && !aligned16(work)) return forge_set_error(FORGE_ERR_INVALID, "add_rmsnorm: work is not 16-byte aligned");
   BwdArgs a = {dy, lddy, dh, lddh, h, ldh, weight, w_dtype, rstd, d, (float*)work, part_pitch(H), rows, H, (float)offset};
   const BwdKernel k = dtype == FORGE_DTYPE_F32 ? pick_bwd<float>(H, dw, dh) : dtype == FORGE_DTYPE_F16 ? pick_bwd<fp16_t>(H, dw, dh) : pick_bwd<bf16_t>(H, dw, dh);
   const int64_t blocks = bwd_blocks(dtype, rows, H);

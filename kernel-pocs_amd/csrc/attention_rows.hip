@@ -291,7 +291,7 @@ int launch_rows(int dtype, const Args& a, int64_t n_queries, void* work, hipStre
   parts.C = chunk_keys(a, parts.n);
   const int64_t most = a.tk <= parts.C ? 1 : a.tk / parts.C + 1;
   if (most > 1) {
-    if (!work) return forge_set_error(FORGE_ERR_INVALID, "attention: work is NULL");
+    if (!work || !aligned16(work)) return forge_set_error(FORGE_ERR_INVALID, "attention: work is NULL or not aligned");
     parts.o = (float*)work;
     parts.m = parts.o + most * parts.n * a.D;
     parts.l = parts.m + most * parts.n;

@@ -263,3 +263,34 @@ def test_entry_point_refusals():
         assert bwd(**{n: None}) == 1, n
     assert L.forge_add_rmsnorm_bwd_workspace(2, 100, 64) == 25 * 64 * 4
     assert L.forge_add_rmsnorm_bwd_workspace(2, -1, 64) == -1
+
+
+@pytest.mark.gpu
+def test_gradients_are_tensors_of_their_own():
+    """x's and the residual's gradient are the same values: changing one's in place leaves the other's."""
+    from kernels.rmsnorm import add_rmsnorm
+
+    x, r, w = (torch.randn(*s, device="cuda").requires_grad_(True) for s in ((5, 64), (5, 64), (64,)))
+    y, h = add_rmsnorm(x, r, w)
+    (y.sum() + h.sum()).backward()
+    before = r.grad.clone()
+    assert torch.equal(x.grad, before)
+    x.grad.zero_()
+    assert torch.equal(r.grad, before)
+    # one tensor for both
+    x.grad = None
+    y, h = add_rmsnorm(x, x, w)
+    (y.sum() + h.sum()).backward()
+    d = x.grad.clone()
+    a, b = x.detach().clone().requires_grad_(True), x.detach().clone().requires_grad_(True)
+    y, h = add_rmsnorm(a, b, w)
+    (y.sum() + h.sum()).backward()
+    assert torch.equal(d, a.grad + b.grad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,H", [(FP32, 3), (BF16, 7), (FP16, 8), (FP32, 4), (BF16, 9), (BF16, 8191), (FP32, 8191), (BF16, 16377)])
+def test_rows_about_a_vector_and_about_each_kernel(dtype, H):
+    _check(37, H, dtype, dtype, pad=3)
+    x, res, w, _, _ = _make(37, H, dtype, dtype, 0.0, pad=3)
+    _check8(x, res, w, 0.0)

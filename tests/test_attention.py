@@ -155,6 +155,12 @@ def test_entry_point_refusals():
         assert fwd(**{at: [24, 0, 512, 64]}) == 1 and b"aligned" in L.forge_last_error()
         assert fwd(**{at: [16, 0, 516, 64]}) == 1
         assert fwd(**{at: [16, 0, 1 << 23, 64]}) == 1 and b"stride" in L.forge_last_error()
+    # 2049 keys of one sequence are read in chunks
+    assert L.forge_attention_fwd_workspace(1, 1, 1, 2049, 4, 2, 64) == (2049 // 128 + 1) * 4 * 66 * 4
+    long = (1, 1, 2049, 4, 2, 64)
+    args = [2, *rows, *rows, *rows, *rows, None, None, 16, 16, *long, 0.1, 1]
+    assert L.forge_attention_fwd(*args, None, None) == 1 and L.forge_attention_fwd(*args, 24, None) == 1
+    assert b"work" in L.forge_last_error()
     assert fwd(low=16) == 1 and fwd(dtype=1, low=24) == 1 and b"low" in L.forge_last_error()
 
     def bwd(dtype=2, lse=16, low=None, work=16):
@@ -406,3 +412,40 @@ def test_values_that_are_not_finite_where_they_are_not_seen(lens_q, lens_k, H, k
 def test_few_keys_and_many_heads(lens_q, lens_k, H, kv, D, dtype):
     """Gradients of keys whose heads go to several workgroups (heads that the parts do not divide)."""
     _check(lens_q, lens_k, H, kv, D, dtype, tail_q=3, tail_k=40)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_few_tokens_with_gradients_over_many_chunks(dtype):
+    """Long caches, whose chunks are joined, then trained through: 1 and 2 tokens, none, of 3000 keys and less."""
+    _check([1, 2, 0, 1], [3000, 1, 5, 700], 8, 2, 128, dtype, tail_q=1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("train", [False, True])
+def test_one_long_sequence_among_empty_ones(train):
+    """As many tokens as few a sequence would be, all of one sequence."""
+    lens = [0] * 40 + [150] + [0] * 39
+    _check(lens, lens, 4, 2, 64, BF16, train=train)
+
+
+@pytest.mark.gpu
+def test_expanded_keys_and_one_tensor_for_all():
+    """One key head expanded to four (stride 0), and q = k = v: gradients add up."""
+    from kernels.attention import forge_varlen_attention
+
+    g = torch.Generator().manual_seed(0)
+    q, one = torch.randn(90, 4, 64, generator=g).to(BF16), torch.randn(90, 1, 64, generator=g).to(BF16)
+    do = torch.randn(90, 4, 64, generator=g).to(BF16).cuda()
+    cu = torch.tensor([0, 50, 90], device="cuda", dtype=torch.int32)
+    qg, kg = q.cuda().requires_grad_(True), one.cuda().requires_grad_(True)
+    out = forge_varlen_attention(qg, kg.expand(-1, 4, -1), kg.expand(-1, 4, -1), cu)
+    want = forge_varlen_attention(qg, kg.repeat(1, 4, 1), kg.repeat(1, 4, 1), cu)
+    assert torch.equal(out, want)
+    for a, b in zip(torch.autograd.grad(out, (qg, kg), do), torch.autograd.grad(want, (qg, kg), do)):
+        assert (a.float() - b.float()).abs().max() <= 0.02 * b.float().abs().max()  # (8 roundings of parts as they are added)
+    same = q.cuda().requires_grad_(True)
+    (a,) = torch.autograd.grad(forge_varlen_attention(same, same, same, cu), same, do)
+    leaves = [q.cuda().requires_grad_(True) for _ in range(3)]
+    parts = torch.autograd.grad(forge_varlen_attention(*leaves, cu), leaves, do)
+    assert (a.float() - sum(p.float() for p in parts)).abs().max() <= 0.02 * a.float().abs().max()
