@@ -778,8 +778,8 @@ int forge_transpose_2b_batch(int n, const void* const* src, const int64_t* ld_sr
  * the batch strides are not used), 16-byte aligned, unit stride in D, row strides
  * below 2^23.  A query that sees no key has out = 0.  lse (fp32 [queries][H], or
  * NULL): the natural logarithm of the sum, -inf without keys.  low (int8
- * [queries][H][D], fp16 only, or NULL): for the gradients, what the rounding of
- * out took, in 254ths of a step.
+ * [queries][H][D], 16-byte aligned, or NULL): for the gradients, what the rounding
+ * of out took, in 254ths of a step.
  * work: forge_attention_fwd_workspace bytes, 16-byte aligned (0: may be NULL). */
 int64_t forge_attention_fwd_workspace(int varlen, int64_t B, int64_t tq, int64_t tk, int64_t H, int64_t Hkv,
                                       int64_t D);
@@ -790,8 +790,8 @@ int forge_attention_fwd(int dtype, const void* q, int64_t q_batch, int64_t q_row
                         const int32_t* cu_q, const int32_t* cu_k, int64_t B, int64_t tq, int64_t tk,
                         int64_t H, int64_t Hkv, int64_t D, float scale, int causal, void* work, void* stream);
 
-/* Gradients of q, k and v from that of out, with out, lse and (fp16) low as the
- * forward left them; dk and dv are summed over a group's heads.  Sums have a fixed
+/* Gradients of q, k and v from that of out, with out, lse and low as the forward
+ * left them; dk and dv are summed over a group's heads.  Sums have a fixed
  * order.  work: forge_attention_bwd_workspace bytes. */
 int64_t forge_attention_bwd_workspace(int varlen, int64_t B, int64_t tq, int64_t tk, int64_t H, int64_t Hkv, int64_t D);
 int forge_attention_bwd(int dtype, const void* dout, int64_t do_batch, int64_t do_row, int64_t do_head,

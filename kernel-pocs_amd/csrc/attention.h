@@ -43,7 +43,7 @@ struct Rows {  // [batch][row][head][D] with unit stride in D
 struct Args {
   Rows q, k, v, o, dout, dq, dk, dv;  // o: an output of the forward, an input of the backward
   float* lse;                         // [queries][H] natural logarithms
-  int8_t* low;                        // [queries][H][D], what the rounding of o to fp16 left, or NULL
+  int8_t* low;                        // [queries][H][D], what the rounding of o left, or NULL
   float* delta;                       // [queries][H], sum of o dout (backward)
   const int32_t* cu_q;
   const int32_t* cu_k;
@@ -394,20 +394,22 @@ __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d)
   *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(a, b), pack2<T>(c, d));
 }
 
-// What rounding x to fp16 took, in 254ths of a step of the rounded value r: delta =
-// sum o dout is formed of r + low (a sum over few of dout's signs else misses by a step of o,
-// which every ds of the row then has: a third of the error of dq and dk).  bf16 keeps
-// none: ds itself is rounded 8 times as coarsely there.
+// What rounding x took, in 254ths of a step of the rounded value r: delta = sum o dout
+// is formed of r + low.  (Of r alone it misses by roundings of o, and every ds of the
+// row then has that error: some 15% more in dq and dk, for a byte a value.)
+template <class T>
 __device__ __forceinline__ float low_step(float r) {
-  return fmaxf(__uint_as_float(__float_as_uint(r) & 0x7f800000u), 0x1p-14f) * (0x1p-10f / 254.f);
+  const float e = __uint_as_float(__float_as_uint(r) & 0x7f800000u);
+  return std::is_same_v<T, fp16_t> ? fmaxf(e, 0x1p-14f) * (0x1p-10f / 254.f) : fmaxf(e, 0x1p-100f) * (0x1p-7f / 254.f);
 }
+template <class T>
 __device__ __forceinline__ uint32_t low_byte(float x) {
-  const float r = to_f32((fp16_t)x);
-  return (uint32_t)(int)rintf(fminf(fmaxf((x - r) / low_step(r), -127.f), 127.f)) & 255u;
+  const float r = to_f32(from_f32<T>(x));
+  return (uint32_t)(int)rintf(fminf(fmaxf((x - r) / low_step<T>(r), -127.f), 127.f)) & 255u;
 }
 template <class T>
 __device__ __forceinline__ void store_low4(int8_t* p, float a, float b, float c, float d) {
-  *reinterpret_cast<uint32_t*>(p) = low_byte(a) | low_byte(b) << 8 | low_byte(c) << 16 | low_byte(d) << 24;
+  *reinterpret_cast<uint32_t*>(p) = low_byte<T>(a) | low_byte<T>(b) << 8 | low_byte<T>(c) << 16 | low_byte<T>(d) << 24;
 }
 
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }

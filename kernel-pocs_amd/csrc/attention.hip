@@ -87,7 +87,7 @@ extern "C" int forge_attention_fwd(int dtype, const void* q, int64_t q_batch, in
   a.o = {out, o_batch, o_row, o_head};
   a.lse = lse;
   a.low = low;
-  if (low && (dtype != FORGE_DTYPE_F16 || !aligned16(low))) return forge_set_error(FORGE_ERR_INVALID, "attention: low is kept of fp16 only, 16-byte aligned");
+  if (!aligned16(low)) return forge_set_error(FORGE_ERR_INVALID, "attention: low is not 16-byte aligned");
   const int64_t nb = cu_q ? 1 : B, n = nb * tq;
   if (int e = check_rows("q", a.q, nb, tq, H)) return e;
   if (int e = check_rows("k", a.k, nb, tk, Hkv)) return e;
@@ -142,8 +142,7 @@ extern "C" int forge_attention_bwd(int dtype, const void* dout, int64_t do_batch
   if (int e = check_rows("dq", a.dq, nb, tq, H)) return e;
   if (int e = check_rows("dk", a.dk, nb, tk, Hkv)) return e;
   if (int e = check_rows("dv", a.dv, nb, tk, Hkv)) return e;
-  if (n > 0 && (!lse || !work)) return forge_set_error(FORGE_ERR_INVALID, "attention: lse or work is NULL");
-  if (n > 0 && dtype == FORGE_DTYPE_F16 && !low) return forge_set_error(FORGE_ERR_INVALID, "attention: fp16 needs low");
+  if (n > 0 && (!lse || !low || !work)) return forge_set_error(FORGE_ERR_INVALID, "attention: lse, low or work is NULL");
   if (!aligned16(work) || !aligned16(low)) return forge_set_error(FORGE_ERR_INVALID, "attention: work or low is not aligned");
   a.delta = (float*)work;
   a.parts = n > 0 ? dkv_parts(a) : 1;

@@ -10,8 +10,8 @@
 // times as large, and ds times a power of two from 2^14 down to 1, a wave's choice that
 // falls, with its sums, when one of its ds would pass fp16's largest value.  The sums
 // are taken back at the end.  All of that is exact.
-// 8 causal sequences of 16384 tokens, 32 heads of 128 on 8: 50 us (5.4 TB/s), 520 and 690
-// (both 950 TFLOP/s: matrix pipes and power, as in the forward).
+// 8 causal sequences of 16384 tokens, 32 heads of 128 on 8: 62 us (5.4 TB/s), 510 and 680
+// (both 960 TFLOP/s: matrix pipes and power, as in the forward).
 // As in the forward, products are laid out so that p and ds stay in the
 // registers that they are computed in: keys x queries for dq, queries x keys for
 // dk and dv.
@@ -57,14 +57,11 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(Args a, float* shift, i
     float sum = 0.f;
     for (int c = 8 * (lane % 16); c < a.D; c += 128) {
       const Vec16<T> x = load16(o + c), y = load16(d + c);
-      uint2 low = make_uint2(0, 0);
-      if constexpr (std::is_same_v<T, fp16_t>) low = *reinterpret_cast<const uint2*>(a.low + p * a.D + c);
+      const uint2 low = *reinterpret_cast<const uint2*>(a.low + p * a.D + c);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        float f = to_f32(x.v[i]);
-        if constexpr (std::is_same_v<T, fp16_t>)
-          f = __builtin_fmaf((float)(int8_t)((i < 4 ? low.x : low.y) >> (8 * (i % 4))), low_step(f), f);
-        sum += f * to_f32(y.v[i]);
+        const float f = to_f32(x.v[i]);
+        sum += __builtin_fmaf((float)(int8_t)((i < 4 ? low.x : low.y) >> (8 * (i % 4))), low_step<T>(f), f) * to_f32(y.v[i]);
       }
     }
 #pragma unroll

@@ -170,10 +170,9 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a
       const int d = 32 * db + 8 * i + 4 * h;
       if (d >= a.D) continue;
       store4(op + d, o[db][4 * i] * inv, o[db][4 * i + 1] * inv, o[db][4 * i + 2] * inv, o[db][4 * i + 3] * inv);
-      if constexpr (std::is_same_v<T, fp16_t>)
-        if (a.low)
-          store_low4<T>(a.low + (row * a.H + head) * a.D + d, o[db][4 * i] * inv, o[db][4 * i + 1] * inv, o[db][4 * i + 2] * inv,
-                        o[db][4 * i + 3] * inv);
+      if (a.low)
+        store_low4<T>(a.low + (row * a.H + head) * a.D + d, o[db][4 * i] * inv, o[db][4 * i + 1] * inv, o[db][4 * i + 2] * inv,
+                      o[db][4 * i + 3] * inv);
     }
   if (h == 0 && a.lse) a.lse[row * a.H + head] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * LN2;
 }

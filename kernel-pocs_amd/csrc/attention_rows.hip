@@ -179,8 +179,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_rows_kernel(Args a, Parts par
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] *= inv;
         store4(row_ptr<T>(a.o, sq.batch, sq.start + t, hd) + d, v[0], v[1], v[2], v[3]);
-        if constexpr (std::is_same_v<T, fp16_t>)
-          if (a.low) store_low4<T>(a.low + (q * a.H + hd) * a.D + d, v[0], v[1], v[2], v[3]);
+        if (a.low) store_low4<T>(a.low + (q * a.H + hd) * a.D + d, v[0], v[1], v[2], v[3]);
         if (d == 0 && a.lse) a.lse[q * a.H + hd] = total == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(total)) * LN2;
       } else {
         const int64_t at_part = at.tile * parts.n + q * a.H + hd;
@@ -247,8 +246,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(Args a, Parts parts) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] *= inv;
     store4(op + 4 * lane, v[0], v[1], v[2], v[3]);
-    if constexpr (std::is_same_v<T, fp16_t>)
-      if (a.low) store_low4<T>(a.low + p * a.D + 4 * lane, v[0], v[1], v[2], v[3]);
+    if (a.low) store_low4<T>(a.low + p * a.D + 4 * lane, v[0], v[1], v[2], v[3]);
   }
   if (lane == 0 && a.lse) a.lse[p] = total == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(total)) * LN2;
 }

@@ -12,7 +12,9 @@ and no gradient.
 fp16 and bf16, head_dim a multiple of 8 up to 256, any number of heads on a
 divisor of it.  Products take 16-bit operands (the probabilities and, backward,
 their gradients are rounded to them) and sum in fp32; each result is rounded
-once.  Every sum has a fixed order, forward and backward.  Queries, keys and
+once.  Every sum has a fixed order, forward and backward.  A key or value that is
+not finite stays with the queries that see it; a query, or a gradient that comes
+in, that is not may also make gradients of the next keys (up to 63) NaN.  Queries, keys and
 values are read where they lie (columns of one projection's output, HF's
 transposed views); rows that are not 16-byte aligned are copied first.
 """
@@ -77,7 +79,7 @@ def _forward(q, k, v, cu_q, cu_k, scale, causal, layout, want_lse, train=False):
     out = _new(q.shape, q, layout)
     varlen = layout is _Layout.packed
     lse = low = None
-    if train and q.dtype == torch.float16:  # what out's rounding took, for the gradients
+    if train:  # what out's rounding took, for the gradients
         low = torch.empty(out.numel(), dtype=torch.int8, device=q.device)
     if want_lse:
         lse = torch.empty((q.shape[0], q.shape[1]) if varlen else (q.shape[0], q.shape[2], q.shape[1]),
@@ -117,8 +119,8 @@ def _backward(dout, q, k, v, out, lse, low, cu_q, cu_k, scale, causal, layout):
 class ForgeAttentionFunction(torch.autograd.Function):
     """forward(ctx, q, k, v, cu_q, cu_k, scale, causal, packed) -> (out, lse) on
     arguments that the entry points have checked and laid out; saves them with
-    out and lse (fp16: and a byte a value of what out's rounding took), and the
-    backward computes the probabilities again."""
+    out, lse and a byte a value of what out's rounding took, and the backward computes
+    the probabilities again."""
 
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, scale, causal, packed):

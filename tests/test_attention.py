@@ -161,14 +161,14 @@ def test_entry_point_refusals():
     args = [2, *rows, *rows, *rows, *rows, None, None, 16, 16, *long, 0.1, 1]
     assert L.forge_attention_fwd(*args, None, None) == 1 and L.forge_attention_fwd(*args, 24, None) == 1
     assert b"work" in L.forge_last_error()
-    assert fwd(low=16) == 1 and fwd(dtype=1, low=24) == 1 and b"low" in L.forge_last_error()
+    assert fwd(low=24) == 1 and b"low" in L.forge_last_error()
 
-    def bwd(dtype=2, lse=16, low=None, work=16):
+    def bwd(dtype=2, lse=16, low=16, work=16):
         return L.forge_attention_bwd(dtype, *(rows * 5), lse, low, *(rows * 3), 16, 16, 1, 4, 4, 4, 2, 64, 0.1, 1, work, None)
 
-    assert bwd(lse=None) == 1 and b"lse or work" in L.forge_last_error()
+    assert bwd(lse=None) == 1 and bwd(low=None) == 1 and b"lse, low or work" in L.forge_last_error()
     assert bwd(work=None) == 1 and bwd(work=24) == 1
-    assert bwd(dtype=1) == 1 and bwd(dtype=1, low=24) == 1 and b"low" in L.forge_last_error()
+    assert bwd(dtype=0) == 2 and bwd(low=24) == 1 and b"low" in L.forge_last_error()
     assert L.forge_attention_bwd_workspace(1, 1, 4, 4, 4, 2, 64) == 4 * 4 * 2 * 4
     # few keys, many heads: 16 parts of 300 keys
     assert L.forge_attention_bwd_workspace(0, 1, 300, 300, 16, 1, 64) == 300 * 16 * 2 * 4 + 16 * 300 * 2 * 64 * 4
