@@ -449,3 +449,43 @@ def test_expanded_keys_and_one_tensor_for_all():
     leaves = [q.cuda().requires_grad_(True) for _ in range(3)]
     parts = torch.autograd.grad(forge_varlen_attention(*leaves, cu), leaves, do)
     assert (a.float() - sum(p.float() for p in parts)).abs().max() <= 0.02 * a.float().abs().max()
+
+
+@pytest.mark.gpu
+def test_captured_gradients_of_few_keys():
+    """The pass whose heads go to several workgroups and are joined, captured and replayed with other values and
+    other lengths of the same total, an eager pass between: the same bits."""
+    from kernels.attention import forge_varlen_attention
+
+    g = torch.Generator().manual_seed(0)
+    q = torch.randn(600, 16, 64, generator=g).to(FP16).cuda().requires_grad_(True)
+    k, v = (torch.randn(600, 1, 64, generator=g).to(FP16).cuda().requires_grad_(True) for _ in range(2))
+    do = torch.randn(600, 16, 64, generator=g).to(FP16).cuda()
+    cu = torch.tensor([0, 200, 600], device="cuda", dtype=torch.int32)
+
+    def step():
+        out = forge_varlen_attention(q, k, v, cu)
+        grads = torch.autograd.grad(out, (q, k, v), do)
+        return (out.detach(), *grads)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static = step()
+    for i, at in enumerate(([0, 200, 600], [0, 1, 600], [0, 600, 600], [0, 300, 500])):
+        with torch.no_grad():
+            cu.copy_(torch.tensor(at, dtype=torch.int32))
+            for t in (q, k, v, do):
+                t.copy_(torch.randn(t.shape, generator=g).to(FP16))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in static]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b), f"replay {i}"
+        torch.cuda.synchronize()
