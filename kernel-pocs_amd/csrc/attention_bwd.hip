@@ -4,14 +4,14 @@
 //   dq_i = scale sum_j ds_ij k_j,       a workgroup to 128 queries of a head;
 //   dv_j = sum_i p_ij dout_i, dk_j = scale sum_i ds_ij q_i over the queries of the
 //   group's heads,                      a workgroup to 128 keys of a kv head,
-// with p_ij = exp2((s_ij - lse_i / scale) c), c = scale log2(e), computed again and ds_ij = p_ij (dout_i . v_j -
-// delta_i).  p and ds are rounded to 16 bits as operands; every sum is in fp32.
+// with p_ij = exp2((s_ij - lse_i / scale) c), c = scale log2(e), computed again and
+// ds_ij = p_ij (dout_i . v_j - delta_i).  p and ds are rounded to 16 bits as operands; every sum is in fp32.
 // fp16 has few small values (2^-14 is the last with 11 bits), so there p is 2^14
 // times as large, and ds times a power of two from 2^14 down to 1, a wave's choice that
 // falls, with its sums, when one of its ds would pass fp16's largest value.  The sums
 // are taken back at the end.  All of that is exact.
-// 8 causal sequences of 16384 tokens, 32 heads of 128 on 8: 62 us (5.4 TB/s), 510 and 680
-// (both 960 TFLOP/s: matrix pipes and power, as in the forward).
+// 8 causal sequences, 16384 tokens in all, 32 heads of 128 on 8: 62 us (5.4 TB/s),
+// 510 and 680 (both 960 TFLOP/s: matrix pipes and power, as in the forward).
 // As in the forward, products are laid out so that p and ds stay in the
 // registers that they are computed in: keys x queries for dq, queries x keys for
 // dk and dv.

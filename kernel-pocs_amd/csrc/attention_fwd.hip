@@ -11,7 +11,7 @@
 // the rounding of the result.
 //
 // A workgroup of 4 waves takes 128 queries of one head, 32 a wave; tiles of 64
-// keys and values come by LDS-DMA into a ring of two.  8 causal sequences of 16384
+// keys and values come by LDS-DMA into a ring of two.  8 causal sequences, 16384
 // tokens, 32 heads of 128 on 8: 390 to 410 us, 820 TFLOP/s.  The matrix pipes set
 // the time, with the power they leave (1150 where the data are zeros); 8 waves to
 // 256 queries, or 64 queries a wave, were slower (870 and 754 where this ran 890).
