@@ -827,7 +827,7 @@ int forge_add_rmsnorm_int8(int dtype, int w_dtype, const void* x, int64_t ldx, c
                            const void* weight, void* h, int8_t* q, int64_t ldq, float* scale, int64_t rows,
                            int64_t H, double eps, double offset, void* stream);
 
-/* d = dh + rstd g - h rstd^3 mean(g h), g = dy (weight + offset): the gradient of x and of
+/* d = dh + rstd (g - h rstd (rstd mean(g h))), g = dy (weight + offset): the gradient of x and of
  * the residual, from those of y and h (dh may be NULL); dw = sum over rows of dy h
  * rstd in a fixed order, of the weight's type (dw NULL: not formed; with rows == 0 it is
  * not written).  work: forge_add_rmsnorm_bwd_workspace bytes for dw. */

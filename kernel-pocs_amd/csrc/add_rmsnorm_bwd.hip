@@ -1,6 +1,8 @@
 // Backward of the RMS norm with the residual's addition:
-//   g = dy (w + offset),  d = dh + rstd g - h rstd^3 mean(g h)   (x's and the residual's)
+//   g = dy (w + offset),  d = dh + rstd (g - h rstd (rstd mean(g h)))   (x's and the residual's)
 //   dw = sum over rows of dy h rstd
+// (multiplied in this order: rstd^3 itself is infinite for rows of 1e-13, and a
+// subnormal for those of 1e13 and more)
 // with dh the gradient that reaches h by the residual stream.  Reads dy, dh and h
 // and writes d once.  A workgroup adds its rows' dw in registers (thread t its
 // own columns) and writes one partial row; a second launch adds those in order.
@@ -89,12 +91,12 @@ __global__ __launch_bounds__(threads_of<TPR>) void add_rmsnorm_bwd_kernel(BwdArg
     }
     dot = row_sum<TPR>(dot, sums[flip]);
     if (!on) return;
-    const float rstd = NV > 0 ? s.rstd : a.rstd[row], k = rstd * rstd * rstd * dot * inv_h;
+    const float rstd = NV > 0 ? s.rstd : a.rstd[row], k = rstd * (rstd * dot * inv_h);
     auto finish = [&](const Vec<T>& x, const Vec<T>& y, const Vec<T>& g, const float (&wv)[VN], int vec) {
       Vec<T> d;
       float f[VN];
 #pragma unroll
-      for (int i = 0; i < VN; ++i) f[i] = g.get(i) + (rstd * (y.get(i) * wv[i]) - x.get(i) * k);
+      for (int i = 0; i < VN; ++i) f[i] = g.get(i) + rstd * (y.get(i) * wv[i] - x.get(i) * k);
       d.set(f);
       const int c = vec * VN;
       store_part((T*)a.d + row * a.H + c, d, (int)min((int64_t)VN, a.H - c));

@@ -294,3 +294,22 @@ def test_rows_about_a_vector_and_about_each_kernel(dtype, H):
     _check(37, H, dtype, dtype, pad=3)
     x, res, w, _, _ = _make(37, H, dtype, dtype, 0.0, pad=3)
     _check8(x, res, w, 0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("H", [3, 520, 2305, 20001])
+@pytest.mark.parametrize("size,eps", [(1e-16, 0.0), (1e-13, 0.0), (1e13, 1e-6), (1e15, 1e-6), (1e16, 1e-6)])
+def test_gradients_of_rows_of_any_size(size, eps, H, dtype):
+    """Rows whose rstd has no cube in fp32 (rstd 1e13: infinite, 1e-15: a subnormal of one bit)."""
+    from kernels.rmsnorm import add_rmsnorm
+
+    x, res, w, dy, _ = _make(5, H, dtype, dtype, 0.0, seed=H)
+    x, res = ((t.double() * size).to(dtype) for t in (x, res))
+    ref = fwd_bwd(x, res, w, dy, None, eps, 0.0)
+    leaves = [t.cuda().requires_grad_(True) for t in (x, res, w)]
+    got = torch.autograd.grad(add_rmsnorm(*leaves, eps=eps)[0], leaves, dy.cuda())
+    k = 400 if H > 4096 else 100
+    for t in got[:2]:
+        _within(t, ref.d, ref.d_terms, 2 * k, "d")
+    _within(got[2], ref.dw, ref.dw_terms, 181, "dw")
