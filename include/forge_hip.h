@@ -822,7 +822,7 @@ int forge_add_rmsnorm_fwd(int dtype, int w_dtype, const void* x, int64_t ldx, co
 /* The same with y in 8 bits: with t = h (weight + offset) and a = max |t| of a row, q =
  * round_half_even(127 t / a) of exact arithmetic and scale = a rstd / 127, y = q scale.
  * q [rows][ldq], 16-byte aligned, ldq >= H a multiple of 16, zeros behind H.  A row
- * with an infinity or NaN: scale NaN. */
+ * with an infinity or NaN, or whose t passes fp32's largest value: scale NaN. */
 int forge_add_rmsnorm_int8(int dtype, int w_dtype, const void* x, int64_t ldx, const void* residual, int64_t ldr,
                            const void* weight, void* h, int8_t* q, int64_t ldq, float* scale, int64_t rows,
                            int64_t H, double eps, double offset, void* stream);

@@ -200,7 +200,9 @@ __global__ __launch_bounds__(threads_of<TPR>) void add_rmsnorm_kernel(FwdArgs a)
         below = __uint_as_float(inv - (WIDE ? 6 : 1));
         above = __uint_as_float(inv + (WIDE ? 6 : 1));
       }
-      if (tid == 0) a.scale[row] = bad ? __builtin_nanf("") : (float)top64 * rstd / 127.f;
+      // (a rstd may pass fp32's range where a rstd / 127 does not)
+      if (tid == 0)
+        a.scale[row] = bad ? __builtin_nanf("") : SUMS ? (float)(top64 * (double)rstd / 127.0) : (float)top64 / 127.f;
     }
     auto write = [&](const Vec<T>& v, const float* wv, int vec) {
       const int c = vec * VN;

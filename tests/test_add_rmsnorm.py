@@ -313,3 +313,13 @@ def test_gradients_of_rows_of_any_size(size, eps, H, dtype):
     for t in got[:2]:
         _within(t, ref.d, ref.d_terms, 2 * k, "d")
     _within(got[2], ref.dw, ref.dw_terms, 181, "dw")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e30, 1e36, 1e38])
+@pytest.mark.parametrize("H", [64, 5001])
+def test_int8_scales_of_large_weights(size, H):
+    """a rstd / 127 is finite where a rstd is not."""
+    x = torch.full((3, H), 1e-3)
+    x[:, :2] = torch.tensor([1.0, -0.5])
+    _check8(x, None, torch.full((H,), size), 0.0)
