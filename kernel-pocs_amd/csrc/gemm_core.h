@@ -455,9 +455,19 @@ __device__ __forceinline__ void tile_coords(int64_t tiles_m, int64_t tiles_n, in
   tn = (int)(in / gm);
 }
 
-// An accumulator of 8-bit products to its value in C.
-__device__ __forceinline__ float scale_i8(int acc, float row, float col, float bias) {
+// An accumulator of 8-bit products to its value in C: the sum rounded to fp32, times the
+// row's scale, times the column's plus the bias, each rounded.  The sum (below 2^31) times
+// a row's scale above 2^96 may pass fp32's range where the value does not; from
+// FAR_SCALE on the column's comes first, which with such a row passes it only where the
+// value does too.  (A product below the range is a multiple of its smallest step, and
+// exact.)
+constexpr float FAR_SCALE = 0x1p90f;
+__device__ __forceinline__ float scale_i8_near(int acc, float row, float col, float bias) {
   return __builtin_fmaf((float)acc * row, col, bias);
+}
+__device__ __forceinline__ float scale_i8(int acc, float row, float col, float bias) {
+  const bool far = row > FAR_SCALE;
+  return scale_i8_near(acc, far ? col : row, far ? row : col, bias);
 }
 template <class O>
 __device__ __forceinline__ float bias_i8(const EpiArgs& ep, int64_t n) {

@@ -230,3 +230,44 @@ def test_entry_point_refusals():
     assert L.forge_transpose_1b(None, 8, 4, 8, 16, 16, None) == 1
     assert L.forge_transpose_1b(16, 7, 4, 8, 16, 16, None) == 1
     assert L.forge_quantize_rows(2, 16, 8, None, 16, 8, 16, 2, 8, None) == 1
+
+
+# sizes of each engine: rows, tiles in parts of K, both kinds of tiles, large tiles with and without aligned rows
+_ENGINES = [(4, 64, 64), (50, 1024, 512), (100, 1024, 4096), (333, 257, 130), (1000, 4096, 128), (2600, 3000, 300),
+            (2600, 3001, 48)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,out_dtype", [(BF16, BF16), (FP32, FP32), (FP32, FP16)])
+@pytest.mark.parametrize("m,n,k", _ENGINES)
+def test_sums_times_one_scale_past_the_largest_value(m, n, k, dtype, out_dtype):
+    """Rows of 1e35 and weights of 1e-33, rows of 1e-30 and weights of 1e30 beside rows of usual size: the products
+    of the integers and one of the scales are past fp32's range, or below it, and the results are not."""
+    from kernels.int8 import Int8Weight, int8_linear
+
+    g = torch.Generator().manual_seed(m)
+    rows = torch.ones(m, 1)
+    w, ws = _weight(n, k)
+    for large in (True, False):
+        rows[::3] = 1e35 if large else 1e-30
+        x = (torch.randn(m, k, generator=g) * rows).to(dtype)
+        scale = ws * (1e-33 if large else 1e30)
+        if not large:
+            x[1::3], x[2::3] = x[1::3] * 1e-29, x[2::3] * 0
+        b = torch.randn(n, generator=g).to(out_dtype)
+        ref, terms = linear(*quantize(x), w, scale, b)
+        y = int8_linear(x.cuda(), Int8Weight(w.cuda(), scale.cuda()), b.cuda(), out_dtype=out_dtype)
+        if out_dtype == FP16:  # (what passes the type's own largest value is infinite)
+            over = ref.abs() >= 65520
+            near = (ref.abs() - 65520).abs() < 1
+            assert torch.equal(torch.isinf(y.cpu())[~near], over[~near])
+            y, ref, terms = y.cpu()[~over & ~near], ref[~over & ~near], terms[~over & ~near]
+        _within(y, ref, terms, 6, "y")
+    # scales that are not finite, and products of 0 with a large scale
+    x = torch.randn(m, k, generator=g)
+    x[0] = 3e38
+    scale = ws.clone()
+    scale[0], scale[-1] = 3e38, float("nan")
+    w[0] = 0
+    y = int8_linear(x.cuda(), Int8Weight(w.cuda(), scale.cuda()), out_dtype=FP32)
+    assert bool(y[:, -1].isnan().all()) and (n == 1 or bool((y[:, 0] == 0).all()))
