@@ -100,7 +100,7 @@ def quantize_int8_rows(x: torch.Tensor) -> Int8Rows:
 
 class Int8Weight:
     """A frozen weight [N, K] of 8-bit integers with a scale for each of its N channels,
-    laid out for the kernels (a copy).  backward: also its transpose, which the
+    laid out for the kernels (a copy of both).  backward: also its transpose, which the
     gradient of the activations reads."""
 
     def __init__(self, values: torch.Tensor, scale: torch.Tensor, *, backward: bool = False):
@@ -117,10 +117,10 @@ class Int8Weight:
         self.shape = values.shape
         self.padded = torch.zeros(n, _pitch(k), dtype=torch.int8, device=values.device)
         self.padded[:, :k] = values
-        self._finish(scale, backward)
+        self._finish(scale.detach().clone(memory_format=torch.contiguous_format), backward)
 
     def _finish(self, scale, backward):
-        self.scale = scale.detach().contiguous()
+        self.scale = scale
         self.transposed = None
         if backward:
             n, k = self.shape

@@ -271,3 +271,21 @@ def test_sums_times_one_scale_past_the_largest_value(m, n, k, dtype, out_dtype):
     w[0] = 0
     y = int8_linear(x.cuda(), Int8Weight(w.cuda(), scale.cuda()), out_dtype=FP32)
     assert bool(y[:, -1].isnan().all()) and (n == 1 or bool((y[:, 0] == 0).all()))
+
+
+@pytest.mark.gpu
+def test_a_weight_is_a_copy():
+    """Values and scales that are changed in place afterwards, also between a forward and its backward."""
+    from kernels.int8 import Int8Weight, int8_linear
+
+    w, ws = (t.cuda() for t in _weight(40, 64))
+    for scale in (ws, torch.stack([ws, ws], 1)[:, 0]):  # contiguous or not
+        values, scale = w.clone(), scale.clone() if scale.is_contiguous() else scale
+        weight = Int8Weight(values, scale, backward=True)
+        x = torch.randn(3, 64, device="cuda", requires_grad=True)
+        y = int8_linear(x, weight)
+        (dx,) = torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)
+        values.zero_()
+        scale.zero_()
+        assert torch.equal(int8_linear(x, weight), y)
+        assert torch.equal(torch.autograd.grad(y, x, torch.ones_like(y))[0], dx)
