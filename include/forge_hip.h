@@ -844,12 +844,15 @@ int forge_quantize_rows(int dtype, const void* x, int64_t ldx, const float* col_
 /* C[m, n] = (sum_k a[m, k] b[n, k]) row_scale[m] col_scale[n] + bias[n]: the sum exact in
  * 32-bit integers (K up to 2^17), C (fp32, bf16 or fp16, pitch ldc) rounded once.  a
  * [M][lda], b [N][ldb]: 16-byte aligned, pitches multiples of 16 below 2^22, zeros from K
- * to the next multiple of 16.  bias: C's type, or NULL.  work: forge_int8_gemm_workspace
- * bytes, 16-byte aligned (0: may be NULL). */
+ * to the next multiple of 16.  bias: C's type (_typed: fp32, bf16 or fp16), or NULL.  work:
+ * forge_int8_gemm_workspace bytes, 16-byte aligned (0: may be NULL). */
 int64_t forge_int8_gemm_workspace(int64_t M, int64_t N, int64_t K);
 int forge_int8_gemm(const int8_t* a, int64_t lda, const float* row_scale, const int8_t* b, int64_t ldb,
                     const float* col_scale, const void* bias, void* c, int64_t ldc, int c_dtype, int64_t M,
                     int64_t N, int64_t K, void* work, void* stream);
+int forge_int8_gemm_typed(const int8_t* a, int64_t lda, const float* row_scale, const int8_t* b, int64_t ldb,
+                          const float* col_scale, const void* bias, int bias_dtype, void* c, int64_t ldc,
+                          int c_dtype, int64_t M, int64_t N, int64_t K, void* work, void* stream);
 
 /* forge_quantize_rows and forge_int8_gemm of the result in one call: C = x w^T with
  * the rows of x (times x_col_scale, or NULL) in 8 bits.  work:
@@ -858,6 +861,9 @@ int64_t forge_int8_linear_workspace(int64_t M, int64_t N, int64_t K);
 int forge_int8_linear(int x_dtype, const void* x, int64_t ldx, const float* x_col_scale, const int8_t* w,
                       int64_t ldw, const float* w_scale, const void* bias, void* c, int64_t ldc, int c_dtype,
                       int64_t M, int64_t N, int64_t K, void* work, void* stream);
+int forge_int8_linear_typed(int x_dtype, const void* x, int64_t ldx, const float* x_col_scale, const int8_t* w,
+                            int64_t ldw, const float* w_scale, const void* bias, int bias_dtype, void* c,
+                            int64_t ldc, int c_dtype, int64_t M, int64_t N, int64_t K, void* work, void* stream);
 
 /* dst[c, r] = src[r, c] of 8-bit values, zeros in dst's columns from `rows` to ld_dst. */
 int forge_transpose_1b(const int8_t* src, int64_t ld_src, int64_t rows, int64_t cols, int8_t* dst, int64_t ld_dst,

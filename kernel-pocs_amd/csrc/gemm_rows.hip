@@ -124,7 +124,7 @@ __global__ __launch_bounds__(NW * 64) void gemm_rows_kernel(GemmArgs args) {
       if constexpr (OutOf<T>::i8) {
         typedef out_t<T> O;
         ((O*)ep.c)[m * ep.ldc + n + q] =
-            from_f32<O>(scale_i8(v[0][q], ep.row_scale[m], ep.col_scale[n + q], bias_i8<O>(ep, n + q)));
+            from_f32<O>(scale_i8(v[0][q], ep.row_scale[m], ep.col_scale[n + q], bias_i8(ep, n + q)));
       } else if constexpr (ND == 2) {
         const float e = v[0][q], g = v[1][q];
         if (ep.e) {

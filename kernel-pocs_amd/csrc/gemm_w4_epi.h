@@ -804,7 +804,7 @@ __device__ __forceinline__ void w4_epilogue_i8(const GemmArgs& args, const i32x4
   const int tid = threadIdx.x, cl = 4 * (lane / 16);
   float* scales = reinterpret_cast<float*>(smem + W4_SCALES);
   const int64_t sm = min(m0 + tid, M - 1), sn = min(n0 + tid, N - 1);
-  const float row_scale = ep.row_scale[sm], col_scale = ep.col_scale[sn], col_bias = bias_i8<O>(ep, sn);
+  const float row_scale = ep.row_scale[sm], col_scale = ep.col_scale[sn], col_bias = bias_i8(ep, sn);
   // A tile with a scale from FAR_SCALE on: 2^26 goes from the rows' scales to the columns',
   // so that no sum times a row's passes fp32's range (a column's that would is the largest
   // value: with such a row C is infinite all the same, or 0).  Of rows below 2^-100 in

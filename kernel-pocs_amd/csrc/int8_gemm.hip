@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256) void join_i8_kernel(const int* parts, int64_t 
   const float row = ep.row_scale[m];
 #pragma unroll
   for (int q = 0; q < 4; ++q)
-    if (c + q < N) ((O*)ep.c)[m * ep.ldc + c + q] = from_f32<O>(scale_i8(sum[q], row, ep.col_scale[c + q], bias_i8<O>(ep, c + q)));
+    if (c + q < N) ((O*)ep.c)[m * ep.ldc + c + q] = from_f32<O>(scale_i8(sum[q], row, ep.col_scale[c + q], bias_i8(ep, c + q)));
 }
 
 template <class O>
@@ -107,13 +107,19 @@ extern "C" int64_t forge_int8_gemm_workspace(int64_t M, int64_t N, int64_t K) {
   return p.split > 1 ? p.split * M * part_pitch(N) * 4 : 0;
 }
 
-extern "C" int forge_int8_gemm(const int8_t* a, int64_t lda, const float* row_scale, const int8_t* b, int64_t ldb,
-                               const float* col_scale, const void* bias, void* c, int64_t ldc, int c_dtype, int64_t M,
-                               int64_t N, int64_t K, void* work, void* stream) {
+static int check_types(const char* what, int c_dtype, const void* bias, int bias_dtype) {
+  auto known = [](int t) { return t == FORGE_DTYPE_F32 || t == FORGE_DTYPE_F16 || t == FORGE_DTYPE_BF16; };
+  if (!known(c_dtype)) return forge_set_error(FORGE_ERR_UNSUPPORTED, "%s: C dtype %d", what, c_dtype);
+  if (bias && !known(bias_dtype)) return forge_set_error(FORGE_ERR_UNSUPPORTED, "%s: bias dtype %d", what, bias_dtype);
+  return FORGE_OK;
+}
+
+extern "C" int forge_int8_gemm_typed(const int8_t* a, int64_t lda, const float* row_scale, const int8_t* b, int64_t ldb,
+                                     const float* col_scale, const void* bias, int bias_dtype, void* c, int64_t ldc,
+                                     int c_dtype, int64_t M, int64_t N, int64_t K, void* work, void* stream) {
   if (M < 0 || N < 0 || K < 0 || K > (int64_t(1) << 17))
     return forge_set_error(FORGE_ERR_INVALID, "int8_gemm: sizes (K up to 2^17, where a sum fits 32 bits)");
-  if (c_dtype != FORGE_DTYPE_F32 && c_dtype != FORGE_DTYPE_F16 && c_dtype != FORGE_DTYPE_BF16)
-    return forge_set_error(FORGE_ERR_UNSUPPORTED, "int8_gemm: C dtype %d", c_dtype);
+  if (int e = check_types("int8_gemm", c_dtype, bias, bias_dtype)) return e;
   if (M == 0 || N == 0) return FORGE_OK;
   const int64_t kp = (K + 15) / 16 * 16;
   if (!row_scale || !col_scale || !c || (K > 0 && (!a || !b))) return forge_set_error(FORGE_ERR_INVALID, "int8_gemm: an array is NULL");
@@ -138,6 +144,7 @@ extern "C" int forge_int8_gemm(const int8_t* a, int64_t lda, const float* row_sc
   g.ep.row_scale = row_scale;
   g.ep.col_scale = col_scale;
   g.ep.bias = bias;
+  g.ep.bias_dtype = bias_dtype;
   g.ep.vec_ok = aligned16(c) && ldc % 8 == 0;
   const Plan p = plan_i8(M, N, kp);
   if (p.split > 1 && (!work || !aligned16(work))) return forge_set_error(FORGE_ERR_INVALID, "int8_gemm: work is NULL or not aligned");
@@ -145,6 +152,12 @@ extern "C" int forge_int8_gemm(const int8_t* a, int64_t lda, const float* row_sc
   if (c_dtype == FORGE_DTYPE_F32) return launch_i8<float>(c_dtype, g, p, (int*)work, s);
   if (c_dtype == FORGE_DTYPE_F16) return launch_i8<fp16_t>(c_dtype, g, p, (int*)work, s);
   return launch_i8<bf16_t>(c_dtype, g, p, (int*)work, s);
+}
+
+extern "C" int forge_int8_gemm(const int8_t* a, int64_t lda, const float* row_scale, const int8_t* b, int64_t ldb,
+                               const float* col_scale, const void* bias, void* c, int64_t ldc, int c_dtype, int64_t M,
+                               int64_t N, int64_t K, void* work, void* stream) {
+  return forge_int8_gemm_typed(a, lda, row_scale, b, ldb, col_scale, bias, c_dtype, c, ldc, c_dtype, M, N, K, work, stream);
 }
 
 // The rows of x in 8 bits and their product in one call: work holds the integers,
@@ -156,10 +169,11 @@ extern "C" int64_t forge_int8_linear_workspace(int64_t M, int64_t N, int64_t K) 
   return own < 0 ? -1 : rows8_bytes(M, (K + 15) / 16 * 16) + own;
 }
 
-extern "C" int forge_int8_linear(int x_dtype, const void* x, int64_t ldx, const float* x_col_scale, const int8_t* w, int64_t ldw,
-                                 const float* w_scale, const void* bias, void* c, int64_t ldc, int c_dtype, int64_t M, int64_t N,
-                                 int64_t K, void* work, void* stream) {
+extern "C" int forge_int8_linear_typed(int x_dtype, const void* x, int64_t ldx, const float* x_col_scale, const int8_t* w,
+                                       int64_t ldw, const float* w_scale, const void* bias, int bias_dtype, void* c, int64_t ldc,
+                                       int c_dtype, int64_t M, int64_t N, int64_t K, void* work, void* stream) {
   if (M < 0 || N < 0 || K < 0) return forge_set_error(FORGE_ERR_INVALID, "int8_linear: sizes");
+  if (int e = check_types("int8_linear", c_dtype, bias, bias_dtype)) return e;
   if (M == 0 || N == 0) return FORGE_OK;
   if (!work || !aligned16(work)) return forge_set_error(FORGE_ERR_INVALID, "int8_linear: work is NULL or not aligned");
   const int64_t kp = (K + 15) / 16 * 16;
@@ -170,7 +184,14 @@ extern "C" int forge_int8_linear(int x_dtype, const void* x, int64_t ldx, const 
     if (int e = forge_quantize_rows(x_dtype, x, ldx, x_col_scale, q, kp, scale, M, K, stream)) return e;
   if (K == 0)
     if (int e = forge_zero(scale, M * 4, stream)) return e;
-  return forge_int8_gemm(q, kp, scale, w, ldw, w_scale, bias, c, ldc, c_dtype, M, N, K, q + rows8_bytes(M, kp), stream);
+  return forge_int8_gemm_typed(q, kp, scale, w, ldw, w_scale, bias, bias_dtype, c, ldc, c_dtype, M, N, K, q + rows8_bytes(M, kp),
+                               stream);
+}
+
+extern "C" int forge_int8_linear(int x_dtype, const void* x, int64_t ldx, const float* x_col_scale, const int8_t* w, int64_t ldw,
+                                 const float* w_scale, const void* bias, void* c, int64_t ldc, int c_dtype, int64_t M, int64_t N,
+                                 int64_t K, void* work, void* stream) {
+  return forge_int8_linear_typed(x_dtype, x, ldx, x_col_scale, w, ldw, w_scale, bias, c_dtype, c, ldc, c_dtype, M, N, K, work, stream);
 }
 
 // dst[c][r] = src[r][c] of 8-bit values, 64 x 64 tiles through LDS, zeros in the

@@ -251,11 +251,17 @@ forge_add_rmsnorm_bwd = _decl(
 forge_quantize_rows = _decl("forge_quantize_rows", [c_int, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_vp])
 forge_int8_gemm = _decl(
     "forge_int8_gemm", [c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_int] + [c_i64] * 3 + [c_vp, c_vp])
+forge_int8_gemm_typed = _decl(
+    "forge_int8_gemm_typed",
+    [c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_int, c_vp, c_i64, c_int] + [c_i64] * 3 + [c_vp, c_vp])
 forge_int8_gemm_workspace = _decl("forge_int8_gemm_workspace", [c_i64] * 3, c_i64)
 forge_int8_linear_workspace = _decl("forge_int8_linear_workspace", [c_i64] * 3, c_i64)
 forge_int8_linear = _decl(
     "forge_int8_linear",
     [c_int, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_int] + [c_i64] * 3 + [c_vp, c_vp])
+forge_int8_linear_typed = _decl(
+    "forge_int8_linear_typed",
+    [c_int, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_vp, c_int, c_vp, c_i64, c_int] + [c_i64] * 3 + [c_vp, c_vp])
 forge_transpose_1b = _decl("forge_transpose_1b", [c_vp] + [c_i64] * 3 + [c_vp, c_i64, c_vp])
 
 # Every symbol include/forge_hip.h declares (checked by the CPU test suite).
@@ -275,7 +281,7 @@ EXPORTED = [
     "forge_rmsnorm_fwd", "forge_rmsnorm_bwd", "forge_rmsnorm_bwd_workspace",
     "forge_attention_fwd", "forge_attention_fwd_workspace", "forge_attention_bwd", "forge_attention_bwd_workspace",
     "forge_add_rmsnorm_fwd", "forge_add_rmsnorm_int8", "forge_add_rmsnorm_bwd", "forge_add_rmsnorm_bwd_workspace",
-    "forge_quantize_rows", "forge_int8_gemm", "forge_int8_gemm_workspace", "forge_int8_linear",
+    "forge_quantize_rows", "forge_int8_gemm", "forge_int8_gemm_workspace", "forge_int8_linear", "forge_int8_gemm_typed", "forge_int8_linear_typed",
     "forge_int8_linear_workspace", "forge_transpose_1b",
 ]
 

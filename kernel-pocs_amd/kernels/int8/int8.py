@@ -152,15 +152,20 @@ class Int8Weight:
         return self.values.float() * self.scale.unsqueeze(1)
 
 
+def _bias_code(bias):
+    return 0 if bias is None else L.dtype_code(bias.dtype)
+
+
 def _product(q, scale, w, w_scale, bias, dtype, n, k):
     out = torch.empty(q.shape[0], n, dtype=dtype, device=q.device)
     if out.numel():
         nbytes = L.forge_int8_gemm_workspace(q.shape[0], n, k)
         work = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
         with L.on_device(q):
-            L.check(L.forge_int8_gemm(q.data_ptr(), q.shape[1], scale.data_ptr(), w.data_ptr(), w.shape[1],
-                                      w_scale.data_ptr(), L.ptr(bias), out.data_ptr(), n, L.dtype_code(dtype), q.shape[0],
-                                      n, k, L.ptr(work), L.stream_of(q)), "forge_int8_gemm")
+            L.check(L.forge_int8_gemm_typed(q.data_ptr(), q.shape[1], scale.data_ptr(), w.data_ptr(), w.shape[1],
+                                            w_scale.data_ptr(), L.ptr(bias), _bias_code(bias), out.data_ptr(), n,
+                                            L.dtype_code(dtype), q.shape[0], n, k, L.ptr(work), L.stream_of(q)),
+                    "forge_int8_gemm")
     return out
 
 
@@ -171,9 +176,9 @@ def _linear(x2, col_scale, w, w_scale, bias, dtype, n, k):
     if rows and n:
         work = torch.empty(L.forge_int8_linear_workspace(rows, n, k), dtype=torch.uint8, device=device)
         with L.on_device(x2):
-            L.check(L.forge_int8_linear(L.dtype_code(x2.dtype), x2.data_ptr(), _ld(x2), L.ptr(col_scale), w.data_ptr(),
-                                        w.shape[1], w_scale.data_ptr(), L.ptr(bias), out.data_ptr(), n,
-                                        L.dtype_code(dtype), rows, n, k, work.data_ptr(), L.stream_of(x2)),
+            L.check(L.forge_int8_linear_typed(L.dtype_code(x2.dtype), x2.data_ptr(), _ld(x2), L.ptr(col_scale), w.data_ptr(),
+                                              w.shape[1], w_scale.data_ptr(), L.ptr(bias), _bias_code(bias), out.data_ptr(),
+                                              n, L.dtype_code(dtype), rows, n, k, work.data_ptr(), L.stream_of(x2)),
                     "forge_int8_linear")
     return out
 
@@ -199,6 +204,7 @@ class Int8LinearFunction(torch.autograd.Function):
 def int8_linear(x: Union[torch.Tensor, Int8Rows], weight: Int8Weight, bias: Optional[torch.Tensor] = None, *,
                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """x [..., K] times weight [N, K], plus bias [N]: [..., N] in out_dtype (default x's type).
+    The bias is added in fp32, whatever its type.
 
     x in fp16, bf16 or fp32 is rounded to 8 bits by rows; Int8Rows
     (quantize_int8_rows, add_rmsnorm_int8) are taken as they are.  A gradient of x
@@ -223,7 +229,7 @@ def int8_linear(x: Union[torch.Tensor, Int8Rows], weight: Int8Weight, bias: Opti
         if torch.is_grad_enabled() and bias.requires_grad:
             raise ValueError("the bias of an int8_linear is frozen; add a trained one to the result")
         L.refuse_tangents(bias)
-        bias = bias.to(dtype).contiguous()
+        bias = (bias if bias.dtype in _DTYPES else bias.float()).contiguous()
     if ready:
         return _product(x.padded, x.scale, weight.padded, weight.scale, bias, dtype, n, k).view(*x.shape[:-1], n)
     if torch.is_grad_enabled() and x.requires_grad:

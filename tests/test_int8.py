@@ -289,3 +289,37 @@ def test_a_weight_is_a_copy():
         scale.zero_()
         assert torch.equal(int8_linear(x, weight), y)
         assert torch.equal(torch.autograd.grad(y, x, torch.ones_like(y))[0], dx)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bias_dtype", [FP32, BF16, FP16, torch.float64])
+@pytest.mark.parametrize("m,n,k", _ENGINES)
+def test_a_bias_of_another_type(m, n, k, bias_dtype):
+    """Added as it is: only the sum is rounded to the output's type."""
+    from kernels.int8 import Int8Weight, int8_linear, quantize_int8_rows
+
+    g = torch.Generator().manual_seed(n)
+    w, ws = _weight(n, k)
+    b = (torch.randn(n, generator=g, dtype=torch.float64) * 3).to(bias_dtype)
+    weight = Int8Weight(w.cuda(), ws.cuda(), backward=True)
+    for dtype in (BF16, FP16, FP32):
+        x = torch.randn(m, k, generator=g).to(dtype)
+        ref, terms = linear(*quantize(x), w, ws, b)
+        y = int8_linear(x.cuda(), weight, b.cuda())
+        _within(y, ref, terms, 7, "y")  # (a float64 bias: its rounding to fp32 besides)
+        assert torch.equal(int8_linear(quantize_int8_rows(x.cuda()), weight, b.cuda()), y)
+        assert torch.equal(int8_linear(x.cuda().requires_grad_(True), weight, b.cuda()), y)
+
+
+def test_entry_points_with_a_bias_type():
+    from forge_hip import _lib as L
+
+    def gemm(bias=16, bias_dtype=0, K=64):
+        return L.forge_int8_gemm_typed(16, 64, 16, 16, 64, 16, bias, bias_dtype, 16, 40, 2, 4, 40, K, None, None)
+
+    def lin(bias=16, bias_dtype=0, x=16):
+        return L.forge_int8_linear_typed(2, x, 64, None, 16, 64, 16, bias, bias_dtype, 16, 40, 2, 4, 40, 64, 16, None)
+
+    assert gemm(bias_dtype=3) == 2 and gemm(bias_dtype=-1) == 2 and b"bias" in L.forge_last_error()
+    assert lin(bias_dtype=3) == 2 and b"bias" in L.forge_last_error()
+    assert gemm(bias=None, bias_dtype=3, K=-1) == 1 and lin(bias=None, bias_dtype=3, x=None) == 1
