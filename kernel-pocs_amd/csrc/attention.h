@@ -56,6 +56,13 @@ struct Args {
   int parts;                          // 1: dk and dv are written as they are
 };
 
+// The forward's p = exp2(s c - m), m the running maximum of s c less P_UP.  fp16's
+// smallest step is 2^-24: with p up to 1 the keys more than 17 below a maximum (in
+// natural units) counted for nothing in o, however many they are, and in full in l.
+// Held 2^9 times as large, as far as the maximum's steps of 2^6 let it, p has them to 2^-34.
+template <class T>
+constexpr float P_UP = std::is_same_v<T, fp16_t> ? 9.f : 0.f;
+
 template <class T> __device__ __forceinline__ T* row_ptr(const Rows& r, int64_t batch, int64_t row, int head) {
   return (T*)r.p + batch * r.batch + row * r.row + head * r.head;
 }

@@ -1,8 +1,8 @@
 // Attention forward for gfx950.
 //
 // One pass over the keys with a running maximum m and sum l a query:
-//   S^T = K Q^T (keys x queries), p = exp2(s c - m c) with c = scale log2(e),
-//   O^T += V^T P^T, and at the end o = O / l, lse = m scale + ln l.
+//   S^T = K Q^T (keys x queries), p = exp2(s c - m) with c = scale log2(e),
+//   O^T += V^T P^T, and at the end o = O / l, lse = (m + log2 l) ln 2.
 // Both products are formed transposed, so that a lane of v_mfma_f32_32x32x16
 // holds one query's scores (the maximum and the sum are in-lane, with one exchange
 // between the halves of the wave), and those registers, rounded to 16 bits,
@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a
 
   f32x16 o[DB];
   const float c = a.scale * LOG2E;
-  float m, l;  // m: in units of log2; l: this half's sum
+  float m, l;  // m: the maximum less P_UP, in units of log2; l: this half's sum
 
   // keys that this lane's query sees, and those that every query of the wave does
   const int sees = a.causal ? min(sk.len, iq + shift + 1) : sk.len;
@@ -109,8 +109,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
-    top = fmaxf(top, other_half(top)) * c;
-    // m follows the maximum by steps of SLACK at least: p stays below 2^SLACK, and
+    top = __builtin_fmaf(fmaxf(top, other_half(top)), c, -P_UP<T>);
+    // m follows the maximum by steps of SLACK at least: p stays below 2^(SLACK + P_UP), and
     // the sums are seldom scaled (a new maximum, however small, comes up in one of
     // 32 queries at almost every tile)
     if (__any(top > m + SLACK)) {

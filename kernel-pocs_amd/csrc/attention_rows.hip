@@ -17,7 +17,7 @@ namespace fattn {
 
 struct Parts {      // sums of a chunk: [chunk of its sequence][query * H + head]
   float* o;         // [D], relative to 2^m
-  float* m;         // maximum, in units of log2
+  float* m;         // maximum less P_UP, in units of log2
   float* l;         // sum
   int64_t n;        // queries * H
   int C;            // keys a chunk
@@ -108,7 +108,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_rows_kernel(Args a, Parts par
           if (k0 + 8 * (r / 4) + 4 * h + r % 4 >= sees) s[r] = -__builtin_inff();
           top = fmaxf(top, s[r]);
         }
-        top = fmaxf(top, other_half(top)) * c;
+        top = __builtin_fmaf(fmaxf(top, other_half(top)), c, -P_UP<T>);
         const float up = fmaxf(top, m), f = exp2_hw(m - up);
         m = up;
         l *= f;

@@ -489,3 +489,28 @@ def test_captured_gradients_of_few_keys():
         for a, b in zip(got, step()):
             assert torch.equal(a, b), f"replay {i}"
         torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("where", [0, -1])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("queries", [1, 8, 300])
+@pytest.mark.parametrize("keys,above", [(16384, 17.4), (16384, 19.0), (3000, 16.9)])
+def test_many_small_probabilities_in_fp16(keys, above, queries, causal, where):
+    """One key far above all others, whose probabilities (2^-24 to 2^-27 of its) are below fp16's smallest steps, and
+    whose sum is the result.  Each is off by 2^-34 of the largest at most (held 2^9 times as large, half a step of
+    2^-24), by its rounding (2^-11 of it) and by that of the result."""
+    from kernels.attention import forge_varlen_attention
+
+    k, v = torch.zeros(keys, 1, 64, dtype=FP16), torch.ones(keys, 1, 64, dtype=FP16)
+    k[where, 0, 0], v[where] = above, 0
+    q = torch.zeros(queries, 2, 64, dtype=FP16)
+    q[:, :, 0] = 1
+    cu_q, cu_k = (torch.tensor([0, n], device="cuda", dtype=torch.int32) for n in (queries, keys))
+    out = forge_varlen_attention(q.cuda(), k.cuda(), v.cuda(), cu_q, cu_k, scale=1.0, causal=causal).double().cpu()
+    for i in range(queries):
+        sees = keys - queries + i + 1 if causal else keys
+        s = k[:sees, 0, 0].double()
+        ref = torch.softmax(s, 0) @ v[:sees, 0].double()
+        err = ref * 2 * 2.0 ** -11 * (1 + 2.0 ** -8) + sees * 2.0 ** -34 + 2.0 ** -25
+        assert bool(((out[i] - ref).abs() <= err).all()), (i, out[i, 0, 0].item(), ref[0].item())
