@@ -300,8 +300,8 @@ struct ColFrag {
 
 // Keys that a query does not see have p = 0, but 0 times an infinity or NaN is NaN,
 // and a product takes 16 keys at once.  Kernels run as if there were none; where
-// a causal sum comes out as NaN they run again with such values apart: added to the
-// sums of the queries that see them, and zeros in the tile.  (Seldom runs: few
+// a causal sum comes out as NaN or infinite they run again with such values apart: added
+// to the sums of the queries that see them, and zeros in the tile.  (Seldom runs: few
 // registers, not speed.  No value of a finite tile passes through any of this.)
 template <class T, int DP>
 struct Special {
@@ -339,18 +339,37 @@ struct Special {
         }
     }
   }
-  // zeros in their places, by waves `wave` of `waves`
-  static __device__ __forceinline__ void clear(char* tile, int r0, int n, int wave, int waves) {
+  // zeros in their places, and the others times `by`, a power of two (not in fp16); by
+  // waves `wave` of `waves`
+  static __device__ __forceinline__ void clear(char* tile, int r0, int n, int wave, int waves, float by = 1.f) {
 #pragma unroll 1
     for (int row = r0 + wave; row < r0 + n; row += waves)
       for (int w = threadIdx.x % 64; w < DP / 2; w += 64) {
         uint32_t* p = reinterpret_cast<uint32_t*>(row_at(tile, row)) + w;
-        const uint32_t x = *p;
-        if (is(x) || is(x >> 16)) *p = (is(x) ? 0 : x & 0xffff) | (is(x >> 16) ? 0 : x & 0xffff0000u);
+        uint32_t x = *p;
+        if (!is(x) && !is(x >> 16) && by == 1.f) continue;
+        x = (is(x) ? 0 : x & 0xffff) | (is(x >> 16) ? 0 : x & 0xffff0000u);
+        if (by != 1.f)
+          x = __float_as_uint(__uint_as_float(x << 16) * by) >> 16 | (__float_as_uint(__uint_as_float(x & 0xffff0000u) * by) & 0xffff0000u);
+        *p = x;
       }
   }
 };
 
+// The second run's factor of the values, a power of two, for n keys: sums of p below 2^6
+// times values near bf16's largest pass fp32's range, and the result, divided by the sum
+// of p, does not.  With it they do not either, and no other bit changes but of values
+// below 2^-87.  (fp16's values are far from that.)
+template <class T>
+__device__ __forceinline__ float v_down(int n) {
+  n = __builtin_amdgcn_readfirstlane(n);  // (the same in all lanes, and held once)
+  return std::is_same_v<T, fp16_t> ? 1.f : __uint_as_float((uint32_t)(127 - 7 - (32 - __builtin_clz(n | 1))) << 23);
+}
+// whether a first run with values that are not finite is to be followed by a second
+template <class T>
+__device__ __forceinline__ bool second_run(bool hides) { return hides || !std::is_same_v<T, fp16_t>; }
+
+// (infinities among them)
 template <int N>
 __device__ __forceinline__ bool any_nan(const f32x16 (&sums)[N]) {
   float t = 0.f;

@@ -74,6 +74,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a
   f32x16 o[DB];
   const float c = a.scale * LOG2E;
   float m, l;  // m: the maximum less P_UP, in units of log2; l: this half's sum
+  float down = 1.f;  // of the values, in the second run
 
   // keys that this lane's query sees, and those that every query of the wave does
   const int sees = a.causal ? min(sk.len, iq + shift + 1) : sk.len;
@@ -133,7 +134,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a
     if constexpr (apart) {
       Special<T, DP>::add(o, vt, 0, BN, k0, sees, false);
       __syncthreads();
-      Special<T, DP>::clear(vt, 0, BN, wave, 4);
+      Special<T, DP>::clear(vt, 0, BN, wave, 4, down);
       __syncthreads();
     }
 #pragma unroll
@@ -157,10 +158,13 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a
     }
   };
   run(std::false_type());
-  if (a.causal && any_of_4_waves(smem, wave, any_nan(o))) run(std::true_type());
+  if (second_run<T>(a.causal) && any_of_4_waves(smem, wave, any_nan(o))) {
+    down = v_down<T>(sk.len);
+    run(std::true_type());
+  }
   l += other_half(l);
   if (!live) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;  // (a row without keys)
+  const float inv = l == 0.f ? 0.f : 1.f / (l * down);  // (a row without keys)
   T* op = row_ptr<T>(a.o, sq.batch, sq.start + iq, head);
   const int64_t row = a.cu_q ? sq.start + iq : sq.batch * a.tq + iq;
 #pragma unroll

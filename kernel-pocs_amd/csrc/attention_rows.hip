@@ -15,10 +15,10 @@
 
 namespace fattn {
 
-struct Parts {      // sums of a chunk: [chunk of its sequence][query * H + head]
-  float* o;         // [D], relative to 2^m
+struct Parts {      // of a chunk: [chunk of its sequence][query * H + head]
+  float* o;         // [D], its output (divided by its sum)
   float* m;         // maximum less P_UP, in units of log2
-  float* l;         // sum
+  float* l;         // sum of p, relative to 2^m
   int64_t n;        // queries * H
   int C;            // keys a chunk
 };
@@ -82,7 +82,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_rows_kernel(Args a, Parts par
       qf[ks] = __builtin_bit_cast(bf16x8, v);
     }
     f32x16 o[DB];
-    float m, l;
+    float m, l, down = 1.f;  // down: of the values, in the second run
     const int sees = a.causal ? min(sk.len, token + shift + 1) : sk.len;
     auto run = [&](auto apart) __attribute__((always_inline)) {
 #pragma unroll
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_rows_kernel(Args a, Parts par
         }
         if constexpr (apart) {  // (the wave's own ring; its LDS accesses keep their order)
           Special<T, DP>::add(o, vt, 0, 32, k0, sees, false);
-          Special<T, DP>::clear(vt, 0, 32, 0, 1);
+          Special<T, DP>::clear(vt, 0, 32, 0, 1, down);
           wait_dma<0>();
         }
 #pragma unroll
@@ -137,7 +137,8 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_rows_kernel(Args a, Parts par
       }
     };
     run(std::false_type());
-    if (a.causal && sq.len > 1 && mine > 0 && __any(any_nan(o))) {  // (a token alone sees every key)
+    if (second_run<T>(a.causal && sq.len > 1) && mine > 0 && __any(any_nan(o))) {  // (a token alone sees every key)
+      down = v_down<T>(sk.len);
       wait_dma<0>();  // the reads of the ring are done
       issue(0);
       if (mine > 1) issue(1);
@@ -146,13 +147,16 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_rows_kernel(Args a, Parts par
     l += other_half(l);
     wait_dma<0>();
     barrier();  // every wave is done with its ring
+    // outputs of parts are joined, not sums: those may be past fp32's range where the
+    // output is not
+    const float part_inv = l == 0.f ? 0.f : 1.f / (l * down);
     float* sums = reinterpret_cast<float*>(smem) + wave * 32 * PITCH + (lane % 32) * PITCH;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         *reinterpret_cast<f32x4*>(sums + 32 * db + 8 * i + 4 * h) =
-            f32x4{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]};
+            f32x4{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]} * part_inv;
     if (h == 0) {
       stat[wave * 32 + lane] = m;
       stat[(NW + wave) * 32 + lane] = l;
@@ -164,20 +168,21 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_rows_kernel(Args a, Parts par
       float top = stat[r];
 #pragma unroll
       for (int w = 1; w < NW; ++w) top = fmaxf(top, stat[w * 32 + r]);
-      float total = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+      float total = 0.f, f[NW], v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        const float f = exp2_hw(stat[w * 32 + r] - top);
-        total += stat[(NW + w) * 32 + r] * f;
+        f[w] = stat[(NW + w) * 32 + r] * exp2_hw(stat[w * 32 + r] - top);
+        total += f[w];
+      }
+      const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
         const f32x4 y = *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(smem) + (w * 32 + r) * PITCH + d);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] += y[j] * f;
+        for (int j = 0; j < 4; ++j) v[j] += y[j] * (f[w] * inv);
       }
       const int64_t q = (a.cu_q ? sq.start : sq.batch * a.tq) + t;
       if (n_chunk == 1) {
-        const float inv = total == 0.f ? 0.f : 1.f / total;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] *= inv;
         store4(row_ptr<T>(a.o, sq.batch, sq.start + t, hd) + d, v[0], v[1], v[2], v[3]);
         if (a.low) store_low4<T>(a.low + (q * a.H + hd) * a.D + d, v[0], v[1], v[2], v[3]);
         if (d == 0 && a.lse) a.lse[q * a.H + hd] = total == 0.f ? -__builtin_inff() : (top + __builtin_amdgcn_logf(total)) * LN2;
@@ -238,13 +243,11 @@ __global__ __launch_bounds__(256) void attn_join_kernel(Args a, Parts parts) {
     float v[4] = {0.f, 0.f, 0.f, 0.f};
     for (int i = 0; i < n; ++i) {
       const int64_t at = i * parts.n + p;
-      const float f = exp2_hw(parts.m[at] - top);
+      const float f = parts.l[at] * exp2_hw(parts.m[at] - top) * inv;
       const f32x4 y = *reinterpret_cast<const f32x4*>(parts.o + at * a.D + 4 * lane);
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] += y[j] * f;
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] *= inv;
     store4(op + 4 * lane, v[0], v[1], v[2], v[3]);
     if (a.low) store_low4<T>(a.low + p * a.D + 4 * lane, v[0], v[1], v[2], v[3]);
   }

@@ -514,3 +514,31 @@ def test_many_small_probabilities_in_fp16(keys, above, queries, causal, where):
         ref = torch.softmax(s, 0) @ v[:sees, 0].double()
         err = ref * 2 * 2.0 ** -11 * (1 + 2.0 ** -8) + sees * 2.0 ** -34 + 2.0 ** -25
         assert bool(((out[i] - ref).abs() <= err).all()), (i, out[i, 0, 0].item(), ref[0].item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e36, 8e37])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lens_q,lens_k", [([1, 1], [3000, 40]), ([3], [900]), ([200, 5], [200, 1300])])
+def test_values_near_the_largest(lens_q, lens_k, causal, size):
+    """Sums of probabilities times values pass fp32's range before they are divided by the probabilities' sum; the
+    results do not.  Small values beside them keep their accuracy, and keys that are not finite stay apart."""
+    from kernels.attention import forge_varlen_attention
+
+    q, k, v, do = _make(lens_q, lens_k, 4, 2, 72, BF16)
+    v = (v.float().clamp(-4, 4) * size).to(BF16)
+    v[:, :, 1] = (v[:, :, 1].float() * (1e-20 / size)).to(BF16)
+    v[:, :, 2] = v[:, :, 2].abs()
+    at_q, at_k = _offsets(lens_q), _offsets(lens_k)
+    unit, tiny = _unit(BF16)
+    ref = packed_fwd_bwd(q, k, v, do * 0, at_q, at_k, 72 ** -0.5, causal, unit, tiny)
+    cu_q, cu_k = (torch.tensor(a, device="cuda", dtype=torch.int32) for a in (at_q, at_k))
+    out, lse = forge_varlen_attention(q.cuda(), k.cuda(), v.cuda(), cu_q, cu_k, causal=causal, return_lse=True)
+    # (a result's error is a share of its own column's terms: the bound of each is made of |v| of that column)
+    _within(out, ref.o, ref.o_err, "out")
+    _within(lse, ref.lse, ref.lse_err, "lse")
+    if causal and lens_q[0] > 3:
+        bad = _special(v, list(range(100, 200, 2)), [float("nan"), float("inf")])
+        got = forge_varlen_attention(q.cuda(), k.cuda(), bad.cuda(), cu_q, cu_k)
+        _within(got[:100], ref.o[:100], ref.o_err[:100], "rows that do not see them")
+        assert bool(got[103:200].isnan().any(-1).all()) and bool(got[200:].isfinite().all())
