@@ -776,8 +776,8 @@ int forge_transpose_2b_batch(int n, const void* const* src, const int64_t* ld_sr
  *   dense (cu_q = cu_k = NULL): B sequences of tq queries and tk keys.
  * Rows lie at base + sequence * batch + row * row + head * head (elements; varlen:
  * the batch strides are not used), 16-byte aligned, unit stride in D, row strides
- * below 2^23.  A query that sees no key has out = 0.  lse (fp32 [queries][H], or
- * NULL): the natural logarithm of the sum, -inf without keys.  low (int8
+ * below 2^23.  A query that sees no key has out = 0, one that sees scores of -inf alone NaN.
+ * lse (fp32 [queries][H], or NULL): the natural logarithm of the sum, -inf for both.  low (int8
  * [queries][H][D], 16-byte aligned, or NULL): for the gradients, what the rounding
  * of out took, in 254ths of a step.
  * work: forge_attention_fwd_workspace bytes, 16-byte aligned (0: may be NULL). */

@@ -5,7 +5,7 @@
 //   o_i = sum_j p_ij v_j,  p_ij = exp(s_ij - lse_i),  s_ij = scale q_i . k_j,
 // over the keys j that query i sees: all of its sequence's, or (causal) j <= i +
 // len_k - len_q, so that the last query sees every key.  A query that sees
-// none has o = 0 and lse = -inf.
+// none has o = 0 and lse = -inf; one whose scores are all -inf has o = NaN, as softmax.
 //
 // Sequences: cu_q and cu_k hold the B + 1 offsets of each, or are NULL for B
 // dense sequences of len_q and len_k rows.  Row i of sequence s lies at base +
@@ -365,6 +365,10 @@ __device__ __forceinline__ float v_down(int n) {
   n = __builtin_amdgcn_readfirstlane(n);  // (the same in all lanes, and held once)
   return std::is_same_v<T, fp16_t> ? 1.f : __uint_as_float((uint32_t)(127 - 7 - (32 - __builtin_clz(n | 1))) << 23);
 }
+// 1 / l of a query that has no probability: of one that sees no key 0, and so are its sums;
+// of one whose keys' scores are all -inf NaN, which its softmax is.
+__device__ __forceinline__ float nothing(int sees) { return sees > 0 ? __builtin_nanf("") : 0.f; }
+
 // whether a first run with values that are not finite is to be followed by a second
 template <class T>
 __device__ __forceinline__ bool second_run(bool hides) { return hides || !std::is_same_v<T, fp16_t>; }

@@ -69,8 +69,9 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(Args a, float* shift, i
     if (lane % 16 == 0) {
       const float l = a.lse[row * a.H + head];
       a.delta[head * n_rows + row] = -sum;
-      // a query without keys: exp(scale (s - inf)) = 0
-      shift[head * n_rows + row] = l == -__builtin_inff() ? -__builtin_inff() : -l / a.scale;
+      // a query without keys: exp(scale (s - inf)) = 0; one that sees scores of -inf alone
+      // (o, and so the sum, is NaN): NaN, where it sees keys
+      shift[head * n_rows + row] = l != -__builtin_inff() ? -l / a.scale : sum == sum ? l : sum;
     }
   }
 }

@@ -164,7 +164,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a
   }
   l += other_half(l);
   if (!live) return;
-  const float inv = l == 0.f ? 0.f : 1.f / (l * down);  // (a row without keys)
+  const float inv = l == 0.f ? nothing(sees) : 1.f / (l * down);
   T* op = row_ptr<T>(a.o, sq.batch, sq.start + iq, head);
   const int64_t row = a.cu_q ? sq.start + iq : sq.batch * a.tq + iq;
 #pragma unroll

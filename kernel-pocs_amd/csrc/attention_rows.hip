@@ -174,7 +174,8 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_rows_kernel(Args a, Parts par
         f[w] = stat[(NW + w) * 32 + r] * exp2_hw(stat[w * 32 + r] - top);
         total += f[w];
       }
-      const float inv = total == 0.f ? 0.f : 1.f / total;
+      // (of a chunk of several 0: the join looks at them all)
+      const float inv = total != 0.f ? 1.f / total : n_chunk == 1 ? nothing(a.causal ? min(sk.len, t + shift + 1) : sk.len) : 0.f;
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
         const f32x4 y = *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(smem) + (w * 32 + r) * PITCH + d);
@@ -209,21 +210,22 @@ __global__ __launch_bounds__(256) void attn_join_kernel(Args a, Parts parts) {
   const int head = (int)(p % a.H);
   Span sk = {0, 0, 0};
   int64_t batch = 0, row = q;
+  int behind = 0;  // queries of the sequence behind this one
   if (!a.cu_q) {
     batch = q / a.tq;
     row = q % a.tq;
     sk = span_of(nullptr, a.B, a.tk, (int)batch);
+    behind = (int)(a.tq - 1 - row);
   } else {
     for (int base = 0; base < a.B; base += 64) {
       const int s = base + lane;
-      bool in = false;
-      if (s < a.B) {
-        const Span sq = span_of(a.cu_q, a.B, a.tq, s);
-        in = q >= sq.start && q < sq.start + sq.len;
-      }
-      const uint64_t found = __ballot(in);
+      Span sq = {0, 0, 0};
+      if (s < a.B) sq = span_of(a.cu_q, a.B, a.tq, s);
+      const uint64_t found = __ballot(q >= sq.start && q < sq.start + sq.len);
       if (found) {
-        sk = span_of(a.cu_k, a.B, a.tk, base + __builtin_ctzll(found));
+        const int at = __builtin_ctzll(found);
+        sk = span_of(a.cu_k, a.B, a.tk, base + at);
+        behind = __builtin_amdgcn_readlane((int)(sq.start + sq.len - 1 - q), at);
         break;
       }
     }
@@ -236,7 +238,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(Args a, Parts parts) {
   float total = 0.f;
   for (int i = lane; i < n; i += 64) total += parts.l[i * parts.n + p] * exp2_hw(parts.m[i * parts.n + p] - top);
   total = wave_sum(total);
-  const float inv = total == 0.f ? 0.f : 1.f / total;
+  const float inv = total != 0.f ? 1.f / total : nothing(a.causal ? sk.len - behind : sk.len);
   T* op = row_ptr<T>(a.o, batch, row, head);
   const int vecs = a.D / 4;
   if (lane < vecs) {

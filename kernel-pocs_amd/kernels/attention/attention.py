@@ -7,7 +7,8 @@ over the keys that query i sees: all of its sequence's or, causal, those j <= i 
 len_k - len_q (the last query sees every key: a prompt, a prompt that continues
 earlier tokens, or one token against a sequence's keys).  A query that sees no
 key (a sequence without keys, or more queries than keys) has out = 0, lse = -inf
-and no gradient.
+and no gradient.  One that sees keys whose scores are all -inf has no softmax: out and
+the gradients that it takes part in are NaN, lse is -inf.
 
 fp16 and bf16, head_dim a multiple of 8 up to 256, any number of heads on a
 divisor of it.  Products take 16-bit operands (the probabilities and, backward,

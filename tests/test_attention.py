@@ -542,3 +542,42 @@ def test_values_near_the_largest(lens_q, lens_k, causal, size):
         got = forge_varlen_attention(q.cuda(), k.cuda(), bad.cuda(), cu_q, cu_k)
         _within(got[:100], ref.o[:100], ref.o_err[:100], "rows that do not see them")
         assert bool(got[103:200].isnan().any(-1).all()) and bool(got[200:].isfinite().all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lens_q,lens_k,row", [([1, 1], [40, 9], 0), ([1, 2], [5000, 30], 0), ([2, 1], [300, 70], 1),
+                                               ([200, 60], [200, 60], 37), ([100, 30], [60, 30], 90)])
+def test_scores_that_are_all_minus_infinity(lens_q, lens_k, row, causal, dtype):
+    """A query that sees keys, all with a score of -inf, has no probabilities: NaN, as in the softmax of its row, and so
+    are the gradients that it takes part in.  One that sees no key has zeros."""
+    from kernels.attention import forge_varlen_attention
+
+    q, k, v, do = _make(lens_q, lens_k, 4, 2, 64, dtype)
+    k[:, :, 0] = 1
+    q[:, :, 0] = 0
+    bad = q.clone()
+    bad[row, 1, 0] = float("-inf")
+    cu_q, cu_k = (torch.tensor(_offsets(n), device="cuda", dtype=torch.int32) for n in (lens_q, lens_k))
+
+    def run(q):
+        leaves = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+        out, lse = forge_varlen_attention(*leaves, cu_q, cu_k, causal=causal, return_lse=True)
+        return [t.detach() for t in (out, lse, *torch.autograd.grad(out, leaves, do.cuda()))]
+
+    (out, lse, dq, dk, dv), plain = run(bad), run(q)
+    assert bool(out[row, 1].isnan().all()) and lse[row, 1] == -math.inf and bool(dq[row, 1].isnan().all())
+    sees = row + lens_k[0] - lens_q[0] + 1 if causal else lens_k[0]
+    assert bool(dk[:sees, 0].isnan().all()) and bool(dv[:sees, 0].isnan().all())
+    others = torch.ones(sum(lens_q), 4, dtype=torch.bool)
+    others[row, 1] = False
+    for a, b in zip((out, lse, dq), plain):
+        assert torch.equal(a[others], b[others])
+    for a, b in zip((dk, dv), plain[3:]):
+        assert torch.equal(a[:, 1], b[:, 1]) and torch.equal(a[lens_k[0]:], b[lens_k[0]:])
+    none = [i for i in range(lens_q[0]) if causal and i + lens_k[0] - lens_q[0] < 0]
+    assert bool((out[none] == 0).all()) and bool((lse[none] == -math.inf).all()) and bool((dq[none] == 0).all())
+    # the definition's, in float64
+    s = bad[row, 1].double() @ k[:sees, 0].double().T
+    assert bool((s == -math.inf).all()) and bool(torch.softmax(s, 0).isnan().all())
