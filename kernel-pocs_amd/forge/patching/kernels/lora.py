@@ -373,12 +373,12 @@ def attention_args(module, query, key, value, attention_mask, kwargs):
     """(causal, offsets of the packed queries, of their keys, or None and None) when
     forge_attention or forge_varlen_attention is the attention that this call asks
     for, else None.  Taken: fp16 and bf16 GPU tensors without a mask, dropout, soft
-    cap or weights to return, and without a window that hides a key; one token
-    against its cache, or as many queries as keys.  As in the model's own
-    implementations "eager" without a mask sees every key and the others are causal
-    where module.is_causal says so; cu_seq_lens_q and cu_seq_lens_k (the "flash_attention"
-    implementations' arguments) give sequences packed into one row, and such an
-    implementation may find them in position_ids instead, so then it runs itself.
+    cap or weights to return, without a window that hides a key and without arguments
+    that are not known; one token against its cache, or as many queries as keys.  As in
+    the model's own implementations "eager" without a mask sees every key and the others
+    are causal where module.is_causal says so; cu_seq_lens_q and cu_seq_lens_k (the
+    "flash_attention" implementations' arguments) give sequences packed into one row, and
+    such an implementation may find them in position_ids instead, so then it runs itself.
     Implementations of other names run themselves."""
     if attention_mask is not None or not query.is_cuda or any(_is_dtensor(t) for t in (query, key, value)):
         return None
@@ -391,7 +391,8 @@ def attention_args(module, query, key, value, attention_mask, kwargs):
         return None
     if getattr(module, "attn_logit_softcapping", None) is not None:
         return None
-    if any(v is not None and v is not False and n not in _NEUTRAL for n, v in kwargs.items()):
+    # (False is a choice too: is_causal=False comes before the module's is_causal)
+    if any(v is not None and n not in _NEUTRAL and not (n == "output_attentions" and v is False) for n, v in kwargs.items()):
         return None
     window = _sliding_window(module)
     if window is not None and window < keys:

@@ -184,3 +184,24 @@ def test_sequences_packed_into_one_row(monkeypatch):
             alone = m(x[:, a:b], (cos[:, a:b], sin[:, a:b]), None)[0].float()
             assert (got[:, a:b] - alone).abs().max() <= 0.02 * alone.abs().max()
     assert calls == ["forge_varlen_attention"] + ["forge_attention"] * 3
+
+
+@pytest.mark.gpu
+def test_calls_that_say_whether_they_are_causal(monkeypatch):
+    """is_causal of a call comes before the module's: such calls run the model's implementation, as do calls with
+    any other argument that is not known, False among them."""
+    from forge.patching.kernels.lora import attention_args
+
+    calls = _counted(monkeypatch)
+    module, rot = _attn()
+    x = torch.randn(1, 37, 512, device="cuda", dtype=BF16)
+    tables = rot(x, torch.arange(37, device="cuda")[None])
+    plain, patched = _patched(copy.deepcopy(module)), _patched(copy.deepcopy(module), attention="forge")
+    for value in (False, True):
+        with torch.no_grad():
+            want, got = (m(x, tables, None, is_causal=value)[0] for m in (plain, patched))
+        assert torch.equal(got, want) and calls == []
+    q, k = (torch.zeros(2, h, 5, 128, device="cuda", dtype=BF16) for h in (4, 2))
+    assert attention_args(module, q, k, k, None, {"is_causal": False}) is None
+    assert attention_args(module, q, k, k, None, {"some_option": False}) is None
+    assert attention_args(module, q, k, k, None, {"is_causal": None, "output_attentions": False}) == (True, None, None)
