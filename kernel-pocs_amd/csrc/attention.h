@@ -302,7 +302,8 @@ struct ColFrag {
 // and a product takes 16 keys at once.  Kernels run as if there were none; where
 // a causal sum comes out as NaN or infinite they run again with such values apart: added
 // to the sums of the queries that see them, and zeros in the tile.  (Seldom runs: few
-// registers, not speed.  No value of a finite tile passes through any of this.)
+// registers, not speed.  No value of a finite tile passes through any of this.)  For the
+// keys' gradients it is 16 queries at once, and they know beforehand.
 template <class T, int DP>
 struct Special {
   typedef Tile<DP> L;
@@ -318,9 +319,9 @@ struct Special {
     }
     return __any(any);
   }
-  // those of rows r0 .. r0 + n - 1, the keys from key0, of the keys before `sees`; as
-  // they are (times a p above 0) or as NaN
-  static __device__ __forceinline__ void add(f32x16 (&sums)[DP / 32], char* tile, int r0, int n, int key0, int sees, bool as_nan) {
+  // those of rows r0 .. r0 + n - 1 whose number, first + j, is from `lo` on and below `hi`;
+  // as they are (times a p above 0) or as NaN
+  static __device__ __forceinline__ void add(f32x16 (&sums)[DP / 32], char* tile, int r0, int n, int first, int lo, int hi, bool as_nan) {
     const int h = threadIdx.x % 64 / 32;
 #pragma unroll 1
     for (int j = 0; j < n; ++j) {
@@ -335,7 +336,7 @@ struct Special {
           const int d = 32 * db + 8 * (r / 4) + 4 * h + r % 4;
           const uint16_t x = *reinterpret_cast<const uint16_t*>(p + ((d / 8 ^ L::f(row)) << 4) + d % 8 * 2);
           const float v = as_nan ? __builtin_nanf("") : to_f32(__builtin_bit_cast(T, x));
-          sums[db][r] += is(x) && key0 + j < sees ? v : 0.f;
+          sums[db][r] += is(x) && first + j >= lo && first + j < hi ? v : 0.f;
         }
     }
   }

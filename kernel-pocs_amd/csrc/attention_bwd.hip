@@ -31,7 +31,8 @@ __device__ __forceinline__ void keep_in_range(f32x16& ds, float& unit, f32x16 (&
       float top = 0.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(ds[r]));
-      if (unit < 0x1p-13f || !__any(top > 65504.f)) return;
+      // (an infinite ds makes its own lane's sums so, whatever the unit)
+      if (unit < 0x1p-13f || !__any(top > 65504.f && top < __builtin_inff())) return;
       unit *= 0.25f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) ds[r] *= 0.25f;
@@ -43,11 +44,21 @@ __device__ __forceinline__ void keep_in_range(f32x16& ds, float& unit, f32x16 (&
   }
 }
 
-// rows [batch][row] of the query side, one wave to a (row, head) at a time
+// whether a row has values that are not; by 16 lanes
+template <class T>
+__device__ __forceinline__ bool not_finite(const T* p, int D, int lane) {
+  float t = 0.f;
+#pragma unroll 1
+  for (int d = lane % 16; d < D; d += 16) t = __builtin_fmaf(to_f32(p[d]), 0.f, t);
+#pragma unroll
+  for (int off = 8; off >= 1; off /= 2) t += __shfl_xor(t, off, 64);
+  return t != t;
+}
+
+// rows [batch][row] of the query side, 16 lanes to a (row, head) at a time
 template <class T>
 __global__ __launch_bounds__(256) void attn_delta_kernel(Args a, float* shift, int64_t n_rows, int64_t pairs) {
   const int lane = threadIdx.x % 64;
-  // 16 lanes to a (row, head), D / 8 chunks of 8
   for (int64_t p = ((int64_t)blockIdx.x * 256 + threadIdx.x) / 16; p < pairs; p += (int64_t)gridDim.x * 16) {
     const int64_t row = p / a.H;
     const int head = (int)(p % a.H);
@@ -66,8 +77,12 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(Args a, float* shift, i
     }
 #pragma unroll
     for (int off = 8; off >= 1; off /= 2) sum += __shfl_xor(sum, off, 64);
+    const float l = a.lse[row * a.H + head];
+    // The dk, dv kernel looks here for rows of q and dout that are not finite: the sum is
+    // not where dout is not, nor where q is not, as o is NaN then.  But of a query without
+    // keys o is 0, whatever it holds.
+    if (l == -__builtin_inff() && a.causal && not_finite(row_ptr<T>(a.q, batch, r, head), a.D, lane)) sum = __builtin_nanf("");
     if (lane % 16 == 0) {
-      const float l = a.lse[row * a.H + head];
       a.delta[head * n_rows + row] = -sum;
       // a query without keys: exp(scale (s - inf)) = 0; one that sees scores of -inf alone
       // (o, and so the sum, is NaN): NaN, where it sees keys
@@ -167,7 +182,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dq_kernel(Args a,
       keep_in_range<T>(s, unit, acc);
       if constexpr (apart) {  // (the sign of ds is not known: NaN)
         __syncthreads();        // every wave has its scores of these keys
-        Special<T, DP>::add(acc, kt, 32 * kb, 32, k0, sees, true);
+        Special<T, DP>::add(acc, kt, 32 * kb, 32, k0, 0, sees, true);
         __syncthreads();
         Special<T, DP>::clear(kt, 32 * kb, 32, wave, 4);
         __syncthreads();
@@ -239,7 +254,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
   const bool live = jk < sk.len;
   const int shift = sk.len - sq.len;
   bf16x8 kf[KS], vf[KS];
-  {
+  // (in each of the two loops' branches: registers that both share went to scratch memory)
+  auto load_own = [&]() __attribute__((always_inline)) {
     const T* kp = row_ptr<T>(a.k, sk.batch, sk.start + (live ? jk : 0), it.kv);
     const T* vp = row_ptr<T>(a.v, sk.batch, sk.start + (live ? jk : 0), it.kv);
 #pragma unroll
@@ -253,7 +269,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
       kf[ks] = __builtin_bit_cast(bf16x8, v);
       vf[ks] = __builtin_bit_cast(bf16x8, w);
     }
-  }
+  };
   // the first query that sees a key of the tile, and tiles of queries from there, of
   // each of the group's heads in turn
   const int first = a.causal ? max(0, k0 - shift) / BQ * BQ : 0;
@@ -286,6 +302,16 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
   fc.setup(lane);
   for (int& x : fr.base) asm("" : "+v"(x += TILES));
   for (int& x : fc.base) asm("" : "+v"(x += TILES));
+  // Whether a query that sees some of these keys and not all, or is in a tile with such
+  // (from `first` on), has a q or dout that is not finite (delta tells): its p and ds of
+  // the others are 0, but their products with it are NaN.
+  bool odd = false;
+  if (a.causal && n_t > 0) {
+    const int n = min(sq.len, k0 + BN - 1 - shift) - first;
+    const int64_t row = (a.cu_q ? sq.start : sq.batch * a.tq) + first;
+    for (int head = it.kv * G + g_lo; head < it.kv * G + g_hi; ++head)
+      for (int i = threadIdx.x; i < n; i += 256) odd |= !__builtin_isfinite(a.delta[head * n_rows + row + i]);
+  }
   f32x16 dk[DB], dv[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db)
@@ -295,20 +321,20 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
   float unit = 1.f;
 
   int tile_i = first;
-  auto step = [&](bool more, int slot) __attribute__((always_inline)) {
+  auto step = [&](bool more, int slot, auto apart) __attribute__((always_inline)) {
     wait_dma<0>();
     barrier();
     if (more) issue(1 - slot);
     const int t_i = tile_i;
     tile_i = tile_i + BQ < sq.len ? tile_i + BQ : first;
-    const char* qt = smem + slot * 2 * Dma::BYTES;
-    const char* dt = qt + Dma::BYTES;
+    char* qt = smem + slot * 2 * Dma::BYTES;
+    char* dt = qt + Dma::BYTES;
 #pragma unroll
     for (int qb = 0; qb < BQ / 32; ++qb) {
       __builtin_amdgcn_sched_barrier(0);
       const int i0 = t_i + 32 * qb;
       // (causal: the last query of the block sees nothing of this wave's keys)
-      if (i0 >= sq.len || wk >= sk.len || (a.causal && i0 + 31 + shift < wk)) continue;
+      if (i0 >= sq.len || (!apart && (wk >= sk.len || (a.causal && i0 + 31 + shift < wk)))) continue;
       f32x16 s, dp;  // begin with -lse / scale and -delta of their queries
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -340,6 +366,15 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
       }
       if constexpr (DK) keep_in_range<T>(dp, unit, dk);
       __builtin_amdgcn_sched_barrier(0);
+      if constexpr (apart) {  // (the fragments read the tiles TILES behind qt and dt)
+        __syncthreads();      // every wave has its scores of these queries
+        if constexpr (DK) Special<T, DP>::add(dk, qt + TILES, 32 * qb, 32, i0, jk - shift, sq.len, true);
+        if constexpr (DV) Special<T, DP>::add(dv, dt + TILES, 32 * qb, 32, i0, jk - shift, sq.len, false);
+        __syncthreads();
+        if constexpr (DK) Special<T, DP>::clear(qt + TILES, 32 * qb, 32, wave, 4);
+        if constexpr (DV) Special<T, DP>::clear(dt + TILES, 32 * qb, 32, wave, 4);
+        __syncthreads();
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const bf16x8 p = pack_acc<T>(s, i), ds = pack_acc<T>(dp, i);
@@ -352,9 +387,17 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
     }
   };
   if (n_t > 0) issue(0);
-  for (int t = 0; t < n_t; t += 2) {
-    step(t + 1 < n_t, 0);
-    if (t + 1 < n_t) step(t + 2 < n_t, 1);
+  // (through slot 1's statistics, which are not under way yet)
+  if (a.causal && any_of_4_waves(smem + TILES / 2, wave, odd)) {
+    load_own();
+#pragma unroll 1
+    for (int t = 0; t < n_t; ++t) step(t + 1 < n_t, t % 2, std::true_type());
+  } else {
+    load_own();
+    for (int t = 0; t < n_t; t += 2) {
+      step(t + 1 < n_t, 0, std::false_type());
+      if (t + 1 < n_t) step(t + 2 < n_t, 1, std::false_type());
+    }
   }
   if (!live) return;
   const float p_one = exp2f(-P_BITS<T>), back = a.scale * p_one / unit;

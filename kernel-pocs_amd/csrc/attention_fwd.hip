@@ -132,7 +132,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a
         s[kb][r] = p;
       }
     if constexpr (apart) {
-      Special<T, DP>::add(o, vt, 0, BN, k0, sees, false);
+      Special<T, DP>::add(o, vt, 0, BN, k0, 0, sees, false);
       __syncthreads();
       Special<T, DP>::clear(vt, 0, BN, wave, 4, down);
       __syncthreads();

@@ -122,7 +122,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_rows_kernel(Args a, Parts par
           l += s[r];
         }
         if constexpr (apart) {  // (the wave's own ring; its LDS accesses keep their order)
-          Special<T, DP>::add(o, vt, 0, 32, k0, sees, false);
+          Special<T, DP>::add(o, vt, 0, 32, k0, 0, sees, false);
           Special<T, DP>::clear(vt, 0, 32, 0, 1, down);
           wait_dma<0>();
         }

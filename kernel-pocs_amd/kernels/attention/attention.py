@@ -14,10 +14,10 @@ fp16 and bf16, head_dim a multiple of 8 up to 256, any number of heads on a
 divisor of it.  Products take 16-bit operands (the probabilities and, backward,
 their gradients are rounded to them) and sum in fp32; each result is rounded
 once.  Every sum has a fixed order, forward and backward.  A key or value that is
-not finite stays with the queries that see it; a query, or a gradient that comes
-in, that is not may also make gradients of the next keys (up to 63) NaN.  Queries, keys and
-values are read where they lie (columns of one projection's output, HF's
-transposed views); rows that are not 16-byte aligned are copied first.
+not finite stays with the queries that see it, and a query, or a gradient that comes
+in, with the keys that it sees.  Queries, keys and values are read where they lie
+(columns of one projection's output, HF's transposed views); rows that are not 16-byte
+aligned are copied first.
 """
 from __future__ import annotations
 

@@ -581,3 +581,40 @@ def test_scores_that_are_all_minus_infinity(lens_q, lens_k, row, causal, dtype):
     # the definition's, in float64
     s = bad[row, 1].double() @ k[:sees, 0].double().T
     assert bool((s == -math.inf).all()) and bool(torch.softmax(s, 0).isnan().all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("H,kv,D", [(2, 1, 64), (4, 2, 128), (2, 2, 256), (3, 1, 40), (16, 1, 64)])
+@pytest.mark.parametrize("lens_q,lens_k,row", [([300, 90], [300, 90], 100), ([3, 7], [330, 40], 1), ([100, 40], [60, 40], 45),
+                                               ([100, 40], [60, 40], 20), ([70], [500], 33)])
+def test_queries_and_gradients_that_are_not_finite(lens_q, lens_k, row, H, kv, D, dtype):
+    """NaN and infinities in a query or in the gradient of an output: the gradients of the keys and values that it does
+    not see are as they are without, bit by bit, and so are the other queries'."""
+    from kernels.attention import forge_varlen_attention
+
+    q, k, v, do = _make(lens_q, lens_k, H, kv, D, dtype)
+    cu_q, cu_k = (torch.tensor(_offsets(n), device="cuda", dtype=torch.int32) for n in (lens_q, lens_k))
+    inf, nan = float("inf"), float("nan")
+
+    def run(q, do):
+        leaves = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+        out = forge_varlen_attention(*leaves, cu_q, cu_k)
+        return torch.autograd.grad(out, leaves, do.cuda())
+
+    sees = max(0, row + lens_k[0] - lens_q[0] + 1)  # keys that the row's query sees
+    plain = run(q, do)
+    for values in ([nan], [inf], [-inf, nan, inf]):
+        head = 0
+        for bad in (run(_special(q, [row], values), do), run(q, _special(do, [row], values)),
+                    run(_special(q, [row], values), _special(do, [row], values))):
+            assert torch.equal(bad[0][:row], plain[0][:row]) and torch.equal(bad[0][row + 1:], plain[0][row + 1:])
+            for a, b in zip(bad[1:], plain[1:]):
+                assert torch.equal(a[sees:], b[sees:]) and torch.equal(a[:, 1:], b[:, 1:])
+            if sees:  # and where it is seen, nothing is hidden
+                assert not bool(bad[1][:sees, head].isfinite().all(-1).any())
+    # a value's gradient: p times the infinity, in its column alone
+    dv = run(q, _special(do, [row], [inf]))[2]
+    want = plain[2].clone()
+    want[:sees, 0, 0] = inf
+    assert torch.equal(dv, want)
