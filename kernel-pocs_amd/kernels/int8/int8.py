@@ -17,6 +17,7 @@ same way: e = dy w_scale, quantized by rows, times the transposed weight.
 """
 from __future__ import annotations
 
+import math
 from typing import Optional, Union
 
 import torch
@@ -46,13 +47,31 @@ def _ld(x2: torch.Tensor) -> int:
 
 
 class Int8Rows:
-    """Rows in 8 bits: `padded` [rows, pitch] (zeros behind K), `scale` [rows] in fp32,
-    the shape and type of what they stand for."""
+    """Rows in 8 bits: `padded` [rows, pitch] (K to the next multiple of 16 or more, zeros
+    behind K), `scale` [rows] in fp32, the shape and type of what they stand for."""
 
     __slots__ = ("padded", "scale", "shape", "dtype")
 
-    def __init__(self, padded, scale, shape, dtype):
-        self.padded, self.scale, self.shape, self.dtype = padded, scale, torch.Size(shape), dtype
+    def __init__(self, padded: torch.Tensor, scale: torch.Tensor, shape, dtype: torch.dtype):
+        shape = torch.Size(shape)
+        if dtype not in _DTYPES:
+            raise TypeError(f"Int8Rows stand for fp16, bf16 or fp32, got {dtype}")
+        rows = math.prod(shape[:-1])
+        if (len(shape) < 1 or padded.dim() != 2 or padded.dtype != torch.int8 or not padded.is_contiguous()
+                or padded.shape[0] != rows or padded.shape[1] < shape[-1] or padded.shape[1] % 16):
+            raise ValueError(f"Int8Rows of {tuple(shape)} need contiguous int8 rows of a multiple of 16 columns, got "
+                             f"{padded.dtype} {tuple(padded.shape)}")
+        if scale.shape != (rows,) or scale.dtype != torch.float32 or not scale.is_contiguous() or scale.device != padded.device:
+            raise ValueError(f"Int8Rows need contiguous fp32 scales [{rows}] on {padded.device}, got {scale.dtype} "
+                             f"{tuple(scale.shape)} on {scale.device}")
+        self.padded, self.scale, self.shape, self.dtype = padded, scale, shape, dtype
+
+    @classmethod
+    def _of(cls, padded, scale, shape, dtype) -> "Int8Rows":
+        """Of this package's own making: without the checks."""
+        self = cls.__new__(cls)
+        self.padded, self.scale, self.shape, self.dtype = padded, scale, shape, dtype
+        return self
 
     @property
     def values(self) -> torch.Tensor:
@@ -95,7 +114,7 @@ def quantize_int8_rows(x: torch.Tensor) -> Int8Rows:
     if torch.is_grad_enabled() and x.requires_grad:
         raise ValueError("quantize_int8_rows has no gradient; pass x itself to int8_linear, or a detached x")
     L.refuse_tangents(x)
-    return Int8Rows(*_quantize(_rows(x)), x.shape, x.dtype)
+    return Int8Rows._of(*_quantize(_rows(x)), x.shape, x.dtype)
 
 
 class Int8Weight:

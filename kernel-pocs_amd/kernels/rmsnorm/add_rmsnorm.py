@@ -138,7 +138,7 @@ def add_rmsnorm_int8(x: torch.Tensor, residual: Optional[torch.Tensor], weight: 
                     "forge_add_rmsnorm_int8")
     else:
         scale.zero_()
-    return Int8Rows(q, scale, x.shape, x.dtype), x if h is None else h
+    return Int8Rows._of(q, scale, x.shape, x.dtype), x if h is None else h
 
 
 __all__ = ["ForgeAddRMSNormFunction", "add_rmsnorm", "add_rmsnorm_int8"]

@@ -323,3 +323,19 @@ def test_entry_points_with_a_bias_type():
     assert gemm(bias_dtype=3) == 2 and gemm(bias_dtype=-1) == 2 and b"bias" in L.forge_last_error()
     assert lin(bias_dtype=3) == 2 and b"bias" in L.forge_last_error()
     assert gemm(bias=None, bias_dtype=3, K=-1) == 1 and lin(bias=None, bias_dtype=3, x=None) == 1
+
+
+def test_rows_that_the_kernels_cannot_read_are_refused():
+    from kernels.int8 import Int8Rows
+
+    q, s = torch.zeros(6, 32, dtype=torch.int8), torch.zeros(6)
+    assert Int8Rows(q, s, (2, 3, 20), BF16).values.shape == (2, 3, 20)
+    for padded, scale, shape in ((q.float(), s, (6, 20)), (q[0], s, (6, 20)), (q, s.double(), (6, 20)), (q, s.half(), (6, 20)),
+                                 (q, s[:5], (6, 20)), (q, s.view(6, 1), (6, 20)), (q, s, (5, 20)), (q, s, (2, 4, 20)),
+                                 (q, s, (6, 40)), (q, s, ()), (q[:, :24], s, (6, 20)), (q[:, 1:17], s, (6, 16)),
+                                 (torch.zeros(6, 24, dtype=torch.int8), s, (6, 20)), (q, torch.zeros(12)[::2], (6, 20)),
+                                 (q, s.to("meta"), (6, 20)), (q.t(), torch.zeros(32), (32, 6))):
+        with pytest.raises(ValueError, match="Int8Rows"):
+            Int8Rows(padded, scale, shape, BF16)
+    with pytest.raises(TypeError, match="fp16, bf16 or fp32"):
+        Int8Rows(q, s, (6, 20), torch.float64)
