@@ -34,7 +34,7 @@ def _pitch(k: int) -> int:
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """x as [rows, K] with a unit stride in K."""
-    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    x2 = x if x.dim() == 2 else x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
     if x2.is_contiguous():
         return x2
     if x2.stride(-1) != 1 and x2.shape[-1] > 1 or (x2.shape[0] > 1 and x2.stride(0) < x2.shape[-1]):

@@ -323,3 +323,16 @@ def test_int8_scales_of_large_weights(size, H):
     x = torch.full((3, H), 1e-3)
     x[:, :2] = torch.tensor([1.0, -0.5])
     _check8(x, None, torch.full((H,), size), 0.0)
+
+
+@pytest.mark.gpu
+def test_rows_without_columns():
+    from kernels.rmsnorm import add_rmsnorm, add_rmsnorm_int8
+
+    w = torch.ones(0, device="cuda", requires_grad=True)
+    x = torch.zeros(2, 3, 0, device="cuda", requires_grad=True)
+    y, h = add_rmsnorm(x, x, w)
+    assert y.shape == h.shape == (2, 3, 0)
+    assert [g.shape for g in torch.autograd.grad((y, h), (x, w), (y, h))] == [(2, 3, 0), (0,)]
+    rows, h = add_rmsnorm_int8(x.detach(), None, w.detach())
+    assert rows.values.shape == (2, 3, 0) and rows.scale.shape == (6,)

@@ -339,3 +339,22 @@ def test_rows_that_the_kernels_cannot_read_are_refused():
             Int8Rows(padded, scale, shape, BF16)
     with pytest.raises(TypeError, match="fp16, bf16 or fp32"):
         Int8Rows(q, s, (6, 20), torch.float64)
+
+
+@pytest.mark.gpu
+def test_no_columns_and_no_channels_with_leading_dimensions():
+    from kernels.int8 import Int8Weight, int8_linear, quantize_int8_rows
+
+    empty = Int8Weight(torch.zeros(3, 0, dtype=torch.int8, device="cuda"), torch.ones(3, device="cuda"), backward=True)
+    b = torch.arange(3.0, device="cuda")
+    x = torch.zeros(2, 4, 0, device="cuda", requires_grad=True)
+    y = int8_linear(x, empty, b)
+    assert torch.equal(y, b.expand(2, 4, 3)) and torch.autograd.grad(y, x, torch.ones_like(y))[0].shape == (2, 4, 0)
+    rows = quantize_int8_rows(x.detach())
+    assert rows.values.shape == (2, 4, 0) and torch.equal(int8_linear(rows, empty, b), b.expand(2, 4, 3))
+    none = Int8Weight(torch.zeros(0, 64, dtype=torch.int8, device="cuda"), torch.ones(0, device="cuda"), backward=True)
+    x = torch.randn(2, 4, 64, device="cuda", requires_grad=True)
+    y = int8_linear(x, none)
+    assert y.shape == (2, 4, 0) and torch.equal(torch.autograd.grad(y, x, torch.ones_like(y))[0], torch.zeros_like(x))
+    one = torch.zeros(0, device="cuda")
+    assert torch.equal(int8_linear(one, empty, b), b)
