@@ -117,10 +117,17 @@ def quantize_int8_rows(x: torch.Tensor) -> Int8Rows:
     return Int8Rows._of(*_quantize(_rows(x)), x.shape, x.dtype)
 
 
+def _check_sums(shape, backward):
+    """A product sums over the columns, the gradient of x over the channels."""
+    if shape[1] > MAX_K or (backward and shape[0] > MAX_K):
+        raise ValueError(f"a sum over more than {MAX_K} products does not fit 32 bits, got {tuple(shape)}"
+                         + (" with backward=True" if backward else ""))
+
+
 class Int8Weight:
     """A frozen weight [N, K] of 8-bit integers with a scale for each of its N channels,
-    laid out for the kernels (a copy of both).  backward: also its transpose, which the
-    gradient of the activations reads."""
+    laid out for the kernels (a copy of both).  K up to 2^17.  backward: also its
+    transpose, which the gradient of the activations reads; N up to 2^17 then."""
 
     def __init__(self, values: torch.Tensor, scale: torch.Tensor, *, backward: bool = False):
         if values.dim() != 2 or values.dtype != torch.int8:
@@ -130,8 +137,7 @@ class Int8Weight:
         if scale.device != values.device:
             raise ValueError(f"values and scale must be on one device, got {values.device} and {scale.device}")
         n, k = values.shape
-        if k > MAX_K or n > MAX_K:
-            raise ValueError(f"a sum over more than {MAX_K} products does not fit 32 bits, got {tuple(values.shape)}")
+        _check_sums(values.shape, backward)
         L.require_gpu(values)
         self.shape = values.shape
         self.padded = torch.zeros(n, _pitch(k), dtype=torch.int8, device=values.device)
@@ -155,8 +161,9 @@ class Int8Weight:
     def from_float(cls, weight: torch.Tensor, *, backward: bool = False) -> "Int8Weight":
         """weight [N, K] rounded by channels, as rows of activations are."""
         _check_float(weight, "weight")
-        if weight.dim() != 2 or max(weight.shape) > MAX_K:
-            raise ValueError(f"weight must be a matrix of at most {MAX_K} rows and columns, got {tuple(weight.shape)}")
+        if weight.dim() != 2:
+            raise ValueError(f"weight must be a matrix [N, K], got {tuple(weight.shape)}")
+        _check_sums(weight.shape, backward)
         self = cls.__new__(cls)
         self.shape = weight.shape
         self.padded, scale = _quantize(_rows(weight.detach()))

@@ -358,3 +358,21 @@ def test_no_columns_and_no_channels_with_leading_dimensions():
     assert y.shape == (2, 4, 0) and torch.equal(torch.autograd.grad(y, x, torch.ones_like(y))[0], torch.zeros_like(x))
     one = torch.zeros(0, device="cuda")
     assert torch.equal(int8_linear(one, empty, b), b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 50, 300])
+def test_more_channels_than_a_gradient_can_sum(m):
+    """More than 2^17 channels (an output layer's vocabulary): a product sums over the columns, only the gradient over
+    the channels."""
+    _check(m, (1 << 17) + 37, 48, BF16, bias=True, train=False)
+
+
+def test_a_gradient_over_too_many_channels_is_refused():
+    from kernels.int8 import Int8Weight
+
+    n = (1 << 17) + 1
+    with pytest.raises(ValueError, match="32 bits"):
+        Int8Weight(torch.zeros(n, 1, dtype=torch.int8), torch.zeros(n), backward=True)
+    with pytest.raises(RuntimeError, match="GPU"):
+        Int8Weight(torch.zeros(n, 1, dtype=torch.int8), torch.zeros(n))
