@@ -153,7 +153,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dq_kernel(Args a,
   f32x16 acc[DB];
   const int sees = a.causal ? min(sk.len, iq + shift + 1) : sk.len;
   const int all_see = a.causal ? min(sk.len, wq + shift + 1) : sk.len;
-  const int any_sees = a.causal ? min(sk.len, min(wq + 32, sq.len) + shift) : (wq < sq.len ? sk.len : 0);
+  const int any_sees = wq >= sq.len ? 0 : a.causal ? min(sk.len, min(wq + 32, sq.len) + shift) : sk.len;
 
   auto step = [&](int t, int slot, auto apart) __attribute__((always_inline)) {
     wait_dma<0>();

@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_fwd_kernel(Args a
   // keys that this lane's query sees, and those that every query of the wave does
   const int sees = a.causal ? min(sk.len, iq + shift + 1) : sk.len;
   const int all_see = a.causal ? min(sk.len, wq + shift + 1) : sk.len;
-  const int any_sees = a.causal ? min(sk.len, min(wq + 32, sq.len) + shift) : (wq < sq.len ? sk.len : 0);
+  const int any_sees = wq >= sq.len ? 0 : a.causal ? min(sk.len, min(wq + 32, sq.len) + shift) : sk.len;
 
   // (slot: a constant where the call is, so that it is part of the reads' immediates)
   auto step = [&](int t, int slot, auto apart) __attribute__((always_inline)) {
