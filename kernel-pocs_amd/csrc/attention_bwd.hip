@@ -65,6 +65,7 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(Args a, float* shift, i
     const int64_t batch = a.cu_q ? 0 : row / a.tq, r = a.cu_q ? row : row % a.tq;
     const T* o = row_ptr<T>(a.o, batch, r, head);
     const T* d = row_ptr<T>(a.dout, batch, r, head);
+    const float l = a.lse[p];
     float sum = 0.f;
     for (int c = 8 * (lane % 16); c < a.D; c += 128) {
       const Vec16<T> x = load16(o + c), y = load16(d + c);
@@ -77,7 +78,6 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(Args a, float* shift, i
     }
 #pragma unroll
     for (int off = 8; off >= 1; off /= 2) sum += __shfl_xor(sum, off, 64);
-    const float l = a.lse[row * a.H + head];
     // The dk, dv kernel looks here for rows of q and dout that are not finite: the sum is
     // not where dout is not, nor where q is not, as o is NaN then.  But of a query without
     // keys o is 0, whatever it holds.
@@ -254,8 +254,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
   const bool live = jk < sk.len;
   const int shift = sk.len - sq.len;
   bf16x8 kf[KS], vf[KS];
-  // (in each of the two loops' branches: registers that both share went to scratch memory)
-  auto load_own = [&]() __attribute__((always_inline)) {
+  {
     const T* kp = row_ptr<T>(a.k, sk.batch, sk.start + (live ? jk : 0), it.kv);
     const T* vp = row_ptr<T>(a.v, sk.batch, sk.start + (live ? jk : 0), it.kv);
 #pragma unroll
@@ -269,7 +268,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
       kf[ks] = __builtin_bit_cast(bf16x8, v);
       vf[ks] = __builtin_bit_cast(bf16x8, w);
     }
-  };
+  }
   // the first query that sees a key of the tile, and tiles of queries from there, of
   // each of the group's heads in turn
   const int first = a.causal ? max(0, k0 - shift) / BQ * BQ : 0;
@@ -321,7 +320,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
   float unit = 1.f;
 
   int tile_i = first;
-  auto step = [&](bool more, int slot, auto apart) __attribute__((always_inline)) {
+  auto step = [&](bool more, int slot, auto apart, auto on_k, auto on_v) __attribute__((always_inline)) {
     wait_dma<0>();
     barrier();
     if (more) issue(1 - slot);
@@ -350,7 +349,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
       for (int ks = 0; ks < KS; ++ks) s = mfma32<T>(fr.read(qt, 32 * qb, ks), kf[ks], s);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
-        if constexpr (DK) dp = mfma32<T>(fr.read(dt, 32 * qb, ks), vf[ks], dp);
+        if constexpr (on_k) dp = mfma32<T>(fr.read(dt, 32 * qb, ks), vf[ks], dp);
       if (a.causal && i0 + shift < wk + 31) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -364,15 +363,15 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
         s[r] = exp2_hw(P_BITS<T> ? __builtin_fmaf(s[r], c, P_BITS<T>) : s[r] * c);
         dp[r] *= s[r] * unit;
       }
-      if constexpr (DK) keep_in_range<T>(dp, unit, dk);
+      if constexpr (on_k) keep_in_range<T>(dp, unit, dk);
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (apart) {  // (the fragments read the tiles TILES behind qt and dt)
         __syncthreads();      // every wave has its scores of these queries
-        if constexpr (DK) Special<T, DP>::add(dk, qt + TILES, 32 * qb, 32, i0, jk - shift, sq.len, true);
-        if constexpr (DV) Special<T, DP>::add(dv, dt + TILES, 32 * qb, 32, i0, jk - shift, sq.len, false);
+        if constexpr (on_k) Special<T, DP>::add(dk, qt + TILES, 32 * qb, 32, i0, jk - shift, sq.len, true);
+        if constexpr (on_v) Special<T, DP>::add(dv, dt + TILES, 32 * qb, 32, i0, jk - shift, sq.len, false);
         __syncthreads();
-        if constexpr (DK) Special<T, DP>::clear(qt + TILES, 32 * qb, 32, wave, 4);
-        if constexpr (DV) Special<T, DP>::clear(dt + TILES, 32 * qb, 32, wave, 4);
+        if constexpr (on_k) Special<T, DP>::clear(qt + TILES, 32 * qb, 32, wave, 4);
+        if constexpr (on_v) Special<T, DP>::clear(dt + TILES, 32 * qb, 32, wave, 4);
         __syncthreads();
       }
 #pragma unroll
@@ -380,56 +379,69 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_dkv_kernel(Args a
         const bf16x8 p = pack_acc<T>(s, i), ds = pack_acc<T>(dp, i);
 #pragma unroll
         for (int db = 0; db < DB; ++db) {
-          if constexpr (DV) dv[db] = mfma32<T>(fc.read(dt, 32 * qb + 16 * i, db), p, dv[db]);
-          if constexpr (DK) dk[db] = mfma32<T>(fc.read(qt, 32 * qb + 16 * i, db), ds, dk[db]);
+          if constexpr (on_v) dv[db] = mfma32<T>(fc.read(dt, 32 * qb + 16 * i, db), p, dv[db]);
+          if constexpr (on_k) dk[db] = mfma32<T>(fc.read(qt, 32 * qb + 16 * i, db), ds, dk[db]);
         }
       }
     }
   };
-  if (n_t > 0) issue(0);
-  // (through slot 1's statistics, which are not under way yet)
-  if (a.causal && any_of_4_waves(smem + TILES / 2, wave, odd)) {
-    load_own();
-#pragma unroll 1
-    for (int t = 0; t < n_t; ++t) step(t + 1 < n_t, t % 2, std::true_type());
-  } else {
-    load_own();
-    for (int t = 0; t < n_t; t += 2) {
-      step(t + 1 < n_t, 0, std::false_type());
-      if (t + 1 < n_t) step(t + 2 < n_t, 1, std::false_type());
+  auto store = [&](auto on_k, auto on_v) __attribute__((always_inline)) {
+    if (!live) return;
+    const float p_one = exp2f(-P_BITS<T>), back = a.scale * p_one / unit;
+    if (a.parts > 1) {
+      const int64_t n_k = a.cu_k ? a.tk : a.tk * a.B, row = (a.cu_k ? sk.start : sk.batch * a.tk) + jk;
+      float* p = a.part + ((it.g * n_k + row) * a.Hkv + it.kv) * 2 * a.D;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = 32 * db + 8 * i + 4 * h;
+          if (d >= a.D) continue;
+          if constexpr (on_k)
+            *reinterpret_cast<f32x4*>(p + d) = f32x4{dk[db][4 * i], dk[db][4 * i + 1], dk[db][4 * i + 2], dk[db][4 * i + 3]} * back;
+          if constexpr (on_v)
+            *reinterpret_cast<f32x4*>(p + a.D + d) = f32x4{dv[db][4 * i], dv[db][4 * i + 1], dv[db][4 * i + 2], dv[db][4 * i + 3]} * p_one;
+        }
+      return;
     }
-  }
-  if (!live) return;
-  const float p_one = exp2f(-P_BITS<T>), back = a.scale * p_one / unit;
-  if (a.parts > 1) {
-    const int64_t n_k = a.cu_k ? a.tk : a.tk * a.B, row = (a.cu_k ? sk.start : sk.batch * a.tk) + jk;
-    float* p = a.part + ((it.g * n_k + row) * a.Hkv + it.kv) * 2 * a.D;
+    T* kp = row_ptr<T>(a.dk, sk.batch, sk.start + jk, it.kv);
+    T* vp = row_ptr<T>(a.dv, sk.batch, sk.start + jk, it.kv);
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int d = 32 * db + 8 * i + 4 * h;
         if (d >= a.D) continue;
-        if constexpr (DK)
-          *reinterpret_cast<f32x4*>(p + d) = f32x4{dk[db][4 * i], dk[db][4 * i + 1], dk[db][4 * i + 2], dk[db][4 * i + 3]} * back;
-        if constexpr (DV)
-          *reinterpret_cast<f32x4*>(p + a.D + d) = f32x4{dv[db][4 * i], dv[db][4 * i + 1], dv[db][4 * i + 2], dv[db][4 * i + 3]} * p_one;
+        if constexpr (on_k)
+          store4(kp + d, dk[db][4 * i] * back, dk[db][4 * i + 1] * back, dk[db][4 * i + 2] * back,
+                 dk[db][4 * i + 3] * back);
+        if constexpr (on_v) store4(vp + d, dv[db][4 * i] * p_one, dv[db][4 * i + 1] * p_one, dv[db][4 * i + 2] * p_one, dv[db][4 * i + 3] * p_one);
       }
+  };
+  typedef std::bool_constant<DK> WithK;
+  typedef std::bool_constant<DV> WithV;
+  if (n_t > 0) issue(0);
+  // (through slot 1's statistics, which are not under way yet)
+  if (a.causal && any_of_4_waves(smem + TILES / 2, wave, odd)) {
+    // dk and dv one after the other: together they take more registers than there are
+    auto pass = [&](auto on_k, auto on_v) __attribute__((always_inline)) {
+      tile_i = next_i = first;
+      next_head = it.kv * G + g_lo;
+      __syncthreads();
+      if (n_t > 0) issue(0);
+#pragma unroll 1
+      for (int t = 0; t < n_t; ++t) step(t + 1 < n_t, t % 2, std::true_type(), on_k, on_v);
+      store(on_k, on_v);
+    };
+    if constexpr (DK) pass(WithK(), std::false_type());
+    if constexpr (DV) pass(std::false_type(), WithV());
     return;
   }
-  T* kp = row_ptr<T>(a.dk, sk.batch, sk.start + jk, it.kv);
-  T* vp = row_ptr<T>(a.dv, sk.batch, sk.start + jk, it.kv);
-#pragma unroll
-  for (int db = 0; db < DB; ++db)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = 32 * db + 8 * i + 4 * h;
-      if (d >= a.D) continue;
-      if constexpr (DK)
-        store4(kp + d, dk[db][4 * i] * back, dk[db][4 * i + 1] * back, dk[db][4 * i + 2] * back,
-               dk[db][4 * i + 3] * back);
-      if constexpr (DV) store4(vp + d, dv[db][4 * i] * p_one, dv[db][4 * i + 1] * p_one, dv[db][4 * i + 2] * p_one, dv[db][4 * i + 3] * p_one);
-    }
+  for (int t = 0; t < n_t; t += 2) {
+    step(t + 1 < n_t, 0, std::false_type(), WithK(), WithV());
+    if (t + 1 < n_t) step(t + 2 < n_t, 1, std::false_type(), WithK(), WithV());
+  }
+  store(WithK(), WithV());
 }
 
 // dk and dv: the sums of the parts, in order.  4 values a thread.
