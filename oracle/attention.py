@@ -39,14 +39,17 @@ def head_fwd_bwd(q, k, v, do, scale, causal, unit, tiny, tiny_bwd=None):
     mag = scale * q.abs() @ k.abs().T
     rel = torch.where(sees, (mag + mag.amax(-1, keepdim=True) if m else mag) * depth * u32 + (m + 16) * u32, 0.0)
     p_err = p * (unit + rel) + (tiny + FLUSH) * sees
-    o_err = p_err @ v.abs() + (rel * p).sum(-1, keepdim=True) * (p @ v.abs()) + o.abs() * unit + tiny
+    sum_err = p_err @ v.abs() + (rel * p).sum(-1, keepdim=True) * (p @ v.abs())
+    o_err = sum_err + o.abs() * unit + tiny
     lse_err = (rel * p).sum(-1) + (lse.abs().nan_to_num(0.0, 0.0, 0.0) + 1) * 8 * u32
     dp = do @ v.T
     delta = (do * o).sum(-1, keepdim=True)
     ds = p * (dp - delta)
     dp_mag = do.abs() @ v.abs().T
-    # delta is formed from the rounded o
-    delta_err = (do.abs() * (o_err + depth * u32 * o.abs())).sum(-1, keepdim=True)
+    # delta is formed of o before its rounding, but for half a 254th of a step (a step: twice the largest
+    # rounding, unit |o| at least, or tiny)
+    half_part = (o.abs() * unit + tiny) / 254
+    delta_err = (do.abs() * (sum_err + half_part + depth * u32 * o.abs())).sum(-1, keepdim=True)
     # (a probability below the smallest normal of fp32 is 0: off by FLUSH, and ds by that times its other factor)
     ds_err = p * (delta_err + dp_mag * depth * u32) + ds.abs() * (unit + 3 * rel) + (tiny_bwd + FLUSH * (dp - delta).abs()) * sees
     pv_err = p * (unit + 3 * rel) + (tiny_bwd + FLUSH) * sees

@@ -618,3 +618,87 @@ def test_queries_and_gradients_that_are_not_finite(lens_q, lens_k, row, H, kv, D
     want = plain[2].clone()
     want[:sees, 0, 0] = inf
     assert torch.equal(dv, want)
+
+
+def _spacing(r, dtype):
+    """The spacing of the type's values at r (of the smallest at 0)."""
+    e = torch.where(r == 0, 0.0, torch.ldexp(torch.ones_like(r), torch.frexp(r).exponent - 1))
+    return e.clamp(min=2.0 ** -14) * 2.0 ** -10 if dtype == FP16 else e.clamp(min=2.0 ** -100) * 2.0 ** -7
+
+
+# what writes an output: the tiles' kernel, that of few tokens, and the join of its chunks
+_WRITERS = [([70, 5], [70, 130]), ([1, 2], [100, 17]), ([1, 2], [300, 8])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("D", [64, 40, 128, 200, 256])
+@pytest.mark.parametrize("lens_q,lens_k", _WRITERS)
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -15, 300.0])
+def test_what_the_rounding_of_an_output_took(size, lens_q, lens_k, D, dtype):
+    """The byte a value that the gradients' delta is formed with, in 254ths of a step: with it an output is that of
+    exact arithmetic to half of such a part and the fp32 sums' roundings.  Scores of 0, so that all probabilities are
+    one power of two and are not rounded; fp16's subnormals among the outputs."""
+    from kernels.attention.attention import _forward, _Layout
+
+    _, k, v, _ = _make(lens_q, lens_k, 4, 2, D, dtype)
+    v = (v.float() * size).to(dtype)
+    q = torch.zeros(sum(lens_q), 4, D, dtype=dtype)
+    at_q, at_k = _offsets(lens_q), _offsets(lens_k)
+    cu_q, cu_k = (torch.tensor(a, device="cuda", dtype=torch.int32) for a in (at_q, at_k))
+    out, _, low = _forward(q.cuda(), k.cuda(), v.cuda(), cu_q, cu_k, 1.0, True, _Layout.packed, True, True)
+    out, low = out.double().cpu(), low.view(out.shape).double().cpu()
+    for n in range(len(lens_q)):
+        for i in range(at_q[n], at_q[n + 1]):
+            seen = v[at_k[n]:at_k[n + 1] - (at_q[n + 1] - 1 - i)].double().repeat_interleave(2, 1)
+            if len(seen) == 0:
+                continue
+            sums = (len(seen) + 24) * 2.0 ** -24 * seen.abs().mean(0)
+            step = _spacing(out[i], dtype) / 254
+            assert low[i].abs().max() <= 127
+            over = (out[i] + low[i] * step - seen.mean(0)).abs() - (0.5 + 2.0 ** -12) * step - sums
+            assert over.max() <= 0, (i, over.max().item(), step.max().item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("D", [64, 136])
+@pytest.mark.parametrize("lens_q,lens_k", _WRITERS)
+def test_gradients_without_the_outputs_rounding(lens_q, lens_k, D, dtype):
+    """Values that are half a and half the type's next value: their mean, the output, lies between the two and its
+    rounding is as large as every dout . v - delta.  delta of the rounded output misses by |dout| times half a step, all
+    of ds; delta as it is by a 254th of that, and the bound below is made of the latter."""
+    from kernels.attention import forge_varlen_attention
+
+    eps = torch.finfo(dtype).eps
+    unit, tiny = _unit(dtype)
+    T, Tk, u32 = sum(lens_q), sum(lens_k), 2.0 ** -24
+    q = torch.full((T, 2, D), 2.0 ** -6, dtype=dtype)
+    k = torch.ones(Tk, 1, D, dtype=dtype)
+    v = torch.full((Tk, 1, D), 1.5, dtype=dtype)
+    v[1::2] += eps
+    do = (torch.rand(T, 2, D, generator=torch.Generator().manual_seed(0)) + 0.5).to(dtype)
+    at_q, at_k = _offsets(lens_q), _offsets([n // 2 * 2 for n in lens_k])
+    cu_q, cu_k = (torch.tensor(a, device="cuda", dtype=torch.int32) for a in (at_q, at_k))
+    leaves = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    out = forge_varlen_attention(*leaves, cu_q, cu_k, causal=False, scale=1.0)
+    dq, dk = (t.double().cpu() for t in torch.autograd.grad(out, leaves[:2], do.cuda()))
+    want_dk, err_dk = torch.zeros(Tk, D).double(), torch.zeros(Tk, D).double()
+    for n in range(len(lens_q)):
+        rows, keys = slice(at_q[n], at_q[n + 1]), slice(at_k[n], at_k[n + 1])
+        m = at_k[n + 1] - at_k[n]
+        for h in range(2):
+            r = head_fwd_bwd(q[rows, h], k[keys, 0], v[keys, 0], do[rows, h], 1.0, False, 0.0, 0.0)
+            d = do[rows, h].double()
+            sums = (D + m + 24) * u32 * 1.6 * d.sum(-1)  # of dout . v, of delta, and of the output in it
+            delta_err = (0.5 + 2.0 ** -12) / 254 * eps * d.sum(-1) + 2 * sums
+            ds = (d @ v[keys, 0].double().T - (d * r.o).sum(-1, keepdim=True)) / m
+            rel = (2 * D * 2.0 ** -6 * (D + 8) + 2 * m + 32) * u32  # of a probability
+            ds_err = (delta_err.unsqueeze(1) + sums.unsqueeze(1)) / m + ds.abs() * (unit + 4 * rel) + tiny * 2.0 ** -14
+            bound = (ds_err.sum(1) + (m + 16) * u32 * ds.abs().sum(1)).unsqueeze(1) * torch.ones(D) + tiny
+            missed = 0.4 * eps * d.sum(-1, keepdim=True)  # (what delta of the rounded output would do to dq)
+            assert bool((bound < 0.5 * missed).all())
+            assert bool(((dq[rows, h] - r.dq).abs() <= bound).all()), (n, h)
+            want_dk[keys] += r.dk
+            err_dk[keys] += (ds_err + (len(d) + 16) * u32 * ds.abs()).T @ q[rows, h].double()
+    assert bool(((dk[:, 0] - want_dk).abs() <= err_dk + want_dk.abs() * unit + tiny).all())
