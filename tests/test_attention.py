@@ -702,3 +702,52 @@ def test_gradients_without_the_outputs_rounding(lens_q, lens_k, D, dtype):
             want_dk[keys] += r.dk
             err_dk[keys] += (ds_err + (len(d) + 16) * u32 * ds.abs()).T @ q[rows, h].double()
     assert bool(((dk[:, 0] - want_dk).abs() <= err_dk + want_dk.abs() * unit + tiny).all())
+
+
+@pytest.mark.gpu
+def test_a_cache_with_room_to_grow():
+    """Tokens appended in place: sequences without queries stand for the room behind each sequence's keys, whatever it
+    holds.  Steps of one and more tokens, eager and in a captured call that is replayed as the offsets move."""
+    from kernels.attention import forge_varlen_attention
+
+    H, kv, D, room, held = 8, 2, 64, [700, 40, 300], [600, 0, 129]
+    starts, steps = _offsets(room), 6
+    g = torch.Generator().manual_seed(0)
+    cache = torch.full((2, sum(room) + 500, kv, D), float("nan"), dtype=BF16)
+    for s, n in zip(starts, held):
+        cache[:, s:s + n] = torch.randn(2, n, kv, D, generator=g).to(BF16)
+    kc, vc = cache.cuda()
+    q = torch.zeros(3, H, D, dtype=BF16, device="cuda")
+    # a sequence of the batch, then its room, which has no queries
+    cu_q = torch.tensor([0, 1, 1, 2, 2, 3, 3], dtype=torch.int32, device="cuda")
+    cu_k = torch.zeros(7, dtype=torch.int32, device="cuda")
+
+    def step():
+        return forge_varlen_attention(q, kc, vc, cu_q, cu_k)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for t in range(steps):
+        new = torch.randn(2, 3, kv, D, generator=g).to(BF16)
+        for i, s in enumerate(starts[:3]):
+            cache[:, s + held[i]] = new[:, i]
+            kc[s + held[i]], vc[s + held[i]] = new[0, i].cuda(), new[1, i].cuda()
+            held[i] += 1
+        q.copy_(torch.randn(3, H, D, generator=g).to(BF16))
+        cu_k.copy_(torch.tensor([x for i, s in enumerate(starts[:3]) for x in (s, s + held[i])] + [starts[3]], dtype=torch.int32))
+        out = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, captured), t
+        for i, s in enumerate(starts[:3]):
+            keys = slice(s, s + held[i])
+            for h in range(H):
+                r = head_fwd_bwd(q[i:i + 1, h].cpu(), cache[0, keys, h * kv // H], cache[1, keys, h * kv // H],
+                                 torch.zeros(1, D), D ** -0.5, True, *_unit(BF16))
+                _within(out[i:i + 1, h], r.o, r.o_err, (t, i, h))
