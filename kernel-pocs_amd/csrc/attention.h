@@ -374,15 +374,16 @@ __device__ __forceinline__ float nothing(int sees) { return sees > 0 ? __builtin
 template <class T>
 __device__ __forceinline__ bool second_run(bool hides) { return hides || !std::is_same_v<T, fp16_t>; }
 
-// (infinities among them)
+// (infinities among them; in four chains)
 template <int N>
 __device__ __forceinline__ bool any_nan(const f32x16 (&sums)[N]) {
-  float t = 0.f;
+  float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) t = __builtin_fmaf(sums[i][r], 0.f, t);
-  return t != t;
+    for (int r = 0; r < 16; ++r) t[r % 4] = __builtin_fmaf(sums[i][r], 0.f, t[r % 4]);
+  const float all = t[0] + t[1] + (t[2] + t[3]);
+  return all != all;
 }
 
 // Whether any of the workgroup's 4 waves has it; through 16 bytes of LDS that no wave

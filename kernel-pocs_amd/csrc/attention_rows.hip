@@ -32,8 +32,8 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_rows_kernel(Args a, Parts par
   constexpr int RING = NW * 2 * 2 * Dma::BYTES, SUMS = NW * 32 * PITCH * 4;
   // (one array: beside a second one the compiler waits for all LDS-DMA before it reads)
   constexpr int STAT = RING > SUMS ? RING : SUMS;
-  __shared__ __attribute__((aligned(1024))) char smem[STAT + 2 * NW * 32 * 4];
-  float* const stat = reinterpret_cast<float*>(smem + STAT);  // [2][NW][32]: maxima and sums
+  __shared__ __attribute__((aligned(1024))) char smem[STAT + 3 * NW * 32 * 4];
+  float* const stat = reinterpret_cast<float*>(smem + STAT);  // [3][NW][32]: maxima, sums of p, 1 / down
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), h = lane / 32;
   const int G = a.H / a.Hkv, kv = blockIdx.y;
   const TileAt at = find_tile(a.cu_k, a.B, a.tk, parts.C, blockIdx.x, 1);
@@ -147,19 +147,17 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_rows_kernel(Args a, Parts par
     l += other_half(l);
     wait_dma<0>();
     barrier();  // every wave is done with its ring
-    // outputs of parts are joined, not sums: those may be past fp32's range where the
-    // output is not
-    const float part_inv = l == 0.f ? 0.f : 1.f / (l * down);
     float* sums = reinterpret_cast<float*>(smem) + wave * 32 * PITCH + (lane % 32) * PITCH;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         *reinterpret_cast<f32x4*>(sums + 32 * db + 8 * i + 4 * h) =
-            f32x4{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]} * part_inv;
+            f32x4{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]};
     if (h == 0) {
       stat[wave * 32 + lane] = m;
       stat[(NW + wave) * 32 + lane] = l;
+      stat[(2 * NW + wave) * 32 + lane] = 1.f / down;
     }
     __syncthreads();
     const int rows = min(32, n_rows - r0), vecs = a.D / 4;
@@ -168,11 +166,14 @@ __global__ __launch_bounds__(NW * 64, 1) void attn_rows_kernel(Args a, Parts par
       float top = stat[r];
 #pragma unroll
       for (int w = 1; w < NW; ++w) top = fmaxf(top, stat[w * 32 + r]);
+      // (divided by the sum first: the waves' sums may be past fp32's range together, or
+      // without their factors)
       float total = 0.f, f[NW], v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        f[w] = stat[(NW + w) * 32 + r] * exp2_hw(stat[w * 32 + r] - top);
-        total += f[w];
+        f[w] = exp2_hw(stat[w * 32 + r] - top);
+        total += stat[(NW + w) * 32 + r] * f[w];
+        f[w] *= stat[(2 * NW + w) * 32 + r];
       }
       // (of a chunk of several 0: the join looks at them all)
       const float inv = total != 0.f ? 1.f / total : n_chunk == 1 ? nothing(a.causal ? min(sk.len, t + shift + 1) : sk.len) : 0.f;
