@@ -467,7 +467,7 @@ __device__ __forceinline__ float scale_i8_near(int acc, float row, float col, fl
   return __builtin_fmaf((float)acc * row, col, bias);
 }
 __device__ __forceinline__ float scale_i8(int acc, float row, float col, float bias) {
-  const bool far = row > FAR_SCALE;
+  const bool far = __builtin_fabsf(row) > FAR_SCALE;
   return scale_i8_near(acc, far ? col : row, far ? row : col, bias);
 }
 // By halves of 32 bits, or the same 16 bits twice, and selects: with a branch on the type

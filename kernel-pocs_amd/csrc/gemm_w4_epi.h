@@ -795,6 +795,31 @@ __device__ __forceinline__ void w4_epilogue_staged_dual(const GemmArgs& args, f3
 // ---------------------------------------------------------------------------
 constexpr int W4_SCALES = 160 * 1024 - 3 * 256 * 4;  // byte offset in the ring: row, column scales, bias
 
+// The rows of a tile from FAR_SCALE on, once more, from the operands: a thread to a
+// column.  Seldom runs.  (With scale_i8's choice among the epilogue's instructions, or a
+// branch to a second one, [8192, 14336], K = 4096 took 389 us; 382 without, and with this.)
+template <class O>
+__device__ __forceinline__ void far_rows_i8(const GemmArgs& args, int64_t m0, int64_t n0) {
+  const Seg& sg = args.segs[0];
+  const EpiArgs& ep = args.ep;
+  const int64_t n = n0 + threadIdx.x, rows = min((int64_t)256, args.M - m0);
+#pragma unroll 1
+  for (int64_t m = m0; m < m0 + rows; ++m) {
+    const float row = ep.row_scale[m];
+    if (!(fabsf(row) > FAR_SCALE) || n >= args.N) continue;
+    const char* a = (const char*)(sg.a + m * sg.lda);
+    const char* b = (const char*)(sg.b + n * sg.ldb);
+    int sum = 0;
+#pragma unroll 1
+    for (int64_t k = 0; k < 2 * sg.k; k += 16) {
+      const i32x4 x = *reinterpret_cast<const i32x4*>(a + k), y = *reinterpret_cast<const i32x4*>(b + k);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum = __builtin_amdgcn_sdot4(x[i], y[i], sum, false);
+    }
+    ((O*)ep.c)[m * ep.ldc + n] = from_f32<O>(scale_i8(sum, row, ep.col_scale[n], bias_i8(ep, n)));
+  }
+}
+
 template <class O, bool VEC>
 __device__ __forceinline__ void w4_epilogue_i8(const GemmArgs& args, const i32x4 (&acc)[8][8], int64_t m0, int64_t n0, int lane,
                                                int wm, int wn, char* smem) {
@@ -805,20 +830,14 @@ __device__ __forceinline__ void w4_epilogue_i8(const GemmArgs& args, const i32x4
   float* scales = reinterpret_cast<float*>(smem + W4_SCALES);
   const int64_t sm = min(m0 + tid, M - 1), sn = min(n0 + tid, N - 1);
   const float row_scale = ep.row_scale[sm], col_scale = ep.col_scale[sn], col_bias = bias_i8(ep, sn);
-  // A tile with a scale from FAR_SCALE on: 2^26 goes from the rows' scales to the columns',
-  // so that no sum times a row's passes fp32's range (a column's that would is the largest
-  // value: with such a row C is infinite all the same, or 0).  Of rows below 2^-100 in
-  // such a tile bits are lost.  Every wave looks at all of the tile's rows, in registers
-  // and without a branch: [8192, 14336], K = 4096 took 381 us before and takes 382, 389 with
-  // the scales read again behind the barrier and a branch.
+  // (whether any of the tile's rows is far: every wave looks at all of them)
   float top = 0.f;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) top = fmaxf(top, ep.row_scale[min(m0 + 64 * r + lane, M - 1)]);
+  for (int r = 0; r < 4; ++r) top = fmaxf(top, fabsf(ep.row_scale[min(m0 + 64 * r + lane, M - 1)]));
   const bool far = __any(top > FAR_SCALE);
-  const float up = far ? col_scale * 0x1p26f : col_scale;
   lds_barrier();  // the main loop's LDS reads are done in every wave
-  scales[tid] = far ? row_scale * 0x1p-26f : row_scale;
-  scales[256 + tid] = far && up > __FLT_MAX__ ? __FLT_MAX__ : up;
+  scales[tid] = row_scale;
+  scales[256 + tid] = col_scale;
   scales[512 + tid] = col_bias;
   lds_barrier();
   float row[8];
@@ -907,6 +926,11 @@ __device__ __forceinline__ void w4_epilogue_i8(const GemmArgs& args, const i32x4
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (and read, before the other half is written)
     }
+  }
+  if (far) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's values are written,
+    __syncthreads();                                  // and every wave's
+    far_rows_i8<O>(args, m0, n0);
   }
 }
 

@@ -376,3 +376,28 @@ def test_a_gradient_over_too_many_channels_is_refused():
         Int8Weight(torch.zeros(n, 1, dtype=torch.int8), torch.zeros(n), backward=True)
     with pytest.raises(RuntimeError, match="GPU"):
         Int8Weight(torch.zeros(n, 1, dtype=torch.int8), torch.zeros(n))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", _ENGINES)
+def test_large_scales_that_are_negative(m, n, k):
+    """Of rows and of channels, where a caller's have signs: as large ones, and 0 times the largest is 0."""
+    from kernels.int8 import Int8Rows, Int8Weight, int8_linear
+
+    g = torch.Generator().manual_seed(m)
+    w, ws = _weight(n, k)
+    pitch = (k + 15) // 16 * 16
+    q = torch.randint(-127, 128, (m, pitch), generator=g).to(torch.int8)
+    q[:, k:] = 0
+    q[1 % m] = 0
+    scale = torch.rand(m, generator=g) + 0.5
+    scale[::2] *= -1e34
+    scale[1 % m] = -1e36
+    ws = ws * 1e-33
+    ws[::3] *= -1
+    ws[-1] = -3e38
+    y = int8_linear(Int8Rows(q.cuda(), scale.cuda(), (m, k), FP32), Int8Weight(w.cuda(), ws.cuda())).cpu()
+    ref, terms = linear(q[:, :k], scale, w, ws)
+    over = ref.abs() > 3.4e38
+    assert bool((y[1 % m] == 0).all()) and torch.equal(torch.isinf(y), over)
+    _within(y[~over], ref[~over], terms[~over], 6, "y")
