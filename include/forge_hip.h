@@ -769,7 +769,7 @@ int forge_transpose_2b_batch(int n, const void* const* src, const int64_t* ld_sr
 /* out_i = sum_j p_ij v_j, p_ij = exp(scale q_i.k_j - lse_i), over the keys that
  * query i sees: its sequence's, with causal != 0 those j <= i + len_k - len_q.
  * H heads on Hkv key heads (head h reads h / (H / Hkv)), D a multiple of 8 up
- * to 256, fp16 or bf16, fp32 sums.
+ * to 256, fp16 or bf16, fp32 sums; scale from 2^-100 to 2^100.
  *   varlen: cu_q, cu_k hold B + 1 int32 offsets into tq queries and tk keys,
  *     not decreasing; rows before the first and behind the last get zeros.
  *     Offsets are read on the device only and clamped to the arrays.

@@ -38,7 +38,8 @@ static int check_sizes(int dtype, const Args& a) {
     return forge_set_error(FORGE_ERR_INVALID, "attention: %d heads on %d key heads", a.H, a.Hkv);
   if ((a.cu_q == nullptr) != (a.cu_k == nullptr))
     return forge_set_error(FORGE_ERR_INVALID, "attention: offsets of one side only");
-  if (!(a.scale > 0.f && a.scale < __builtin_inff())) return forge_set_error(FORGE_ERR_INVALID, "attention: scale");
+  // (the backward divides lse by it, and all multiply it by log2(e))
+  if (!(a.scale >= 0x1p-100f && a.scale <= 0x1p100f)) return forge_set_error(FORGE_ERR_INVALID, "attention: scale %g", a.scale);
   return FORGE_OK;
 }
 

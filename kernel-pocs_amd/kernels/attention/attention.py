@@ -31,6 +31,7 @@ _DTYPES = (torch.float16, torch.bfloat16)
 _INTEGERS = (torch.int32, torch.int64)
 MAX_HEAD_DIM = 256
 _MAX_ROW = 1 << 23  # elements from one token to the next
+_SCALES = (2.0 ** -100, 2.0 ** 100)  # lse / scale and scale log2(e) within fp32
 
 
 def _rows_ok(t, strides):
@@ -159,8 +160,8 @@ def _check(q, k, v, dims, scale):
     heads, kv_heads = q.shape[1], k.shape[1]
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
         raise ValueError(f"{heads} heads need a number of key heads that divides them, got {kv_heads}")
-    if scale is not None and not 0.0 < scale < float("inf"):
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if scale is not None and not _SCALES[0] <= scale <= _SCALES[1]:
+        raise ValueError(f"scale must be positive, from 2^-100 to 2^100, got {scale}")
 
 
 def _offsets(name, cu, rows, device, validate):

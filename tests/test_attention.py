@@ -751,3 +751,22 @@ def test_a_cache_with_room_to_grow():
                 r = head_fwd_bwd(q[i:i + 1, h].cpu(), cache[0, keys, h * kv // H], cache[1, keys, h * kv // H],
                                  torch.zeros(1, D), D ** -0.5, True, *_unit(BF16))
                 _within(out[i:i + 1, h], r.o, r.o_err, (t, i, h))
+
+
+def test_scales_that_fp32_cannot_divide_by_are_refused():
+    from forge_hip import _lib as L
+    from kernels.attention import forge_varlen_attention
+
+    t, cu = torch.zeros(4, 2, 64, dtype=BF16), torch.tensor([0, 4], dtype=torch.int32)
+    rows = [16, 0, 512, 64]
+    for scale in (1e-38, 1e-31, 1e31):
+        with pytest.raises(ValueError, match="positive, from"):
+            forge_varlen_attention(t, t, t, cu, scale=scale)
+        assert L.forge_attention_fwd(2, *(rows * 4), None, None, 16, 16, 1, 4, 4, 4, 2, 64, scale, 1, None, None) == 1
+        assert b"scale" in L.forge_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [1e-30, 1e-20])
+def test_small_scales(scale):
+    _check([70, 3], [70, 40], 4, 2, 64, BF16, scale=scale)
