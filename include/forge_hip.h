@@ -842,7 +842,7 @@ int forge_quantize_rows(int dtype, const void* x, int64_t ldx, const float* col_
                         float* scale, int64_t rows, int64_t H, void* stream);
 
 /* C[m, n] = (sum_k a[m, k] b[n, k]) row_scale[m] col_scale[n] + bias[n]: the sum exact in
- * 32-bit integers (K up to 2^17), C (fp32, bf16 or fp16, pitch ldc) rounded once.  a
+ * 32-bit integers (K up to 2^17), C (fp32, bf16 or fp16, pitch ldc) formed of it in fp32.  a
  * [M][lda], b [N][ldb]: 16-byte aligned, pitches multiples of 16 below 2^22, zeros from K
  * to the next multiple of 16.  bias: C's type (_typed: fp32, bf16 or fp16), or NULL.  work:
  * forge_int8_gemm_workspace bytes, 16-byte aligned (0: may be NULL). */

@@ -459,7 +459,7 @@ __global__ __launch_bounds__(256) void attn_dkv_join_kernel(Args a, int64_t n_k)
 }
 
 // Parts of a group's heads, a workgroup each (13 sequences of 3001 tokens, 14 heads of 64
-// on 2: 80 workgroups 84 us, 480 33 and 5 for the join): where the tiles of keys alone would
+// on 2: 80 workgroups 84 us, 480 35 and 5 for the join): where the tiles of keys alone would
 // leave CUs without work (two workgroups a CU are resident), and where a
 // workgroup has at least 16 tiles of queries to go through (a tile takes longer than
 // its share of the join).

@@ -12,9 +12,12 @@
 //
 // A workgroup of 4 waves takes 128 queries of one head, 32 a wave; tiles of 64
 // keys and values come by LDS-DMA into a ring of two.  8 causal sequences, 16384
-// tokens, 32 heads of 128 on 8: 390 to 410 us, 820 TFLOP/s.  The matrix pipes set
-// the time, with the power they leave (1150 where the data are zeros); 8 waves to
-// 256 queries, or 64 queries a wave, were slower (870 and 754 where this ran 890).
+// tokens, 32 heads of 128 on 8: 390 to 410 us, 820 TFLOP/s.  Of its parts MFMA alone
+// reaches 1680, with LDS-DMA and barriers 1270, with the reads of LDS 1020: each wave
+// reads all of a tile for itself, 1024 cycles of LDS beside 1031 of MFMA, and the softmax
+// stands between its two products (power adds to that: 1150 where the data are
+// zeros).  8 waves to 256 queries, or 64 queries a wave, were slower (870 and 754 where
+// this ran 890).
 #include "attention.h"
 
 namespace fattn {

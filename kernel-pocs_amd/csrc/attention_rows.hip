@@ -9,8 +9,8 @@
 // ring of its own, without barriers.  The waves' sums are joined in LDS; those of
 // several chunks by a second launch.  Every sum has a fixed order.
 //
-// 32 sequences of 131072 keys in all, 8 kv heads of 128, a token each: 104 us, keys and
-// values at 5.2 TB/s, and 6 for the join.  4 tokens and 2004 keys: 8 and 5 us.
+// 32 sequences of 131072 keys in all, 8 kv heads of 128, a token each: 106 us, keys and
+// values at 5.1 TB/s, and 6 for the join.  4 tokens and 2004 keys: 9 and 5 us.
 #include "attention.h"
 
 namespace fattn {

@@ -1338,8 +1338,7 @@ void gemm_dma_kernel(GemmArgs args) {
           }
       }
     }
-    if constexpr (!std::is_same_v<T, I8<int>>)
-    epilogue<out_t<T>, BM, BN, WAVES_M, WAVES_N, EPI>(args, acc, m0, n0, lane, wm, wn);
+    if constexpr (!std::is_same_v<T, I8<int>>) epilogue<out_t<T>, BM, BN, WAVES_M, WAVES_N, EPI>(args, acc, m0, n0, lane, wm, wn);
   }
 }
 

@@ -2,7 +2,7 @@
 //   C[m, n] = (sum_k a[m, k] b[n, k]) row_scale[m] col_scale[n] + bias[n]
 // a [M][K] and b [N][K], K-contiguous with pitches that are multiples of 16
 // bytes and zeros from K to the next multiple of 16.  The sum is exact in 32-bit
-// integers; C is rounded once, to fp32, bf16 or fp16.
+// integers; C is formed of it in fp32 (scale_i8) and rounded to fp32, bf16 or fp16.
 //
 // The engines are those of the 16-bit products (gemm_w4.h, gemm_core.h,
 // gemm_rows.hip), which see two values as one 16-bit word: the matrix
@@ -63,7 +63,7 @@ static Plan plan_i8(int64_t M, int64_t N, int64_t K) {
 
 static int64_t part_pitch(int64_t N) { return (N + 3) / 4 * 4; }
 
-// C from the integers of the parts of K: still exact, and rounded once.
+// C from the integers of the parts of K, whose sum is still exact.
 template <class O>
 __global__ __launch_bounds__(256) void join_i8_kernel(const int* parts, int64_t stride, int n, int64_t M, int64_t N, int64_t vecs,
                                                       EpiArgs ep) {

@@ -7,8 +7,9 @@ that is found as they come:
     q = round(127 x / a), a = max |x| of the row,  scale = a / 127
     y = (sum_k q[m, k] w[n, k]) scale[m] w_scale[n] + bias[n]
 
-The integers are those of exact arithmetic (half to even), their sum is exact, and y
-is rounded once.  A row with an infinity or NaN has a NaN scale, so all that is
+The integers are those of exact arithmetic (half to even) and their sum is exact.  y is
+formed of it in fp32 (the sum, its product with a scale, and that with the other plus
+the bias are rounded) and then rounded to its type.  A row with an infinity or NaN has a NaN scale, so all that is
 computed of it is NaN; a row of zeros has scale 0.
 
 Weights are frozen: there is no gradient for them or the bias.  The gradient of x
