@@ -387,7 +387,7 @@ def attention_args(module, query, key, value, attention_mask, kwargs):
     D, queries, keys = query.shape[-1], query.shape[2], key.shape[2]
     if D < 8 or D % 8 or D > 256 or key.shape != value.shape or key.shape[-1] != D or query.shape[1] % key.shape[1]:
         return None
-    if module.training and float(getattr(module, "attention_dropout", 0.0)) != 0.0 or not module.scaling > 0.0:
+    if module.training and float(getattr(module, "attention_dropout", 0.0)) != 0.0 or not 2.0 ** -100 <= module.scaling <= 2.0 ** 100:
         return None
     if getattr(module, "attn_logit_softcapping", None) is not None:
         return None

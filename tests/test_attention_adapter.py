@@ -205,3 +205,14 @@ def test_calls_that_say_whether_they_are_causal(monkeypatch):
     assert attention_args(module, q, k, k, None, {"is_causal": False}) is None
     assert attention_args(module, q, k, k, None, {"some_option": False}) is None
     assert attention_args(module, q, k, k, None, {"is_causal": None, "output_attentions": False}) == (True, None, None)
+
+
+@pytest.mark.gpu
+def test_scales_that_forge_attention_refuses_run_the_models_implementation():
+    from forge.patching.kernels.lora import attention_args
+
+    module, _ = _attn()
+    q, k = (torch.zeros(2, h, 5, 128, device="cuda", dtype=BF16) for h in (4, 2))
+    for scale, taken in ((128 ** -0.5, True), (0.0, False), (-1.0, False), (1e-38, False), (1e38, False), (float("nan"), False)):
+        module.scaling = scale
+        assert (attention_args(module, q, k, k, None, {}) is not None) == taken, scale
